@@ -18,6 +18,11 @@ from dominusultra_b200.attention import (  # noqa: F401
     dominus_ultra_prefill,
     precompute_rope_cos_sin,
 )
+from dominusultra_b200.paged import (  # noqa: F401
+    dominus_ultra_decode_paged,
+    dominus_ultra_paged_tables,
+    dominus_ultra_paged_write,
+)
 
 __all__ = ["precompute_rope_cos_sin", "dominus_ultra_prefill", "dominus_ultra_decode"]
 

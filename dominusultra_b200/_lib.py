@@ -79,6 +79,9 @@ SIGNATURES = {
         _i, [_vp, _vp, ctypes.POINTER(_vp), _i, _i, _i, _i, _vp, _i, _vp, _vp]
     ),
     "du_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _ll, _vp]),
+    "du_paged_tables": (_i, [_vp] * 8 + [_i] * 5 + [_vp]),
+    "du_paged_write": (_i, [_vp] * 10 + [_i] * 7 + [_ll, _vp]),
+    "du_decode_paged": (_i, [_vp] * 10 + [_i] * 8 + [_f, _ll, _vp]),
     "du_selftest_wait_timeout": (_i, [_i, _vp]),
     "du_read_status": (_i, [ctypes.POINTER(ctypes.c_uint), _i]),
 }

@@ -16,9 +16,11 @@
 #include <string>
 
 #include "../../include/dominus_ultra_b200.h"
+#include "decode_paged_sm100.cuh"
 #include "decode_sm100.cuh"
 #include "decode_tc_sm100.cuh"
 #include "exchange_sm100.cuh"
+#include "paged_sm100.cuh"
 #include "prefill_fa1_sm100.cuh"
 #include "prefill_fa_sm100.cuh"
 #include "prefill_sm100.cuh"
@@ -1256,6 +1258,211 @@ int noalloc_scratch_address(void** out) {
 }
 
 }  // namespace
+
+// ------------------------------------------------------------------- paged 8-bit KV cache
+namespace {
+
+// Sizes shared by the paged entry points: block ids and slots are int32, and a block is a power
+// of two between 16 and 128 tokens (whole blocks fill the 128-key tiles of the decode).
+int check_paged(int Hkv, int num_blocks, int block_size) {
+  if (num_blocks <= 0 || Hkv <= 0) return fail(DU_ERR_INVALID, "num_blocks and num_kv_heads must be positive");
+  if (block_size < 16 || block_size > 128 || (block_size & (block_size - 1)) != 0)
+    return fail(DU_ERR_UNSUPPORTED, "block_size must be 16, 32, 64 or 128");
+  if (static_cast<long long>(num_blocks) * block_size > 0x7fffffffLL ||
+      static_cast<long long>(num_blocks) * Hkv > 0x7fffffffLL)
+    return fail(DU_ERR_UNSUPPORTED, "the cache holds more than 2^31 - 1 slots or (block, head) pairs");
+  return DU_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+template <int D, bool BF16, int WPI>
+int launch_paged_write_t(const du::PagedWriteParams& prm, cudaStream_t st) {
+  const long long items = static_cast<long long>(prm.B) * prm.pages * prm.Hkv * 2;
+  const long long ctas = (items + 4 / WPI - 1) / (4 / WPI);
+  if (ctas > 0x7fffffffLL) return fail(DU_ERR_UNSUPPORTED, "too many (request, block, head) items for one launch");
+  du::paged_write_kernel<D, BF16, WPI><<<static_cast<unsigned>(ctas), 128, 0, st>>>(prm);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
+  return DU_OK;
+}
+
+template <int D, bool BF16>
+int launch_paged_write_d(const du::PagedWriteParams& prm, cudaStream_t st) {
+  // Chunk pairs of the largest item: a warp takes up to four per lane, else four warps share it.
+  const int rows = prm.T < prm.block ? prm.T : prm.block;
+  if (static_cast<long long>(rows) * (D / 16) <= 128) return launch_paged_write_t<D, BF16, 1>(prm, st);
+  return launch_paged_write_t<D, BF16, 4>(prm, st);
+}
+
+template <bool BF16>
+int launch_paged_write(const du::PagedWriteParams& prm, int D, cudaStream_t st) {
+  switch (D) {
+    case 16: return launch_paged_write_d<16, BF16>(prm, st);
+    case 32: return launch_paged_write_d<32, BF16>(prm, st);
+    case 64: return launch_paged_write_d<64, BF16>(prm, st);
+    case 128: return launch_paged_write_d<128, BF16>(prm, st);
+    default: return launch_paged_write_d<256, BF16>(prm, st);
+  }
+}
+
+template <bool BF16>
+int launch_decode_paged(const du::DecodePagedParams& prm, int D, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(prm.Hq), static_cast<unsigned>(prm.B));
+  switch (D) {
+    case 16: du::decode_paged_kernel<16, BF16><<<grid, 256, 0, st>>>(prm); break;
+    case 32: du::decode_paged_kernel<32, BF16><<<grid, 256, 0, st>>>(prm); break;
+    case 64: du::decode_paged_kernel<64, BF16><<<grid, 256, 0, st>>>(prm); break;
+    case 128: du::decode_paged_kernel<128, BF16><<<grid, 256, 0, st>>>(prm); break;
+    default: du::decode_paged_kernel<256, BF16><<<grid, 256, 0, st>>>(prm); break;
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged decode launch");
+  return DU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int du_paged_tables(int* block_table, const int* cache_seqlens, const int* new_seqlens,
+                    int* free_blocks, const int* free_state, int* slots, int* seqlens_out,
+                    int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
+                    int max_new, void* stream) {
+  g_last_error.clear();
+  int rc = check_paged(1, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (B <= 0 || max_blocks <= 0 || max_new < 0)
+    return fail(DU_ERR_INVALID, "batch and max_blocks must be positive and max_new not negative");
+  if (B > du::PAGED_MAX_BATCH)
+    return fail(DU_ERR_UNSUPPORTED, "paged tables take at most 8192 requests in one call");
+  if (static_cast<long long>(B) * max_blocks > 0x7fffffffLL ||
+      static_cast<long long>(max_blocks) * block_size > 0x7fffffffLL - 128)
+    return fail(DU_ERR_UNSUPPORTED, "the block table holds more than 2^31 - 1 entries, or a row more tokens");
+  if (!block_table || !cache_seqlens || !new_seqlens || !free_blocks || !free_state ||
+      (!slots && max_new > 0) || !seqlens_out || !free_state_out)
+    return fail(DU_ERR_INVALID, "null pointer argument");
+  const void* ptrs[] = {block_table, cache_seqlens, new_seqlens, free_blocks, free_state, slots, seqlens_out, free_state_out};
+  for (const void* q : ptrs)
+    if (!aligned4(q)) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
+  const void* ins[] = {cache_seqlens, new_seqlens, free_state};
+  for (const void* q : ins)
+    if (q == seqlens_out || q == free_state_out || (slots && q == slots))
+      return fail(DU_ERR_INVALID, "the outputs must not be the inputs (every block of threads reads those)");
+  du::PagedTablesParams prm{};
+  prm.table = block_table;
+  prm.old_lens = cache_seqlens;
+  prm.new_lens = new_seqlens;
+  prm.ring = free_blocks;
+  prm.state = free_state;
+  prm.slots = slots;
+  prm.lens_out = seqlens_out;
+  prm.state_out = free_state_out;
+  prm.B = B;
+  prm.width = max_blocks;
+  prm.N = num_blocks;
+  prm.block = block_size;
+  prm.T = max_new;
+  // A CTA for each 2048 slots (four per thread), at most one per SM.
+  long long grid = (static_cast<long long>(B) * max_new + 4 * du::PAGED_TABLES_THREADS - 1) /
+                   (4 * du::PAGED_TABLES_THREADS);
+  const long long sms = sm_count();
+  grid = grid < 1 ? 1 : (grid > sms ? sms : grid);
+  const int smem = 2 * B * static_cast<int>(sizeof(int));
+  // (an attribute of the largest batch, once per device: the kernel's shared memory is 64 KB then)
+  cudaError_t e = ensure_smem_attr(du::paged_tables_kernel, 2 * du::PAGED_MAX_BATCH * static_cast<int>(sizeof(int)));
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged tables)");
+  du::paged_tables_kernel<<<static_cast<unsigned>(grid), du::PAGED_TABLES_THREADS, smem,
+                            static_cast<cudaStream_t>(stream)>>>(prm);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged tables launch");
+  return DU_OK;
+}
+
+int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                   float* k_scale, float* v_scale, const int* slots, const int* cache_seqlens,
+                   const void* cos, const void* sin, int B, int Hkv, int T, int D, int num_blocks,
+                   int block_size, int dtype, long long rope_positions, void* stream) {
+  g_last_error.clear();
+  int rc = check_common(B, Hkv, Hkv, T, D, dtype);
+  if (rc != DU_OK) return rc;
+  rc = check_paged(Hkv, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (!k_new || !v_new || !k_cache || !v_cache || !k_scale || !v_scale || !slots || !cache_seqlens || !cos || !sin)
+    return fail(DU_ERR_INVALID, "null pointer argument");
+  if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      !aligned16(cos) || !aligned16(sin))
+    return fail(DU_ERR_INVALID, "k_new, v_new, the caches and the rope tables must be 16-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(slots) || !aligned4(cache_seqlens))
+    return fail(DU_ERR_INVALID, "scales, slots and cache_seqlens must be 4-byte aligned");
+  if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
+  du::PagedWriteParams prm{};
+  prm.k = k_new;
+  prm.v = v_new;
+  prm.k8 = static_cast<uint8_t*>(k_cache);
+  prm.v8 = static_cast<uint8_t*>(v_cache);
+  prm.ks = k_scale;
+  prm.vs = v_scale;
+  prm.slots = slots;
+  prm.past = cache_seqlens;
+  prm.cos = cos;
+  prm.sin = sin;
+  prm.positions = rope_positions;
+  prm.B = B;
+  prm.Hkv = Hkv;
+  prm.T = T;
+  prm.N = num_blocks;
+  prm.block = block_size;
+  prm.pages = static_cast<int>((static_cast<long long>(T) + 2LL * block_size - 2) / block_size);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DU_DTYPE_BF16 ? launch_paged_write<true>(prm, D, st) : launch_paged_write<false>(prm, D, st);
+}
+
+int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                    const float* v_scale, const int* block_table, const int* cache_seqlens,
+                    const void* cos, const void* sin, void* out, int B, int Hq, int Hkv, int D,
+                    int num_blocks, int block_size, int max_blocks, int dtype, float scale,
+                    long long rope_positions, void* stream) {
+  g_last_error.clear();
+  int rc = check_common(B, Hq, Hkv, 1, D, dtype);
+  if (rc != DU_OK) return rc;
+  rc = check_paged(Hkv, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (max_blocks <= 0) return fail(DU_ERR_INVALID, "max_blocks must be positive");
+  if (static_cast<long long>(max_blocks) * block_size > 0x7fffffffLL - 128)
+    return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^31 - 129 tokens");
+  if (B > 65535) return fail(DU_ERR_UNSUPPORTED, "at most 65535 sequences per call");
+  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !cache_seqlens || !cos || !sin || !out)
+    return fail(DU_ERR_INVALID, "null pointer argument");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(cos) || !aligned16(sin) || !aligned16(out))
+    return fail(DU_ERR_INVALID, "q, out, the caches and the rope tables must be 16-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(cache_seqlens))
+    return fail(DU_ERR_INVALID, "scales, block_table and cache_seqlens must be 4-byte aligned");
+  if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
+  du::DecodePagedParams prm{};
+  prm.q = q;
+  prm.k8 = static_cast<const uint8_t*>(k_cache);
+  prm.v8 = static_cast<const uint8_t*>(v_cache);
+  prm.ks = k_scale;
+  prm.vs = v_scale;
+  prm.table = block_table;
+  prm.lens = cache_seqlens;
+  prm.cos = cos;
+  prm.sin = sin;
+  prm.out = out;
+  prm.positions = rope_positions;
+  prm.B = B;
+  prm.Hq = Hq;
+  prm.Hkv = Hkv;
+  prm.N = num_blocks;
+  prm.block = block_size;
+  prm.width = max_blocks;
+  prm.scale_log2 = scale * 1.4426950408889634f;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DU_DTYPE_BF16 ? launch_decode_paged<true>(prm, D, st) : launch_decode_paged<false>(prm, D, st);
+}
+
+}  // extern "C"
 
 extern "C" {
 

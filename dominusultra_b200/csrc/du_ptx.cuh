@@ -19,7 +19,8 @@
 
 // Status words written by device code (the first error wins until the host resets them):
 //   code 5, a bounded wait expired: [1] wait-site id, [2] blockIdx.x, [3] blockIdx.y;
-//   code 6, a per-sequence cache length out of range: [1] sequence index, [2] the length.
+//   code 6, a per-sequence cache length out of range: [1] sequence index, [2] the length;
+//   code 7, a block id or slot out of range: [1] sequence index, [2] the value (ring: head, count).
 __device__ unsigned int g_du_status[4];
 
 #ifdef DU_TRACE

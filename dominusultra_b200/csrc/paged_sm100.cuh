@@ -1,0 +1,398 @@
+// Paged KV cache held in 8 bits (e4m3, one fp32 scale per block of tokens and KV head): the
+// block tables and slot maps of a step, and the writer of the new tokens' keys and values. The
+// attention that reads the cache is in decode_paged_sm100.cuh.
+#pragma once
+
+#include "du_ptx.cuh"
+
+namespace du {
+
+// ---------------------------------------------------------------------------------------------
+// e4m3 helpers
+// ---------------------------------------------------------------------------------------------
+// Two fp32 values to a packed e4m3 pair (a in the low byte), nearest-even, saturating at 448.
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+  return r;
+}
+
+// A packed e4m3 pair widened to fp32 (exact).
+__device__ __forceinline__ float2 e4m3x2_widen(uint32_t p) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(p)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Block tables and slot maps
+// ---------------------------------------------------------------------------------------------
+struct PagedTablesParams {
+  int* table;           // [B, width], updated in place
+  const int* old_lens;  // [B] tokens cached
+  const int* new_lens;  // [B] tokens wanted
+  int* ring;            // [N] free block ids: a ring, taken at its head, given back at its tail
+  const int* state;     // {head, count} of the ring
+  int* slots;           // [B, T]
+  int* lens_out;        // [B]
+  int* state_out;       // {head, count}
+  int B, width, N, block, T;
+};
+
+constexpr int PAGED_TABLES_THREADS = 512;
+constexpr int PAGED_MAX_BATCH = 8192;  // two prefix sums per request in shared memory (64 KB)
+
+// A request's pages before and after, as asked for. A request whose lengths are out of range
+// asks for what it has.
+struct PagedAsk {
+  int old_len, new_len, old_pages, new_pages;
+  bool bad;
+};
+__device__ __forceinline__ PagedAsk paged_ask(const PagedTablesParams& p, int b, bool ring_ok) {
+  PagedAsk a;
+  a.old_len = p.old_lens[b];
+  a.new_len = p.new_lens[b];
+  const int cap = p.width * p.block;  // (the host checks that it fits)
+  a.bad = a.old_len < 0 || a.old_len > cap || a.new_len < 0 || a.new_len > cap ||
+          a.new_len - a.old_len > p.T;
+  if (a.bad || !ring_ok) a.new_len = a.old_len;
+  const int o = min(max(a.old_len, 0), cap), n = min(max(a.new_len, 0), cap);
+  a.old_pages = (o + p.block - 1) / p.block;
+  a.new_pages = (n + p.block - 1) / p.block;
+  return a;
+}
+
+// Last index with off[i] <= x (off is non-decreasing, off[0] = 0): among requests with equal
+// offsets that is the one that holds element x, since those before it hold none.
+__device__ __forceinline__ int paged_owner(const int* off, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Block tables and slot maps of a step from the requests' lengths, in one launch.
+//
+// pages(n) = ceil(n / block). Request b needs need_b = max(0, pages(new_b) - pages(old_b)) more
+// blocks and gives back max(0, pages(old_b) - pages(new_b)); it is served if need_b = 0 or the
+// needs of requests 0..b sum to at most the free blocks. Taken entries, in (request, page) order,
+// get the ring's blocks from its head on; given-back entries go behind its tail. The two ranges
+// of the ring never meet (free + given back <= N), entries that are read as held blocks lie
+// before every entry that is written, and a slot's new block is read from the ring, so no CTA
+// waits for another: every CTA repeats the scan of the lengths (two loads per request, L2) and
+// takes a share of the entries and slots. Bound by latency: the loads of the lengths, the scan,
+// the loads of ring or table.
+__global__ void __launch_bounds__(PAGED_TABLES_THREADS) paged_tables_kernel(const PagedTablesParams p) {
+  extern __shared__ int sm_off[];  // take[B], give[B]: exclusive prefix sums
+  __shared__ int warp_sum[2][PAGED_TABLES_THREADS / 32];
+  __shared__ int served_sum[PAGED_TABLES_THREADS / 32];
+  int* take = sm_off;
+  int* give = sm_off + p.B;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int NW = PAGED_TABLES_THREADS / 32;
+
+  const int head = p.state[0], count = p.state[1];
+  bool ring_ok = head >= 0 && head < p.N && count >= 0 && count <= p.N;
+
+  int carry_t = 0, carry_g = 0, taken_max = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    carry_t = carry_g = taken_max = 0;
+    for (int b0 = 0; b0 < p.B; b0 += PAGED_TABLES_THREADS) {
+      const int b = b0 + tid;
+      int need = 0, back = 0;
+      if (b < p.B) {
+        const PagedAsk a = paged_ask(p, b, ring_ok);
+        need = max(0, a.new_pages - a.old_pages);
+        back = max(0, a.old_pages - a.new_pages);
+        if (a.bad && blockIdx.x == 0 && pass == 0)
+          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.new_lens[b]));
+      }
+      int it = need, ig = back;  // inclusive scans
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, it, o), g = __shfl_up_sync(0xffffffffu, ig, o);
+        if (lane >= o) {
+          it += t;
+          ig += g;
+        }
+      }
+      if (lane == 31) {
+        warp_sum[0][warp] = it;
+        warp_sum[1][warp] = ig;
+      }
+      __syncthreads();
+      int bt = carry_t, bg = carry_g, tt = 0, tg = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const int xt = warp_sum[0][w], xg = warp_sum[1][w];
+        if (w < warp) {
+          bt += xt;
+          bg += xg;
+        }
+        tt += xt;
+        tg += xg;
+      }
+      it += bt;
+      ig += bg;
+      if (b < p.B) {
+        take[b] = it - need;
+        give[b] = ig - back;
+        if (need > 0 && it <= count) taken_max = max(taken_max, it);
+      }
+      carry_t += tt;
+      carry_g += tg;
+      __syncthreads();
+    }
+    // More given back than the ring has room for: the ring's state is not the tables'. Nothing
+    // changes hands then (scanned once more with every request kept as it is).
+    if (!ring_ok || static_cast<long long>(count) + carry_g <= p.N) break;
+    ring_ok = false;
+  }
+  if (!ring_ok && blockIdx.x == 0 && tid == 0)
+    record_error(7u, static_cast<unsigned>(head), static_cast<unsigned>(count));
+  // Blocks taken: the largest prefix sum of needs that the free blocks cover.
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) taken_max = max(taken_max, __shfl_xor_sync(0xffffffffu, taken_max, o));
+  if (lane == 0) served_sum[warp] = taken_max;
+  __syncthreads();
+  int taken = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) taken = max(taken, served_sum[w]);
+  const int given = carry_g;
+
+  const long long first = static_cast<long long>(blockIdx.x) * PAGED_TABLES_THREADS + tid;
+  const long long step = static_cast<long long>(gridDim.x) * PAGED_TABLES_THREADS;
+  auto ring_at = [&](long long i) { return static_cast<int>((static_cast<long long>(head) + i) % p.N); };
+  for (long long a = first; a < taken; a += step) {
+    const int b = paged_owner(take, p.B, static_cast<int>(a));
+    const PagedAsk q = paged_ask(p, b, ring_ok);
+    p.table[static_cast<long long>(b) * p.width + q.old_pages + (a - take[b])] = p.ring[ring_at(a)];
+  }
+  for (long long f = first; f < given; f += step) {
+    const int b = paged_owner(give, p.B, static_cast<int>(f));
+    const PagedAsk q = paged_ask(p, b, ring_ok);
+    p.ring[ring_at(count + f)] = p.table[static_cast<long long>(b) * p.width + q.new_pages + (f - give[b])];
+  }
+  const long long n_slots = static_cast<long long>(p.B) * p.T;
+  for (long long i = first; i < n_slots; i += step) {
+    const int b = static_cast<int>(i / p.T), t = static_cast<int>(i - static_cast<long long>(b) * p.T);
+    const PagedAsk q = paged_ask(p, b, ring_ok);
+    const int need = q.new_pages - q.old_pages;
+    const bool served = need <= 0 || take[b] + need <= count;
+    int slot = -1;
+    // (a bad request asks for no more than it has: no new token)
+    if (served && t < q.new_len - q.old_len) {
+      const int pos = q.old_len + t, page = pos / p.block;
+      const int id = page < q.old_pages ? p.table[static_cast<long long>(b) * p.width + page]
+                                        : p.ring[ring_at(take[b] + page - q.old_pages)];
+      // an id outside the cache gives no slot (the block table was damaged)
+      if (id >= 0 && id < p.N) slot = id * p.block + (pos - page * p.block);
+      else record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(id));
+    }
+    p.slots[i] = slot;
+  }
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < p.B; b += PAGED_TABLES_THREADS) {
+      const PagedAsk q = paged_ask(p, b, ring_ok);
+      const int need = q.new_pages - q.old_pages;
+      p.lens_out[b] = (need <= 0 || take[b] + need <= count) ? q.new_len : q.old_len;
+    }
+    if (tid == 0) {
+      p.state_out[0] = ring_ok ? ring_at(taken) : head;
+      p.state_out[1] = ring_ok ? count - taken + given : count;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Writer
+// ---------------------------------------------------------------------------------------------
+struct PagedWriteParams {
+  const void* k;     // [B, Hkv, T, D] 16-bit, not rotated
+  const void* v;     // [B, Hkv, T, D]
+  uint8_t* k8;       // [N, Hkv, block, D] e4m3
+  uint8_t* v8;
+  float* ks;         // [N, Hkv]
+  float* vs;
+  const int* slots;  // [B, T]: block * block_size + row, -1: no token
+  const int* past;   // [B]: position of the request's first new token
+  const void* cos;   // [positions, D/2]
+  const void* sin;
+  long long positions;
+  int B, Hkv, T, N, block, pages;  // pages: blocks that one request's T tokens can touch
+};
+
+// a + b rounded to odd: the exact sum when it has 24 bits, else the neighbour of it whose last
+// bit is set. Rounding that to e4m3 gives what rounding the exact sum would (no double rounding).
+__device__ __forceinline__ float add_to_odd(float a, float b) {
+  const float s = __fadd_rn(a, b);
+  const float bb = __fsub_rn(s, a);
+  const float err = __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb));
+  const int i = __float_as_int(s);
+  if (err != 0.f && (i & 1) == 0 && (i & 0x7f800000) != 0x7f800000)
+    return __int_as_float(((err > 0.f) == (s > 0.f)) ? i + 1 : i - 1);
+  return s;
+}
+
+// The smallest power of two of at least 2^-64 whose 448-fold covers amax (its bits given); NaN
+// when amax is not finite.
+__device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return __int_as_float(0x7fc00000);
+  // amax = f 2^x with f in [1, 2): 448 = 1.75 2^8
+  const int x = static_cast<int>(amax_bits >> 23) - 127;
+  const int e = max((amax_bits & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7, -64);
+  return __int_as_float((e + 127) << 23);
+}
+
+// Quantises the new tokens of a call into the cache: keys rotated at their positions, one scale
+// per (block, KV head) and per cache.
+//
+// A work item is (request, block that its tokens touch, KV head, key or value); WPI warps take
+// it, a thread a pair of 16-byte chunks i, i + D/2 of a row at a time, which is what a rotation
+// pairs up. First the largest magnitude of the item's rows, from which the scale follows: the
+// smallest power of two with amax <= 448 scale, or the block's present scale where that is
+// larger and the block holds rows already. Then the rows again (out of L1), scaled and rounded
+// once. Products of two 16-bit values are exact in fp32, their sum is rounded to odd and the
+// scale is a power of two, so each byte is the e4m3 value nearest to the exact quotient. Where a
+// block's scale grows, its present rows are scaled down and rounded again; that is exact but
+// for what falls below the format's normal range. A block with a value that is not finite gets
+// the scale NaN, which every attention over it then returns.
+//
+// Bound by HBM for prompts: 2 bytes read and 1 written per value; by the chain of loads (slots,
+// rows, scale) for single tokens.
+template <int D, bool BF16, int WPI>
+__global__ void __launch_bounds__(128) paged_write_kernel(const PagedWriteParams p) {
+  constexpr int PAIRS = D / 16;  // chunk pairs per row
+  constexpr int NT = 32 * WPI;   // threads per item
+  constexpr int IPC = 4 / WPI;   // items per CTA
+  __shared__ uint32_t warp_max[4];
+  const int lane_i = threadIdx.x % NT;  // thread within the item
+  const long long items = static_cast<long long>(p.B) * p.pages * p.Hkv * 2;
+  const long long item = static_cast<long long>(blockIdx.x) * IPC + threadIdx.x / NT;
+  // Uniform over the item's threads. With WPI = 4 the whole CTA is one item, so its barriers
+  // are reached by all or none.
+  if (item >= items) return;
+  const bool is_v = (item & 1) != 0;
+  const long long i2 = item >> 1;
+  const int h = static_cast<int>(i2 % p.Hkv);
+  const long long i3 = i2 / p.Hkv;
+  const int pg = static_cast<int>(i3 % p.pages);
+  const int b = static_cast<int>(i3 / p.pages);
+
+  const int past = p.past[b];
+  const int row0 = past >= 0 ? past % p.block : 0;  // row of the request's first new token
+  const int t0 = pg == 0 ? 0 : pg * p.block - row0;
+  if (t0 >= p.T) return;
+  const int r0 = pg == 0 ? row0 : 0;  // the block's first row that this call writes
+  const int n = min(p.T - t0, p.block - r0);
+  const int* slot_row = p.slots + static_cast<long long>(b) * p.T + t0;
+  const int slot0 = slot_row[0];
+  if (slot0 < 0) return;  // no token here
+  const int blk = slot0 / p.block;
+  if (past < 0 || blk >= p.N || slot0 - blk * p.block != r0) {
+    if (lane_i == 0) record_error(past < 0 ? 6u : 7u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : slot0));
+    return;
+  }
+  const long long cell = static_cast<long long>(blk) * p.Hkv + h;
+  float* scale = (is_v ? p.vs : p.ks) + cell;
+  uint8_t* out = (is_v ? p.v8 : p.k8) + cell * p.block * D;
+  const float had = r0 > 0 ? *scale : 0.f;
+  const uint8_t* x = static_cast<const uint8_t*>(is_v ? p.v : p.k) +
+                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0) * (2 * D);
+
+  // The 16 values of chunk pair (r, c), rotated for keys; false for a row without a token.
+  auto values = [&](int r, int c, float (&y1)[8], float (&y2)[8]) -> bool {
+    if (slot_row[r] != slot0 + r) return false;
+    const long long pos = static_cast<long long>(past) + t0 + r;
+    if (!is_v && pos >= p.positions) return false;
+    const uint4 a = ldg_v4(x + static_cast<long long>(r) * (2 * D) + c * 16);
+    const uint4 d = ldg_v4(x + static_cast<long long>(r) * (2 * D) + D + c * 16);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, dw[4] = {d.x, d.y, d.z, d.w};
+    if (is_v) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
+        y1[2 * e] = u.x;
+        y1[2 * e + 1] = u.y;
+        y2[2 * e] = w.x;
+        y2[2 * e + 1] = w.y;
+      }
+      return true;
+    }
+    const uint4 cv = ldg_v4(static_cast<const uint8_t*>(p.cos) + pos * D + c * 16);
+    const uint4 sv = ldg_v4(static_cast<const uint8_t*>(p.sin) + pos * D + c * 16);
+    const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 u = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
+      const float2 cc = unpack2<BF16>(cw[e]), ss = unpack2<BF16>(sw[e]);
+      y1[2 * e] = add_to_odd(__fmul_rn(u.x, cc.x), -__fmul_rn(w.x, ss.x));
+      y1[2 * e + 1] = add_to_odd(__fmul_rn(u.y, cc.y), -__fmul_rn(w.y, ss.y));
+      y2[2 * e] = add_to_odd(__fmul_rn(w.x, cc.x), __fmul_rn(u.x, ss.x));
+      y2[2 * e + 1] = add_to_odd(__fmul_rn(w.y, cc.y), __fmul_rn(u.y, ss.y));
+    }
+    return true;
+  };
+
+  uint32_t top = 0;  // bits of the largest magnitude: NaN above infinity above every number
+  for (int u = lane_i; u < n * PAIRS; u += NT) {
+    const int r = u / PAIRS, c = u % PAIRS;
+    float y1[8], y2[8];
+    if (values(r, c, y1, y2)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        top = max(top, max(__float_as_uint(y1[e]) & 0x7fffffffu, __float_as_uint(y2[e]) & 0x7fffffffu));
+    } else if (c == 0 && slot_row[r] >= 0) {
+      const bool far = slot_row[r] == slot0 + r;
+      record_error(far ? 6u : 7u, static_cast<unsigned>(b), static_cast<unsigned>(far ? past + t0 + r : slot_row[r]));
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (WPI > 1) {
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPI; ++w) top = max(top, warp_max[w]);
+  } else {
+    __syncwarp();  // every lane has read the present scale
+  }
+  float unit = paged_unit(top);
+  if (r0 > 0 && (unit <= had || had != had)) unit = had;  // (a NaN on either side stays)
+  if (lane_i == 0) *scale = unit;
+  const bool poison = unit != unit;
+  const float inv = 1.0f / unit;
+  for (int u = lane_i; u < n * PAIRS; u += NT) {
+    const int r = u / PAIRS, c = u % PAIRS;
+    float y1[8], y2[8];
+    if (!values(r, c, y1, y2)) continue;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w[e] = e4m3x2(y1[4 * e] * inv, y1[4 * e + 1] * inv) | (e4m3x2(y1[4 * e + 2] * inv, y1[4 * e + 3] * inv) << 16);
+      w[2 + e] = e4m3x2(y2[4 * e] * inv, y2[4 * e + 1] * inv) | (e4m3x2(y2[4 * e + 2] * inv, y2[4 * e + 3] * inv) << 16);
+    }
+    if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
+    uint8_t* row = out + static_cast<long long>(r0 + r) * D;
+    *reinterpret_cast<uint2*>(row + 8 * c) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(row + D / 2 + 8 * c) = make_uint2(w[2], w[3]);
+  }
+  if (r0 > 0 && unit > had) {
+    // The present rows under the larger scale.
+    const float f = had * inv;
+    for (int u = lane_i; u < r0 * D / 16; u += NT) {
+      uint4* q = reinterpret_cast<uint4*>(out) + u;
+      const uint4 o = *q;
+      uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 lo = e4m3x2_widen(w[e] & 0xffffu), hi = e4m3x2_widen(w[e] >> 16);
+        w[e] = e4m3x2(lo.x * f, lo.y * f) | (e4m3x2(hi.x * f, hi.y * f) << 16);
+      }
+      *q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+}  // namespace du

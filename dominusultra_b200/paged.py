@@ -1,0 +1,359 @@
+"""Paged KV cache held in 8 bits: block tables, the cache's writer and its single-token attention.
+
+The serving step around ``dominus_ultra_decode`` (reference ``dominus_ultra.py:504-583``, which
+reads one contiguous 16-bit cache of one length) with the cache cut into blocks of tokens and held
+as e4m3 with one scale per (block, KV head):
+
+* ``k_cache``, ``v_cache``: ``[num_blocks, num_kv_heads, block_size, head_dim]``
+  ``torch.float8_e4m3fn``, ``block_size`` 16, 32, 64 or 128; keys are stored rotated;
+* ``k_scale``, ``v_scale``: ``[num_blocks, num_kv_heads]`` fp32;
+* ``block_table``: ``[batch, max_blocks]`` int32, the blocks of each request in order.
+
+A step is ``dominus_ultra_paged_tables`` (blocks and slots for the new tokens),
+``dominus_ultra_paged_write`` (their keys and values) and ``dominus_ultra_decode_paged``. Lengths
+and tables stay on the GPU: no call synchronises, and each can be captured into a CUDA graph.
+"""
+
+from __future__ import annotations
+
+from typing import Tuple
+
+import torch
+
+from . import _lib
+from .attention import (
+    _aligned,
+    _dtype_code,
+    _OnDevice,
+    _ptr,
+    _stream,
+    _validate_attention_tensors,
+    _validate_head_dim,
+)
+
+__all__ = [
+    "dominus_ultra_paged_tables",
+    "dominus_ultra_paged_write",
+    "dominus_ultra_decode_paged",
+]
+
+
+def _validate_block_size(block_size: int) -> None:
+    if block_size not in (16, 32, 64, 128):
+        raise ValueError("block_size must be 16, 32, 64 or 128")
+
+
+def _validate_int32(name: str, t: torch.Tensor, device: torch.device) -> None:
+    if t.dtype != torch.int32:
+        raise ValueError(f"{name} must be an int32 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must be on the same CUDA device as the other tensors")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _lengths(name: str, t: torch.Tensor, batch: int) -> None:
+    if t.ndim != 1 or t.shape[0] != batch:
+        raise ValueError(f"{name} must have shape [batch]")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be an int32 or int64 tensor")
+
+
+def _check_host_lengths(name: str, t: torch.Tensor, hi: int) -> None:
+    """Range check of lengths that are on the CPU (those on the GPU are checked there)."""
+    bad = [(i, n) for i, n in enumerate(t.tolist()) if n < 0 or n > hi]
+    if bad:
+        raise ValueError(f"{name}[{bad[0][0]}] = {bad[0][1]} is outside [0, {hi}]")
+
+
+def _check_host_table(table: torch.Tensor, lengths: torch.Tensor, block_size: int, num_blocks: int) -> None:
+    """Range check of the block ids that `lengths` tokens use, for a table on the CPU."""
+    for b, n in enumerate(lengths.tolist()):
+        used = table[b, : -(-n // block_size)]
+        bad = ((used < 0) | (used >= num_blocks)).nonzero()
+        if bad.numel():
+            page = int(bad[0])
+            raise ValueError(f"block_table[{b}, {page}] = {int(used[page])} is outside [0, {num_blocks - 1}]")
+
+
+def _device_int32(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Lengths as a contiguous int32 tensor on `device`; 64-bit ones out of int32's range stay out
+    of every length's range."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, 2**31 - 1).to(torch.int32)
+    return t.to(device).contiguous()
+
+
+def _validate_paged_cache(k_cache, v_cache, k_scale, v_scale, device) -> None:
+    if k_cache.ndim != 4 or v_cache.ndim != 4:
+        raise ValueError("k_cache and v_cache must be rank-4 tensors")
+    num_blocks, hkv, block_size, _ = k_cache.shape
+    if v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape")
+    if num_blocks <= 0 or hkv <= 0:
+        raise ValueError("num_blocks and num_kv_heads must be positive")
+    _validate_block_size(block_size)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"{name} must use float8_e4m3fn")
+        if t.device != device:
+            raise ValueError("all attention tensors must be on the same CUDA device")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.data_ptr() % 16:
+            raise ValueError(f"{name} must be 16-byte aligned")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.shape != (num_blocks, hkv):
+            raise ValueError(f"{name} must have shape [num_blocks, num_kv_heads]")
+        if t.dtype != torch.float32:
+            raise ValueError(f"{name} must use float32")
+        if t.device != device:
+            raise ValueError("all attention tensors must be on the same CUDA device")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+
+
+def _validate_tables_like(cos, sin, head_dim, device, dtype) -> None:
+    """The rope tables but for their length: the positions are known on the GPU only."""
+    expected_tail = (head_dim // 2,)
+    if cos.ndim != 2 or sin.ndim != 2:
+        raise ValueError("cos and sin must be rank-2 [positions, head_dim // 2] tensors")
+    if cos.shape[0] < 1 or sin.shape[0] < 1:
+        raise ValueError("cos and sin must contain at least 1 positions")
+    if cos.shape[1:] != expected_tail or sin.shape[1:] != expected_tail:
+        raise ValueError(f"cos and sin must have trailing shape {expected_tail}")
+    if cos.device != device or sin.device != device:
+        raise ValueError("cos and sin must be on the same device as the attention tensors")
+    if cos.dtype != dtype or sin.dtype != dtype:
+        raise ValueError("cos and sin must have the same dtype as the attention tensors")
+    if not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError("cos and sin must be contiguous")
+
+
+def dominus_ultra_paged_tables(
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    new_seqlens: torch.Tensor,
+    free_blocks: torch.Tensor,
+    free_state: torch.Tensor,
+    block_size: int,
+    max_new: int,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """
+    Block tables and slot map of a step, from the requests' lengths (``du_paged_tables``).
+
+    Request ``b`` holds ``cache_seqlens[b]`` tokens and wants ``new_seqlens[b]``: more (up to
+    ``max_new`` more), fewer (a rejected draft), or 0 (a request that ends). Requests that grow
+    over a block's end take blocks from the ring of free ones, in order of ``b`` from its head, as
+    long as the needs up to a request are covered; a request that is not served keeps its length.
+    Requests that shrink give blocks back behind the ring's tail, free from the next call on.
+
+    ``block_table`` (new entries) and ``free_blocks`` (given-back ids) are updated in place; the
+    lengths and ``free_state`` are not: pass the returned ones to the next call, or copy them
+    into the same tensors inside a captured graph.
+
+    Args:
+        block_table: [batch, max_blocks] int32
+        cache_seqlens: [batch] integer tokens cached (int32 or int64; on the CPU they are checked
+            here, on the GPU a bad request is left as it is and ``_lib.read_status()`` reports 6)
+        new_seqlens: [batch] integer tokens wanted
+        free_blocks: [num_blocks] int32, a ring of free block ids
+        free_state: [2] int32, {head, count} of the ring
+        block_size: 16, 32, 64 or 128
+        max_new: columns of the slot map
+
+    Returns:
+        Tuple of:
+            - slots: [batch, max_new] int32, ``block * block_size + row`` of each new token, -1
+              where there is none
+            - seqlens: [batch] int32, the lengths that the requests have now
+            - free_state: [2] int32
+    """
+    if block_table.ndim != 2 or block_table.shape[0] <= 0 or block_table.shape[1] <= 0:
+        raise ValueError("block_table must be a non-empty [batch, max_blocks] tensor")
+    batch, max_blocks = block_table.shape
+    _validate_block_size(block_size)
+    if max_new < 0:
+        raise ValueError("max_new must not be negative")
+    _lengths("cache_seqlens", cache_seqlens, batch)
+    _lengths("new_seqlens", new_seqlens, batch)
+    if free_blocks.ndim != 1 or free_blocks.shape[0] <= 0:
+        raise ValueError("free_blocks must be a non-empty [num_blocks] tensor")
+    if free_state.shape != (2,):
+        raise ValueError("free_state must have shape [2]")
+    if not block_table.is_cuda:
+        raise ValueError("DominusUltra kernels require CUDA tensors")
+    device = block_table.device
+    _validate_int32("block_table", block_table, device)
+    _validate_int32("free_blocks", free_blocks, device)
+    _validate_int32("free_state", free_state, device)
+    for name, t in (("cache_seqlens", cache_seqlens), ("new_seqlens", new_seqlens)):
+        if t.device.type == "cpu":
+            _check_host_lengths(name, t, max_blocks * block_size)
+        elif t.device != device:
+            raise ValueError(f"{name} must be on the device of block_table (or on the CPU)")
+
+    lib = _lib.load()
+    with _OnDevice(device):
+        old, new = _device_int32(cache_seqlens, device), _device_int32(new_seqlens, device)
+        slots = torch.empty((batch, max_new), dtype=torch.int32, device=device)
+        seqlens = torch.empty((batch,), dtype=torch.int32, device=device)
+        state = torch.empty((2,), dtype=torch.int32, device=device)
+        rc = lib.du_paged_tables(
+            _ptr(block_table), _ptr(old), _ptr(new), _ptr(free_blocks), _ptr(free_state),
+            _ptr(slots), _ptr(seqlens), _ptr(state), batch, max_blocks, free_blocks.shape[0],
+            block_size, max_new, _stream(device),
+        )
+    _lib.check(rc, "du_paged_tables")
+    return slots, seqlens, state
+
+
+def dominus_ultra_paged_write(
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    slots: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+) -> None:
+    """
+    Write new tokens' keys and values into the paged 8-bit cache, in place (``du_paged_write``).
+
+    Token ``t`` of request ``b`` rotates at position ``cache_seqlens[b] + t`` and goes to
+    ``slots[b, t]``. Each (block, KV head) of keys and of values has a scale, a power of two: the
+    smallest that covers the rows written, or the present one where the block holds earlier rows
+    and theirs is larger; when it grows, the earlier rows are rescaled. Values are rounded once, to
+    the nearest e4m3 value. A value that is not finite makes its block's scale NaN.
+
+    Requests must not share a block that they write to; blocks that are only read may be shared.
+
+    Args:
+        k_new, v_new: [batch, num_kv_heads, T, head_dim], keys not rotated (one token each, or
+            whole prompts as ``dominus_ultra_prefill`` takes them)
+        k_cache, v_cache: [num_blocks, num_kv_heads, block_size, head_dim] float8_e4m3fn
+        k_scale, v_scale: [num_blocks, num_kv_heads] fp32
+        slots: [batch, T] int32 from ``dominus_ultra_paged_tables``, -1 for no token
+        cache_seqlens: [batch] integer lengths before these tokens (what the tables call took)
+        cos, sin: tables from precompute_rope_cos_sin covering the new positions
+    """
+    if k_new.ndim != 4 or v_new.ndim != 4 or k_cache.ndim != 4 or v_cache.ndim != 4:
+        raise ValueError("k_new, v_new, k_cache, and v_cache must be rank-4 tensors")
+    B, Hkv, T, D = k_new.shape
+    if B <= 0 or Hkv <= 0 or T <= 0:
+        raise ValueError("batch, heads, and sequence length must be positive")
+    if v_new.shape != k_new.shape:
+        raise ValueError("k_new and v_new must have the same shape")
+    if k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        raise ValueError("the caches must have k_new's head count and head_dim")
+    if slots.shape != (B, T):
+        raise ValueError("slots must have shape [batch, T]")
+    _lengths("cache_seqlens", cache_seqlens, B)
+    _validate_head_dim(D)
+    _validate_attention_tensors(k_new, v_new)
+    device = k_new.device
+    _validate_paged_cache(k_cache, v_cache, k_scale, v_scale, device)
+    _validate_int32("slots", slots, device)
+    _validate_tables_like(cos, sin, D, device, k_new.dtype)
+    positions = min(cos.shape[0], sin.shape[0])
+    if cache_seqlens.device.type == "cpu":
+        _check_host_lengths("cache_seqlens", cache_seqlens, positions)
+    elif cache_seqlens.device != device:
+        raise ValueError("cache_seqlens must be on the device of k_new (or on the CPU)")
+
+    lib = _lib.load()
+    with _OnDevice(device):
+        k_new, v_new, cos, sin = (_aligned(t) for t in (k_new, v_new, cos, sin))
+        past = _device_int32(cache_seqlens, device)
+        rc = lib.du_paged_write(
+            _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+            _ptr(slots), _ptr(past), _ptr(cos), _ptr(sin), B, Hkv, T, D, k_cache.shape[0],
+            k_cache.shape[2], _dtype_code(k_new.dtype), positions, _stream(device),
+        )
+    _lib.check(rc, "du_paged_write")
+
+
+def dominus_ultra_decode_paged(
+    q_new: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+) -> torch.Tensor:
+    """
+    Decode-phase attention over the paged 8-bit cache (``du_decode_paged``).
+
+    ``cache_seqlens[b]`` counts the cached tokens with the new one (what
+    ``dominus_ultra_paged_tables`` returned, after ``dominus_ultra_paged_write``): the query
+    rotates at ``cache_seqlens[b] - 1`` and attends to keys ``0..cache_seqlens[b] - 1``, as
+    ``dominus_ultra_decode_kvcache`` does with an append. A request of length 0 gives zeros. Rows of
+    a block behind the length are never used, whatever they hold.
+
+    Lengths and table are read on the GPU: a length out of range gives zeros, a block id out of
+    range NaN, and ``_lib.read_status()`` reports code 6 or 7. Given on the CPU, they are checked
+    here.
+
+    Args:
+        q_new: [batch, num_heads, 1, head_dim]
+        k_cache, v_cache: [num_blocks, num_kv_heads, block_size, head_dim] float8_e4m3fn
+        k_scale, v_scale: [num_blocks, num_kv_heads] fp32, positive
+        block_table: [batch, max_blocks] int32
+        cache_seqlens: [batch] integer lengths
+        cos, sin: tables from precompute_rope_cos_sin covering every length
+
+    Returns:
+        Output tensor of shape [batch, num_heads, 1, head_dim]
+    """
+    if q_new.ndim != 4 or k_cache.ndim != 4 or v_cache.ndim != 4:
+        raise ValueError("q_new, k_cache, and v_cache must be rank-4 tensors")
+    B, Hq, _, D = q_new.shape
+    if q_new.shape[2] != 1:
+        raise ValueError("q_new must contain exactly one sequence position")
+    if B <= 0 or Hq <= 0:
+        raise ValueError("batch and heads must be positive")
+    Hkv = k_cache.shape[1]
+    if Hkv <= 0 or Hq % Hkv != 0:
+        raise ValueError("num_query_heads must be divisible by num_kv_heads")
+    if k_cache.shape[3] != D:
+        raise ValueError("the caches must have q_new's head_dim")
+    if block_table.ndim != 2 or block_table.shape[0] != B or block_table.shape[1] <= 0:
+        raise ValueError("block_table must have shape [batch, max_blocks]")
+    _lengths("cache_seqlens", cache_seqlens, B)
+    _validate_head_dim(D)
+    _validate_attention_tensors(q_new)
+    device = q_new.device
+    _validate_paged_cache(k_cache, v_cache, k_scale, v_scale, device)
+    _validate_tables_like(cos, sin, D, device, q_new.dtype)
+    num_blocks, _, block_size, _ = k_cache.shape
+    max_blocks = block_table.shape[1]
+    positions = min(cos.shape[0], sin.shape[0])
+    if cache_seqlens.device.type == "cpu":
+        _check_host_lengths("cache_seqlens", cache_seqlens, min(max_blocks * block_size, positions))
+        if block_table.device.type == "cpu":
+            _check_host_table(block_table, cache_seqlens, block_size, num_blocks)
+    elif cache_seqlens.device != device:
+        raise ValueError("cache_seqlens must be on the device of q_new (or on the CPU)")
+    if block_table.device.type == "cpu" and block_table.dtype == torch.int32:
+        block_table = block_table.to(device)
+    _validate_int32("block_table", block_table, device)
+
+    lib = _lib.load()
+    with _OnDevice(device):
+        q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
+        lens = _device_int32(cache_seqlens, device)
+        out = torch.empty_like(q_new)
+        rc = lib.du_decode_paged(
+            _ptr(q_new), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+            _ptr(block_table), _ptr(lens), _ptr(cos), _ptr(sin), _ptr(out), B, Hq, Hkv, D,
+            num_blocks, block_size, max_blocks, _dtype_code(q_new.dtype), 1.0 / (D**0.5),
+            positions, _stream(device),
+        )
+    _lib.check(rc, "du_decode_paged")
+    return out

@@ -29,6 +29,7 @@ extern "C" {
 #define DU_ERR_WORKSPACE 4   /* workspace missing or too small */
 #define DU_ERR_TIMEOUT 5     /* a bounded device-side wait expired (see du_read_status) */
 #define DU_STATUS_BAD_SEQLEN 6 /* device status only: a per-sequence cache length out of range */
+#define DU_STATUS_BAD_BLOCK 7  /* device status only: a block id, slot or free-ring state out of range */
 
 #define DU_DTYPE_F16 0
 #define DU_DTYPE_BF16 1
@@ -236,6 +237,76 @@ int du_decode_noalloc(const void* q, const void* k_cache, const void* v_cache, c
                       int dtype, float scale, long long rope_positions, void* stream);
 
 /*
+ * Paged KV cache held in 8 bits (no counterpart in the reference, whose decode reads one
+ * contiguous 16-bit cache, dominus_ultra.py:504-583). Three calls make up a generation step:
+ * du_paged_tables gives requests their blocks, du_paged_write quantises the new tokens' keys and
+ * values into them, du_decode_paged attends. Lengths, tables and slots live on the device and are
+ * read there: no call synchronises, and captured CUDA graphs stay valid as requests grow.
+ *
+ *   caches  [num_blocks, Hkv, block_size, D] e4m3 (8-bit, S.1111.111 not a number): a value is its
+ *           8-bit value times the scale of its (block, KV head). Keys are stored rotated.
+ *   scales  [num_blocks, Hkv] fp32, one for keys and one for values, positive.
+ *   block_table [B, max_blocks] int32: entry p of a row is the block of tokens
+ *           [p block_size, (p + 1) block_size) of that request. Only entries of cached tokens
+ *           are read.
+ *   block_size is 16, 32, 64 or 128.
+ *
+ * A length, block id or slot out of range cannot be an argument error (the host never sees it): no
+ * access leaves the buffers, the outcome is stated per call, and du_read_status reports code 6
+ * (lengths) or 7 (blocks, slots, ring) with the request and the value.
+ */
+
+/*
+ * Block tables and slot maps of a step. cache_seqlens [B] tokens cached, new_seqlens [B] tokens
+ * wanted: more (at most max_new more), fewer, or 0 for a request that ends. A request that grows
+ * over a block's end takes blocks from free_blocks [num_blocks], a ring with free_state = {head,
+ * count}: in request order, from the head; a request is served if the needs of the requests up to
+ * it are covered, else it keeps its length and gets no slot. A request that shrinks gives its
+ * blocks beyond ceil(new / block_size) back behind the ring's tail; they are free from the next
+ * call on. Writes the new entries of block_table (others stay as they are), the ring's new
+ * entries, slots [B, max_new] (block * block_size + row of token cache_seqlens[b] + t, -1 where
+ * there is no such token), seqlens_out [B] (new_seqlens where served, else cache_seqlens) and
+ * free_state_out [2]; the inputs cache_seqlens, new_seqlens and free_state are not changed and
+ * must not be the outputs. A request with a length below 0 or beyond the table's row, or with more
+ * than max_new new tokens, is left as it is (code 6); a ring state that does not fit num_blocks
+ * leaves every request as it is (code 7). B <= 8192; max_new may be 0 (slots is not used then).
+ */
+int du_paged_tables(int* block_table, const int* cache_seqlens, const int* new_seqlens,
+                    int* free_blocks, const int* free_state, int* slots, int* seqlens_out,
+                    int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
+                    int max_new, void* stream);
+
+/*
+ * New tokens into the cache. k_new, v_new [B, Hkv, T, D] (keys not rotated: token t of request b
+ * rotates at cache_seqlens[b] + t), slots [B, T] as du_paged_tables gives them (-1: no token;
+ * consecutive tokens of a request have consecutive positions), cache_seqlens [B] the lengths
+ * before these tokens. Per (block, KV head), for keys and values each: the scale is the smallest
+ * power of two (2^-64 at least) with which the new rows' magnitudes stay within 448, or the
+ * present scale where that is larger and the block holds earlier rows; each value is the e4m3 value
+ * nearest to its quotient. Where the scale grows, the earlier rows are rescaled. A block that
+ * gets a value that is not finite gets the scale NaN. Rows of other slots are left as they are.
+ * Requests must not share a block that they write to. A token whose slot is not where its
+ * position belongs, or whose position the tables do not reach, is not written (codes 7, 6).
+ */
+int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                   float* k_scale, float* v_scale, const int* slots, const int* cache_seqlens,
+                   const void* cos, const void* sin, int B, int Hkv, int T, int D, int num_blocks,
+                   int block_size, int dtype, long long rope_positions, void* stream);
+
+/*
+ * Single-token attention over the cache. q [B, Hq, D] (rotated here at cache_seqlens[b] - 1, the
+ * position of the newest cached token, which the query sees), out [B, Hq, D], cache_seqlens [B]
+ * the cached tokens with the new one. A request of length 0 gives zeros; a length below 0, beyond
+ * the table's row or beyond rope_positions gives zeros and code 6; a block id out of range
+ * gives NaN and code 7.
+ */
+int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                    const float* v_scale, const int* block_table, const int* cache_seqlens,
+                    const void* cos, const void* sin, void* out, int B, int Hq, int Hkv, int D,
+                    int num_blocks, int block_size, int max_blocks, int dtype, float scale,
+                    long long rope_positions, void* stream);
+
+/*
  * Failure-detection self-test (no counterpart in the reference): launches one CTA whose
  * bounded wait can never complete -- an mbarrier nothing arrives at -- with a limit of
  * timeout_us microseconds (1..1000000). The kernel records DU_ERR_TIMEOUT in the status words
@@ -247,8 +318,10 @@ int du_selftest_wait_timeout(int timeout_us, void* stream);
  * Read the device status words (the first device-side error since the last reset):
  *   words[0] = 0 ok;
  *   DU_ERR_TIMEOUT: a bounded wait expired, [1] wait site, [2..3] block index;
- *   DU_STATUS_BAD_SEQLEN: du_decode_kvcache met a cache length out of range, [1] sequence
- *   index, [2] the length (as unsigned).
+ *   DU_STATUS_BAD_SEQLEN: du_decode_kvcache or a paged call met a cache length out of range, [1]
+ *   sequence index, [2] the length (as unsigned);
+ *   DU_STATUS_BAD_BLOCK: a paged call met a block id or slot out of range, [1] sequence index,
+ *   [2] the value, or a ring state, [1] head, [2] count.
  * Synchronises the current device. reset != 0 clears them. Returns DU_OK or DU_ERR_CUDA.
  */
 int du_read_status(unsigned int* words4, int reset);
