@@ -25,6 +25,7 @@ DU_DTYPE_F16 = 0
 DU_DTYPE_BF16 = 1
 DU_DTYPE_F32 = 2
 
+DU_PAGED_TICKETS = 1024  # int32 words of tickets a paged decode takes (see the header)
 DU_NOALLOC_SCRATCH_BYTES = 4 << 20  # scratch held by du_decode_noalloc (see the header)
 
 _vp = ctypes.c_void_p
@@ -81,7 +82,8 @@ SIGNATURES = {
     "du_decode_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _ll, _vp]),
     "du_paged_tables": (_i, [_vp] * 8 + [_i] * 5 + [_vp]),
     "du_paged_write": (_i, [_vp] * 10 + [_i] * 7 + [_ll, _vp]),
-    "du_decode_paged": (_i, [_vp] * 10 + [_i] * 8 + [_f, _ll, _vp]),
+    "du_decode_paged_workspace_size": (_sz, [_i] * 6),
+    "du_decode_paged": (_i, [_vp] * 10 + [_i] * 8 + [_f, _ll, _vp, _vp, _sz, _vp]),
     "du_selftest_wait_timeout": (_i, [_i, _vp]),
     "du_read_status": (_i, [ctypes.POINTER(ctypes.c_uint), _i]),
 }

@@ -1,9 +1,37 @@
-// Single-token attention over the paged 8-bit KV cache (layout in paged_sm100.cuh).
+// Single-token attention over the paged 8-bit KV cache (layout in paged_sm100.cuh), on tcgen05.
 //
 // Per request b with n cached tokens (the query's own among them) and query head h of KV head g:
 //   q' = R(n - 1) q            s_j = (q' . k8_j) ks[page_j, g] scale       j < n
 //   out = sum_j softmax(s)_j v8_j vs[page_j, g]
 // The cached keys are rotated already. A request without tokens gives zeros.
+//
+// The call streams the cache once (1 byte per value) and should run at HBM speed: about 23 bytes
+// per clock and SM. Widening each byte on the CUDA cores would take most of their issue slots, so
+// the cached bytes go to the tensor cores as they are (kind::f8f6f4, e4m3 x e4m3 -> fp32) and the
+// few operands on the other side are carried as sums of e4m3 parts instead:
+//   x = x1 + x2 / 16 + x3 / 256,  x1 = e4m3(x), x2 = e4m3(16 (x - x1)), x3 = e4m3(16 (16 (x - x1) - x2))
+// Each part holds 4 significant bits of what the parts before it left, so three carry 12 bits: half
+// a step of 2^-12, as fp16 operands would. The parts are rows of their own in tiles that are
+// mostly empty otherwise, so they cost no tensor time:
+//   S^T = K8 Q^T     M = 128 keys of a chunk, N = 16 or 32 (three parts of the unit's heads),
+//                    K = head_dim. A = the K tile as TMA left it, B = the query parts.
+//   O  += P V8       M = 128, N = head_dim, K = 128 keys. A = P, B = the V tile as TMA left it
+//                    (MN-major). Row 32 w + t HPU + h: part t of head h's weights at warp w's keys.
+// One key per TMEM lane, so the softmax is one thread per key, and each of its four warps keeps a
+// reference maximum, a sum and rows of O of its own over its 32 keys of every chunk: no
+// reduction across warps per chunk. The value scale joins the weight before it is split: with
+// u_j = s_j + log2 vs_j (log2 domain) the carried weight is 2^(u_j - m) = w_j vs_j and the sum
+// takes it divided by vs_j. m moves only when some u exceeds it by 8 (then to 4 below that
+// maximum), so the weights stay within 2^8 < 448 and the largest one of a warp is at least 1;
+// a weight's last part ends at an absolute 2^-18.
+//
+// Work: the requests' chunks of 128 keys, unit by unit (unit: request, KV head, group of up to
+// HPU query heads), cut into equal ranges, one per CTA of a persistent grid. Lengths are read on
+// the device; every CTA repeats the sum over them. A unit within one CTA is written at once; the
+// fragments of others leave fp32 partials, and the CTA that leaves the last one joins them.
+//
+// Warps: 0-3 softmax, combine and output; 4 TMA (K, V and scales of each chunk); 5 TMEM and MMA;
+// 6 walks the fragments and prepares their query parts, one fragment ahead. Every wait is bounded.
 #pragma once
 
 #include "paged_sm100.cuh"
@@ -12,8 +40,6 @@ namespace du {
 
 struct DecodePagedParams {
   const void* q;        // [B, Hq, D]
-  const uint8_t* k8;    // [N, Hkv, block, D] e4m3
-  const uint8_t* v8;
   const float* ks;      // [N, Hkv]
   const float* vs;
   const int* table;     // [B, width]
@@ -21,89 +47,796 @@ struct DecodePagedParams {
   const void* cos;      // [positions, D/2]
   const void* sin;
   void* out;            // [B, Hq, D]
+  int* cnt;             // [gridDim.x] tickets, zero between calls
+  float* part;          // [2 gridDim.x][HPU][D + 2]: out, log2 of the sum, unused
   long long positions;
-  int B, Hq, Hkv, N, block, width;
+  int D, bf16;
+  int B, Hq, Hkv, G, N, width;
+  int block, block_log2;
+  int n_gchunk, heads;  // groups of `heads` query heads per KV head (the last may hold fewer)
   float scale_log2;
 };
 
-// One CTA per (query head, request); a warp takes a key at a time, a lane the row's elements
-// lane, lane + 32, ...; running maximum and sum per warp, joined at the end.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(256) decode_paged_kernel(const DecodePagedParams p) {
-  constexpr int EPL = (D + 31) / 32;
-  constexpr int NW = 8;
-  __shared__ float sm_q[D], sm_o[NW][D], sm_m[NW], sm_l[NW];
-  const int h = blockIdx.x, b = blockIdx.y, kvh = h / (p.Hq / p.Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int n = p.lens[b];
-  if (n < 0 || n > p.width * p.block || n > p.positions) {
-    if (threadIdx.x == 0) record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(n));
-    n = 0;
+// A CTA takes at least this many chunks.
+constexpr int DECODE_PAGED_MIN_PER = 2;
+__device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
+
+// cp.async of 4 bytes, and an arrival on `bar` once this thread's earlier cp.async have landed.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem] * B[smem], e4m3 operands, fp32 accumulate, one CTA.
+__device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The three e4m3 parts of two values (packed fp16, |value| <= 256), each part packed as a pair.
+__device__ __forceinline__ void e4m3_parts2(uint32_t x, uint32_t (&t)[3]) {
+  uint32_t r = x;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    uint16_t e;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(e) : "r"(r));
+    t[i] = e;
+    if (i < 2) {
+      uint32_t f;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(e));
+      const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&f));
+      const __half2 s = __hmul2(d, __float2half2_rn(16.0f));  // exact: d has at most 7 bits
+      r = *reinterpret_cast<const uint32_t*>(&s);
+    }
   }
-  auto at16 = [&](const void* base, long long i) {
-    if constexpr (BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
-    else return __half2float(static_cast<const __half*>(base)[i]);
-  };
-  if (n > 0)
-    for (int d = threadIdx.x; d < D / 2; d += 256) {
-      const long long qr = (static_cast<long long>(b) * p.Hq + h) * D, tr = static_cast<long long>(n - 1) * (D / 2);
-      const float x1 = at16(p.q, qr + d), x2 = at16(p.q, qr + D / 2 + d);
-      const float c = at16(p.cos, tr + d), s = at16(p.sin, tr + d);
-      sm_q[d] = (x1 * c - x2 * s) * p.scale_log2;
-      sm_q[d + D / 2] = (x2 * c + x1 * s) * p.scale_log2;
+}
+
+template <int DP_, int HPU_>
+struct DecodePagedShape {
+  static constexpr int DP = DP_;    // head_dim (32 for head_dim 16: the upper half is zero)
+  static constexpr int HPU = HPU_;  // query heads per unit
+  static constexpr int NQ = 3 * HPU <= 16 ? 16 : 32;  // rows of the query tile
+  static constexpr int CK = 128;    // keys per chunk
+  static constexpr int SPAN = DP < 128 ? DP : 128;    // bytes per row of a swizzled block
+  static constexpr int NBLK = DP / SPAN;
+  static constexpr int TILE = CK * DP;
+  static constexpr int STAGE = 2 * TILE;
+  // Two CTAs per SM where their tiles allow: one CTA's four softmax warps keep up with half an
+  // SM's share of the bandwidth at head_dim 64 and below, and their start and end overlap.
+  static constexpr int CTAS = DP <= 64 ? 2 : 1;
+  static constexpr int P_BYTES = CK * 128;            // [key][128 rows] bytes, 128-byte swizzle
+  static constexpr int Q_BYTES = ((NQ * DP + 1023) / 1024) * 1024;
+  static constexpr int ROW = DP + 4;                  // floats per row of the combine area
+  static constexpr int MRG_BYTES = ((4 * HPU * ROW + 8 * HPU) * 4 + 127) / 128 * 128;
+  static constexpr int FIXED = 2 * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2304;
+  static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
+  static constexpr int NSTG_FIT = (BUDGET - FIXED) / STAGE;
+  static constexpr int NSTG = NSTG_FIT > 8 ? 8 : NSTG_FIT;
+  static constexpr int OFF_P = NSTG * STAGE;
+  static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
+  static constexpr int OFF_MRG = OFF_Q + 2 * Q_BYTES;
+  static constexpr int OFF_SC = OFF_MRG + MRG_BYTES;  // [NSTG][2][8] scales of a chunk's blocks
+  static constexpr int OFF_FRAG = OFF_SC + NSTG * 64; // [2] fragment entries of 16 words
+  static constexpr int OFF_QS = OFF_FRAG + 2 * 64;    // [2][HPU] score factor of each head
+  static constexpr int OFF_BAR = OFF_QS + 2 * 32;
+  static constexpr int B_KFULL = 0, B_KEMPTY = NSTG, B_VFULL = 2 * NSTG, B_VEMPTY = 3 * NSTG,
+                       B_QFULL = 4 * NSTG, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
+                       B_SEMPTY = B_QFULL + 6, B_PFULL = B_QFULL + 8, B_PDONE = B_QFULL + 10,
+                       B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13;
+  static constexpr int N_BAR = B_DRAIN + 1;
+  static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;  // 16 words
+  static constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
+  static constexpr int TM_S = 0;           // S^T: two buffers of NQ columns
+  static constexpr int TM_O = 64;          // O: DP columns
+  static constexpr int TMEM_COLS = TM_O + DP <= 128 ? 128 : (TM_O + DP <= 256 ? 256 : 512);
+  static constexpr int NTHREADS = 224;
+  static_assert(3 * HPU <= 32, "a warp's rows of P");
+  static_assert(NSTG >= 2, "at least two stages");
+  static_assert(SMEM_BYTES <= (CTAS == 2 ? 115712 : 232448), "shared memory budget");
+  static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
+};
+
+// The range of chunks of this CTA and where it starts, found once per CTA (shared memory).
+struct PagedStart {
+  long long cur, hi, per;  // chunks [cur, hi) of the flattened sequence, chunks per CTA
+  long long base;          // first chunk of request b
+  int b, pad;
+};
+
+// One fragment, as warp 6 leaves it for the MMA and softmax warps (16 words).
+struct PagedFrag {
+  int kind;       // 1 a fragment, 0 the end
+  int b, h0, nh;  // request, first query head, heads
+  int chunks;     // 0: a request without tokens
+  int keys;       // keys of the fragment
+  int nf, c0;     // fragments of the unit, CTA of the first
+  int slot;       // partial slot when nf > 1
+  int pad[7];
+};
+
+// Walks a CTA's range fragment by fragment.
+struct PagedWalk {
+  long long cur, hi, per, base;
+  int b;
+  __device__ __forceinline__ void init(const PagedStart& s) {
+    cur = s.cur;
+    hi = s.hi;
+    per = s.per;
+    base = s.base;
+    b = s.b;
+  }
+  __device__ __forceinline__ static int tokens(const DecodePagedParams& p, int b) {
+    const int n = p.lens[b];
+    return (n < 0 || n > p.width * p.block || n > p.positions) ? 0 : n;
+  }
+  __device__ __forceinline__ static int chunks(int n) { return n > 128 ? (n + 127) >> 7 : 1; }
+  // unit: KV head * n_gchunk + group; [kbeg, kend) tokens.
+  __device__ __forceinline__ bool next(const DecodePagedParams& p, PagedFrag& f, int& unit, int& kbeg,
+                                       int& len) {
+    if (cur >= hi) return false;
+    const int ups = p.Hkv * p.n_gchunk;
+    int n, nc;
+    while (true) {
+      n = tokens(p, b);
+      nc = chunks(n);
+      const long long end = base + static_cast<long long>(nc) * ups;
+      if (cur < end) break;
+      base = end;
+      ++b;
     }
+    const long long in = cur - base;
+    unit = static_cast<int>(in / nc);
+    const long long ub = base + static_cast<long long>(unit) * nc;  // the unit's first chunk
+    const int j0 = static_cast<int>(cur - ub);
+    const long long e = min(hi, ub + nc);
+    const int j1 = static_cast<int>(e - ub);
+    const int kvh = unit / p.n_gchunk, gch = unit - kvh * p.n_gchunk;
+    f.kind = 1;
+    f.b = b;
+    f.h0 = kvh * p.G + gch * p.heads;
+    f.nh = min(p.heads, p.G - gch * p.heads);
+    kbeg = j0 << 7;
+    len = n;
+    f.keys = min(n, j1 << 7) - kbeg;
+    f.chunks = f.keys > 0 ? j1 - j0 : 0;
+    f.c0 = static_cast<int>(ub / per);
+    f.nf = static_cast<int>((ub + nc - 1) / per) - f.c0 + 1;
+    f.slot = 2 * static_cast<int>(blockIdx.x) + (j0 > 0 ? 0 : 1);
+    cur = e;
+    return true;
+  }
+};
+
+template <int DP, int HPU>
+__global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePagedShape<DP, HPU>::CTAS)
+    decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const DecodePagedParams p) {
+  using S = DecodePagedShape<DP, HPU>;
+  constexpr int CK = S::CK, SPAN = S::SPAN, NSTG = S::NSTG, NQ = S::NQ, ROW = S::ROW;
+  constexpr uint32_t SWZ = swizzle_code(SPAN);
+  constexpr uint32_t IDESC_QK = idesc_f16(128, NQ, 0, 0, 0, 0);  // (format 0 of kind::f8f6f4: e4m3)
+  constexpr uint32_t IDESC_PV = idesc_f16(128, DP, 0, 0, 1, 1);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_u32 = smem_u32(smem_raw);
+  const uint32_t sbase = (raw_u32 + 1023u) & ~1023u;
+  uint8_t* sgen = smem_raw + (sbase - raw_u32);
+  auto bar = [&](int i) -> uint32_t { return sbase + S::OFF_BAR + 8u * static_cast<uint32_t>(i); };
+  auto KFULL = [&](int s) { return bar(S::B_KFULL + s); };    // K and scales of a stage landed
+  auto KEMPTY = [&](int s) { return bar(S::B_KEMPTY + s); };  // QK read K, each softmax warp its scales
+  auto VFULL = [&](int s) { return bar(S::B_VFULL + s); };
+  auto VEMPTY = [&](int s) { return bar(S::B_VEMPTY + s); };  // PV read V
+  auto QFULL = [&](int i) { return bar(S::B_QFULL + i); };    // fragment entry and query parts written
+  auto QEMPTY = [&](int i) { return bar(S::B_QEMPTY + i); };  // last QK issued and done, entry read
+  auto SFULL = [&](int i) { return bar(S::B_SFULL + i); };
+  auto SEMPTY = [&](int i) { return bar(S::B_SEMPTY + i); };
+  auto PFULL = [&](int i) { return bar(S::B_PFULL + i); };
+  auto PDONE = [&](int i) { return bar(S::B_PDONE + i); };    // PV of even / odd chunks complete
+  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_DRAIN = bar(S::B_DRAIN);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(sgen + S::OFF_MISC);
+  volatile int* failed = reinterpret_cast<volatile int*>(misc + 1);
+  volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
+  volatile int* verdict = reinterpret_cast<volatile int*>(misc + 3);  // last of the unit's fragments
+  PagedStart* start = reinterpret_cast<PagedStart*>(misc + 4);
+  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_MRG);  // o [4][HPU][ROW], m [4][HPU], l [4][HPU]
+  float* mrg_m = mrg + 4 * HPU * ROW;
+  float* mrg_l = mrg_m + 4 * HPU;
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+
+  if (tid == 128) {
+    for (int s = 0; s < NSTG; ++s) {
+      mbar_init(KFULL(s), 1 + 32);
+      mbar_init(KEMPTY(s), 1 + 4);
+      mbar_init(VFULL(s), 1);
+      mbar_init(VEMPTY(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(QFULL(i), 32);
+      mbar_init(QEMPTY(i), 1 + 4);
+      mbar_init(SFULL(i), 1);
+      mbar_init(SEMPTY(i), 4);
+      mbar_init(PFULL(i), 128);
+      mbar_init(PDONE(i), 1);
+    }
+    mbar_init(BAR_MRG, 128);
+    mbar_init(BAR_DRAIN, 1);
+    *failed = 0;
+    *emitted = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 5) {
+    tmem_alloc(sbase + S::OFF_MISC, S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  // Rows of P that are no warp's own and rows of the query tiles beyond the parts stay zero.
+  for (int i = tid; i < (2 * S::P_BYTES + 2 * S::Q_BYTES) / 16; i += S::NTHREADS)
+    st_shared_v4(sbase + S::OFF_P + 16 * i, make_uint4(0, 0, 0, 0));
+  // This CTA's range: every thread sums the chunks of a run of requests, the runs are summed over
+  // the CTA, and the thread whose run holds the range's first chunk finds the request.
+  {
+    long long* wsum = reinterpret_cast<long long*>(mrg);
+    constexpr int NW = S::NTHREADS / 32;
+    const int ups = p.Hkv * p.n_gchunk;
+    const int run = (p.B + S::NTHREADS - 1) / S::NTHREADS;
+    const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int n = PagedWalk::tokens(p, b);
+      if (blockIdx.x == 0 && n != p.lens[b])
+        record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
+      mine += PagedWalk::chunks(n);
+    }
+    mine *= ups;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    long long before = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const long long x = wsum[w];
+      if (w < warp) before += x;
+      total += x;
+    }
+    long long per = (total + gridDim.x - 1) / gridDim.x;
+    if (per < DECODE_PAGED_MIN_PER) per = DECODE_PAGED_MIN_PER;
+    const long long cur = per * blockIdx.x;
+    if (tid == 0) {
+      start->cur = cur;
+      start->hi = min(total, cur + per);
+      start->per = per;
+    }
+    if (cur >= before && cur < before + mine) {
+      int b = b0;
+      long long base = before;
+      while (true) {
+        const long long nb = static_cast<long long>(PagedWalk::chunks(PagedWalk::tokens(p, b))) * ups;
+        if (cur < base + nb) break;
+        base += nb;
+        ++b;
+      }
+      start->b = b;
+      start->base = base;
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
   __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[EPL];
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc);
+
+  if (warp == 4) {
+    // ------------------------------------------------------------------ TMA: K, V, scales
+    PagedWalk walk;
+    walk.init(*start);
+    PagedFrag f;
+    int unit, kbeg, len, g = 0;
+    bool ok = true;
+    while (ok && walk.next(p, f, unit, kbeg, len)) {
+      const int kvh = unit / p.n_gchunk;
+      const int* row = p.table + static_cast<long long>(f.b) * p.width;
+      const int page0 = kbeg >> p.block_log2;
+      const int pages = (f.keys + p.block - 1) >> p.block_log2;  // of the fragment
+      const int ppc = CK >> p.block_log2;                        // per whole chunk: 1, 2, 4, 8
+      // Lane l holds the ids of blocks at + l and, loaded ahead, at + 32 + l.
+      int id = lane < pages ? row[page0 + lane] : 0;
+      int id_next = lane + 32 < pages ? row[page0 + 32 + lane] : 0;
+      int at = 0;
+      for (int j = 0; j < f.chunks; ++j, ++g) {
+        const int first = j * ppc;
+        if (first >= at + 32) {
+          at += 32;
+          id = id_next;
+          id_next = at + 32 + lane < pages ? row[page0 + at + 32 + lane] : 0;
+        }
+        const int here = min(ppc, pages - first);
+        const int s = g % NSTG;
+        const uint32_t st = sbase + s * S::STAGE;
+        int mine = __shfl_sync(0xffffffffu, id, (first - at) + (lane & 7));
+        const bool in = (lane & 7) < here;
+        const bool bad = in && (mine < 0 || mine >= p.N);
+        if (bad && lane < 8) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(mine));
+        const long long cell = bad ? static_cast<long long>(p.N) * p.Hkv  // beyond the map: zeros
+                                   : static_cast<long long>(mine) * p.Hkv + kvh;
+        if (g >= NSTG) ok = mbar_wait(KEMPTY(s), ((g / NSTG) - 1) & 1, failed, 800);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        const uint32_t bytes = static_cast<uint32_t>(here << p.block_log2) * DP;
+        if (lane == 0) mbar_expect_tx(KFULL(s), bytes);
+        __syncwarp();
+        if (in && lane < 16) {
+          const float* src = (lane < 8 ? p.ks : p.vs) + cell;
+          cp_async4(sbase + S::OFF_SC + s * 64 + lane * 4, bad ? &g_du_paged_nan : src);
+        }
+        cp_async_arrive(KFULL(s));
+        if (in && lane < 8)
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-  for (int j = warp; j < n; j += NW) {
-    const int id = p.table[static_cast<long long>(b) * p.width + j / p.block];
-    if (id < 0 || id >= p.N) {
-      if (lane == 0) record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(id));
-      m = __int_as_float(0x7fc00000);
-      break;
-    }
-    const long long cell = static_cast<long long>(id) * p.Hkv + kvh;
-    const long long row = (cell * p.block + j % p.block) * D;
-    float dot = 0.f, vv[EPL];
+          for (int nb = 0; nb < S::NBLK; ++nb)
+            tma_load_3d(st + nb * CK * SPAN + (lane << p.block_log2) * SPAN, &tm_k, KFULL(s), nb * SPAN, 0,
+                        static_cast<int>(cell));
+        if (g >= NSTG) ok = mbar_wait(VEMPTY(s), ((g / NSTG) - 1) & 1, failed, 801);
+        if (!(ok = __all_sync(0xffffffffu, ok))) {
+          ++g;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(VFULL(s), bytes);
+        __syncwarp();
+        if (in && lane < 8)
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const int d = lane + 32 * e;
-      vv[e] = 0.f;
-      if (d < D) {
-        dot = fmaf(sm_q[d], e4m3x2_widen(p.k8[row + d]).x, dot);
-        vv[e] = e4m3x2_widen(p.v8[row + d]).x;
+          for (int nb = 0; nb < S::NBLK; ++nb)
+            tma_load_3d(st + S::TILE + nb * CK * SPAN + (lane << p.block_log2) * SPAN, &tm_v, VFULL(s), nb * SPAN,
+                        0, static_cast<int>(cell));
       }
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float s = dot * p.ks[cell], mn = s > m ? s : m;
-    const float a = ex2(m - mn), w = ex2(s - mn), wv = w * p.vs[cell];
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] = acc[e] * a + wv * vv[e];
-    m = mn;
-  }
-  if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < EPL; ++e)
-    if (lane + 32 * e < D) sm_o[warp][lane + 32 * e] = acc[e];
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float M = -INFINITY, L = 0.f, A = 0.f;
-    for (int w = 0; w < NW; ++w) M = (sm_m[w] > M || sm_m[w] != sm_m[w]) ? sm_m[w] : M;
-    for (int w = 0; w < NW; ++w) {
-      const float f = (sm_m[w] == -INFINITY && M == M) ? 0.f : ex2(sm_m[w] - M);
-      L += sm_l[w] * f;
-      A += sm_o[w][d] * f;
+    // The last copies land before the CTA may exit. (After a failed wait a stage's V may never
+    // have been issued: that wait runs into its own limit.)
+    for (int j = g > NSTG ? g - NSTG : 0; j < g; ++j) {
+      mbar_wait_drain(KFULL(j % NSTG), (j / NSTG) & 1, 802);
+      mbar_wait_drain(VFULL(j % NSTG), (j / NSTG) & 1, 803);
     }
-    const float val = n > 0 ? A / L : 0.f;
-    const long long o = (static_cast<long long>(b) * p.Hq + h) * D + d;
-    if constexpr (BF16) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(val);
-    else static_cast<__half*>(p.out)[o] = __float2half_rn(val);
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    bool ok = true;
+    int g = 0;
+    for (int it = 0; ok; ++it) {
+      const int qb = it & 1;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 810)))) break;
+      const PagedFrag* f = reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + qb * 64);
+      const int kind = f->kind, n = f->chunks;
+      if (kind == 0) break;
+      if (n == 0) {
+        if (leader) mbar_arrive(QEMPTY(qb));
+        __syncwarp();
+        continue;
+      }
+      const uint64_t dq = smem_desc(sbase + S::OFF_Q + qb * S::Q_BYTES, 16, 8 * SPAN, SWZ);
+      for (int j = 0; j <= n; ++j) {
+        if (j < n) {  // S of chunk j
+          const int gj = g + j, s = gj % NSTG;
+          ok = mbar_wait(KFULL(s), (gj / NSTG) & 1, failed, 811);
+          if (ok && gj >= 2) ok = mbar_wait(SEMPTY(gj & 1), ((gj >> 1) - 1) & 1, failed, 812);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t dk = smem_desc(sbase + s * S::STAGE, 16, 8 * SPAN, SWZ);
+#pragma unroll
+            for (int kk = 0; kk < DP / 32; ++kk) {
+              const uint32_t off_k = ((kk * 32) / SPAN) * CK * SPAN + (kk * 32) % SPAN;
+              const uint32_t off_q = ((kk * 32) / SPAN) * NQ * SPAN + (kk * 32) % SPAN;
+              umma_f8_ss(tmem + S::TM_S + (gj & 1) * NQ, dk + (off_k >> 4), dq + (off_q >> 4), IDESC_QK,
+                         kk > 0 ? 1u : 0u);
+            }
+            umma_commit(SFULL(gj & 1));
+            umma_commit(KEMPTY(s));
+            if (j == n - 1) umma_commit(QEMPTY(qb));
+          }
+          __syncwarp();
+        }
+        if (j > 0) {  // O of chunk j - 1
+          const int gj = g + j - 1, s = gj % NSTG;
+          ok = mbar_wait(PFULL(gj & 1), (gj >> 1) & 1, failed, 813);
+          if (ok) ok = mbar_wait(VFULL(s), (gj / NSTG) & 1, failed, 814);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t dp = smem_desc(sbase + S::OFF_P + (gj & 1) * S::P_BYTES, 16, 1024, 2);
+            const uint64_t dv = smem_desc(sbase + s * S::STAGE + S::TILE, CK * SPAN, 8 * SPAN, SWZ);
+#pragma unroll
+            for (int kk = 0; kk < CK / 32; ++kk)
+              umma_f8_ss(tmem + S::TM_O, dp + static_cast<uint64_t>((kk * 32 * 128) >> 4),
+                         dv + static_cast<uint64_t>((kk * 32 * SPAN) >> 4), IDESC_PV,
+                         (j > 1 || kk > 0) ? 1u : 0u);
+            umma_commit(PDONE(gj & 1));
+            umma_commit(VEMPTY(s));
+          }
+          __syncwarp();
+        }
+      }
+      g += n;
+    }
+    if (leader) {
+      umma_commit(BAR_DRAIN);
+      mbar_wait_drain(BAR_DRAIN, 0, 815);
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    // ------------------------------------------------------------------ fragments and queries
+    PagedWalk walk;
+    walk.init(*start);
+    const int D = p.D, half = D >> 1;
+    auto at16 = [&](const void* base, long long i) -> float {
+      return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i])
+                    : __half2float(static_cast<const __half*>(base)[i]);
+    };
+    for (int it = 0;; ++it) {
+      const int qb = it & 1;
+      PagedFrag f;
+      int unit, kbeg, len;
+      const bool more = walk.next(p, f, unit, kbeg, len);
+      // (the loads go out before the wait for the entry)
+      constexpr int EPL = DP >= 64 ? DP / 64 : 1;  // element pairs per lane
+      float x1[HPU][EPL], x2[HPU][EPL];
+      if (more && f.chunks > 0) {
+        float c[EPL], sn[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          const int d = lane + 32 * e;
+          const long long tr = static_cast<long long>(len - 1) * half + d;
+          c[e] = d < half ? at16(p.cos, tr) : 0.f;
+          sn[e] = d < half ? at16(p.sin, tr) : 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < HPU; ++h)
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            const int d = lane + 32 * e;
+            const long long qr = (static_cast<long long>(f.b) * p.Hq + f.h0 + h) * D + d;
+            const bool on = h < f.nh && d < half;
+            const float a = on ? at16(p.q, qr) : 0.f, b = on ? at16(p.q, qr + half) : 0.f;
+            x1[h][e] = a;
+            x2[h][e] = b;
+          }
+#pragma unroll
+        for (int h = 0; h < HPU; ++h)
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            const float a = x1[h][e], b = x2[h][e];
+            x1[h][e] = a * c[e] - b * sn[e];
+            x2[h][e] = b * c[e] + a * sn[e];
+          }
+      }
+      if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
+      if (more && f.chunks > 0) {
+        // Row n of the tile, element d: a swizzled K-major byte.
+        auto put = [&](int n, int d, uint32_t byte) {
+          const uint32_t o = swz_chunk_offset<SPAN>(NQ, n, d >> 4) + (d & 15);
+          sgen[S::OFF_Q + qb * S::Q_BYTES + o] = static_cast<uint8_t>(byte);
+        };
+#pragma unroll
+        for (int h = 0; h < HPU; ++h) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e)
+            top = max(top, max(__float_as_uint(x1[h][e]) & 0x7fffffffu, __float_as_uint(x2[h][e]) & 0x7fffffffu));
+          top = __reduce_max_sync(0xffffffffu, top);
+          const float u = paged_unit(top);  // a power of two: the row fits e4m3 divided by it
+          const float inv = 1.0f / u;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            const int d = lane + 32 * e;
+            float y1 = x1[h][e] * inv, y2 = x2[h][e] * inv;
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+              const uint32_t pr = e4m3x2(y1, y2);
+              const float2 w = e4m3x2_widen(pr);
+              y1 = (y1 - w.x) * 16.0f;
+              y2 = (y2 - w.y) * 16.0f;
+              if (d < half) {
+                put(t * HPU + h, d, pr & 0xffu);
+                put(t * HPU + h, d + half, pr >> 8);
+              }
+            }
+          }
+          if (lane == 0) reinterpret_cast<float*>(sgen + S::OFF_QS)[qb * HPU + h] = u * p.scale_log2;
+        }
+        fence_proxy_async_smem();
+      }
+      if (lane == 0) {
+        if (!more) f.kind = 0;
+        *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + qb * 64) = f;
+      }
+      __syncwarp();
+      mbar_arrive(QFULL(qb));
+      if (!more) break;
+    }
+  } else {
+    // ------------------------------------------------------------------ warps 0-3: softmax
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    bool ok = true;
+    int g = 0, mq = 0;
+    for (int it = 0; ok; ++it) {
+      const int qb = it & 1;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 830)))) break;
+      const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + qb * 64);
+      float qs[HPU];
+#pragma unroll
+      for (int h = 0; h < HPU; ++h) qs[h] = reinterpret_cast<const float*>(sgen + S::OFF_QS)[qb * HPU + h];
+      __syncwarp();
+      if (f.kind == 0) break;
+      if (lane == 0) mbar_arrive(QEMPTY(qb));
+      auto store_out = [&](long long row, int d, float val) {
+        if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[row * p.D + d] = __float2bfloat16_rn(val);
+        else static_cast<__half*>(p.out)[row * p.D + d] = __float2half_rn(val);
+      };
+      const long long row0 = static_cast<long long>(f.b) * p.Hq + f.h0;
+      if (f.chunks == 0) {
+        for (int i = tid; i < f.nh * p.D; i += 128) store_out(row0 + i / p.D, i % p.D, 0.f);
+        if (tid == 0) *emitted = it + 1;
+        continue;
+      }
+      float m[HPU], l[HPU];
+#pragma unroll
+      for (int h = 0; h < HPU; ++h) {
+        m[h] = -1e30f;
+        l[h] = 0.f;
+      }
+      for (int j = 0; j < f.chunks; ++j) {
+        const int gj = g + j, s = gj % NSTG;
+        const int left = f.keys - j * CK;  // keys of this chunk and those behind it
+        const bool valid = tid < left;
+        ok = mbar_wait(KFULL(s), (gj / NSTG) & 1, failed, 831);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        const float* sc = reinterpret_cast<const float*>(sgen + S::OFF_SC + s * 64);
+        const float ksc = valid ? sc[tid >> p.block_log2] : 1.0f;
+        float vsc = valid ? sc[8 + (tid >> p.block_log2)] : 1.0f;
+        if (vsc < 0x1p-64f) vsc = 0x1p-64f;  // (the writer's smallest; a NaN stays)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(KEMPTY(s));
+        const float lv = lg2(vsc), rv = __fdividef(1.0f, vsc);
+        ok = mbar_wait(SFULL(gj & 1), (gj >> 1) & 1, failed, 832);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+        float sv[NQ];
+#pragma unroll
+        for (int c = 0; c < NQ; c += 16) tmem_ld16(tmem + lane_off + S::TM_S + (gj & 1) * NQ + c, sv + c);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(SEMPTY(gj & 1));
+        float u[HPU];
+        bool over = false;
+#pragma unroll
+        for (int h = 0; h < HPU; ++h) {
+          const float dot = fmaf(sv[2 * HPU + h], 0x1p-8f, fmaf(sv[HPU + h], 0x1p-4f, sv[h]));
+          u[h] = valid ? fmaf(dot, qs[h] * ksc, lv) : -INFINITY;
+          over |= u[h] > m[h] + 8.0f;
+        }
+        float alpha[HPU];
+        const bool moved = __any_sync(0xffffffffu, over);
+        if (moved) {
+#pragma unroll
+          for (int h = 0; h < HPU; ++h) {
+            const float mx = warp_max(u[h]);
+            const float mn = mx > m[h] + 8.0f ? mx - 4.0f : m[h];
+            alpha[h] = ex2(m[h] - mn);
+            l[h] *= alpha[h];
+            m[h] = mn;
+          }
+        }
+        float pe[HPU];
+#pragma unroll
+        for (int h = 0; h < HPU; ++h) {
+          pe[h] = ex2(u[h] - m[h]);
+          l[h] = fmaf(pe[h], rv, l[h]);
+        }
+        // Parts of the weights, rows t HPU + h of this warp: 3 HPU bytes of the key's row of P.
+        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if constexpr (HPU == 1) {
+          uint32_t t[3];
+          e4m3_parts2(pack2<false>(pe[0], 0.f), t);
+          w[0] = (t[0] & 0xffu) | ((t[1] & 0xffu) << 8) | ((t[2] & 0xffu) << 16);
+        } else if constexpr (HPU == 2) {
+          uint32_t t[3];
+          e4m3_parts2(pack2<false>(pe[0], pe[1]), t);
+          w[0] = t[0] | (t[1] << 16);
+          w[1] = t[2];
+        } else {
+#pragma unroll
+          for (int h = 0; h < HPU; h += 4) {
+            uint32_t a[3], b[3];
+            e4m3_parts2(pack2<false>(pe[h], pe[h + 1]), a);
+            e4m3_parts2(pack2<false>(pe[h + 2], pe[h + 3]), b);
+#pragma unroll
+            for (int t = 0; t < 3; ++t) w[t * (HPU / 4) + h / 4] = a[t] | (b[t] << 16);
+          }
+        }
+        // P buffer gj & 1 was last read by PV(gj - 2); a moved reference rescales O, which holds
+        // PV up to gj - 1 of this fragment.
+        if (gj >= 2) ok = mbar_wait(PDONE(gj & 1), ((gj >> 1) - 1) & 1, failed, 833);
+        if (ok && moved && j > 0) ok = mbar_wait(PDONE((gj - 1) & 1), ((gj - 1) >> 1) & 1, failed, 834);
+        if (ok && left < CK) ok = mbar_wait(VFULL(s), (gj / NSTG) & 1, failed, 835);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+        if (moved && j > 0) {
+          float al = 1.0f;
+#pragma unroll
+          for (int h = 0; h < HPU; ++h) al = (lane % HPU) == h ? alpha[h] : al;
+          // (a row that was zero and whose reference was none yet: alpha is 0, O is 0)
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            float o[16];
+            tmem_ld16(tmem + lane_off + S::TM_O + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= al;
+            tmem_st16(tmem + lane_off + S::TM_O + c, o);
+          }
+          tmem_wait_st();
+        }
+        const uint32_t prow = sbase + S::OFF_P + (gj & 1) * S::P_BYTES + tid * 128;
+        st_shared_v4(prow + (((2 * warp) ^ (tid & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+        if constexpr (HPU == 8)
+          st_shared_v4(prow + (((2 * warp + 1) ^ (tid & 7)) << 4), make_uint4(w[4], w[5], w[6], w[7]));
+        if (!valid) {
+          // Rows behind the last key may hold anything, a NaN among it, and 0 x NaN is a NaN.
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c)
+            st_shared_v4(sbase + s * S::STAGE + S::TILE + ((c * 16) / SPAN) * CK * SPAN + tid * SPAN + (c * 16) % SPAN,
+                         make_uint4(0, 0, 0, 0));
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(PFULL(gj & 1));
+      }
+      if (!ok) break;
+      g += f.chunks;
+      // Combine the warps: O rows 32 w + t HPU + h, parts joined by shuffles.
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) & 1), ((g - 1) >> 1) & 1, failed, 836)))) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c0 = 0; c0 < DP; c0 += 32) {
+        float o[32];
+        tmem_ld16(tmem + lane_off + S::TM_O + c0, o);
+        tmem_ld16(tmem + lane_off + S::TM_O + c0 + 16, o + 16);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float a = __shfl_down_sync(0xffffffffu, o[i], HPU), b = __shfl_down_sync(0xffffffffu, o[i], 2 * HPU);
+          o[i] = fmaf(b, 0x1p-8f, fmaf(a, 0x1p-4f, o[i]));
+        }
+        if (lane < HPU) {
+          float4* dst = reinterpret_cast<float4*>(mrg + (warp * HPU + lane) * ROW + c0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();
+#pragma unroll
+      for (int h = 0; h < HPU; ++h) {
+        float x = l[h];
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (lane == 0) {
+          mrg_m[warp * HPU + h] = m[h];
+          mrg_l[warp * HPU + h] = x;
+        }
+      }
+      mbar_arrive(BAR_MRG);
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
+      ++mq;
+      for (int i = tid; i < f.nh * p.D; i += 128) {
+        const int h = i / p.D, d = i - h * p.D;
+        float M = mrg_m[h];
+#pragma unroll
+        for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, mrg_m[w2 * HPU + h]);
+        float A = 0.f, L = 0.f;
+#pragma unroll
+        for (int w2 = 0; w2 < 4; ++w2) {
+          const float wt = ex2(mrg_m[w2 * HPU + h] - M);
+          A = fmaf(mrg[(w2 * HPU + h) * ROW + d], wt, A);
+          L = fmaf(mrg_l[w2 * HPU + h], wt, L);
+        }
+        const float val = A / L;
+        if (f.nf == 1) {
+          store_out(row0 + h, d, val);
+        } else {
+          float* ps = p.part + (static_cast<long long>(f.slot) * HPU + h) * (p.D + 2);
+          ps[d] = val;
+          if (d == 0) ps[p.D] = M + lg2(L);
+        }
+      }
+      // The combine area is free again (and the partial stored) once every thread is here.
+      mbar_arrive(BAR_MRG);
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 838)))) break;
+      ++mq;
+      if (f.nf > 1) {
+        // A ticket on the unit's counter. The partial stores reach thread 0 through the barrier; its
+        // acquire-release add makes them visible before the ticket and, after the last ticket,
+        // the other fragments' partials visible to this CTA.
+        if (tid == 0) {
+          const int last = atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1;
+          if (last) p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
+          *verdict = last;
+          *emitted = it + 1;
+        }
+        mbar_arrive(BAR_MRG);
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 839)))) break;
+        ++mq;
+        if (*verdict) {
+          for (int i = tid; i < f.nh * p.D; i += 128) {
+            const int h = i / p.D, d = i - h * p.D;
+            float M = -INFINITY, A = 0.f, L = 0.f;
+#pragma unroll 4
+            for (int k = 0; k < f.nf; ++k) {
+              const long long sl = k == 0 ? 2LL * f.c0 + 1 : 2LL * (f.c0 + k);
+              const float* ps = p.part + (sl * HPU + h) * (p.D + 2);
+              const float x = __ldcg(ps + p.D), o = __ldcg(ps + d);
+              const float mn = fmaxf(M, x);
+              const float a = M == -INFINITY ? 0.f : ex2(M - mn), b = ex2(x - mn);
+              A = fmaf(A, a, o * b);
+              L = fmaf(L, a, b);
+              M = mn;
+            }
+            store_out(row0 + h, d, A / L);
+          }
+        }
+      } else if (tid == 0) {
+        *emitted = it + 1;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*failed) {
+    // A wait ran out (reported in the status words): NaN for what this CTA still owes, and its
+    // tickets, so that the counters return to zero.
+    PagedWalk walk;
+    walk.init(*start);
+    PagedFrag f;
+    int unit, kbeg, len;
+    const float nan = __int_as_float(0x7fc00000);
+    for (int it = 0; walk.next(p, f, unit, kbeg, len); ++it) {
+      if (it < *emitted) continue;
+      for (int i = tid; i < f.nh * p.D; i += S::NTHREADS) {
+        const int h = i / p.D, d = i - h * p.D;
+        const long long o = (static_cast<long long>(f.b) * p.Hq + f.h0 + h) * p.D + d;
+        if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(nan);
+        else static_cast<__half*>(p.out)[o] = __float2half_rn(nan);
+        if (f.nf > 1) {
+          float* ps = p.part + (static_cast<long long>(f.slot) * HPU + h) * (p.D + 2);
+          ps[d] = nan;
+          if (d == 0) ps[p.D] = nan;
+        }
+      }
+      __threadfence();
+      __syncthreads();
+      if (f.nf > 1 && tid == 0 && atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1) p.cnt[f.c0] = 0;
+    }
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::TMEM_COLS);
   }
 }
 

@@ -1306,19 +1306,79 @@ int launch_paged_write(const du::PagedWriteParams& prm, int D, cudaStream_t st) 
   }
 }
 
-template <bool BF16>
-int launch_decode_paged(const du::DecodePagedParams& prm, int D, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(prm.Hq), static_cast<unsigned>(prm.B));
-  switch (D) {
-    case 16: du::decode_paged_kernel<16, BF16><<<grid, 256, 0, st>>>(prm); break;
-    case 32: du::decode_paged_kernel<32, BF16><<<grid, 256, 0, st>>>(prm); break;
-    case 64: du::decode_paged_kernel<64, BF16><<<grid, 256, 0, st>>>(prm); break;
-    case 128: du::decode_paged_kernel<128, BF16><<<grid, 256, 0, st>>>(prm); break;
-    default: du::decode_paged_kernel<256, BF16><<<grid, 256, 0, st>>>(prm); break;
-  }
-  cudaError_t e = cudaGetLastError();
+// Query heads per unit of the paged decode: the group of a KV head in equal parts of at most 8.
+int paged_group_chunks(int G) { return (G + 7) / 8; }
+int paged_unit_heads(int G) { return (G + paged_group_chunks(G) - 1) / paged_group_chunks(G); }
+int paged_hpu(int heads) { return heads <= 1 ? 1 : (heads <= 2 ? 2 : (heads <= 4 ? 4 : 8)); }
+
+// CTAs of the persistent grid: the resident ones, or as many as a full block table could occupy.
+int paged_grid(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
+  const long long ctas = static_cast<long long>(sm_count()) * (D <= 64 ? 2 : 1);
+  const long long units = static_cast<long long>(B) * Hkv * paged_group_chunks(Hq / Hkv);
+  const long long per_unit = (static_cast<long long>(max_blocks) * block_size + 127) / 128;
+  const long long most = (units * per_unit + du::DECODE_PAGED_MIN_PER - 1) / du::DECODE_PAGED_MIN_PER;
+  return static_cast<int>(most < ctas ? most : ctas);
+}
+
+size_t paged_ws_bytes(int grid, int Hq, int Hkv, int D) {
+  return 2 * static_cast<size_t>(grid) * paged_hpu(paged_unit_heads(Hq / Hkv)) * (D + 2) * sizeof(float);
+}
+
+// 3-D map over a paged cache [cells, block, D] of bytes (a cell: one block of one KV head): box
+// {span, block, 1}. head_dim 16 takes boxes of 32 bytes, zero-filled beyond the row.
+int encode_map_paged(CUtensorMap* map, const void* base, int D, int block, long long cells, int span) {
+  auto fn = get_encode_fn();
+  if (fn == nullptr) return fail(DU_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(block), static_cast<cuuint64_t>(cells)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(D) * block};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(span), static_cast<cuuint32_t>(block), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = span == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                             : CU_TENSOR_MAP_SWIZZLE_32B;
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(DU_ERR_CUDA, "cuTensorMapEncodeTiled (paged cache) failed with CUresult " + std::to_string(r));
+  return DU_OK;
+}
+
+template <int DP, int HPU>
+int launch_decode_paged_t(const void* k8, const void* v8, const du::DecodePagedParams& prm, int grid, cudaStream_t st) {
+  using S = du::DecodePagedShape<DP, HPU>;
+  CUtensorMap tk, tv;
+  const long long cells = static_cast<long long>(prm.N) * prm.Hkv;
+  int rc;
+  if ((rc = encode_map_paged(&tk, k8, prm.D, prm.block, cells, S::SPAN)) != DU_OK) return rc;
+  if ((rc = encode_map_paged(&tv, v8, prm.D, prm.block, cells, S::SPAN)) != DU_OK) return rc;
+  auto kern = du::decode_paged_kernel<DP, HPU>;
+  cudaError_t e = ensure_smem_attr(kern, S::SMEM_BYTES);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged decode)");
+  kern<<<static_cast<unsigned>(grid), S::NTHREADS, S::SMEM_BYTES, st>>>(tk, tv, prm);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged decode launch");
   return DU_OK;
+}
+
+template <int DP>
+int launch_decode_paged_h(const void* k8, const void* v8, const du::DecodePagedParams& prm, int grid, cudaStream_t st) {
+  switch (paged_hpu(prm.heads)) {
+    case 1: return launch_decode_paged_t<DP, 1>(k8, v8, prm, grid, st);
+    case 2: return launch_decode_paged_t<DP, 2>(k8, v8, prm, grid, st);
+    case 4: return launch_decode_paged_t<DP, 4>(k8, v8, prm, grid, st);
+    default: return launch_decode_paged_t<DP, 8>(k8, v8, prm, grid, st);
+  }
+}
+
+int launch_decode_paged(const void* k8, const void* v8, const du::DecodePagedParams& prm, int grid, cudaStream_t st) {
+  switch (prm.D) {
+    case 16:
+    case 32: return launch_decode_paged_h<32>(k8, v8, prm, grid, st);
+    case 64: return launch_decode_paged_h<64>(k8, v8, prm, grid, st);
+    case 128: return launch_decode_paged_h<128>(k8, v8, prm, grid, st);
+    default: return launch_decode_paged_h<256>(k8, v8, prm, grid, st);
+  }
 }
 
 }  // namespace
@@ -1418,11 +1478,18 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
   return dtype == DU_DTYPE_BF16 ? launch_paged_write<true>(prm, D, st) : launch_paged_write<false>(prm, D, st);
 }
 
+size_t du_decode_paged_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
+  if (check_common(B, Hq, Hkv, 1, D, DU_DTYPE_BF16) != DU_OK || check_paged(Hkv, 1, block_size) != DU_OK || max_blocks <= 0)
+    return 0;
+  return paged_ws_bytes(paged_grid(B, Hq, Hkv, D, block_size, max_blocks), Hq, Hkv, D);
+}
+
 int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                     const float* v_scale, const int* block_table, const int* cache_seqlens,
                     const void* cos, const void* sin, void* out, int B, int Hq, int Hkv, int D,
                     int num_blocks, int block_size, int max_blocks, int dtype, float scale,
-                    long long rope_positions, void* stream) {
+                    long long rope_positions, int* tickets, void* workspace, size_t workspace_bytes,
+                    void* stream) {
   g_last_error.clear();
   int rc = check_common(B, Hq, Hkv, 1, D, dtype);
   if (rc != DU_OK) return rc;
@@ -1431,18 +1498,21 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   if (max_blocks <= 0) return fail(DU_ERR_INVALID, "max_blocks must be positive");
   if (static_cast<long long>(max_blocks) * block_size > 0x7fffffffLL - 128)
     return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^31 - 129 tokens");
-  if (B > 65535) return fail(DU_ERR_UNSUPPORTED, "at most 65535 sequences per call");
-  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !cache_seqlens || !cos || !sin || !out)
+  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !cache_seqlens || !cos || !sin || !out ||
+      !tickets)
     return fail(DU_ERR_INVALID, "null pointer argument");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(cos) || !aligned16(sin) || !aligned16(out))
     return fail(DU_ERR_INVALID, "q, out, the caches and the rope tables must be 16-byte aligned");
-  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(cache_seqlens))
-    return fail(DU_ERR_INVALID, "scales, block_table and cache_seqlens must be 4-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(cache_seqlens) || !aligned4(tickets))
+    return fail(DU_ERR_INVALID, "scales, block_table, cache_seqlens and tickets must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
+  if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
+  const int grid = paged_grid(B, Hq, Hkv, D, block_size, max_blocks);
+  if (grid > DU_PAGED_TICKETS) return fail(DU_ERR_UNSUPPORTED, "more resident blocks of threads than tickets");
+  if (!workspace || workspace_bytes < paged_ws_bytes(grid, Hq, Hkv, D) || !aligned16(workspace))
+    return fail(DU_ERR_WORKSPACE, "workspace missing, misaligned or smaller than du_decode_paged_workspace_size");
   du::DecodePagedParams prm{};
   prm.q = q;
-  prm.k8 = static_cast<const uint8_t*>(k_cache);
-  prm.v8 = static_cast<const uint8_t*>(v_cache);
   prm.ks = k_scale;
   prm.vs = v_scale;
   prm.table = block_table;
@@ -1450,16 +1520,23 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.cos = cos;
   prm.sin = sin;
   prm.out = out;
+  prm.cnt = tickets;
+  prm.part = static_cast<float*>(workspace);
   prm.positions = rope_positions;
+  prm.D = D;
+  prm.bf16 = dtype == DU_DTYPE_BF16;
   prm.B = B;
   prm.Hq = Hq;
   prm.Hkv = Hkv;
+  prm.G = Hq / Hkv;
   prm.N = num_blocks;
-  prm.block = block_size;
   prm.width = max_blocks;
+  prm.block = block_size;
+  prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
+  prm.n_gchunk = paged_group_chunks(prm.G);
+  prm.heads = paged_unit_heads(prm.G);
   prm.scale_log2 = scale * 1.4426950408889634f;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DU_DTYPE_BF16 ? launch_decode_paged<true>(prm, D, st) : launch_decode_paged<false>(prm, D, st);
+  return launch_decode_paged(k_cache, v_cache, prm, grid, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

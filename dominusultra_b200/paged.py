@@ -16,13 +16,16 @@ and tables stay on the GPU: no call synchronises, and each can be captured into 
 
 from __future__ import annotations
 
+import threading
 from typing import Tuple
 
 import torch
 
 from . import _lib
 from .attention import (
+    _RETIRED,
     _aligned,
+    _cached_workspace,
     _dtype_code,
     _OnDevice,
     _ptr,
@@ -128,6 +131,58 @@ def _validate_tables_like(cos, sin, head_dim, device, dtype) -> None:
         raise ValueError("cos and sin must have the same dtype as the attention tensors")
     if not cos.is_contiguous() or not sin.is_contiguous():
         raise ValueError("cos and sin must be contiguous")
+
+
+_WS_SIZES = {}
+
+
+def _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, device) -> int:
+    key = (B, Hq, Hkv, D, block_size, max_blocks, device.index)
+    n = _WS_SIZES.get(key)
+    if n is None:
+        n = int(_lib.load().du_decode_paged_workspace_size(B, Hq, Hkv, D, block_size, max_blocks))
+        _WS_SIZES[key] = n
+    return n
+
+
+# Tickets for calls under a graph capture, handed out of zeroed slabs: [slab, words used] per device.
+# A graph's tickets and workspace are its own for good, so any two graphs may be replayed at once.
+_SLAB_WORDS = 1024 * _lib.DU_PAGED_TICKETS
+_SLABS = {}
+_SLAB_LOCK = threading.Lock()
+
+
+def _decode_scratch(nbytes: int, device: torch.device, stream: int):
+    """(tickets, workspace, keep-alive tensors) of a paged decode on torch's current stream.
+
+    Eager calls share a pair per (device, stream): calls on one stream run in order. A call that
+    is being captured gets a workspace from the graph's own memory and tickets of its own.
+    """
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    capturing = torch.cuda.is_current_stream_capturing()
+    if not capturing:
+        tickets, _ = _cached_workspace("decode_paged_tickets", 4 * _lib.DU_PAGED_TICKETS, device, stream)
+        ws, _ = _cached_workspace("decode_paged", nbytes, device, stream)
+        slab = _SLABS.get(index)
+        if slab is None or slab[1] > _SLAB_WORDS // 2:
+            # (a copy from the host has ended when it returns: the zeros are there for any stream)
+            zeros = torch.zeros(_SLAB_WORDS, dtype=torch.int32).to(device)
+            with _SLAB_LOCK:
+                _SLABS[index] = [zeros, 0]
+                if slab is not None:
+                    _RETIRED.append(slab[0])
+        return tickets, ws, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with _SLAB_LOCK:
+        slab = _SLABS.get(index)
+        if slab is not None and slab[1] + _lib.DU_PAGED_TICKETS <= _SLAB_WORDS:
+            tickets = slab[0][slab[1] : slab[1] + _lib.DU_PAGED_TICKETS]
+            slab[1] += _lib.DU_PAGED_TICKETS
+            return tickets.data_ptr(), ws.data_ptr(), ws
+    # no slab yet (the process's first call), or more than half a slab of captures since the last
+    # eager call: zeroed inside the graph, by a node of its own
+    tickets = torch.zeros(_lib.DU_PAGED_TICKETS, dtype=torch.int32, device=device)
+    return tickets.data_ptr(), ws.data_ptr(), (ws, tickets)
 
 
 def dominus_ultra_paged_tables(
@@ -349,11 +404,15 @@ def dominus_ultra_decode_paged(
         q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
         lens = _device_int32(cache_seqlens, device)
         out = torch.empty_like(q_new)
+        stream = _stream(device)
+        nbytes = _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, device)
+        tickets, ws, keep = _decode_scratch(nbytes, device, stream)
         rc = lib.du_decode_paged(
             _ptr(q_new), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
             _ptr(block_table), _ptr(lens), _ptr(cos), _ptr(sin), _ptr(out), B, Hq, Hkv, D,
             num_blocks, block_size, max_blocks, _dtype_code(q_new.dtype), 1.0 / (D**0.5),
-            positions, _stream(device),
+            positions, tickets, ws, nbytes, stream,
         )
+        del keep
     _lib.check(rc, "du_decode_paged")
     return out

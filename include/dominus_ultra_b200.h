@@ -298,13 +298,22 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
  * position of the newest cached token, which the query sees), out [B, Hq, D], cache_seqlens [B]
  * the cached tokens with the new one. A request of length 0 gives zeros; a length below 0, beyond
  * the table's row or beyond rope_positions gives zeros and code 6; a block id out of range
- * gives NaN and code 7.
+ * gives NaN and code 7. The requests' chunks of 128 keys are spread evenly over the GPU; fragments of
+ * a (request, KV head) that lies across CTAs meet in `workspace` (du_decode_paged_workspace_size
+ * bytes, 16-byte aligned, any contents), their CTAs count in `tickets` (DU_PAGED_TICKETS ints, zero
+ * before the first call; every call leaves them zero). Calls that may overlap on the GPU, replayed
+ * graphs among them, need tickets and a workspace each. The
+ * scales may be any positive floats (values of blocks whose value scale is below 2^-64 count as
+ * held at 2^-64).
  */
+#define DU_PAGED_TICKETS 1024
+size_t du_decode_paged_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks);
 int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                     const float* v_scale, const int* block_table, const int* cache_seqlens,
                     const void* cos, const void* sin, void* out, int B, int Hq, int Hkv, int D,
                     int num_blocks, int block_size, int max_blocks, int dtype, float scale,
-                    long long rope_positions, void* stream);
+                    long long rope_positions, int* tickets, void* workspace, size_t workspace_bytes,
+                    void* stream);
 
 /*
  * Failure-detection self-test (no counterpart in the reference): launches one CTA whose

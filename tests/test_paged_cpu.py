@@ -179,7 +179,7 @@ def test_c_abi_rejects_bad_arguments():
 
     def decode(**kw):
         a = dict(q=fake, kc=fake, vc=fake, ks=fake, vs=fake, t=fake, ln=fake, c=fake, s=fake, o=fake, B=1, Hq=4, Hkv=2,
-                 D=64, N=8, bs=16, w=4, dt=_lib.DU_DTYPE_BF16, sc=0.125, rp=64)
+                 D=64, N=8, bs=16, w=4, dt=_lib.DU_DTYPE_BF16, sc=0.125, rp=64, tk=fake, ws=fake, wsb=1 << 30)
         a.update(kw)
         return lib.du_decode_paged(*a.values(), null)
 
@@ -189,6 +189,11 @@ def test_c_abi_rejects_bad_arguments():
     assert decode(t=odd) == _lib.DU_ERR_INVALID and "4-byte" in _lib.last_error()
     assert decode(o=null) == _lib.DU_ERR_INVALID
     assert decode(D=512) == _lib.DU_ERR_UNSUPPORTED
+    assert decode(tk=null) == _lib.DU_ERR_INVALID
+    assert decode(wsb=0) == _lib.DU_ERR_WORKSPACE and decode(ws=null) == _lib.DU_ERR_WORKSPACE
+    assert decode(sc=0.0) == _lib.DU_ERR_INVALID
+    assert lib.du_decode_paged_workspace_size(1, 4, 2, 64, 16, 4) > 0
+    assert lib.du_decode_paged_workspace_size(1, 3, 2, 64, 16, 4) == 0
 
 
 class TestPlain:
