@@ -48,7 +48,7 @@ struct DecodePagedParams {
   const void* sin;
   void* out;            // [B, Hq, D]
   int* cnt;             // [gridDim.x] tickets, zero between calls
-  float* part;          // [2 gridDim.x][HPU][D + 2]: out, log2 of the sum, unused
+  float* part;          // [2 gridDim.x][HPU][D] partial outs, then [2 gridDim.x][HPU] log2 of their sums
   long long positions;
   int D, bf16;
   int B, Hq, Hkv, G, N, width;
@@ -58,7 +58,9 @@ struct DecodePagedParams {
 };
 
 // A CTA takes at least this many chunks.
-constexpr int DECODE_PAGED_MIN_PER = 2;
+constexpr int DECODE_PAGED_MIN_PER = 1;
+// The last fragment's CTA holds a weight per fragment and head where it combines rows otherwise.
+constexpr int DECODE_PAGED_MAX_CTAS = 12 * 36;
 __device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
 
 // cp.async of 4 bytes, and an arrival on `bar` once this thread's earlier cp.async have landed.
@@ -117,8 +119,10 @@ struct DecodePagedShape {
   static constexpr int CTAS = DP <= 64 ? 2 : 1;
   static constexpr int P_BYTES = CK * 128;            // [key][128 rows] bytes, 128-byte swizzle
   static constexpr int Q_BYTES = ((NQ * DP + 1023) / 1024) * 1024;
-  static constexpr int ROW = DP + 4;                  // floats per row of the combine area
-  static constexpr int MRG_BYTES = ((4 * HPU * ROW + 8 * HPU) * 4 + 127) / 128 * 128;
+  static constexpr int CB = DP == 256 ? 64 : DP;      // columns of O combined at a time
+  static constexpr int ROW = CB + 4;                  // floats per row of the combine area
+  static constexpr int MRG_O = 12 * HPU * ROW;        // [4 warps][3 HPU rows][ROW] floats
+  static constexpr int MRG_BYTES = ((MRG_O + 8 * HPU) * 4 + 127) / 128 * 128;
   static constexpr int FIXED = 2 * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2304;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
   static constexpr int NSTG_FIT = (BUDGET - FIXED) / STAGE;
@@ -142,16 +146,17 @@ struct DecodePagedShape {
   static constexpr int TMEM_COLS = TM_O + DP <= 128 ? 128 : (TM_O + DP <= 256 ? 256 : 512);
   static constexpr int NTHREADS = 224;
   static_assert(3 * HPU <= 32, "a warp's rows of P");
+  static_assert(MRG_O >= HPU * DECODE_PAGED_MAX_CTAS, "weights of the last fragment's CTA");
   static_assert(NSTG >= 2, "at least two stages");
   static_assert(SMEM_BYTES <= (CTAS == 2 ? 115712 : 232448), "shared memory budget");
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
-// The range of chunks of this CTA and where it starts, found once per CTA (shared memory).
+// The range of chunks of this CTA and where it starts, found once per CTA (shared memory). The host
+// refuses batches whose block tables could hold 2^31 chunks, so chunk numbers are ints.
 struct PagedStart {
-  long long cur, hi, per;  // chunks [cur, hi) of the flattened sequence, chunks per CTA
-  long long base;          // first chunk of request b
-  int b, pad;
+  int cur, hi, per;  // chunks [cur, hi) of the flattened sequence, chunks per CTA
+  int b, base;       // request that holds `cur`, and its first chunk
 };
 
 // One fragment, as warp 6 leaves it for the MMA and softmax warps (16 words).
@@ -167,8 +172,7 @@ struct PagedFrag {
 
 // Walks a CTA's range fragment by fragment.
 struct PagedWalk {
-  long long cur, hi, per, base;
-  int b;
+  int cur, hi, per, base, b;
   __device__ __forceinline__ void init(const PagedStart& s) {
     cur = s.cur;
     hi = s.hi;
@@ -190,17 +194,16 @@ struct PagedWalk {
     while (true) {
       n = tokens(p, b);
       nc = chunks(n);
-      const long long end = base + static_cast<long long>(nc) * ups;
+      const int end = base + nc * ups;
       if (cur < end) break;
       base = end;
       ++b;
     }
-    const long long in = cur - base;
-    unit = static_cast<int>(in / nc);
-    const long long ub = base + static_cast<long long>(unit) * nc;  // the unit's first chunk
-    const int j0 = static_cast<int>(cur - ub);
-    const long long e = min(hi, ub + nc);
-    const int j1 = static_cast<int>(e - ub);
+    unit = (cur - base) / nc;
+    const int ub = base + unit * nc;  // the unit's first chunk
+    const int j0 = cur - ub;
+    const int e = min(hi, ub + nc);
+    const int j1 = e - ub;
     const int kvh = unit / p.n_gchunk, gch = unit - kvh * p.n_gchunk;
     f.kind = 1;
     f.b = b;
@@ -210,8 +213,8 @@ struct PagedWalk {
     len = n;
     f.keys = min(n, j1 << 7) - kbeg;
     f.chunks = f.keys > 0 ? j1 - j0 : 0;
-    f.c0 = static_cast<int>(ub / per);
-    f.nf = static_cast<int>((ub + nc - 1) / per) - f.c0 + 1;
+    f.c0 = ub / per;
+    f.nf = (ub + nc - 1) / per - f.c0 + 1;
     f.slot = 2 * static_cast<int>(blockIdx.x) + (j0 > 0 ? 0 : 1);
     cur = e;
     return true;
@@ -249,14 +252,22 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
   volatile int* verdict = reinterpret_cast<volatile int*>(misc + 3);  // last of the unit's fragments
   PagedStart* start = reinterpret_cast<PagedStart*>(misc + 4);
-  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_MRG);  // o [4][HPU][ROW], m [4][HPU], l [4][HPU]
-  float* mrg_m = mrg + 4 * HPU * ROW;
+  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_MRG);  // o [4][3 HPU][ROW], m [4][HPU], l [4][HPU]
+  float* mrg_m = mrg + S::MRG_O;
   float* mrg_l = mrg_m + 4 * HPU;
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
 
+  // This CTA's range: every thread sums the chunks of a run of requests, the runs are summed over
+  // the CTA, and the thread whose run holds the range's first chunk finds the request. The first
+  // length of a run is on its way while the barriers are set up.
+  const int ups = p.Hkv * p.n_gchunk;
+  const int run = (p.B + S::NTHREADS - 1) / S::NTHREADS;
+  const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += PagedWalk::chunks(PagedWalk::tokens(p, b));
   if (tid == 128) {
     for (int s = 0; s < NSTG; ++s) {
       mbar_init(KFULL(s), 1 + 32);
@@ -284,62 +295,50 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     tmem_alloc(sbase + S::OFF_MISC, S::TMEM_COLS);
     tmem_relinquish();
   }
-  // Rows of P that are no warp's own and rows of the query tiles beyond the parts stay zero.
-  for (int i = tid; i < (2 * S::P_BYTES + 2 * S::Q_BYTES) / 16; i += S::NTHREADS)
-    st_shared_v4(sbase + S::OFF_P + 16 * i, make_uint4(0, 0, 0, 0));
-  // This CTA's range: every thread sums the chunks of a run of requests, the runs are summed over
-  // the CTA, and the thread whose run holds the range's first chunk finds the request.
   {
-    long long* wsum = reinterpret_cast<long long*>(mrg);
+    int* wsum = reinterpret_cast<int*>(mrg);
     constexpr int NW = S::NTHREADS / 32;
-    const int ups = p.Hkv * p.n_gchunk;
-    const int run = (p.B + S::NTHREADS - 1) / S::NTHREADS;
-    const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) {
-      const int n = PagedWalk::tokens(p, b);
-      if (blockIdx.x == 0 && n != p.lens[b])
-        record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
-      mine += PagedWalk::chunks(n);
-    }
     mine *= ups;
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
     if (lane == 31) wsum[warp] = incl;
     __syncthreads();
-    long long before = incl - mine, total = 0;
+    int before = incl - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const long long x = wsum[w];
+      const int x = wsum[w];
       if (w < warp) before += x;
       total += x;
     }
-    long long per = (total + gridDim.x - 1) / gridDim.x;
+    // (the host keeps total + gridDim.x below 2^31)
+    int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
     if (per < DECODE_PAGED_MIN_PER) per = DECODE_PAGED_MIN_PER;
-    const long long cur = per * blockIdx.x;
+    const int cur = min(static_cast<long long>(per) * blockIdx.x, static_cast<long long>(total));
     if (tid == 0) {
       start->cur = cur;
-      start->hi = min(total, cur + per);
+      start->hi = min(total - cur, per) + cur;
       start->per = per;
     }
-    if (cur >= before && cur < before + mine) {
-      int b = b0;
-      long long base = before;
+    if (cur >= before && cur - before < mine) {
+      int b = b0, base = before;
       while (true) {
-        const long long nb = static_cast<long long>(PagedWalk::chunks(PagedWalk::tokens(p, b))) * ups;
-        if (cur < base + nb) break;
+        const int nb = PagedWalk::chunks(PagedWalk::tokens(p, b)) * ups;
+        if (cur - base < nb) break;
         base += nb;
         ++b;
       }
       start->b = b;
       start->base = base;
     }
+    if (blockIdx.x == 0)
+      for (int b = b0; b < b1; ++b)
+        if (PagedWalk::tokens(p, b) != p.lens[b])
+          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
   }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -484,83 +483,88 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     PagedWalk walk;
     walk.init(*start);
     const int D = p.D, half = D >> 1;
-    auto at16 = [&](const void* base, long long i) -> float {
-      return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i])
-                    : __half2float(static_cast<const __half*>(base)[i]);
-    };
+    // A lane takes element pairs 2 lane + 64 e of each half. The 16-bit words of all heads are
+    // loaded before any is used, whatever their type.
+    constexpr int EPL = DP >= 128 ? DP / 128 : 1;
+    const uint32_t* q32 = static_cast<const uint32_t*>(p.q);
+    auto widen = [&](uint32_t w) -> float2 { return p.bf16 ? unpack2<true>(w) : unpack2<false>(w); };
+    // Rows of the query tiles beyond the parts stay zero.
+    for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
+      st_shared_v4(sbase + S::OFF_Q + 16 * i, make_uint4(0, 0, 0, 0));
+    __syncwarp();
     for (int it = 0;; ++it) {
       const int qb = it & 1;
       PagedFrag f;
       int unit, kbeg, len;
       const bool more = walk.next(p, f, unit, kbeg, len);
-      // (the loads go out before the wait for the entry)
-      constexpr int EPL = DP >= 64 ? DP / 64 : 1;  // element pairs per lane
-      float x1[HPU][EPL], x2[HPU][EPL];
-      if (more && f.chunks > 0) {
-        float c[EPL], sn[EPL];
+      const bool busy = more && f.chunks > 0;
+      uint32_t c[EPL], sn[EPL], xa[HPU][EPL], xb[HPU][EPL];
+      if (busy) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
-          const int d = lane + 32 * e;
-          const long long tr = static_cast<long long>(len - 1) * half + d;
-          c[e] = d < half ? at16(p.cos, tr) : 0.f;
-          sn[e] = d < half ? at16(p.sin, tr) : 0.f;
+          const int d = 2 * lane + 64 * e;
+          const bool on = d < half;
+          const long long tr = (static_cast<long long>(len - 1) * half + d) >> 1;
+          c[e] = on ? static_cast<const uint32_t*>(p.cos)[tr] : 0u;
+          sn[e] = on ? static_cast<const uint32_t*>(p.sin)[tr] : 0u;
         }
 #pragma unroll
         for (int h = 0; h < HPU; ++h)
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
-            const int d = lane + 32 * e;
-            const long long qr = (static_cast<long long>(f.b) * p.Hq + f.h0 + h) * D + d;
-            const bool on = h < f.nh && d < half;
-            const float a = on ? at16(p.q, qr) : 0.f, b = on ? at16(p.q, qr + half) : 0.f;
-            x1[h][e] = a;
-            x2[h][e] = b;
-          }
-#pragma unroll
-        for (int h = 0; h < HPU; ++h)
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            const float a = x1[h][e], b = x2[h][e];
-            x1[h][e] = a * c[e] - b * sn[e];
-            x2[h][e] = b * c[e] + a * sn[e];
+            const int d = 2 * lane + 64 * e;
+            const bool on = d < half && h < f.nh;
+            const long long qr = ((static_cast<long long>(f.b) * p.Hq + f.h0 + h) * D + d) >> 1;
+            xa[h][e] = on ? q32[qr] : 0u;
+            xb[h][e] = on ? q32[qr + (half >> 1)] : 0u;
           }
       }
       if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
-      if (more && f.chunks > 0) {
-        // Row n of the tile, element d: a swizzled K-major byte.
-        auto put = [&](int n, int d, uint32_t byte) {
-          const uint32_t o = swz_chunk_offset<SPAN>(NQ, n, d >> 4) + (d & 15);
-          sgen[S::OFF_Q + qb * S::Q_BYTES + o] = static_cast<uint8_t>(byte);
-        };
+      if (busy) {
+        uint8_t* qt = sgen + S::OFF_Q + qb * S::Q_BYTES;
 #pragma unroll
         for (int h = 0; h < HPU; ++h) {
-          uint32_t top = 0;
+          float2 y1[EPL], y2[EPL];
+          float top = 0.f;
+          bool fine = true;
 #pragma unroll
-          for (int e = 0; e < EPL; ++e)
-            top = max(top, max(__float_as_uint(x1[h][e]) & 0x7fffffffu, __float_as_uint(x2[h][e]) & 0x7fffffffu));
-          top = __reduce_max_sync(0xffffffffu, top);
-          const float u = paged_unit(top);  // a power of two: the row fits e4m3 divided by it
+          for (int e = 0; e < EPL; ++e) {
+            const float2 a = widen(xa[h][e]), b = widen(xb[h][e]), cc = widen(c[e]), ss = widen(sn[e]);
+            y1[e] = make_float2(a.x * cc.x - b.x * ss.x, a.y * cc.y - b.y * ss.y);
+            y2[e] = make_float2(b.x * cc.x + a.x * ss.x, b.y * cc.y + a.y * ss.y);
+            top = max3(top, fabsf(y1[e].x), fabsf(y1[e].y));
+            top = max3(top, fabsf(y2[e].x), fabsf(y2[e].y));
+            fine = fine && y1[e].x - y1[e].x == 0.f && y1[e].y - y1[e].y == 0.f && y2[e].x - y2[e].x == 0.f &&
+                   y2[e].y - y2[e].y == 0.f;
+          }
+          // a power of two: the row divided by it fits e4m3 (NaN for a row that is not finite)
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(top) : 0x7fc00000u);
+          const float u = paged_unit(bits);
           const float inv = 1.0f / u;
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
-            const int d = lane + 32 * e;
-            float y1 = x1[h][e] * inv, y2 = x2[h][e] * inv;
+            const int d = 2 * lane + 64 * e;
+            float2 v1 = make_float2(y1[e].x * inv, y1[e].y * inv), v2 = make_float2(y2[e].x * inv, y2[e].y * inv);
 #pragma unroll
             for (int t = 0; t < 3; ++t) {
-              const uint32_t pr = e4m3x2(y1, y2);
-              const float2 w = e4m3x2_widen(pr);
-              y1 = (y1 - w.x) * 16.0f;
-              y2 = (y2 - w.y) * 16.0f;
+              const uint32_t p1 = e4m3x2(v1.x, v1.y), p2 = e4m3x2(v2.x, v2.y);
+              const float2 w1 = e4m3x2_widen(p1), w2 = e4m3x2_widen(p2);
+              v1 = make_float2((v1.x - w1.x) * 16.0f, (v1.y - w1.y) * 16.0f);
+              v2 = make_float2((v2.x - w2.x) * 16.0f, (v2.y - w2.y) * 16.0f);
               if (d < half) {
-                put(t * HPU + h, d, pr & 0xffu);
-                put(t * HPU + h, d + half, pr >> 8);
+                // row t HPU + h of the tile: swizzled, K-major
+                const int n = t * HPU + h, d2 = d + half;
+                *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d >> 4) + (d & 15)) =
+                    static_cast<uint16_t>(p1);
+                *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d2 >> 4) + (d2 & 15)) =
+                    static_cast<uint16_t>(p2);
               }
             }
           }
           if (lane == 0) reinterpret_cast<float*>(sgen + S::OFF_QS)[qb * HPU + h] = u * p.scale_log2;
         }
-        fence_proxy_async_smem();
       }
+      fence_proxy_async_smem();
       if (lane == 0) {
         if (!more) f.kind = 0;
         *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + qb * 64) = f;
@@ -574,6 +578,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
     int g = 0, mq = 0;
+    // A key's row of P has only its warp's bytes, the rest stays zero.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      st_shared_v4(sbase + S::OFF_P + tid * 128 + 16 * i, make_uint4(0, 0, 0, 0));
+      st_shared_v4(sbase + S::OFF_P + S::P_BYTES + tid * 128 + 16 * i, make_uint4(0, 0, 0, 0));
+    }
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 830)))) break;
@@ -710,27 +720,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       if (!ok) break;
       g += f.chunks;
-      // Combine the warps: O rows 32 w + t HPU + h, parts joined by shuffles.
+      // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h through shared
+      // memory, then a thread sums the 12 of an output.
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) & 1), ((g - 1) >> 1) & 1, failed, 836)))) break;
       tc_fence_after();
-#pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += 32) {
-        float o[32];
-        tmem_ld16(tmem + lane_off + S::TM_O + c0, o);
-        tmem_ld16(tmem + lane_off + S::TM_O + c0 + 16, o + 16);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float a = __shfl_down_sync(0xffffffffu, o[i], HPU), b = __shfl_down_sync(0xffffffffu, o[i], 2 * HPU);
-          o[i] = fmaf(b, 0x1p-8f, fmaf(a, 0x1p-4f, o[i]));
-        }
-        if (lane < HPU) {
-          float4* dst = reinterpret_cast<float4*>(mrg + (warp * HPU + lane) * ROW + c0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
-      }
-      tc_fence_before();
 #pragma unroll
       for (int h = 0; h < HPU; ++h) {
         float x = l[h];
@@ -741,34 +734,53 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           mrg_l[warp * HPU + h] = x;
         }
       }
-      mbar_arrive(BAR_MRG);
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
-      ++mq;
-      for (int i = tid; i < f.nh * p.D; i += 128) {
-        const int h = i / p.D, d = i - h * p.D;
-        float M = mrg_m[h];
+      float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
+      float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
+      for (int cb = 0; cb < DP && ok; cb += S::CB) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < S::CB; c0 += 32) {
+          float o[32];
+          tmem_ld16(tmem + lane_off + S::TM_O + cb + c0, o);
+          tmem_ld16(tmem + lane_off + S::TM_O + cb + c0 + 16, o + 16);
+          tmem_wait_ld();
+          if (lane < 3 * HPU) {
+            float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW + c0);
 #pragma unroll
-        for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, mrg_m[w2 * HPU + h]);
-        float A = 0.f, L = 0.f;
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(BAR_MRG);
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
+        ++mq;
+        const int nd = min(p.D, S::CB);  // (head_dim 16: half of the columns)
+        for (int i = tid; i < f.nh * nd; i += 128) {
+          const int h = i / nd, d = i - h * nd;
+          float M = mrg_m[h];
 #pragma unroll
-        for (int w2 = 0; w2 < 4; ++w2) {
-          const float wt = ex2(mrg_m[w2 * HPU + h] - M);
-          A = fmaf(mrg[(w2 * HPU + h) * ROW + d], wt, A);
-          L = fmaf(mrg_l[w2 * HPU + h], wt, L);
+          for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, mrg_m[w2 * HPU + h]);
+          float A = 0.f, L = 0.f;
+#pragma unroll
+          for (int w2 = 0; w2 < 4; ++w2) {
+            const float wt = ex2(mrg_m[w2 * HPU + h] - M);
+            const float* r = mrg + (w2 * 3 * HPU + h) * ROW + d;
+            A = fmaf(fmaf(r[2 * HPU * ROW], 0x1p-8f, fmaf(r[HPU * ROW], 0x1p-4f, r[0])), wt, A);
+            L = fmaf(mrg_l[w2 * HPU + h], wt, L);
+          }
+          const float val = A / L;
+          if (f.nf == 1) {
+            store_out(row0 + h, cb + d, val);
+          } else {
+            part_o[h * p.D + cb + d] = val;
+            if (cb + d == 0) part_l[f.slot * HPU + h] = M + lg2(L);
+          }
         }
-        const float val = A / L;
-        if (f.nf == 1) {
-          store_out(row0 + h, d, val);
-        } else {
-          float* ps = p.part + (static_cast<long long>(f.slot) * HPU + h) * (p.D + 2);
-          ps[d] = val;
-          if (d == 0) ps[p.D] = M + lg2(L);
-        }
+        // The combine area is free again (and the partial stored) once every thread is here.
+        mbar_arrive(BAR_MRG);
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 838)))) break;
+        ++mq;
       }
-      // The combine area is free again (and the partial stored) once every thread is here.
-      mbar_arrive(BAR_MRG);
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 838)))) break;
-      ++mq;
+      if (!ok) break;
       if (f.nf > 1) {
         // A ticket on the unit's counter. The partial stores reach thread 0 through the barrier; its
         // acquire-release add makes them visible before the ticket and, after the last ticket,
@@ -783,22 +795,62 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 839)))) break;
         ++mq;
         if (*verdict) {
-          for (int i = tid; i < f.nh * p.D; i += 128) {
-            const int h = i / p.D, d = i - h * p.D;
-            float M = -INFINITY, A = 0.f, L = 0.f;
-#pragma unroll 4
-            for (int k = 0; k < f.nf; ++k) {
-              const long long sl = k == 0 ? 2LL * f.c0 + 1 : 2LL * (f.c0 + k);
-              const float* ps = p.part + (sl * HPU + h) * (p.D + 2);
-              const float x = __ldcg(ps + p.D), o = __ldcg(ps + d);
-              const float mn = fmaxf(M, x);
-              const float a = M == -INFINITY ? 0.f : ex2(M - mn), b = ex2(x - mn);
-              A = fmaf(A, a, o * b);
-              L = fmaf(L, a, b);
-              M = mn;
+          // The unit's other fragments are done: their sums' weights first, a warp per head and a
+          // lane per fragment, then the outputs, four columns per thread, eight loads in flight.
+          auto slot_of = [&](int k) { return k == 0 ? 2 * f.c0 + 1 : 2 * (f.c0 + k); };
+          float* wt = mrg;  // [HPU][nf]: nf <= gridDim.x <= DECODE_PAGED_MAX_CTAS
+          for (int h = warp; h < f.nh; h += 4) {
+            float M = -INFINITY, L = 0.f;
+            for (int k = lane; k < f.nf; k += 32) {
+              const float x = __ldcg(part_l + slot_of(k) * HPU + h);
+              wt[h * f.nf + k] = x;
+              M = fmaxf(M, x);
             }
-            store_out(row0 + h, d, A / L);
+            M = warp_max(M);
+            for (int k = lane; k < f.nf; k += 32) {
+              const float e = ex2(wt[h * f.nf + k] - M);
+              wt[h * f.nf + k] = e;
+              L += e;
+            }
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            const float inv = 1.0f / L;
+            for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
           }
+          mbar_arrive(BAR_MRG);
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 840)))) break;
+          ++mq;
+          const int q4 = p.D >> 2;
+          for (int i = tid; i < f.nh * q4; i += 128) {
+            const int h = i / q4, d = 4 * (i - h * q4);
+            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int k0 = 0; k0 < f.nf; k0 += 8) {
+              float4 o[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                o[k] = k0 + k < f.nf
+                           ? __ldcg(reinterpret_cast<const float4*>(
+                                 p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float x = k0 + k < f.nf ? wt[h * f.nf + k0 + k] : 0.f;
+                A.x = fmaf(o[k].x, x, A.x);
+                A.y = fmaf(o[k].y, x, A.y);
+                A.z = fmaf(o[k].z, x, A.z);
+                A.w = fmaf(o[k].w, x, A.w);
+              }
+            }
+            store_out(row0 + h, d, A.x);
+            store_out(row0 + h, d + 1, A.y);
+            store_out(row0 + h, d + 2, A.z);
+            store_out(row0 + h, d + 3, A.w);
+          }
+          // The weights are read: the combine area is free again.
+          mbar_arrive(BAR_MRG);
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 841)))) break;
+          ++mq;
         }
       } else if (tid == 0) {
         *emitted = it + 1;
@@ -824,9 +876,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(nan);
         else static_cast<__half*>(p.out)[o] = __float2half_rn(nan);
         if (f.nf > 1) {
-          float* ps = p.part + (static_cast<long long>(f.slot) * HPU + h) * (p.D + 2);
-          ps[d] = nan;
-          if (d == 0) ps[p.D] = nan;
+          p.part[(static_cast<long long>(f.slot) * HPU + h) * p.D + d] = nan;
+          if (d == 0) p.part[2LL * gridDim.x * HPU * p.D + f.slot * HPU + h] = nan;
         }
       }
       __threadfence();

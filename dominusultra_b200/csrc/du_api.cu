@@ -1313,7 +1313,8 @@ int paged_hpu(int heads) { return heads <= 1 ? 1 : (heads <= 2 ? 2 : (heads <= 4
 
 // CTAs of the persistent grid: the resident ones, or as many as a full block table could occupy.
 int paged_grid(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
-  const long long ctas = static_cast<long long>(sm_count()) * (D <= 64 ? 2 : 1);
+  long long ctas = static_cast<long long>(sm_count()) * (D <= 64 ? 2 : 1);
+  if (ctas > du::DECODE_PAGED_MAX_CTAS) ctas = du::DECODE_PAGED_MAX_CTAS;
   const long long units = static_cast<long long>(B) * Hkv * paged_group_chunks(Hq / Hkv);
   const long long per_unit = (static_cast<long long>(max_blocks) * block_size + 127) / 128;
   const long long most = (units * per_unit + du::DECODE_PAGED_MIN_PER - 1) / du::DECODE_PAGED_MIN_PER;
@@ -1321,7 +1322,7 @@ int paged_grid(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
 }
 
 size_t paged_ws_bytes(int grid, int Hq, int Hkv, int D) {
-  return 2 * static_cast<size_t>(grid) * paged_hpu(paged_unit_heads(Hq / Hkv)) * (D + 2) * sizeof(float);
+  return 2 * static_cast<size_t>(grid) * paged_hpu(paged_unit_heads(Hq / Hkv)) * (D + 1) * sizeof(float);
 }
 
 // 3-D map over a paged cache [cells, block, D] of bytes (a cell: one block of one KV head): box
@@ -1507,8 +1508,11 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
     return fail(DU_ERR_INVALID, "scales, block_table, cache_seqlens and tickets must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
+  if (static_cast<double>(B) * Hkv * paged_group_chunks(Hq / Hkv) *
+          ((static_cast<long long>(max_blocks) * block_size + 127) / 128) > 2147480000.0)
+    return fail(DU_ERR_UNSUPPORTED, "the block tables can hold 2^31 chunks of 128 keys or more");
   const int grid = paged_grid(B, Hq, Hkv, D, block_size, max_blocks);
-  if (grid > DU_PAGED_TICKETS) return fail(DU_ERR_UNSUPPORTED, "more resident blocks of threads than tickets");
+  static_assert(du::DECODE_PAGED_MAX_CTAS <= DU_PAGED_TICKETS, "a ticket for each block of threads");
   if (!workspace || workspace_bytes < paged_ws_bytes(grid, Hq, Hkv, D) || !aligned16(workspace))
     return fail(DU_ERR_WORKSPACE, "workspace missing, misaligned or smaller than du_decode_paged_workspace_size");
   du::DecodePagedParams prm{};
