@@ -30,8 +30,10 @@
 // the device; every CTA repeats the sum over them. A unit within one CTA is written at once; the
 // fragments of others leave fp32 partials, and the CTA that leaves the last one joins them.
 //
-// Warps: 0-3 softmax, combine and output; 4 TMA (K, V and scales of each chunk); 5 TMEM and MMA;
-// 6 walks the fragments and prepares their query parts, one fragment ahead. Every wait is bounded.
+// Warps: 0-3 softmax, combine and output; 4 TMA of K, and the scales; 7 TMA of V (a block of 16 tokens
+// is a copy of 2 KB, and one warp issues a copy in about 100 clocks: half an SM's share of the
+// bandwidth); 5 TMEM and MMA; 6 walks the fragments and prepares their query parts, ahead of the
+// others. Every wait is bounded.
 #pragma once
 
 #include "paged_sm100.cuh"
@@ -57,8 +59,9 @@ struct DecodePagedParams {
   float scale_log2;
 };
 
-// A CTA takes at least this many chunks.
-constexpr int DECODE_PAGED_MIN_PER = 1;
+// Chunks per CTA that whole pieces of units may cost over equal ranges of chunks: a CTA whose range
+// straddles two units combines twice, about three chunks' time.
+constexpr int DECODE_PAGED_PIECE_SLACK = 3;
 // The last fragment's CTA holds a weight per fragment and head where it combines rows otherwise.
 constexpr int DECODE_PAGED_MAX_CTAS = 12 * 36;
 __device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
@@ -123,7 +126,7 @@ struct DecodePagedShape {
   static constexpr int ROW = CB + 4;                  // floats per row of the combine area
   static constexpr int MRG_O = 12 * HPU * ROW;        // [4 warps][3 HPU rows][ROW] floats
   static constexpr int MRG_BYTES = ((MRG_O + 8 * HPU) * 4 + 127) / 128 * 128;
-  static constexpr int FIXED = 2 * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2304;
+  static constexpr int FIXED = 2 * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2560;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
   static constexpr int NSTG_FIT = (BUDGET - FIXED) / STAGE;
   static constexpr int NSTG = NSTG_FIT > 8 ? 8 : NSTG_FIT;
@@ -131,20 +134,24 @@ struct DecodePagedShape {
   static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
   static constexpr int OFF_MRG = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_SC = OFF_MRG + MRG_BYTES;  // [NSTG][2][8] scales of a chunk's blocks
-  static constexpr int OFF_FRAG = OFF_SC + NSTG * 64; // [2] fragment entries of 16 words
-  static constexpr int OFF_QS = OFF_FRAG + 2 * 64;    // [2][HPU] score factor of each head
+  static constexpr int NF = 4;                        // fragment entries in flight
+  static constexpr int OFF_FRAG = OFF_SC + NSTG * 64; // [NF] entries of 16 words
+  static constexpr int OFF_QS = OFF_FRAG + NF * 64;   // [2][HPU] score factor of each head
   static constexpr int OFF_BAR = OFF_QS + 2 * 32;
   static constexpr int B_KFULL = 0, B_KEMPTY = NSTG, B_VFULL = 2 * NSTG, B_VEMPTY = 3 * NSTG,
                        B_QFULL = 4 * NSTG, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
                        B_SEMPTY = B_QFULL + 6, B_PFULL = B_QFULL + 8, B_PDONE = B_QFULL + 10,
-                       B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13;
-  static constexpr int N_BAR = B_DRAIN + 1;
+                       B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13, B_FREE = B_QFULL + 14,
+                       B_TKT = B_QFULL + 15, B_FFULL = B_QFULL + 16,
+                       B_FEMPTY = B_FFULL + NF;
+  static constexpr int N_BAR = B_FEMPTY + NF;
   static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;  // 16 words
   static constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
   static constexpr int TM_S = 0;           // S^T: two buffers of NQ columns
   static constexpr int TM_O = 64;          // O: DP columns
   static constexpr int TMEM_COLS = TM_O + DP <= 128 ? 128 : (TM_O + DP <= 256 ? 256 : 512);
-  static constexpr int NTHREADS = 224;
+  static constexpr int NTHREADS = 256;
+  static constexpr int PEN = 2;            // chunks that a unit's beginning is charged with
   static_assert(3 * HPU <= 32, "a warp's rows of P");
   static_assert(MRG_O >= HPU * DECODE_PAGED_MAX_CTAS, "weights of the last fragment's CTA");
   static_assert(NSTG >= 2, "at least two stages");
@@ -152,11 +159,26 @@ struct DecodePagedShape {
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
-// The range of chunks of this CTA and where it starts, found once per CTA (shared memory). The host
-// refuses batches whose block tables could hold 2^31 chunks, so chunk numbers are ints.
+// x / y for a quotient below 2^20 (x >= 0, y > 0): a float estimate, off by one at most, and a step.
+__device__ __forceinline__ int small_div(int x, int y) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
+  const int r = x - q * y;
+  return q + (r >= y) - (r < 0);
+}
+
+// This CTA's share of the flattened chunks, found by one warp. The host refuses batches whose block
+// tables could hold 2^31 chunks, so chunk numbers are ints.
+//
+// Two plans. pieces > 0: every unit is cut into equal pieces, as many as give no CTA more than one,
+// and this CTA has piece `cur` of request b's units (numbered through them), if cur < hi. Else the
+// CTA has the chunks [cur, hi), which may begin and end inside a unit; request b holds `cur` and
+// starts at chunk `base`; `per` chunks per CTA. There a unit's chunks are preceded by PEN positions
+// that hold none: the price, in chunks, of beginning a fragment and combining its rows, so that CTAs
+// with many short units get fewer chunks.
 struct PagedStart {
-  int cur, hi, per;  // chunks [cur, hi) of the flattened sequence, chunks per CTA
-  int b, base;       // request that holds `cur`, and its first chunk
+  int cur, hi, per;
+  int b, base;
+  int pieces;
 };
 
 // One fragment, as warp 6 leaves it for the MMA and softmax warps (16 words).
@@ -167,56 +189,152 @@ struct PagedFrag {
   int keys;       // keys of the fragment
   int nf, c0;     // fragments of the unit, CTA of the first
   int slot;       // partial slot when nf > 1
-  int pad[7];
+  int kvh, kbeg;  // KV head, first token
+  int len;        // the request's tokens
+  int pad[4];
 };
 
-// Walks a CTA's range fragment by fragment.
+// Walks a CTA's share fragment by fragment.
+template <int PEN>
 struct PagedWalk {
-  int cur, hi, per, base, b;
+  int cur, hi, per, base, b, pieces;
   __device__ __forceinline__ void init(const PagedStart& s) {
     cur = s.cur;
     hi = s.hi;
     per = s.per;
     base = s.base;
     b = s.b;
+    pieces = s.pieces;
   }
   __device__ __forceinline__ static int tokens(const DecodePagedParams& p, int b) {
     const int n = p.lens[b];
     return (n < 0 || n > p.width * p.block || n > p.positions) ? 0 : n;
   }
   __device__ __forceinline__ static int chunks(int n) { return n > 128 ? (n + 127) >> 7 : 1; }
-  // unit: KV head * n_gchunk + group; [kbeg, kend) tokens.
-  __device__ __forceinline__ bool next(const DecodePagedParams& p, PagedFrag& f, int& unit, int& kbeg,
-                                       int& len) {
-    if (cur >= hi) return false;
+  // The CTA's share (a whole warp; `lane` its lane).
+  __device__ __forceinline__ static PagedStart find(const DecodePagedParams& p, int lane) {
+    PagedStart st;
     const int ups = p.Hkv * p.n_gchunk;
-    int n, nc;
-    while (true) {
+    const int grid = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
+    int total = 0;
+#pragma unroll 4
+    for (int b = lane; b < p.B; b += 32) {
+      const int n = tokens(p, b);
+      if (c == 0 && n != p.lens[b]) record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
+      total += chunks(n);
+    }
+    total = static_cast<int>(__reduce_add_sync(0xffffffffu, total));
+    // Pieces: with at most x chunks each, the units of request b make ups ceil(chunks_b / x) of
+    // them. x = per .. per + 3 are tried; beyond that, fragments of equal ranges cost less.
+    bool cut = false;
+    int x = 0;
+    if (p.B * static_cast<long long>(ups) <= grid) {
+      const int per = (total * ups + grid - 1) / grid;
+      int sum[DECODE_PAGED_PIECE_SLACK + 1] = {};
+      for (int b = lane; b < p.B; b += 32) {
+        const int nc = chunks(tokens(p, b));
+#pragma unroll
+        for (int i = 0; i <= DECODE_PAGED_PIECE_SLACK; ++i) sum[i] += small_div(nc + per + i - 1, per + i);
+      }
+#pragma unroll
+      for (int i = DECODE_PAGED_PIECE_SLACK; i >= 0; --i)
+        if (static_cast<int>(__reduce_add_sync(0xffffffffu, sum[i])) * ups <= grid) {
+          cut = true;
+          x = per + i;
+        }
+    }
+    int cur, hi;
+    if (cut) {
+      cur = c;
+      hi = c + 1;
+    } else {
+      total = (total + p.B * PEN) * ups;  // (the host keeps total + gridDim.x below 2^31)
+      x = (total + grid - 1) / grid;
+      cur = static_cast<int>(min(static_cast<long long>(x) * c, static_cast<long long>(total)));
+      hi = min(total - cur, x) + cur;
+    }
+    st.per = x;
+    st.cur = st.hi = st.b = st.base = st.pieces = 0;  // no share
+    // The request that holds `cur`.
+    int before = 0;
+    for (int b0 = 0; b0 < p.B && cur < hi; b0 += 32) {
+      const int b = b0 + lane;
+      int k = 0;
+      if (b < p.B) {
+        const int nc = chunks(tokens(p, b));
+        k = cut ? small_div(nc + x - 1, x) : nc + PEN;
+      }
+      int in = k;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, in, o);
+        if (lane >= o) in += t;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, cur < before + in * ups);
+      if (hit) {
+        const int l = __ffs(static_cast<int>(hit)) - 1;
+        k = __shfl_sync(0xffffffffu, k, l);
+        in = __shfl_sync(0xffffffffu, in, l);
+        st.b = b0 + l;
+        st.base = before + (in - k) * ups;
+        st.cur = cut ? cur - st.base : cur;
+        st.hi = cut ? k * ups : hi;
+        st.pieces = cut ? k : 0;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, in, 31) * ups;
+    }
+    return st;
+  }
+  __device__ __forceinline__ bool next(const DecodePagedParams& p, PagedFrag& f) {
+    int n, nc, unit, j0, j1;
+    if (pieces > 0) {
+      if (cur >= hi) return false;
       n = tokens(p, b);
       nc = chunks(n);
-      const int end = base + nc * ups;
-      if (cur < end) break;
-      base = end;
-      ++b;
+      unit = small_div(cur, pieces);
+      const int piece = cur - unit * pieces;
+      const int q = nc / pieces, r = nc - q * pieces;  // the first r pieces hold a chunk more
+      j0 = piece * q + min(piece, r);
+      j1 = j0 + q + (piece < r);
+      f.c0 = static_cast<int>(blockIdx.x) - piece;
+      f.nf = pieces;
+      cur = hi;
+    } else {
+      const int ups = p.Hkv * p.n_gchunk;
+      do {
+        if (cur >= hi) return false;
+        n = tokens(p, b);
+        nc = chunks(n);
+        const int span = nc + PEN;
+        if (cur - base >= span * ups) {
+          base += span * ups;
+          ++b;
+          j1 = 0;
+          continue;
+        }
+        unit = small_div(cur - base, span);
+        const int ub = base + unit * span + PEN;  // the unit's first chunk
+        const int e = min(hi, ub + nc);
+        j0 = max(cur - ub, 0);
+        j1 = e - ub;
+        f.c0 = small_div(ub, per);
+        f.nf = small_div(ub + nc - 1, per) - f.c0 + 1;
+        cur = e;
+      } while (j1 <= 0);  // (a range that ends before the unit's first chunk)
     }
-    unit = (cur - base) / nc;
-    const int ub = base + unit * nc;  // the unit's first chunk
-    const int j0 = cur - ub;
-    const int e = min(hi, ub + nc);
-    const int j1 = e - ub;
-    const int kvh = unit / p.n_gchunk, gch = unit - kvh * p.n_gchunk;
+    const int kvh = p.n_gchunk == 1 ? unit : small_div(unit, p.n_gchunk);
+    const int gch = unit - kvh * p.n_gchunk;
     f.kind = 1;
     f.b = b;
     f.h0 = kvh * p.G + gch * p.heads;
     f.nh = min(p.heads, p.G - gch * p.heads);
-    kbeg = j0 << 7;
-    len = n;
-    f.keys = min(n, j1 << 7) - kbeg;
+    f.kvh = kvh;
+    f.kbeg = j0 << 7;
+    f.len = n;
+    f.keys = min(n, j1 << 7) - f.kbeg;
     f.chunks = f.keys > 0 ? j1 - j0 : 0;
-    f.c0 = ub / per;
-    f.nf = (ub + nc - 1) / per - f.c0 + 1;
     f.slot = 2 * static_cast<int>(blockIdx.x) + (j0 > 0 ? 0 : 1);
-    cur = e;
     return true;
   }
 };
@@ -226,6 +344,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const DecodePagedParams p) {
   using S = DecodePagedShape<DP, HPU>;
+  using Walk = PagedWalk<S::PEN>;
   constexpr int CK = S::CK, SPAN = S::SPAN, NSTG = S::NSTG, NQ = S::NQ, ROW = S::ROW;
   constexpr uint32_t SWZ = swizzle_code(SPAN);
   constexpr uint32_t IDESC_QK = idesc_f16(128, NQ, 0, 0, 0, 0);  // (format 0 of kind::f8f6f4: e4m3)
@@ -240,13 +359,16 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   auto KEMPTY = [&](int s) { return bar(S::B_KEMPTY + s); };  // QK read K, each softmax warp its scales
   auto VFULL = [&](int s) { return bar(S::B_VFULL + s); };
   auto VEMPTY = [&](int s) { return bar(S::B_VEMPTY + s); };  // PV read V
-  auto QFULL = [&](int i) { return bar(S::B_QFULL + i); };    // fragment entry and query parts written
-  auto QEMPTY = [&](int i) { return bar(S::B_QEMPTY + i); };  // last QK issued and done, entry read
+  auto FFULL = [&](int i) { return bar(S::B_FFULL + i); };    // fragment entry written
+  auto FEMPTY = [&](int i) { return bar(S::B_FEMPTY + i); };  // read by each warp but the walker
+  auto QFULL = [&](int i) { return bar(S::B_QFULL + i); };    // query parts written
+  auto QEMPTY = [&](int i) { return bar(S::B_QEMPTY + i); };  // the fragment's QK done, factors read
   auto SFULL = [&](int i) { return bar(S::B_SFULL + i); };
   auto SEMPTY = [&](int i) { return bar(S::B_SEMPTY + i); };
   auto PFULL = [&](int i) { return bar(S::B_PFULL + i); };
   auto PDONE = [&](int i) { return bar(S::B_PDONE + i); };    // PV of even / odd chunks complete
-  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_DRAIN = bar(S::B_DRAIN);
+  // rows of O in the combine area, rows read (and partials stored), ticket taken
+  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_FREE = bar(S::B_FREE), BAR_TKT = bar(S::B_TKT), BAR_DRAIN = bar(S::B_DRAIN);
   uint32_t* misc = reinterpret_cast<uint32_t*>(sgen + S::OFF_MISC);
   volatile int* failed = reinterpret_cast<volatile int*>(misc + 1);
   volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
@@ -260,14 +382,6 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   const int warp = tid >> 5;
   const int lane = tid & 31;
 
-  // This CTA's range: every thread sums the chunks of a run of requests, the runs are summed over
-  // the CTA, and the thread whose run holds the range's first chunk finds the request. The first
-  // length of a run is on its way while the barriers are set up.
-  const int ups = p.Hkv * p.n_gchunk;
-  const int run = (p.B + S::NTHREADS - 1) / S::NTHREADS;
-  const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += PagedWalk::chunks(PagedWalk::tokens(p, b));
   if (tid == 128) {
     for (int s = 0; s < NSTG; ++s) {
       mbar_init(KFULL(s), 1 + 32);
@@ -283,7 +397,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       mbar_init(PFULL(i), 128);
       mbar_init(PDONE(i), 1);
     }
+    for (int i = 0; i < S::NF; ++i) {
+      mbar_init(FFULL(i), 1);
+      mbar_init(FEMPTY(i), 7);
+    }
     mbar_init(BAR_MRG, 128);
+    mbar_init(BAR_FREE, 128);
+    mbar_init(BAR_TKT, 128);
     mbar_init(BAR_DRAIN, 1);
     *failed = 0;
     *emitted = 0;
@@ -292,126 +412,74 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     tma_prefetch_desc(&tm_v);
   }
   if (warp == 5) {
+    // (Only a predecessor whose CTAs all run or have ended lets this grid start early, and none of
+    // them takes TMEM after that: the columns taken here starve nothing.)
     tmem_alloc(sbase + S::OFF_MISC, S::TMEM_COLS);
     tmem_relinquish();
   }
-  {
-    int* wsum = reinterpret_cast<int*>(mrg);
-    constexpr int NW = S::NTHREADS / 32;
-    mine *= ups;
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
-    }
-    if (lane == 31) wsum[warp] = incl;
-    __syncthreads();
-    int before = incl - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const int x = wsum[w];
-      if (w < warp) before += x;
-      total += x;
-    }
-    // (the host keeps total + gridDim.x below 2^31)
-    int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-    if (per < DECODE_PAGED_MIN_PER) per = DECODE_PAGED_MIN_PER;
-    const int cur = min(static_cast<long long>(per) * blockIdx.x, static_cast<long long>(total));
-    if (tid == 0) {
-      start->cur = cur;
-      start->hi = min(total - cur, per) + cur;
-      start->per = per;
-    }
-    if (cur >= before && cur - before < mine) {
-      int b = b0, base = before;
-      while (true) {
-        const int nb = PagedWalk::chunks(PagedWalk::tokens(p, b)) * ups;
-        if (cur - base < nb) break;
-        base += nb;
-        ++b;
-      }
-      start->b = b;
-      start->base = base;
-    }
-    if (blockIdx.x == 0)
-      for (int b = b0; b < b1; ++b)
-        if (PagedWalk::tokens(p, b) != p.lens[b])
-          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
-  }
+  // Launched as a programmatic dependent: what is above runs beside the stream's previous kernel.
+  griddep_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(misc);
 
-  if (warp == 4) {
-    // ------------------------------------------------------------------ TMA: K, V, scales
-    PagedWalk walk;
-    walk.init(*start);
-    PagedFrag f;
-    int unit, kbeg, len, g = 0;
+  if (warp == 4 || warp == 7) {
+    // ------------------------------------------------------------------ TMA: K and scales, V
+    const bool is_k = warp == 4;
+    const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
+    const uint32_t tile = is_k ? 0u : static_cast<uint32_t>(S::TILE);
+    const int ppc = CK >> p.block_log2;  // blocks of a whole chunk: 1, 2, 4, 8
+    int g = 0;
     bool ok = true;
-    while (ok && walk.next(p, f, unit, kbeg, len)) {
-      const int kvh = unit / p.n_gchunk;
-      const int* row = p.table + static_cast<long long>(f.b) * p.width;
-      const int page0 = kbeg >> p.block_log2;
+    for (int it = 0; ok; ++it) {
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 800)))) break;
+      const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
+      __syncwarp();
+      if (f.kind == 0) break;
+      if (lane == 0) mbar_arrive(FEMPTY(it % S::NF));
+      const int* row = p.table + static_cast<long long>(f.b) * p.width + (f.kbeg >> p.block_log2);
       const int pages = (f.keys + p.block - 1) >> p.block_log2;  // of the fragment
-      const int ppc = CK >> p.block_log2;                        // per whole chunk: 1, 2, 4, 8
       // Lane l holds the ids of blocks at + l and, loaded ahead, at + 32 + l.
-      int id = lane < pages ? row[page0 + lane] : 0;
-      int id_next = lane + 32 < pages ? row[page0 + 32 + lane] : 0;
+      int id = lane < pages ? row[lane] : 0;
+      int id_next = lane + 32 < pages ? row[32 + lane] : 0;
       int at = 0;
       for (int j = 0; j < f.chunks; ++j, ++g) {
         const int first = j * ppc;
         if (first >= at + 32) {
           at += 32;
           id = id_next;
-          id_next = at + 32 + lane < pages ? row[page0 + at + 32 + lane] : 0;
+          id_next = at + 32 + lane < pages ? row[at + 32 + lane] : 0;
         }
         const int here = min(ppc, pages - first);
         const int s = g % NSTG;
-        const uint32_t st = sbase + s * S::STAGE;
-        int mine = __shfl_sync(0xffffffffu, id, (first - at) + (lane & 7));
+        const uint32_t st = sbase + s * S::STAGE + tile;
+        const uint32_t full = is_k ? KFULL(s) : VFULL(s);
+        const int mine = __shfl_sync(0xffffffffu, id, (first - at) + (lane & 7));
         const bool in = (lane & 7) < here;
         const bool bad = in && (mine < 0 || mine >= p.N);
-        if (bad && lane < 8) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(mine));
+        if (bad && is_k && lane < 8) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(mine));
         const long long cell = bad ? static_cast<long long>(p.N) * p.Hkv  // beyond the map: zeros
-                                   : static_cast<long long>(mine) * p.Hkv + kvh;
-        if (g >= NSTG) ok = mbar_wait(KEMPTY(s), ((g / NSTG) - 1) & 1, failed, 800);
+                                   : static_cast<long long>(mine) * p.Hkv + f.kvh;
+        if (g >= NSTG) ok = mbar_wait(is_k ? KEMPTY(s) : VEMPTY(s), ((g / NSTG) - 1) & 1, failed, 801);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        const uint32_t bytes = static_cast<uint32_t>(here << p.block_log2) * DP;
-        if (lane == 0) mbar_expect_tx(KFULL(s), bytes);
+        if (lane == 0) mbar_expect_tx(full, static_cast<uint32_t>(here << p.block_log2) * DP);
         __syncwarp();
-        if (in && lane < 16) {
-          const float* src = (lane < 8 ? p.ks : p.vs) + cell;
-          cp_async4(sbase + S::OFF_SC + s * 64 + lane * 4, bad ? &g_du_paged_nan : src);
-        }
-        cp_async_arrive(KFULL(s));
         if (in && lane < 8)
 #pragma unroll
           for (int nb = 0; nb < S::NBLK; ++nb)
-            tma_load_3d(st + nb * CK * SPAN + (lane << p.block_log2) * SPAN, &tm_k, KFULL(s), nb * SPAN, 0,
+            tma_load_3d(st + nb * CK * SPAN + (lane << p.block_log2) * SPAN, tm, full, nb * SPAN, 0,
                         static_cast<int>(cell));
-        if (g >= NSTG) ok = mbar_wait(VEMPTY(s), ((g / NSTG) - 1) & 1, failed, 801);
-        if (!(ok = __all_sync(0xffffffffu, ok))) {
-          ++g;
-          break;
+        if (is_k) {
+          if (in && lane < 16)
+            cp_async4(sbase + S::OFF_SC + s * 64 + lane * 4, bad ? &g_du_paged_nan : (lane < 8 ? p.ks : p.vs) + cell);
+          cp_async_arrive(full);
         }
-        if (lane == 0) mbar_expect_tx(VFULL(s), bytes);
-        __syncwarp();
-        if (in && lane < 8)
-#pragma unroll
-          for (int nb = 0; nb < S::NBLK; ++nb)
-            tma_load_3d(st + S::TILE + nb * CK * SPAN + (lane << p.block_log2) * SPAN, &tm_v, VFULL(s), nb * SPAN,
-                        0, static_cast<int>(cell));
       }
     }
-    // The last copies land before the CTA may exit. (After a failed wait a stage's V may never
-    // have been issued: that wait runs into its own limit.)
-    for (int j = g > NSTG ? g - NSTG : 0; j < g; ++j) {
-      mbar_wait_drain(KFULL(j % NSTG), (j / NSTG) & 1, 802);
-      mbar_wait_drain(VFULL(j % NSTG), (j / NSTG) & 1, 803);
-    }
+    // The last copies land before the CTA may exit.
+    for (int j = g > NSTG ? g - NSTG : 0; j < g; ++j)
+      mbar_wait_drain(is_k ? KFULL(j % NSTG) : VFULL(j % NSTG), (j / NSTG) & 1, 802);
   } else if (warp == 5) {
     // ------------------------------------------------------------------ MMA issuer
     const bool leader = elect_one();
@@ -419,10 +487,16 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     int g = 0;
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 810)))) break;
-      const PagedFrag* f = reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + qb * 64);
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 810)))) break;
+      const PagedFrag* f = reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       const int kind = f->kind, n = f->chunks;
+      __syncwarp();
       if (kind == 0) break;
+      if (leader) mbar_arrive(FEMPTY(it % S::NF));
+      __syncwarp();
+      // (also without chunks: the queries of entry it are prepared once QEMPTY of entry it - 2 is
+      // complete, so this warp's arrivals stay in their phases)
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 816)))) break;
       if (n == 0) {
         if (leader) mbar_arrive(QEMPTY(qb));
         __syncwarp();
@@ -480,8 +554,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     __syncwarp();
   } else if (warp == 6) {
     // ------------------------------------------------------------------ fragments and queries
-    PagedWalk walk;
-    walk.init(*start);
+    Walk walk;
+    {
+      const PagedStart st = Walk::find(p, lane);
+      if (lane == 0) *start = st;
+      walk.init(st);
+    }
     const int D = p.D, half = D >> 1;
     // A lane takes element pairs 2 lane + 64 e of each half. The 16-bit words of all heads are
     // loaded before any is used, whatever their type.
@@ -492,19 +570,34 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
       st_shared_v4(sbase + S::OFF_Q + 16 * i, make_uint4(0, 0, 0, 0));
     __syncwarp();
-    for (int it = 0;; ++it) {
-      const int qb = it & 1;
-      PagedFrag f;
-      int unit, kbeg, len;
-      const bool more = walk.next(p, f, unit, kbeg, len);
-      const bool busy = more && f.chunks > 0;
+    // Entry k is published before the queries of entry k - 1 are prepared.
+    bool ended = false;
+    for (int k = 0;; ++k) {
+      if (!ended) {
+        PagedFrag f;
+        ended = !walk.next(p, f);
+        if (ended) f.kind = 0;
+        const int e = k % S::NF;
+        if (k >= S::NF && !__all_sync(0xffffffffu, mbar_wait(FEMPTY(e), ((k / S::NF) - 1) & 1, failed, 821))) break;
+        if (lane == 0) {
+          *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + e * 64) = f;
+          mbar_arrive(FFULL(e));
+        }
+        __syncwarp();
+      }
+      if (k == 0) continue;
+      const int it = k - 1, qb = it & 1;
+      // (entry k - 1 stays until the softmax warps have read it, which wait for its queries)
+      const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
+      if (f.kind == 0) break;
+      const bool busy = f.chunks > 0;
       uint32_t c[EPL], sn[EPL], xa[HPU][EPL], xb[HPU][EPL];
       if (busy) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
           const int d = 2 * lane + 64 * e;
           const bool on = d < half;
-          const long long tr = (static_cast<long long>(len - 1) * half + d) >> 1;
+          const long long tr = (static_cast<long long>(f.len - 1) * half + d) >> 1;
           c[e] = on ? static_cast<const uint32_t*>(p.cos)[tr] : 0u;
           sn[e] = on ? static_cast<const uint32_t*>(p.sin)[tr] : 0u;
         }
@@ -565,19 +658,14 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
       }
       fence_proxy_async_smem();
-      if (lane == 0) {
-        if (!more) f.kind = 0;
-        *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + qb * 64) = f;
-      }
       __syncwarp();
       mbar_arrive(QFULL(qb));
-      if (!more) break;
     }
   } else {
     // ------------------------------------------------------------------ warps 0-3: softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
-    int g = 0, mq = 0;
+    int g = 0, mq = 0, tq = 0;  // chunks, combined column blocks, ticket barriers
     // A key's row of P has only its warp's bytes, the rest stays zero.
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -586,14 +674,18 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     }
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
+      const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
+      if (f.kind == 0) break;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 830)))) break;
-      const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + qb * 64);
       float qs[HPU];
 #pragma unroll
       for (int h = 0; h < HPU; ++h) qs[h] = reinterpret_cast<const float*>(sgen + S::OFF_QS)[qb * HPU + h];
       __syncwarp();
-      if (f.kind == 0) break;
-      if (lane == 0) mbar_arrive(QEMPTY(qb));
+      if (lane == 0) {
+        mbar_arrive(QEMPTY(qb));
+        mbar_arrive(FEMPTY(it % S::NF));
+      }
       auto store_out = [&](long long row, int d, float val) {
         if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[row * p.D + d] = __float2bfloat16_rn(val);
         else static_cast<__half*>(p.out)[row * p.D + d] = __float2half_rn(val);
@@ -720,64 +812,97 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       if (!ok) break;
       g += f.chunks;
+      // Sums of the weights: the lanes' sums of HPU heads, halving the heads with the lanes.
+      {
+        int n = HPU;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+          if (n > 1) {
+            n >>= 1;
+#pragma unroll
+            for (int h = 0; h < HPU / 2; ++h)
+              if (h < n) {
+                const float send = (lane & o) ? l[h] : l[h + n], keep = (lane & o) ? l[h + n] : l[h];
+                l[h] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+              }
+          } else {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+          }
+        }
+      }
       // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h through shared
       // memory, then a thread sums the 12 of an output.
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) & 1), ((g - 1) >> 1) & 1, failed, 836)))) break;
       tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < HPU; ++h) {
-        float x = l[h];
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (lane == 0) {
-          mrg_m[warp * HPU + h] = m[h];
-          mrg_l[warp * HPU + h] = x;
-        }
-      }
       float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
       float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
       for (int cb = 0; cb < DP && ok; cb += S::CB) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < S::CB; c0 += 32) {
-          float o[32];
-          tmem_ld16(tmem + lane_off + S::TM_O + cb + c0, o);
-          tmem_ld16(tmem + lane_off + S::TM_O + cb + c0 + 16, o + 16);
+        {
+          float o[S::CB];
+#pragma unroll
+          for (int c = 0; c < S::CB; c += 16) tmem_ld16(tmem + lane_off + S::TM_O + cb + c, o + c);
+          // The rows combined before have been read.
+          if (mq > 0) ok = mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 838);
           tmem_wait_ld();
           if (lane < 3 * HPU) {
-            float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW + c0);
+            float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < S::CB / 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+          if (cb == 0) {
+            // The head of a lane's sum: its top log2(HPU) lane bits.
+            constexpr int LANES = 32 / HPU;
+            if (lane % LANES == 0) mrg_l[warp * HPU + lane / LANES] = l[0];
+            float mm = m[0];
+#pragma unroll
+            for (int h = 1; h < HPU; ++h) mm = lane == h ? m[h] : mm;
+            if (lane < HPU) mrg_m[warp * HPU + lane] = mm;
           }
         }
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_before();
         mbar_arrive(BAR_MRG);
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
-        ++mq;
-        const int nd = min(p.D, S::CB);  // (head_dim 16: half of the columns)
-        for (int i = tid; i < f.nh * nd; i += 128) {
-          const int h = i / nd, d = i - h * nd;
-          float M = mrg_m[h];
+        // Lane w HPU + h: the factor of warp w's rows of head h, 2^(m_w - M) / L.
+        float fac, top;
+        {
+          const int i = lane % (4 * HPU);
+          const float mi = mrg_m[i];
+          top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2 * HPU));
+          fac = ex2(mi - top);
+          float L = mrg_l[i] * fac;
+          L += __shfl_xor_sync(0xffffffffu, L, HPU);
+          L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
+          fac = fac / L;
+          top += lg2(L);  // log2 of the sum
+        }
+        if (f.nf > 1 && cb == 0 && tid < HPU) part_l[f.slot * HPU + tid] = top;
+        // A thread takes a column and every (128 / columns)-th head.
+        const int nd_log2 = p.D >= S::CB ? (S::CB == 128 ? 7 : (S::CB == 64 ? 6 : 5)) : 4;  // (4: head_dim 16)
+        const int d = tid & ((1 << nd_log2) - 1), hg = tid >> nd_log2;
+        const int hs = 128 >> nd_log2;
+        float A[HPU];
 #pragma unroll
-          for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, mrg_m[w2 * HPU + h]);
-          float A = 0.f, L = 0.f;
+        for (int i = 0; i < HPU; ++i) {
+          const int h = (hg + i * hs) & (HPU - 1);  // (taken round where a thread has fewer heads)
+          A[i] = 0.f;
 #pragma unroll
           for (int w2 = 0; w2 < 4; ++w2) {
-            const float wt = ex2(mrg_m[w2 * HPU + h] - M);
+            const float wt = __shfl_sync(0xffffffffu, fac, w2 * HPU + h);
             const float* r = mrg + (w2 * 3 * HPU + h) * ROW + d;
-            A = fmaf(fmaf(r[2 * HPU * ROW], 0x1p-8f, fmaf(r[HPU * ROW], 0x1p-4f, r[0])), wt, A);
-            L = fmaf(mrg_l[w2 * HPU + h], wt, L);
-          }
-          const float val = A / L;
-          if (f.nf == 1) {
-            store_out(row0 + h, cb + d, val);
-          } else {
-            part_o[h * p.D + cb + d] = val;
-            if (cb + d == 0) part_l[f.slot * HPU + h] = M + lg2(L);
+            A[i] = fmaf(fmaf(r[2 * HPU * ROW], 0x1p-8f, fmaf(r[HPU * ROW], 0x1p-4f, r[0])), wt, A[i]);
           }
         }
-        // The combine area is free again (and the partial stored) once every thread is here.
-        mbar_arrive(BAR_MRG);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 838)))) break;
+#pragma unroll
+        for (int i = 0; i < HPU; ++i) {
+          const int h = hg + i * hs;
+          if (h < f.nh) {
+            if (f.nf == 1) store_out(row0 + h, cb + d, A[i]);
+            else part_o[h * p.D + cb + d] = A[i];
+          }
+        }
+        mbar_arrive(BAR_FREE);
         ++mq;
       }
       if (!ok) break;
@@ -786,14 +911,17 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         // acquire-release add makes them visible before the ticket and, after the last ticket,
         // the other fragments' partials visible to this CTA.
         if (tid == 0) {
-          const int last = atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1;
-          if (last) p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
+          int last = 0;
+          if (mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 842)) {
+            last = atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1;
+            if (last) p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
+            *emitted = it + 1;
+          }
           *verdict = last;
-          *emitted = it + 1;
         }
-        mbar_arrive(BAR_MRG);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 839)))) break;
-        ++mq;
+        mbar_arrive(BAR_TKT);
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 839)))) break;
+        ++tq;
         if (*verdict) {
           // The unit's other fragments are done: their sums' weights first, a warp per head and a
           // lane per fragment, then the outputs, four columns per thread, eight loads in flight.
@@ -817,9 +945,9 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
             const float inv = 1.0f / L;
             for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
           }
-          mbar_arrive(BAR_MRG);
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 840)))) break;
-          ++mq;
+          mbar_arrive(BAR_TKT);
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 840)))) break;
+          ++tq;
           const int q4 = p.D >> 2;
           for (int i = tid; i < f.nh * q4; i += 128) {
             const int h = i / q4, d = 4 * (i - h * q4);
@@ -848,9 +976,9 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
             store_out(row0 + h, d + 3, A.w);
           }
           // The weights are read: the combine area is free again.
-          mbar_arrive(BAR_MRG);
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 841)))) break;
-          ++mq;
+          mbar_arrive(BAR_TKT);
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 841)))) break;
+          ++tq;
         }
       } else if (tid == 0) {
         *emitted = it + 1;
@@ -863,12 +991,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   if (*failed) {
     // A wait ran out (reported in the status words): NaN for what this CTA still owes, and its
     // tickets, so that the counters return to zero.
-    PagedWalk walk;
+    Walk walk;
     walk.init(*start);
     PagedFrag f;
-    int unit, kbeg, len;
     const float nan = __int_as_float(0x7fc00000);
-    for (int it = 0; walk.next(p, f, unit, kbeg, len); ++it) {
+    for (int it = 0; walk.next(p, f); ++it) {
       if (it < *emitted) continue;
       for (int i = tid; i < f.nh * p.D; i += S::NTHREADS) {
         const int h = i / p.D, d = i - h * p.D;

@@ -1317,7 +1317,7 @@ int paged_grid(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
   if (ctas > du::DECODE_PAGED_MAX_CTAS) ctas = du::DECODE_PAGED_MAX_CTAS;
   const long long units = static_cast<long long>(B) * Hkv * paged_group_chunks(Hq / Hkv);
   const long long per_unit = (static_cast<long long>(max_blocks) * block_size + 127) / 128;
-  const long long most = (units * per_unit + du::DECODE_PAGED_MIN_PER - 1) / du::DECODE_PAGED_MIN_PER;
+  const long long most = units * per_unit;
   return static_cast<int>(most < ctas ? most : ctas);
 }
 
@@ -1356,7 +1356,9 @@ int launch_decode_paged_t(const void* k8, const void* v8, const du::DecodePagedP
   auto kern = du::decode_paged_kernel<DP, HPU>;
   cudaError_t e = ensure_smem_attr(kern, S::SMEM_BYTES);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged decode)");
-  kern<<<static_cast<unsigned>(grid), S::NTHREADS, S::SMEM_BYTES, st>>>(tk, tv, prm);
+  // A programmatic dependent: its barriers and TMEM are set up beside the stream's previous kernel.
+  e = launch_kernel(kern, dim3(static_cast<unsigned>(grid)), S::NTHREADS, S::SMEM_BYTES, st, true, tk, tv, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged decode launch");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged decode launch");
   return DU_OK;
@@ -1508,8 +1510,9 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
     return fail(DU_ERR_INVALID, "scales, block_table, cache_seqlens and tickets must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
+  if (Hq > 65536) return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads");
   if (static_cast<double>(B) * Hkv * paged_group_chunks(Hq / Hkv) *
-          ((static_cast<long long>(max_blocks) * block_size + 127) / 128) > 2147480000.0)
+          ((static_cast<long long>(max_blocks) * block_size + 127) / 128 + 8) > 2147480000.0)
     return fail(DU_ERR_UNSUPPORTED, "the block tables can hold 2^31 chunks of 128 keys or more");
   const int grid = paged_grid(B, Hq, Hkv, D, block_size, max_blocks);
   static_assert(du::DECODE_PAGED_MAX_CTAS <= DU_PAGED_TICKETS, "a ticket for each block of threads");
