@@ -1276,34 +1276,30 @@ int check_paged(int Hkv, int num_blocks, int block_size) {
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
-template <int D, bool BF16, int WPI>
+template <bool BF16, int WPI>
 int launch_paged_write_t(const du::PagedWriteParams& prm, cudaStream_t st) {
-  const long long items = static_cast<long long>(prm.B) * prm.pages * prm.Hkv * 2;
-  const long long ctas = (items + 4 / WPI - 1) / (4 / WPI);
-  if (ctas > 0x7fffffffLL) return fail(DU_ERR_UNSUPPORTED, "too many (request, block, head) items for one launch");
-  du::paged_write_kernel<D, BF16, WPI><<<static_cast<unsigned>(ctas), 128, 0, st>>>(prm);
-  cudaError_t e = cudaGetLastError();
+  const long long items = static_cast<long long>(prm.pages) * prm.Hkv * 2;  // of a request
+  const long long ctas = WPI == 1 ? (items + 3) / 4 : items;
+  if (items > 0x7fffffffLL || prm.B > 65535)
+    return fail(DU_ERR_UNSUPPORTED, "more than 65535 requests or 2^31 - 1 (block, head) items of one");
+  cudaError_t e = launch_kernel(du::paged_write_kernel<BF16, WPI>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(prm.B)),
+                                WPI == 1 ? 128 : 32 * WPI, 0, st, true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
+  e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
   return DU_OK;
 }
 
-template <int D, bool BF16>
-int launch_paged_write_d(const du::PagedWriteParams& prm, cudaStream_t st) {
-  // Chunk pairs of the largest item: a warp takes up to four per lane, else four warps share it.
-  const int rows = prm.T < prm.block ? prm.T : prm.block;
-  if (static_cast<long long>(rows) * (D / 16) <= 128) return launch_paged_write_t<D, BF16, 1>(prm, st);
-  return launch_paged_write_t<D, BF16, 4>(prm, st);
-}
-
 template <bool BF16>
-int launch_paged_write(const du::PagedWriteParams& prm, int D, cudaStream_t st) {
-  switch (D) {
-    case 16: return launch_paged_write_d<16, BF16>(prm, st);
-    case 32: return launch_paged_write_d<32, BF16>(prm, st);
-    case 64: return launch_paged_write_d<64, BF16>(prm, st);
-    case 128: return launch_paged_write_d<128, BF16>(prm, st);
-    default: return launch_paged_write_d<256, BF16>(prm, st);
-  }
+int launch_paged_write(const du::PagedWriteParams& prm, cudaStream_t st) {
+  // Warps per item: enough for four chunk pairs per thread of the largest item.
+  const int rows = prm.T < prm.block ? prm.T : prm.block;
+  const long long pairs = static_cast<long long>(rows) << (prm.d_log2 - 4);
+  if (pairs <= 128) return launch_paged_write_t<BF16, 1>(prm, st);
+  if (pairs <= 256) return launch_paged_write_t<BF16, 2>(prm, st);
+  if (pairs <= 512) return launch_paged_write_t<BF16, 4>(prm, st);
+  if (pairs <= 1024) return launch_paged_write_t<BF16, 8>(prm, st);
+  return launch_paged_write_t<BF16, 16>(prm, st);
 }
 
 // Query heads per unit of the paged decode: the group of a KV head in equal parts of at most 8.
@@ -1477,8 +1473,10 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
   prm.N = num_blocks;
   prm.block = block_size;
   prm.pages = static_cast<int>((static_cast<long long>(T) + 2LL * block_size - 2) / block_size);
+  prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
+  prm.d_log2 = D == 16 ? 4 : (D == 32 ? 5 : (D == 64 ? 6 : (D == 128 ? 7 : 8)));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DU_DTYPE_BF16 ? launch_paged_write<true>(prm, D, st) : launch_paged_write<false>(prm, D, st);
+  return dtype == DU_DTYPE_BF16 ? launch_paged_write<true>(prm, st) : launch_paged_write<false>(prm, st);
 }
 
 size_t du_decode_paged_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {

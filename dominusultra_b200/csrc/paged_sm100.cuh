@@ -24,6 +24,13 @@ __device__ __forceinline__ float2 e4m3x2_widen(uint32_t p) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Block tables and slot maps
 // ---------------------------------------------------------------------------------------------
@@ -222,18 +229,19 @@ struct PagedWriteParams {
   const void* sin;
   long long positions;
   int B, Hkv, T, N, block, pages;  // pages: blocks that one request's T tokens can touch
+  int d_log2, block_log2;  // head_dim = 2^d_log2, block = 2^block_log2
 };
 
-// a + b rounded to odd: the exact sum when it has 24 bits, else the neighbour of it whose last
-// bit is set. Rounding that to e4m3 gives what rounding the exact sum would (no double rounding).
-__device__ __forceinline__ float add_to_odd(float a, float b) {
-  const float s = __fadd_rn(a, b);
-  const float bb = __fsub_rn(s, a);
-  const float err = __fadd_rn(__fsub_rn(a, __fsub_rn(s, bb)), __fsub_rn(b, bb));
-  const int i = __float_as_int(s);
-  if (err != 0.f && (i & 1) == 0 && (i & 0x7f800000) != 0x7f800000)
-    return __int_as_float(((err > 0.f) == (s > 0.f)) ? i + 1 : i - 1);
-  return s;
+// a b + c for two pairs, rounded to odd: the exact value where it has 24 bits, else the one of its
+// two neighbours whose last bit is set. Rounding that to e4m3 gives what rounding the exact value
+// would (no double rounding), and no inexact value lands on the border of a scale. The neighbours
+// come from rounding down and up: they differ in their last bit unless the value is exact.
+__device__ __forceinline__ uint64_t f2_fma_odd(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t lo, hi;
+  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(lo) : "l"(a), "l"(b), "l"(c));
+  asm("fma.rp.f32x2 %0, %1, %2, %3;" : "=l"(hi) : "l"(a), "l"(b), "l"(c));
+  const float2 l = f2_split(lo), h = f2_split(hi);
+  return f2((__float_as_uint(l.x) & 1u) ? l.x : h.x, (__float_as_uint(l.y) & 1u) ? l.y : h.y);
 }
 
 // The smallest power of two of at least 2^-64 whose 448-fold covers amax (its bits given); NaN
@@ -249,49 +257,71 @@ __device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
 // Quantises the new tokens of a call into the cache: keys rotated at their positions, one scale
 // per (block, KV head) and per cache.
 //
-// A work item is (request, block that its tokens touch, KV head, key or value); WPI warps take
-// it, a thread a pair of 16-byte chunks i, i + D/2 of a row at a time, which is what a rotation
-// pairs up. First the largest magnitude of the item's rows, from which the scale follows: the
-// smallest power of two with amax <= 448 scale, or the block's present scale where that is
-// larger and the block holds rows already. Then the rows again (out of L1), scaled and rounded
-// once. Products of two 16-bit values are exact in fp32, their sum is rounded to odd and the
-// scale is a power of two, so each byte is the e4m3 value nearest to the exact quotient. Where a
-// block's scale grows, its present rows are scaled down and rounded again; that is exact but
-// for what falls below the format's normal range. A block with a value that is not finite gets
-// the scale NaN, which every attention over it then returns.
+// A work item is (request, block that its tokens touch, KV head, key or value); WPI warps take it, a
+// thread at most four pairs of 16-byte chunks i, i + D/2 of a row, which is what a rotation pairs
+// up, held in registers from the load to the store. The largest magnitude of the item's rows
+// gives the scale: the smallest power of two with amax <= 448 scale, or the block's present scale
+// where that is larger and the block holds rows already. Products of two 16-bit values are exact
+// in fp32, their sum is rounded to odd and the scale is a power of two, so each byte is the e4m3
+// value nearest to the exact quotient. Where a block's scale grows, its present rows are scaled
+// down and rounded again; that is exact but for what falls below the format's normal range. A
+// block with a value that is not finite gets the scale NaN, which every attention over it then
+// returns.
 //
-// Bound by HBM for prompts: 2 bytes read and 1 written per value; by the chain of loads (slots,
-// rows, scale) for single tokens.
-template <int D, bool BF16, int WPI>
-__global__ void __launch_bounds__(128) paged_write_kernel(const PagedWriteParams p) {
-  constexpr int PAIRS = D / 16;  // chunk pairs per row
-  constexpr int NT = 32 * WPI;   // threads per item
-  constexpr int IPC = 4 / WPI;   // items per CTA
-  __shared__ uint32_t warp_max[4];
+// Bound by HBM for prompts: 2 bytes read and 1 written per value; by the chain of loads (length,
+// rows and slots, scale) for single tokens.
+template <bool BF16, int WPI>
+__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(const PagedWriteParams p) {
+  constexpr int NT = 32 * WPI;  // threads per item
+  constexpr int NP = 4;         // chunk pairs per thread, at most
+  __shared__ uint32_t warp_max[WPI];
+  griddep_launch_dependents();
+  griddep_wait();
   const int lane_i = threadIdx.x % NT;  // thread within the item
-  const long long items = static_cast<long long>(p.B) * p.pages * p.Hkv * 2;
-  const long long item = static_cast<long long>(blockIdx.x) * IPC + threadIdx.x / NT;
-  // Uniform over the item's threads. With WPI = 4 the whole CTA is one item, so its barriers
-  // are reached by all or none.
-  if (item >= items) return;
+  // With WPI = 1 a warp is an item; else the CTA is one, and its barrier is reached by all or none.
+  const unsigned item = WPI == 1 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
+  const unsigned hh = item >> 1;
+  const int pg = static_cast<int>(hh / static_cast<unsigned>(p.Hkv));
+  if (pg >= p.pages) return;
   const bool is_v = (item & 1) != 0;
-  const long long i2 = item >> 1;
-  const int h = static_cast<int>(i2 % p.Hkv);
-  const long long i3 = i2 / p.Hkv;
-  const int pg = static_cast<int>(i3 % p.pages);
-  const int b = static_cast<int>(i3 / p.pages);
+  const int h = static_cast<int>(hh) - pg * p.Hkv;
+  const int b = blockIdx.y;
 
+  const int D = 1 << p.d_log2;
   const int past = p.past[b];
-  const int row0 = past >= 0 ? past % p.block : 0;  // row of the request's first new token
-  const int t0 = pg == 0 ? 0 : pg * p.block - row0;
+  const int row0 = past >= 0 ? past & (p.block - 1) : 0;  // row of the request's first new token
+  const int t0 = pg == 0 ? 0 : (pg << p.block_log2) - row0;
   if (t0 >= p.T) return;
   const int r0 = pg == 0 ? row0 : 0;  // the block's first row that this call writes
   const int n = min(p.T - t0, p.block - r0);
   const int* slot_row = p.slots + static_cast<long long>(b) * p.T + t0;
+  const uint8_t* x = static_cast<const uint8_t*>(is_v ? p.v : p.k) +
+                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0) * (2 * D);
+  const int pairs_log2 = p.d_log2 - 4;
+  const int units = n << pairs_log2;
+  // Everything whose address is known goes out at once: rows, slots and the rows of the tables.
+  uint4 xa[NP], xb[NP], cv[NP], sv[NP];
+  int slots[NP];
   const int slot0 = slot_row[0];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
+    const long long pos = static_cast<long long>(past) + t0 + r;
+    xa[i] = xb[i] = cv[i] = sv[i] = make_uint4(0, 0, 0, 0);
+    slots[i] = -1;
+    if (u < units) {
+      slots[i] = slot_row[r];
+      xa[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + c * 16);
+      xb[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + D + c * 16);
+      if (!is_v && past >= 0 && pos < p.positions) {
+        cv[i] = ldg_v4(static_cast<const uint8_t*>(p.cos) + pos * D + c * 16);
+        sv[i] = ldg_v4(static_cast<const uint8_t*>(p.sin) + pos * D + c * 16);
+      }
+    }
+  }
   if (slot0 < 0) return;  // no token here
-  const int blk = slot0 / p.block;
-  if (past < 0 || blk >= p.N || slot0 - blk * p.block != r0) {
+  const int blk = slot0 >> p.block_log2;
+  if (past < 0 || blk >= p.N || (slot0 & (p.block - 1)) != r0) {
     if (lane_i == 0) record_error(past < 0 ? 6u : 7u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : slot0));
     return;
   }
@@ -299,79 +329,73 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const PagedWriteParams
   float* scale = (is_v ? p.vs : p.ks) + cell;
   uint8_t* out = (is_v ? p.v8 : p.k8) + cell * p.block * D;
   const float had = r0 > 0 ? *scale : 0.f;
-  const uint8_t* x = static_cast<const uint8_t*>(is_v ? p.v : p.k) +
-                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0) * (2 * D);
 
-  // The 16 values of chunk pair (r, c), rotated for keys; false for a row without a token.
-  auto values = [&](int r, int c, float (&y1)[8], float (&y2)[8]) -> bool {
-    if (slot_row[r] != slot0 + r) return false;
-    const long long pos = static_cast<long long>(past) + t0 + r;
-    if (!is_v && pos >= p.positions) return false;
-    const uint4 a = ldg_v4(x + static_cast<long long>(r) * (2 * D) + c * 16);
-    const uint4 d = ldg_v4(x + static_cast<long long>(r) * (2 * D) + D + c * 16);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, dw[4] = {d.x, d.y, d.z, d.w};
-    if (is_v) {
+  uint64_t y1[NP][4], y2[NP][4];  // pairs of fp32 values
+  unsigned live = 0;              // pairs of rows that hold a token
+  int wrong = -1;                 // a row whose slot or position is not fit, and its code
+  unsigned code = 0;
+  float peak = 0.f;               // the largest magnitude (NaN stays)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 u = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
-        y1[2 * e] = u.x;
-        y1[2 * e + 1] = u.y;
-        y2[2 * e] = w.x;
-        y2[2 * e + 1] = w.y;
-      }
-      return true;
+  for (int i = 0; i < NP; ++i) {
+    const int u = lane_i + i * NT, r = u >> pairs_log2;
+    const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
+    const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
+    bool on = slots[i] == slot0 + r;
+    const bool far = on && !is_v && static_cast<long long>(past) + t0 + r >= p.positions;
+    if (far || (!on && slots[i] >= 0)) {
+      wrong = far ? past + t0 + r : slots[i];
+      code = far ? 6u : 7u;
     }
-    const uint4 cv = ldg_v4(static_cast<const uint8_t*>(p.cos) + pos * D + c * 16);
-    const uint4 sv = ldg_v4(static_cast<const uint8_t*>(p.sin) + pos * D + c * 16);
-    const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+    on = on && !far;
+    live |= on ? 1u << i : 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 u = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
-      const float2 cc = unpack2<BF16>(cw[e]), ss = unpack2<BF16>(sw[e]);
-      y1[2 * e] = add_to_odd(__fmul_rn(u.x, cc.x), -__fmul_rn(w.x, ss.x));
-      y1[2 * e + 1] = add_to_odd(__fmul_rn(u.y, cc.y), -__fmul_rn(w.y, ss.y));
-      y2[2 * e] = add_to_odd(__fmul_rn(w.x, cc.x), __fmul_rn(u.x, ss.x));
-      y2[2 * e + 1] = add_to_odd(__fmul_rn(w.y, cc.y), __fmul_rn(u.y, ss.y));
+      y1[i][e] = widen2<BF16>(aw[e]);
+      y2[i][e] = widen2<BF16>(dw[e]);
     }
-    return true;
-  };
-
-  uint32_t top = 0;  // bits of the largest magnitude: NaN above infinity above every number
-  for (int u = lane_i; u < n * PAIRS; u += NT) {
-    const int r = u / PAIRS, c = u % PAIRS;
-    float y1[8], y2[8];
-    if (values(r, c, y1, y2)) {
+    if (!is_v) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        top = max(top, max(__float_as_uint(y1[e]) & 0x7fffffffu, __float_as_uint(y2[e]) & 0x7fffffffu));
-    } else if (c == 0 && slot_row[r] >= 0) {
-      const bool far = slot_row[r] == slot0 + r;
-      record_error(far ? 6u : 7u, static_cast<unsigned>(b), static_cast<unsigned>(far ? past + t0 + r : slot_row[r]));
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t cc = widen2<BF16>(cw[e]), ss = widen2<BF16>(sw[e]);
+        const uint64_t v = y1[i][e], w = y2[i][e];
+        y1[i][e] = f2_fma_odd(f2_mul(w, f2(-1.f, -1.f)), ss, f2_mul(v, cc));  // (each product is exact)
+        y2[i][e] = f2_fma_odd(v, ss, f2_mul(w, cc));
+      }
     }
+    if (on)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 p1 = f2_split(y1[i][e]), p2 = f2_split(y2[i][e]);
+        peak = max3_abs_nan(peak, p1.x, p1.y);
+        peak = max3_abs_nan(peak, p2.x, p2.y);
+      }
   }
+  if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
+  uint32_t top = __float_as_uint(peak) & 0x7fffffffu;  // NaN above infinity above every number
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (WPI > 1) {
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
-    __syncthreads();
+    __syncthreads();  // (and every thread has read the present scale)
 #pragma unroll
     for (int w = 0; w < WPI; ++w) top = max(top, warp_max[w]);
-  } else {
-    __syncwarp();  // every lane has read the present scale
   }
   float unit = paged_unit(top);
   if (r0 > 0 && (unit <= had || had != had)) unit = had;  // (a NaN on either side stays)
   if (lane_i == 0) *scale = unit;
   const bool poison = unit != unit;
   const float inv = 1.0f / unit;
-  for (int u = lane_i; u < n * PAIRS; u += NT) {
-    const int r = u / PAIRS, c = u % PAIRS;
-    float y1[8], y2[8];
-    if (!values(r, c, y1, y2)) continue;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    if (!(live & (1u << i))) continue;
+    const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
     uint32_t w[4];
+    const uint64_t f = f2(inv, inv);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      w[e] = e4m3x2(y1[4 * e] * inv, y1[4 * e + 1] * inv) | (e4m3x2(y1[4 * e + 2] * inv, y1[4 * e + 3] * inv) << 16);
-      w[2 + e] = e4m3x2(y2[4 * e] * inv, y2[4 * e + 1] * inv) | (e4m3x2(y2[4 * e + 2] * inv, y2[4 * e + 3] * inv) << 16);
+      const float2 a0 = f2_split(f2_mul(y1[i][2 * e], f)), a1 = f2_split(f2_mul(y1[i][2 * e + 1], f));
+      const float2 b0 = f2_split(f2_mul(y2[i][2 * e], f)), b1 = f2_split(f2_mul(y2[i][2 * e + 1], f));
+      w[e] = e4m3x2(a0.x, a0.y) | (e4m3x2(a1.x, a1.y) << 16);
+      w[2 + e] = e4m3x2(b0.x, b0.y) | (e4m3x2(b1.x, b1.y) << 16);
     }
     if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
     uint8_t* row = out + static_cast<long long>(r0 + r) * D;
@@ -381,7 +405,7 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const PagedWriteParams
   if (r0 > 0 && unit > had) {
     // The present rows under the larger scale.
     const float f = had * inv;
-    for (int u = lane_i; u < r0 * D / 16; u += NT) {
+    for (int u = lane_i; u < r0 * (D / 16); u += NT) {
       uint4* q = reinterpret_cast<uint4*>(out) + u;
       const uint4 o = *q;
       uint32_t w[4] = {o.x, o.y, o.z, o.w};
