@@ -232,16 +232,13 @@ struct PagedWriteParams {
   int d_log2, block_log2;  // head_dim = 2^d_log2, block = 2^block_log2
 };
 
-// a b + c for two pairs, rounded to odd: the exact value where it has 24 bits, else the one of its
-// two neighbours whose last bit is set. Rounding that to e4m3 gives what rounding the exact value
-// would (no double rounding), and no inexact value lands on the border of a scale. The neighbours
-// come from rounding down and up: they differ in their last bit unless the value is exact.
-__device__ __forceinline__ uint64_t f2_fma_odd(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t lo, hi;
-  asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(lo) : "l"(a), "l"(b), "l"(c));
-  asm("fma.rp.f32x2 %0, %1, %2, %3;" : "=l"(hi) : "l"(a), "l"(b), "l"(c));
-  const float2 l = f2_split(lo), h = f2_split(hi);
-  return f2((__float_as_uint(l.x) & 1u) ? l.x : h.x, (__float_as_uint(l.y) & 1u) ? l.y : h.y);
+// a b + c rounded to odd: the exact value where it has 24 bits, else the one of its two neighbours
+// whose last bit is set. Rounding that to e4m3 gives what rounding the exact value would (no double
+// rounding), and no inexact value lands on the border of a scale. The neighbours come from
+// rounding down and up: they differ in their last bit unless the value is exact.
+__device__ __forceinline__ float fma_odd(float a, float b, float c) {
+  const float lo = __fmaf_rd(a, b, c), hi = __fmaf_ru(a, b, c);
+  return (__float_as_uint(lo) & 1u) ? lo : hi;
 }
 
 // The smallest power of two of at least 2^-64 whose 448-fold covers amax (its bits given); NaN
@@ -270,23 +267,11 @@ __device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
 //
 // Bound by HBM for prompts: 2 bytes read and 1 written per value; by the chain of loads (length,
 // rows and slots, scale) for single tokens.
-template <bool BF16, int WPI>
-__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(const PagedWriteParams p) {
+template <bool BF16, int WPI, bool IS_V>
+__device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int b, int pg, int h, uint32_t* warp_max) {
   constexpr int NT = 32 * WPI;  // threads per item
   constexpr int NP = 4;         // chunk pairs per thread, at most
-  __shared__ uint32_t warp_max[WPI];
-  griddep_launch_dependents();
-  griddep_wait();
   const int lane_i = threadIdx.x % NT;  // thread within the item
-  // With WPI = 1 a warp is an item; else the CTA is one, and its barrier is reached by all or none.
-  const unsigned item = WPI == 1 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
-  const unsigned hh = item >> 1;
-  const int pg = static_cast<int>(hh / static_cast<unsigned>(p.Hkv));
-  if (pg >= p.pages) return;
-  const bool is_v = (item & 1) != 0;
-  const int h = static_cast<int>(hh) - pg * p.Hkv;
-  const int b = blockIdx.y;
-
   const int D = 1 << p.d_log2;
   const int past = p.past[b];
   const int row0 = past >= 0 ? past & (p.block - 1) : 0;  // row of the request's first new token
@@ -295,14 +280,16 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
   const int r0 = pg == 0 ? row0 : 0;  // the block's first row that this call writes
   const int n = min(p.T - t0, p.block - r0);
   const int* slot_row = p.slots + static_cast<long long>(b) * p.T + t0;
-  const uint8_t* x = static_cast<const uint8_t*>(is_v ? p.v : p.k) +
+  const uint8_t* x = static_cast<const uint8_t*>(IS_V ? p.v : p.k) +
                      ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0) * (2 * D);
   const int pairs_log2 = p.d_log2 - 4;
   const int units = n << pairs_log2;
   // Everything whose address is known goes out at once: rows, slots and the rows of the tables.
+  // (In prompts, where requests' padding makes whole blocks without tokens, those are left first.)
   uint4 xa[NP], xb[NP], cv[NP], sv[NP];
   int slots[NP];
   const int slot0 = slot_row[0];
+  if (p.T > p.block && slot0 < 0) return;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
@@ -313,7 +300,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
       slots[i] = slot_row[r];
       xa[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + c * 16);
       xb[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + D + c * 16);
-      if (!is_v && past >= 0 && pos < p.positions) {
+      if (!IS_V && past >= 0 && pos < p.positions) {
         cv[i] = ldg_v4(static_cast<const uint8_t*>(p.cos) + pos * D + c * 16);
         sv[i] = ldg_v4(static_cast<const uint8_t*>(p.sin) + pos * D + c * 16);
       }
@@ -326,11 +313,11 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
     return;
   }
   const long long cell = static_cast<long long>(blk) * p.Hkv + h;
-  float* scale = (is_v ? p.vs : p.ks) + cell;
-  uint8_t* out = (is_v ? p.v8 : p.k8) + cell * p.block * D;
+  float* scale = (IS_V ? p.vs : p.ks) + cell;
+  uint8_t* out = (IS_V ? p.v8 : p.k8) + cell * p.block * D;
   const float had = r0 > 0 ? *scale : 0.f;
 
-  uint64_t y1[NP][4], y2[NP][4];  // pairs of fp32 values
+  float y1[NP][8], y2[NP][8];
   unsigned live = 0;              // pairs of rows that hold a token
   int wrong = -1;                 // a row whose slot or position is not fit, and its code
   unsigned code = 0;
@@ -341,7 +328,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
     const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
     const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
     bool on = slots[i] == slot0 + r;
-    const bool far = on && !is_v && static_cast<long long>(past) + t0 + r >= p.positions;
+    const bool far = on && !IS_V && static_cast<long long>(past) + t0 + r >= p.positions;
     if (far || (!on && slots[i] >= 0)) {
       wrong = far ? past + t0 + r : slots[i];
       code = far ? 6u : 7u;
@@ -350,25 +337,24 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
     live |= on ? 1u << i : 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      y1[i][e] = widen2<BF16>(aw[e]);
-      y2[i][e] = widen2<BF16>(dw[e]);
-    }
-    if (!is_v) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t cc = widen2<BF16>(cw[e]), ss = widen2<BF16>(sw[e]);
-        const uint64_t v = y1[i][e], w = y2[i][e];
-        y1[i][e] = f2_fma_odd(f2_mul(w, f2(-1.f, -1.f)), ss, f2_mul(v, cc));  // (each product is exact)
-        y2[i][e] = f2_fma_odd(v, ss, f2_mul(w, cc));
+      const float2 v = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
+      if constexpr (IS_V) {
+        y1[i][2 * e] = v.x;
+        y1[i][2 * e + 1] = v.y;
+        y2[i][2 * e] = w.x;
+        y2[i][2 * e + 1] = w.y;
+      } else {
+        // (products of two 16-bit values are exact)
+        const float2 cc = unpack2<BF16>(cw[e]), ss = unpack2<BF16>(sw[e]);
+        y1[i][2 * e] = fma_odd(v.x, cc.x, -__fmul_rn(w.x, ss.x));
+        y1[i][2 * e + 1] = fma_odd(v.y, cc.y, -__fmul_rn(w.y, ss.y));
+        y2[i][2 * e] = fma_odd(w.x, cc.x, __fmul_rn(v.x, ss.x));
+        y2[i][2 * e + 1] = fma_odd(w.y, cc.y, __fmul_rn(v.y, ss.y));
       }
     }
     if (on)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 p1 = f2_split(y1[i][e]), p2 = f2_split(y2[i][e]);
-        peak = max3_abs_nan(peak, p1.x, p1.y);
-        peak = max3_abs_nan(peak, p2.x, p2.y);
-      }
+      for (int e = 0; e < 8; ++e) peak = max3_abs_nan(peak, y1[i][e], y2[i][e]);
   }
   if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
   uint32_t top = __float_as_uint(peak) & 0x7fffffffu;  // NaN above infinity above every number
@@ -389,13 +375,12 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
     if (!(live & (1u << i))) continue;
     const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
     uint32_t w[4];
-    const uint64_t f = f2(inv, inv);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float2 a0 = f2_split(f2_mul(y1[i][2 * e], f)), a1 = f2_split(f2_mul(y1[i][2 * e + 1], f));
-      const float2 b0 = f2_split(f2_mul(y2[i][2 * e], f)), b1 = f2_split(f2_mul(y2[i][2 * e + 1], f));
-      w[e] = e4m3x2(a0.x, a0.y) | (e4m3x2(a1.x, a1.y) << 16);
-      w[2 + e] = e4m3x2(b0.x, b0.y) | (e4m3x2(b1.x, b1.y) << 16);
+      w[e] = e4m3x2(y1[i][4 * e] * inv, y1[i][4 * e + 1] * inv) |
+             (e4m3x2(y1[i][4 * e + 2] * inv, y1[i][4 * e + 3] * inv) << 16);
+      w[2 + e] = e4m3x2(y2[i][4 * e] * inv, y2[i][4 * e + 1] * inv) |
+                 (e4m3x2(y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv) << 16);
     }
     if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
     uint8_t* row = out + static_cast<long long>(r0 + r) * D;
@@ -417,6 +402,21 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(
       *q = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+}
+
+template <bool BF16, int WPI>
+__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(const PagedWriteParams p) {
+  __shared__ uint32_t warp_max[WPI];
+  griddep_launch_dependents();
+  griddep_wait();
+  // With WPI = 1 a warp is an item; else the CTA is one, and its barrier is reached by all or none.
+  const unsigned item = WPI == 1 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
+  const unsigned hh = item >> 1;
+  const int pg = static_cast<int>(hh / static_cast<unsigned>(p.Hkv));
+  if (pg >= p.pages) return;
+  const int h = static_cast<int>(hh) - pg * p.Hkv;
+  if (item & 1) paged_write_item<BF16, WPI, true>(p, blockIdx.y, pg, h, warp_max);
+  else paged_write_item<BF16, WPI, false>(p, blockIdx.y, pg, h, warp_max);
 }
 
 }  // namespace du
