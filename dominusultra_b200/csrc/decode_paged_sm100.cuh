@@ -151,7 +151,9 @@ struct DecodePagedShape {
   static constexpr int TM_O = 64;          // O: DP columns
   static constexpr int TMEM_COLS = TM_O + DP <= 128 ? 128 : (TM_O + DP <= 256 ? 256 : 512);
   static constexpr int NTHREADS = 256;
-  static constexpr int PEN = 2;            // chunks that a unit's beginning is charged with
+  // Chunks that a unit's beginning is charged with (measured with 1, 2, 3, 4, 6: 64 requests of up
+  // to 4096, four heads 82, 75, 69, 68, 70 us; 16 of up to 20001, eight heads 86, 80, 77, 75, 73 us).
+  static constexpr int PEN = HPU == 8 ? 6 : 4;
   static_assert(3 * HPU <= 32, "a warp's rows of P");
   static_assert(MRG_O >= HPU * DECODE_PAGED_MAX_CTAS, "weights of the last fragment's CTA");
   static_assert(NSTG >= 2, "at least two stages");
@@ -159,7 +161,8 @@ struct DecodePagedShape {
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
-// x / y for a quotient below 2^20 (x >= 0, y > 0): a float estimate, off by one at most, and a step.
+// x / y for a quotient of at most 2^21 (x >= 0, y > 0): a float estimate, off by one at most, and a
+// step. (Here: chunks of a request, which the host keeps at 2^20, units of one, CTAs.)
 __device__ __forceinline__ int small_div(int x, int y) {
   int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
   const int r = x - q * y;
@@ -229,19 +232,15 @@ struct PagedWalk {
     bool cut = false;
     int x = 0;
     if (p.B * static_cast<long long>(ups) <= grid) {
-      const int per = (total * ups + grid - 1) / grid;
-      int sum[DECODE_PAGED_PIECE_SLACK + 1] = {};
-      for (int b = lane; b < p.B; b += 32) {
-        const int nc = chunks(tokens(p, b));
-#pragma unroll
-        for (int i = 0; i <= DECODE_PAGED_PIECE_SLACK; ++i) sum[i] += small_div(nc + per + i - 1, per + i);
+      const int per = small_div(total * ups + grid - 1, grid);
+#pragma unroll 1
+      for (x = per; x <= per + DECODE_PAGED_PIECE_SLACK && !cut; ++x) {
+        int sum = 0;
+#pragma unroll 1
+        for (int b = lane; b < p.B; b += 32) sum += small_div(chunks(tokens(p, b)) + x - 1, x);
+        cut = static_cast<int>(__reduce_add_sync(0xffffffffu, sum)) * ups <= grid;
       }
-#pragma unroll
-      for (int i = DECODE_PAGED_PIECE_SLACK; i >= 0; --i)
-        if (static_cast<int>(__reduce_add_sync(0xffffffffu, sum[i])) * ups <= grid) {
-          cut = true;
-          x = per + i;
-        }
+      --x;  // (the one that was tried last)
     }
     int cur, hi;
     if (cut) {
@@ -249,7 +248,7 @@ struct PagedWalk {
       hi = c + 1;
     } else {
       total = (total + p.B * PEN) * ups;  // (the host keeps total + gridDim.x below 2^31)
-      x = (total + grid - 1) / grid;
+      x = (total + grid - 1) / grid;  // (may pass what small_div takes)
       cur = static_cast<int>(min(static_cast<long long>(x) * c, static_cast<long long>(total)));
       hi = min(total - cur, x) + cur;
     }
@@ -294,7 +293,7 @@ struct PagedWalk {
       nc = chunks(n);
       unit = small_div(cur, pieces);
       const int piece = cur - unit * pieces;
-      const int q = nc / pieces, r = nc - q * pieces;  // the first r pieces hold a chunk more
+      const int q = small_div(nc, pieces), r = nc - q * pieces;  // the first r pieces hold a chunk more
       j0 = piece * q + min(piece, r);
       j1 = j0 + q + (piece < r);
       f.c0 = static_cast<int>(blockIdx.x) - piece;
@@ -923,9 +922,22 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 839)))) break;
         ++tq;
         if (*verdict) {
-          // The unit's other fragments are done: their sums' weights first, a warp per head and a
-          // lane per fragment, then the outputs, four columns per thread, eight loads in flight.
+          // The unit's other fragments are done. A thread takes four columns of a head at a time; the
+          // rows of the first KB fragments are on their way while the weights are found (a warp
+          // per head, a lane per fragment).
+          constexpr int KB = S::CTAS == 2 ? 4 : 16;  // (registers)
           auto slot_of = [&](int k) { return k == 0 ? 2 * f.c0 + 1 : 2 * (f.c0 + k); };
+          const int q4 = p.D >> 2, items = f.nh * q4;
+          auto load = [&](float4 (&o)[KB], int i, int k0) {
+            const int h = i / q4, d = 4 * (i - h * q4);
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+              if (i < items && k0 + k < f.nf)
+                o[k] = __ldcg(reinterpret_cast<const float4*>(
+                    p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d));
+          };
+          float4 o[KB];
+          load(o, tid, 0);
           float* wt = mrg;  // [HPU][nf]: nf <= gridDim.x <= DECODE_PAGED_MAX_CTAS
           for (int h = warp; h < f.nh; h += 4) {
             float M = -INFINITY, L = 0.f;
@@ -941,29 +953,23 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
               L += e;
             }
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            for (int o2 = 16; o2 >= 1; o2 >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o2);
             const float inv = 1.0f / L;
             for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
           }
           mbar_arrive(BAR_TKT);
           if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 840)))) break;
           ++tq;
-          const int q4 = p.D >> 2;
-          for (int i = tid; i < f.nh * q4; i += 128) {
+          for (int i = tid; i < items; i += 128) {
             const int h = i / q4, d = 4 * (i - h * q4);
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-            for (int k0 = 0; k0 < f.nf; k0 += 8) {
-              float4 o[8];
+            for (int k0 = 0; k0 < f.nf; k0 += KB) {
+              if (i != tid || k0 > 0) load(o, i, k0);
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                o[k] = k0 + k < f.nf
-                           ? __ldcg(reinterpret_cast<const float4*>(
-                                 p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d))
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float x = k0 + k < f.nf ? wt[h * f.nf + k0 + k] : 0.f;
+              for (int k = 0; k < KB; ++k) {
+                if (k0 + k >= f.nf) break;
+                const float x = wt[h * f.nf + k0 + k];
                 A.x = fmaf(o[k].x, x, A.x);
                 A.y = fmaf(o[k].y, x, A.y);
                 A.z = fmaf(o[k].z, x, A.z);

@@ -1497,8 +1497,8 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   rc = check_paged(Hkv, num_blocks, block_size);
   if (rc != DU_OK) return rc;
   if (max_blocks <= 0) return fail(DU_ERR_INVALID, "max_blocks must be positive");
-  if (static_cast<long long>(max_blocks) * block_size > 0x7fffffffLL - 128)
-    return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^31 - 129 tokens");
+  if (static_cast<long long>(max_blocks) * block_size > (1LL << 27))
+    return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^27 tokens");
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !cache_seqlens || !cos || !sin || !out ||
       !tickets)
     return fail(DU_ERR_INVALID, "null pointer argument");

@@ -302,7 +302,7 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
  * a (request, KV head) that lies across CTAs meet in `workspace` (du_decode_paged_workspace_size
  * bytes, 16-byte aligned, any contents), their CTAs count in `tickets` (DU_PAGED_TICKETS ints, zero
  * before the first call; every call leaves them zero). Calls that may overlap on the GPU, replayed
- * graphs among them, need tickets and a workspace each. The
+ * graphs among them, need tickets and a workspace each. A table row covers at most 2^27 tokens. The
  * scales may be any positive floats (values of blocks whose value scale is below 2^-64 count as
  * held at 2^-64).
  */
