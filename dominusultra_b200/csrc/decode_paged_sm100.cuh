@@ -15,8 +15,9 @@
 // mostly empty otherwise, so they cost no tensor time:
 //   S^T = K8 Q^T     M = 128 keys of a chunk, N = 16 or 32 (three parts of the unit's heads),
 //                    K = head_dim. A = the K tile as TMA left it, B = the query parts.
-//   O  += P V8       M = 128, N = head_dim, K = 128 keys. A = P, B = the V tile as TMA left it
-//                    (MN-major). Row 32 w + t HPU + h: part t of head h's weights at warp w's keys.
+//   O  += P V8       M = 64 or 128, N = head_dim, K = 128 keys. A = P, B = the V tile as TMA left
+//                    it (MN-major). Row (M/4) w + t HPU + h: part t of head h's weights at warp w's
+//                    keys, which TMEM lane 32 w + t HPU + h holds.
 // One key per TMEM lane, so the softmax is one thread per key, and each of its four warps keeps a
 // reference maximum, a sum and rows of O of its own over its 32 keys of every chunk: no
 // reduction across warps per chunk. The value scale joins the weight before it is split: with
@@ -116,30 +117,33 @@ struct DecodePagedShape {
   static constexpr int SPAN = DP < 128 ? DP : 128;    // bytes per row of a swizzled block
   static constexpr int NBLK = DP / SPAN;
   static constexpr int TILE = CK * DP;
-  static constexpr int STAGE = 2 * TILE;
-  // Two CTAs per SM where their tiles allow: one CTA's four softmax warps keep up with half an
-  // SM's share of the bandwidth at head_dim 64 and below, and their start and end overlap.
-  static constexpr int CTAS = DP <= 64 ? 2 : 1;
-  static constexpr int P_BYTES = CK * 128;            // [key][128 rows] bytes, 128-byte swizzle
+  // Two CTAs per SM where their tiles allow: one's softmax, fragment ends and start overlap the
+  // other's copies.
+  static constexpr int CTAS = DP <= 128 ? 2 : 1;
+  static constexpr int NPB = DP == 128 && HPU == 8 ? 1 : 2;  // P buffers
+  static constexpr int PM = HPU <= 4 ? 64 : 128;      // rows of P (M of P V): 16 or 32 per warp
+  static constexpr int P_BYTES = CK * PM;             // [key][PM rows] bytes, swizzled
   static constexpr int Q_BYTES = ((NQ * DP + 1023) / 1024) * 1024;
-  static constexpr int CB = DP == 256 ? 64 : DP;      // columns of O combined at a time
+  static constexpr int CB = DP == 256 ? 64 : (DP == 128 ? 32 : DP);  // columns of O combined at a time
   static constexpr int ROW = CB + 4;                  // floats per row of the combine area
   static constexpr int MRG_O = 12 * HPU * ROW;        // [4 warps][3 HPU rows][ROW] floats
   static constexpr int MRG_BYTES = ((MRG_O + 8 * HPU) * 4 + 127) / 128 * 128;
-  static constexpr int FIXED = 2 * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2560;
+  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2560;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
-  static constexpr int NSTG_FIT = (BUDGET - FIXED) / STAGE;
-  static constexpr int NSTG = NSTG_FIT > 8 ? 8 : NSTG_FIT;
-  static constexpr int OFF_P = NSTG * STAGE;
-  static constexpr int OFF_Q = OFF_P + 2 * P_BYTES;
+  static constexpr int TILES = (BUDGET - FIXED) / TILE;
+  static constexpr int NV = TILES / 2 > 8 ? 8 : TILES / 2;            // stages of V
+  static constexpr int NK = TILES - NV > 8 ? 8 : TILES - NV;          // stages of K and scales
+  static constexpr int OFF_V = NK * TILE;
+  static constexpr int OFF_P = OFF_V + NV * TILE;
+  static constexpr int OFF_Q = OFF_P + NPB * P_BYTES;
   static constexpr int OFF_MRG = OFF_Q + 2 * Q_BYTES;
-  static constexpr int OFF_SC = OFF_MRG + MRG_BYTES;  // [NSTG][2][8] scales of a chunk's blocks
+  static constexpr int OFF_SC = OFF_MRG + MRG_BYTES;  // [NK][2][8] scales of a chunk's blocks
   static constexpr int NF = 4;                        // fragment entries in flight
-  static constexpr int OFF_FRAG = OFF_SC + NSTG * 64; // [NF] entries of 16 words
+  static constexpr int OFF_FRAG = OFF_SC + NK * 64;   // [NF] entries of 16 words
   static constexpr int OFF_QS = OFF_FRAG + NF * 64;   // [2][HPU] score factor of each head
   static constexpr int OFF_BAR = OFF_QS + 2 * 32;
-  static constexpr int B_KFULL = 0, B_KEMPTY = NSTG, B_VFULL = 2 * NSTG, B_VEMPTY = 3 * NSTG,
-                       B_QFULL = 4 * NSTG, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
+  static constexpr int B_KFULL = 0, B_KEMPTY = NK, B_VFULL = 2 * NK, B_VEMPTY = 2 * NK + NV,
+                       B_QFULL = 2 * NK + 2 * NV, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
                        B_SEMPTY = B_QFULL + 6, B_PFULL = B_QFULL + 8, B_PDONE = B_QFULL + 10,
                        B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13, B_FREE = B_QFULL + 14,
                        B_TKT = B_QFULL + 15, B_FFULL = B_QFULL + 16,
@@ -154,9 +158,9 @@ struct DecodePagedShape {
   // Chunks that a unit's beginning is charged with (measured with 1, 2, 3, 4, 6: 64 requests of up
   // to 4096, four heads 82, 75, 69, 68, 70 us; 16 of up to 20001, eight heads 86, 80, 77, 75, 73 us).
   static constexpr int PEN = HPU == 8 ? 6 : 4;
-  static_assert(3 * HPU <= 32, "a warp's rows of P");
+  static_assert(3 * HPU <= PM / 4, "a warp's rows of P");
   static_assert(MRG_O >= HPU * DECODE_PAGED_MAX_CTAS, "weights of the last fragment's CTA");
-  static_assert(NSTG >= 2, "at least two stages");
+  static_assert(NV >= 2 && NK >= 2, "at least two stages");
   static_assert(SMEM_BYTES <= (CTAS == 2 ? 115712 : 232448), "shared memory budget");
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
@@ -344,10 +348,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
                         const DecodePagedParams p) {
   using S = DecodePagedShape<DP, HPU>;
   using Walk = PagedWalk<S::PEN>;
-  constexpr int CK = S::CK, SPAN = S::SPAN, NSTG = S::NSTG, NQ = S::NQ, ROW = S::ROW;
+  constexpr int CK = S::CK, SPAN = S::SPAN, NK = S::NK, NV = S::NV, NPB = S::NPB, NQ = S::NQ, ROW = S::ROW;
   constexpr uint32_t SWZ = swizzle_code(SPAN);
   constexpr uint32_t IDESC_QK = idesc_f16(128, NQ, 0, 0, 0, 0);  // (format 0 of kind::f8f6f4: e4m3)
-  constexpr uint32_t IDESC_PV = idesc_f16(128, DP, 0, 0, 1, 1);
+  constexpr uint32_t IDESC_PV = idesc_f16(S::PM, DP, 0, 0, 1, 1);
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -382,9 +386,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   const int lane = tid & 31;
 
   if (tid == 128) {
-    for (int s = 0; s < NSTG; ++s) {
+    for (int s = 0; s < NK; ++s) {
       mbar_init(KFULL(s), 1 + 32);
       mbar_init(KEMPTY(s), 1 + 4);
+    }
+    for (int s = 0; s < NV; ++s) {
       mbar_init(VFULL(s), 1);
       mbar_init(VEMPTY(s), 1);
     }
@@ -427,7 +433,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     // ------------------------------------------------------------------ TMA: K and scales, V
     const bool is_k = warp == 4;
     const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
-    const uint32_t tile = is_k ? 0u : static_cast<uint32_t>(S::TILE);
+    const uint32_t ring = sbase + (is_k ? 0u : static_cast<uint32_t>(S::OFF_V));
+    const int ns = is_k ? NK : NV;
     const int ppc = CK >> p.block_log2;  // blocks of a whole chunk: 1, 2, 4, 8
     int g = 0;
     bool ok = true;
@@ -451,8 +458,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           id_next = at + 32 + lane < pages ? row[at + 32 + lane] : 0;
         }
         const int here = min(ppc, pages - first);
-        const int s = g % NSTG;
-        const uint32_t st = sbase + s * S::STAGE + tile;
+        const int s = g % ns;
+        const uint32_t st = ring + s * S::TILE;
         const uint32_t full = is_k ? KFULL(s) : VFULL(s);
         const int mine = __shfl_sync(0xffffffffu, id, (first - at) + (lane & 7));
         const bool in = (lane & 7) < here;
@@ -460,7 +467,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (bad && is_k && lane < 8) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(mine));
         const long long cell = bad ? static_cast<long long>(p.N) * p.Hkv  // beyond the map: zeros
                                    : static_cast<long long>(mine) * p.Hkv + f.kvh;
-        if (g >= NSTG) ok = mbar_wait(is_k ? KEMPTY(s) : VEMPTY(s), ((g / NSTG) - 1) & 1, failed, 801);
+        if (g >= ns) ok = mbar_wait(is_k ? KEMPTY(s) : VEMPTY(s), ((g / ns) - 1) & 1, failed, 801);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         if (lane == 0) mbar_expect_tx(full, static_cast<uint32_t>(here << p.block_log2) * DP);
         __syncwarp();
@@ -477,8 +484,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
     }
     // The last copies land before the CTA may exit.
-    for (int j = g > NSTG ? g - NSTG : 0; j < g; ++j)
-      mbar_wait_drain(is_k ? KFULL(j % NSTG) : VFULL(j % NSTG), (j / NSTG) & 1, 802);
+    for (int j = g > ns ? g - ns : 0; j < g; ++j)
+      mbar_wait_drain(is_k ? KFULL(j % ns) : VFULL(j % ns), (j / ns) & 1, 802);
   } else if (warp == 5) {
     // ------------------------------------------------------------------ MMA issuer
     const bool leader = elect_one();
@@ -504,13 +511,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       const uint64_t dq = smem_desc(sbase + S::OFF_Q + qb * S::Q_BYTES, 16, 8 * SPAN, SWZ);
       for (int j = 0; j <= n; ++j) {
         if (j < n) {  // S of chunk j
-          const int gj = g + j, s = gj % NSTG;
-          ok = mbar_wait(KFULL(s), (gj / NSTG) & 1, failed, 811);
+          const int gj = g + j, s = gj % NK;
+          ok = mbar_wait(KFULL(s), (gj / NK) & 1, failed, 811);
           if (ok && gj >= 2) ok = mbar_wait(SEMPTY(gj & 1), ((gj >> 1) - 1) & 1, failed, 812);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
           if (leader) {
-            const uint64_t dk = smem_desc(sbase + s * S::STAGE, 16, 8 * SPAN, SWZ);
+            const uint64_t dk = smem_desc(sbase + s * S::TILE, 16, 8 * SPAN, SWZ);
 #pragma unroll
             for (int kk = 0; kk < DP / 32; ++kk) {
               const uint32_t off_k = ((kk * 32) / SPAN) * CK * SPAN + (kk * 32) % SPAN;
@@ -525,20 +532,20 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           __syncwarp();
         }
         if (j > 0) {  // O of chunk j - 1
-          const int gj = g + j - 1, s = gj % NSTG;
-          ok = mbar_wait(PFULL(gj & 1), (gj >> 1) & 1, failed, 813);
-          if (ok) ok = mbar_wait(VFULL(s), (gj / NSTG) & 1, failed, 814);
+          const int gj = g + j - 1, s = gj % NV;
+          ok = mbar_wait(PFULL(gj % NPB), (gj / NPB) & 1, failed, 813);
+          if (ok) ok = mbar_wait(VFULL(s), (gj / NV) & 1, failed, 814);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
           if (leader) {
-            const uint64_t dp = smem_desc(sbase + S::OFF_P + (gj & 1) * S::P_BYTES, 16, 1024, 2);
-            const uint64_t dv = smem_desc(sbase + s * S::STAGE + S::TILE, CK * SPAN, 8 * SPAN, SWZ);
+            const uint64_t dp = smem_desc(sbase + S::OFF_P + (gj % NPB) * S::P_BYTES, 16, 8 * S::PM, swizzle_code(S::PM));
+            const uint64_t dv = smem_desc(sbase + S::OFF_V + s * S::TILE, CK * SPAN, 8 * SPAN, SWZ);
 #pragma unroll
             for (int kk = 0; kk < CK / 32; ++kk)
-              umma_f8_ss(tmem + S::TM_O, dp + static_cast<uint64_t>((kk * 32 * 128) >> 4),
+              umma_f8_ss(tmem + S::TM_O, dp + static_cast<uint64_t>((kk * 32 * S::PM) >> 4),
                          dv + static_cast<uint64_t>((kk * 32 * SPAN) >> 4), IDESC_PV,
                          (j > 1 || kk > 0) ? 1u : 0u);
-            umma_commit(PDONE(gj & 1));
+            umma_commit(PDONE(gj % NPB));
             umma_commit(VEMPTY(s));
           }
           __syncwarp();
@@ -665,12 +672,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
     int g = 0, mq = 0, tq = 0;  // chunks, combined column blocks, ticket barriers
-    // A key's row of P has only its warp's bytes, the rest stays zero.
+    // A key's row of P has only its warp's bytes (a 16- or 32-byte part), the rest stays zero.
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      st_shared_v4(sbase + S::OFF_P + tid * 128 + 16 * i, make_uint4(0, 0, 0, 0));
-      st_shared_v4(sbase + S::OFF_P + S::P_BYTES + tid * 128 + 16 * i, make_uint4(0, 0, 0, 0));
-    }
+    for (int i = 0; i < NPB * S::PM / 16; ++i)
+      st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + tid * S::PM + 16 * (i % (S::PM / 16)),
+                   make_uint4(0, 0, 0, 0));
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
@@ -702,10 +708,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         l[h] = 0.f;
       }
       for (int j = 0; j < f.chunks; ++j) {
-        const int gj = g + j, s = gj % NSTG;
+        const int gj = g + j, s = gj % NK;
         const int left = f.keys - j * CK;  // keys of this chunk and those behind it
         const bool valid = tid < left;
-        ok = mbar_wait(KFULL(s), (gj / NSTG) & 1, failed, 831);
+        ok = mbar_wait(KFULL(s), (gj / NK) & 1, failed, 831);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         const float* sc = reinterpret_cast<const float*>(sgen + S::OFF_SC + s * 64);
         const float ksc = valid ? sc[tid >> p.block_log2] : 1.0f;
@@ -771,11 +777,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
             for (int t = 0; t < 3; ++t) w[t * (HPU / 4) + h / 4] = a[t] | (b[t] << 16);
           }
         }
-        // P buffer gj & 1 was last read by PV(gj - 2); a moved reference rescales O, which holds
-        // PV up to gj - 1 of this fragment.
-        if (gj >= 2) ok = mbar_wait(PDONE(gj & 1), ((gj >> 1) - 1) & 1, failed, 833);
-        if (ok && moved && j > 0) ok = mbar_wait(PDONE((gj - 1) & 1), ((gj - 1) >> 1) & 1, failed, 834);
-        if (ok && left < CK) ok = mbar_wait(VFULL(s), (gj / NSTG) & 1, failed, 835);
+        // The P buffer was last read by PV(gj - NPB); a moved reference rescales O, which holds PV up
+        // to gj - 1 of this fragment.
+        if (gj >= NPB) ok = mbar_wait(PDONE(gj % NPB), ((gj / NPB) - 1) & 1, failed, 833);
+        if (NPB > 1 && ok && moved && j > 0) ok = mbar_wait(PDONE((gj - 1) % NPB), ((gj - 1) / NPB) & 1, failed, 834);
+        if (ok && left < CK) ok = mbar_wait(VFULL(gj % NV), (gj / NV) & 1, failed, 835);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         if (moved && j > 0) {
@@ -794,20 +800,20 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           }
           tmem_wait_st();
         }
-        const uint32_t prow = sbase + S::OFF_P + (gj & 1) * S::P_BYTES + tid * 128;
-        st_shared_v4(prow + (((2 * warp) ^ (tid & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
-        if constexpr (HPU == 8)
-          st_shared_v4(prow + (((2 * warp + 1) ^ (tid & 7)) << 4), make_uint4(w[4], w[5], w[6], w[7]));
+        const uint32_t pbuf = sbase + S::OFF_P + (gj % NPB) * S::P_BYTES;
+        st_shared_v4(pbuf + swz_chunk_offset<S::PM>(CK, tid, warp * (S::PM / 64)), make_uint4(w[0], w[1], w[2], w[3]));
+        if constexpr (S::PM == 128)
+          st_shared_v4(pbuf + swz_chunk_offset<S::PM>(CK, tid, 2 * warp + 1), make_uint4(w[4], w[5], w[6], w[7]));
         if (!valid) {
           // Rows behind the last key may hold anything, a NaN among it, and 0 x NaN is a NaN.
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c)
-            st_shared_v4(sbase + s * S::STAGE + S::TILE + ((c * 16) / SPAN) * CK * SPAN + tid * SPAN + (c * 16) % SPAN,
+            st_shared_v4(sbase + S::OFF_V + (gj % NV) * S::TILE + ((c * 16) / SPAN) * CK * SPAN + tid * SPAN + (c * 16) % SPAN,
                          make_uint4(0, 0, 0, 0));
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(PFULL(gj & 1));
+        mbar_arrive(PFULL(gj % NPB));
       }
       if (!ok) break;
       g += f.chunks;
@@ -831,7 +837,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h through shared
       // memory, then a thread sums the 12 of an output.
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) & 1), ((g - 1) >> 1) & 1, failed, 836)))) break;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) % NPB), ((g - 1) / NPB) & 1, failed, 836)))) break;
       tc_fence_after();
       float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
       float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
@@ -878,7 +884,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         if (f.nf > 1 && cb == 0 && tid < HPU) part_l[f.slot * HPU + tid] = top;
         // A thread takes a column and every (128 / columns)-th head.
-        const int nd_log2 = p.D >= S::CB ? (S::CB == 128 ? 7 : (S::CB == 64 ? 6 : 5)) : 4;  // (4: head_dim 16)
+        const int nd_log2 = p.D >= S::CB ? (S::CB == 64 ? 6 : 5) : 4;  // (4: head_dim 16)
         const int d = tid & ((1 << nd_log2) - 1), hg = tid >> nd_log2;
         const int hs = 128 >> nd_log2;
         float A[HPU];

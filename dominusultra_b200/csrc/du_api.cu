@@ -1309,7 +1309,7 @@ int paged_hpu(int heads) { return heads <= 1 ? 1 : (heads <= 2 ? 2 : (heads <= 4
 
 // CTAs of the persistent grid: the resident ones, or as many as a full block table could occupy.
 int paged_grid(int B, int Hq, int Hkv, int D, int block_size, int max_blocks) {
-  long long ctas = static_cast<long long>(sm_count()) * (D <= 64 ? 2 : 1);
+  long long ctas = static_cast<long long>(sm_count()) * (D <= 128 ? 2 : 1);
   if (ctas > du::DECODE_PAGED_MAX_CTAS) ctas = du::DECODE_PAGED_MAX_CTAS;
   const long long units = static_cast<long long>(B) * Hkv * paged_group_chunks(Hq / Hkv);
   const long long per_unit = (static_cast<long long>(max_blocks) * block_size + 127) / 128;
