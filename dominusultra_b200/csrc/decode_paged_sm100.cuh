@@ -52,7 +52,7 @@ struct DecodePagedParams {
   void* out;            // [B, Hq, D]
   int* cnt;             // [gridDim.x] tickets, zero between calls
   float* part;          // [2 gridDim.x][HPU][D] partial outs, then [2 gridDim.x][HPU] log2 of their sums
-  long long positions;
+  int max_len;          // tokens that the table's row and the rope tables cover
   int D, bf16;
   int B, Hq, Hkv, G, N, width;
   int block, block_log2;
@@ -215,7 +215,7 @@ struct PagedWalk {
   }
   __device__ __forceinline__ static int tokens(const DecodePagedParams& p, int b) {
     const int n = p.lens[b];
-    return (n < 0 || n > p.width * p.block || n > p.positions) ? 0 : n;
+    return static_cast<unsigned>(n) > static_cast<unsigned>(p.max_len) ? 0 : n;
   }
   __device__ __forceinline__ static int chunks(int n) { return n > 128 ? (n + 127) >> 7 : 1; }
   // The CTA's share (a whole warp; `lane` its lane).
@@ -223,13 +223,13 @@ struct PagedWalk {
     PagedStart st;
     const int ups = p.Hkv * p.n_gchunk;
     const int grid = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
-    int total = 0;
+    // The first 32 requests' chunks stay in a register: most batches are no larger.
+    const int len0 = lane < p.B ? p.lens[lane] : 0;
+    const int nc0 = chunks(static_cast<unsigned>(len0) > static_cast<unsigned>(p.max_len) ? 0 : len0);
+    auto chunks_of = [&](int b) { return b < 32 ? nc0 : chunks(tokens(p, b)); };
+    int total = lane < p.B ? nc0 : 0;
 #pragma unroll 4
-    for (int b = lane; b < p.B; b += 32) {
-      const int n = tokens(p, b);
-      if (c == 0 && n != p.lens[b]) record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
-      total += chunks(n);
-    }
+    for (int b = 32 + lane; b < p.B; b += 32) total += chunks(tokens(p, b));
     total = static_cast<int>(__reduce_add_sync(0xffffffffu, total));
     // Pieces: with at most x chunks each, the units of request b make ups ceil(chunks_b / x) of
     // them. x = per .. per + 3 are tried; beyond that, fragments of equal ranges cost less.
@@ -241,7 +241,7 @@ struct PagedWalk {
       for (x = per; x <= per + DECODE_PAGED_PIECE_SLACK && !cut; ++x) {
         int sum = 0;
 #pragma unroll 1
-        for (int b = lane; b < p.B; b += 32) sum += small_div(chunks(tokens(p, b)) + x - 1, x);
+        for (int b = lane; b < p.B; b += 32) sum += small_div(chunks_of(b) + x - 1, x);
         cut = static_cast<int>(__reduce_add_sync(0xffffffffu, sum)) * ups <= grid;
       }
       --x;  // (the one that was tried last)
@@ -260,11 +260,12 @@ struct PagedWalk {
     st.cur = st.hi = st.b = st.base = st.pieces = 0;  // no share
     // The request that holds `cur`.
     int before = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.B && cur < hi; b0 += 32) {
       const int b = b0 + lane;
       int k = 0;
       if (b < p.B) {
-        const int nc = chunks(tokens(p, b));
+        const int nc = chunks_of(b);
         k = cut ? small_div(nc + x - 1, x) : nc + PEN;
       }
       int in = k;
@@ -424,6 +425,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   }
   // Launched as a programmatic dependent: what is above runs beside the stream's previous kernel.
   griddep_wait();
+  if (warp == 5) griddep_launch_dependents();  // (the columns are taken)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -576,6 +578,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
       st_shared_v4(sbase + S::OFF_Q + 16 * i, make_uint4(0, 0, 0, 0));
     __syncwarp();
+    // Lengths out of range are reported once, by the first CTA.
+    auto report = [&]() {
+      for (int b = lane; b < p.B; b += 32)
+        if (static_cast<unsigned>(p.lens[b]) > static_cast<unsigned>(p.max_len))
+          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
+    };
     // Entry k is published before the queries of entry k - 1 are prepared.
     bool ended = false;
     for (int k = 0;; ++k) {
@@ -591,7 +599,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         __syncwarp();
       }
-      if (k == 0) continue;
+      if (k == 0) {
+        if (blockIdx.x == 0) report();
+        continue;
+      }
       const int it = k - 1, qb = it & 1;
       // (entry k - 1 stays until the softmax warps have read it, which wait for its queries)
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);

@@ -1527,7 +1527,8 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.out = out;
   prm.cnt = tickets;
   prm.part = static_cast<float*>(workspace);
-  prm.positions = rope_positions;
+  const long long cover = static_cast<long long>(max_blocks) * block_size;
+  prm.max_len = static_cast<int>(cover < rope_positions ? cover : rope_positions);
   prm.D = D;
   prm.bf16 = dtype == DU_DTYPE_BF16;
   prm.B = B;
