@@ -124,11 +124,12 @@ struct DecodePagedShape {
   static constexpr int PM = HPU <= 4 ? 64 : 128;      // rows of P (M of P V): 16 or 32 per warp
   static constexpr int P_BYTES = CK * PM;             // [key][PM rows] bytes, swizzled
   static constexpr int Q_BYTES = ((NQ * DP + 1023) / 1024) * 1024;
-  static constexpr int CB = DP == 256 ? 64 : (DP == 128 ? 32 : DP);  // columns of O combined at a time
-  static constexpr int ROW = CB + 4;                  // floats per row of the combine area
-  static constexpr int MRG_O = 12 * HPU * ROW;        // [4 warps][3 HPU rows][ROW] floats
-  static constexpr int MRG_BYTES = ((MRG_O + 8 * HPU) * 4 + 127) / 128 * 128;
-  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + MRG_BYTES + 2560;
+  // Rows of O are combined where P is, CB columns at a time (and P's zeros put back): 4 warps x
+  // 3 HPU rows of ROW floats.
+  static constexpr int CB = DP < 64 ? DP : (DP == 128 && HPU == 8 ? 32 : 64);
+  static constexpr int ROW = CB + 4;
+  static constexpr int ML_BYTES = ((8 * HPU * 4) + 127) / 128 * 128;  // maxima and sums of the warps
+  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + 2560;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
   static constexpr int TILES = (BUDGET - FIXED) / TILE;
   static constexpr int NV = TILES / 2 > 8 ? 8 : TILES / 2;            // stages of V
@@ -136,17 +137,18 @@ struct DecodePagedShape {
   static constexpr int OFF_V = NK * TILE;
   static constexpr int OFF_P = OFF_V + NV * TILE;
   static constexpr int OFF_Q = OFF_P + NPB * P_BYTES;
-  static constexpr int OFF_MRG = OFF_Q + 2 * Q_BYTES;
-  static constexpr int OFF_SC = OFF_MRG + MRG_BYTES;  // [NK][2][8] scales of a chunk's blocks
+  static constexpr int OFF_ML = OFF_Q + 2 * Q_BYTES;
+  static constexpr int OFF_SC = OFF_ML + ML_BYTES;  // [NK][2][8] scales of a chunk's blocks
   static constexpr int NF = 4;                        // fragment entries in flight
   static constexpr int OFF_FRAG = OFF_SC + NK * 64;   // [NF] entries of 16 words
-  static constexpr int OFF_QS = OFF_FRAG + NF * 64;   // [2][HPU] score factor of each head
+  static constexpr int OFF_OWED = OFF_FRAG + NF * 64; // [2] entries of units to join
+  static constexpr int OFF_QS = OFF_OWED + 2 * 64;    // [2][HPU] score factor of each head
   static constexpr int OFF_BAR = OFF_QS + 2 * 32;
   static constexpr int B_KFULL = 0, B_KEMPTY = NK, B_VFULL = 2 * NK, B_VEMPTY = 2 * NK + NV,
                        B_QFULL = 2 * NK + 2 * NV, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
                        B_SEMPTY = B_QFULL + 6, B_PFULL = B_QFULL + 8, B_PDONE = B_QFULL + 10,
                        B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13, B_FREE = B_QFULL + 14,
-                       B_TKT = B_QFULL + 15, B_FFULL = B_QFULL + 16,
+                       B_FFULL = B_QFULL + 15,
                        B_FEMPTY = B_FFULL + NF;
   static constexpr int N_BAR = B_FEMPTY + NF;
   static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;  // 16 words
@@ -159,7 +161,8 @@ struct DecodePagedShape {
   // to 4096, four heads 82, 75, 69, 68, 70 us; 16 of up to 20001, eight heads 86, 80, 77, 75, 73 us).
   static constexpr int PEN = HPU == 8 ? 6 : 4;
   static_assert(3 * HPU <= PM / 4, "a warp's rows of P");
-  static_assert(MRG_O >= HPU * DECODE_PAGED_MAX_CTAS, "weights of the last fragment's CTA");
+  static_assert(12 * HPU * ROW * 4 <= NPB * P_BYTES, "rows of O where P is");
+  static_assert(HPU * DECODE_PAGED_MAX_CTAS * 4 <= NPB * P_BYTES, "weights of a unit's fragments where P is");
   static_assert(NV >= 2 && NK >= 2, "at least two stages");
   static_assert(SMEM_BYTES <= (CTAS == 2 ? 115712 : 232448), "shared memory budget");
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
@@ -371,16 +374,17 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   auto SEMPTY = [&](int i) { return bar(S::B_SEMPTY + i); };
   auto PFULL = [&](int i) { return bar(S::B_PFULL + i); };
   auto PDONE = [&](int i) { return bar(S::B_PDONE + i); };    // PV of even / odd chunks complete
-  // rows of O in the combine area, rows read (and partials stored), ticket taken
-  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_FREE = bar(S::B_FREE), BAR_TKT = bar(S::B_TKT), BAR_DRAIN = bar(S::B_DRAIN);
+  // rows of O in the combine area; rows read (and partials stored)
+  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_FREE = bar(S::B_FREE), BAR_DRAIN = bar(S::B_DRAIN);
   uint32_t* misc = reinterpret_cast<uint32_t*>(sgen + S::OFF_MISC);
   volatile int* failed = reinterpret_cast<volatile int*>(misc + 1);
   volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
-  volatile int* verdict = reinterpret_cast<volatile int*>(misc + 3);  // last of the unit's fragments
+  volatile int* n_owed = reinterpret_cast<volatile int*>(misc + 3);
   PagedStart* start = reinterpret_cast<PagedStart*>(misc + 4);
-  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_MRG);  // o [4][3 HPU][ROW], m [4][HPU], l [4][HPU]
-  float* mrg_m = mrg + S::MRG_O;
+  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_P);  // o [4][3 HPU][ROW]
+  float* mrg_m = reinterpret_cast<float*>(sgen + S::OFF_ML);  // m [4][HPU], l [4][HPU]
   float* mrg_l = mrg_m + 4 * HPU;
+  PagedFrag* owed = reinterpret_cast<PagedFrag*>(sgen + S::OFF_OWED);  // units for this CTA to join
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -409,10 +413,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     }
     mbar_init(BAR_MRG, 128);
     mbar_init(BAR_FREE, 128);
-    mbar_init(BAR_TKT, 128);
     mbar_init(BAR_DRAIN, 1);
     *failed = 0;
     *emitted = 0;
+    *n_owed = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -682,12 +686,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     // ------------------------------------------------------------------ warps 0-3: softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
-    int g = 0, mq = 0, tq = 0;  // chunks, combined column blocks, ticket barriers
-    // A key's row of P has only its warp's bytes (a 16- or 32-byte part), the rest stays zero.
-#pragma unroll
-    for (int i = 0; i < NPB * S::PM / 16; ++i)
-      st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + tid * S::PM + 16 * (i % (S::PM / 16)),
-                   make_uint4(0, 0, 0, 0));
+    int g = 0, mq = 0;  // chunks, combined column blocks
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
@@ -712,6 +711,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (tid == 0) *emitted = it + 1;
         continue;
       }
+      // A key's row of P has only its warp's bytes (a 16- or 32-byte part); the rest is zero, once
+      // the last fragment's rows of O, which lie there too, have been read.
+      if (mq > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 838)))) break;
+#pragma unroll
+      for (int i = 0; i < NPB * S::PM / 16; ++i)
+        st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + tid * S::PM + 16 * (i % (S::PM / 16)),
+                     make_uint4(0, 0, 0, 0));
       float m[HPU], l[HPU];
 #pragma unroll
       for (int h = 0; h < HPU; ++h) {
@@ -852,13 +858,15 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       tc_fence_after();
       float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
       float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
+      float fac = 0.f;
+#pragma unroll 1
       for (int cb = 0; cb < DP && ok; cb += S::CB) {
         {
           float o[S::CB];
 #pragma unroll
           for (int c = 0; c < S::CB; c += 16) tmem_ld16(tmem + lane_off + S::TM_O + cb + c, o + c);
-          // The rows combined before have been read.
-          if (mq > 0) ok = mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 838);
+          // The columns combined before have been read.
+          if (cb > 0) ok = mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 837);
           tmem_wait_ld();
           if (lane < 3 * HPU) {
             float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW);
@@ -880,20 +888,18 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         mbar_arrive(BAR_MRG);
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
         // Lane w HPU + h: the factor of warp w's rows of head h, 2^(m_w - M) / L.
-        float fac, top;
-        {
+        if (cb == 0) {
           const int i = lane % (4 * HPU);
           const float mi = mrg_m[i];
-          top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
+          float top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2 * HPU));
           fac = ex2(mi - top);
           float L = mrg_l[i] * fac;
           L += __shfl_xor_sync(0xffffffffu, L, HPU);
           L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
           fac = fac / L;
-          top += lg2(L);  // log2 of the sum
+          if (f.nf > 1 && tid < HPU) part_l[f.slot * HPU + tid] = top + lg2(L);  // log2 of the sum
         }
-        if (f.nf > 1 && cb == 0 && tid < HPU) part_l[f.slot * HPU + tid] = top;
         // A thread takes a column and every (128 / columns)-th head.
         const int nd_log2 = p.D >= S::CB ? (S::CB == 64 ? 6 : 5) : 4;  // (4: head_dim 16)
         const int d = tid & ((1 << nd_log2) - 1), hg = tid >> nd_log2;
@@ -922,95 +928,91 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         ++mq;
       }
       if (!ok) break;
-      if (f.nf > 1) {
-        // A ticket on the unit's counter. The partial stores reach thread 0 through the barrier; its
-        // acquire-release add makes them visible before the ticket and, after the last ticket,
-        // the other fragments' partials visible to this CTA.
-        if (tid == 0) {
-          int last = 0;
-          if (mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 842)) {
-            last = atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1;
-            if (last) p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
+      if (tid == 0) {
+        if (f.nf > 1) {
+          // A ticket on the unit's counter. The partial stores reach this thread through the barrier;
+          // its acquire-release add makes them visible before the ticket and, after the last
+          // ticket, the other fragments' partials visible to this CTA.
+          if (mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 839)) {
+            if (atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1) {
+              p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
+              owed[*n_owed] = f;
+              *n_owed = *n_owed + 1;
+            }
             *emitted = it + 1;
           }
-          *verdict = last;
+        } else {
+          *emitted = it + 1;
         }
-        mbar_arrive(BAR_TKT);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 839)))) break;
-        ++tq;
-        if (*verdict) {
-          // The unit's other fragments are done. A thread takes four columns of a head at a time; the
-          // rows of the first KB fragments are on their way while the weights are found (a warp
-          // per head, a lane per fragment).
-          constexpr int KB = S::CTAS == 2 ? 4 : 16;  // (registers)
-          auto slot_of = [&](int k) { return k == 0 ? 2 * f.c0 + 1 : 2 * (f.c0 + k); };
-          const int q4 = p.D >> 2, items = f.nh * q4;
-          auto load = [&](float4 (&o)[KB], int i, int k0) {
-            const int h = i / q4, d = 4 * (i - h * q4);
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-              if (i < items && k0 + k < f.nf)
-                o[k] = __ldcg(reinterpret_cast<const float4*>(
-                    p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d));
-          };
-          float4 o[KB];
-          load(o, tid, 0);
-          float* wt = mrg;  // [HPU][nf]: nf <= gridDim.x <= DECODE_PAGED_MAX_CTAS
-          for (int h = warp; h < f.nh; h += 4) {
-            float M = -INFINITY, L = 0.f;
-            for (int k = lane; k < f.nf; k += 32) {
-              const float x = __ldcg(part_l + slot_of(k) * HPU + h);
-              wt[h * f.nf + k] = x;
-              M = fmaxf(M, x);
-            }
-            M = warp_max(M);
-            for (int k = lane; k < f.nf; k += 32) {
-              const float e = ex2(wt[h * f.nf + k] - M);
-              wt[h * f.nf + k] = e;
-              L += e;
-            }
-#pragma unroll
-            for (int o2 = 16; o2 >= 1; o2 >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o2);
-            const float inv = 1.0f / L;
-            for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
-          }
-          mbar_arrive(BAR_TKT);
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 840)))) break;
-          ++tq;
-          for (int i = tid; i < items; i += 128) {
-            const int h = i / q4, d = 4 * (i - h * q4);
-            float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-            for (int k0 = 0; k0 < f.nf; k0 += KB) {
-              if (i != tid || k0 > 0) load(o, i, k0);
-#pragma unroll
-              for (int k = 0; k < KB; ++k) {
-                if (k0 + k >= f.nf) break;
-                const float x = wt[h * f.nf + k0 + k];
-                A.x = fmaf(o[k].x, x, A.x);
-                A.y = fmaf(o[k].y, x, A.y);
-                A.z = fmaf(o[k].z, x, A.z);
-                A.w = fmaf(o[k].w, x, A.w);
-              }
-            }
-            store_out(row0 + h, d, A.x);
-            store_out(row0 + h, d + 1, A.y);
-            store_out(row0 + h, d + 2, A.z);
-            store_out(row0 + h, d + 3, A.w);
-          }
-          // The weights are read: the combine area is free again.
-          mbar_arrive(BAR_TKT);
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_TKT, tq & 1, failed, 841)))) break;
-          ++tq;
-        }
-      } else if (tid == 0) {
-        *emitted = it + 1;
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  // Units whose last ticket was this CTA's, of its first and its last fragment at most. A thread takes
+  // four columns of a head at a time; the rows of the first KB fragments are on their way while
+  // the weights are found, a warp per head, a lane per fragment.
+  for (int e = 0; e < *n_owed; ++e) {
+    const PagedFrag f = owed[e];
+    constexpr int KB = 16;
+    auto slot_of = [&](int k) { return k == 0 ? 2 * f.c0 + 1 : 2 * (f.c0 + k); };
+    const int q4 = p.D >> 2, items = f.nh * q4;
+    auto load = [&](float4 (&o)[KB], int i, int k0) {
+      const int h = small_div(i, q4), d = 4 * (i - h * q4);
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+        if (i < items && k0 + k < f.nf)
+          o[k] = __ldcg(reinterpret_cast<const float4*>(
+              p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d));
+    };
+    float4 o[KB];
+    load(o, tid, 0);
+    const float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
+    float* wt = mrg;  // [HPU][nf]: nf <= gridDim.x <= DECODE_PAGED_MAX_CTAS
+    for (int h = warp; h < f.nh; h += S::NTHREADS / 32) {
+      float M = -INFINITY, L = 0.f;
+      for (int k = lane; k < f.nf; k += 32) {
+        const float x = __ldcg(part_l + slot_of(k) * HPU + h);
+        wt[h * f.nf + k] = x;
+        M = fmaxf(M, x);
+      }
+      M = warp_max(M);
+      for (int k = lane; k < f.nf; k += 32) {
+        const float x = ex2(wt[h * f.nf + k] - M);
+        wt[h * f.nf + k] = x;
+        L += x;
+      }
+#pragma unroll
+      for (int o2 = 16; o2 >= 1; o2 >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o2);
+      const float inv = 1.0f / L;
+      for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
+    }
+    __syncthreads();
+    for (int i = tid; i < items; i += S::NTHREADS) {
+      const int h = small_div(i, q4), d = 4 * (i - h * q4);
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int k0 = 0; k0 < f.nf; k0 += KB) {
+        if (i != tid || k0 > 0) load(o, i, k0);
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          if (k0 + k >= f.nf) break;
+          const float x = wt[h * f.nf + k0 + k];
+          A.x = fmaf(o[k].x, x, A.x);
+          A.y = fmaf(o[k].y, x, A.y);
+          A.z = fmaf(o[k].z, x, A.z);
+          A.w = fmaf(o[k].w, x, A.w);
+        }
+      }
+      const long long at = (static_cast<long long>(f.b) * p.Hq + f.h0 + h) * p.D + d;
+      uint2 w;
+      if (p.bf16) w = make_uint2(pack2<true>(A.x, A.y), pack2<true>(A.z, A.w));
+      else w = make_uint2(pack2<false>(A.x, A.y), pack2<false>(A.z, A.w));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = w;
+    }
+    __syncthreads();
+  }
   if (*failed) {
     // A wait ran out (reported in the status words): NaN for what this CTA still owes, and its
     // tickets, so that the counters return to zero.
