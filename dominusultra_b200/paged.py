@@ -16,6 +16,7 @@ and tables stay on the GPU: no call synchronises, and each can be captured into 
 
 from __future__ import annotations
 
+import contextlib
 import threading
 from typing import Tuple
 
@@ -25,10 +26,7 @@ from . import _lib
 from .attention import (
     _RETIRED,
     _aligned,
-    _cached_workspace,
-    _dtype_code,
     _OnDevice,
-    _ptr,
     _stream,
     _validate_attention_tensors,
     _validate_head_dim,
@@ -41,8 +39,23 @@ __all__ = [
 ]
 
 
+_I32, _I64, _F32, _E4M3 = torch.int32, torch.int64, torch.float32, torch.float8_e4m3fn
+_F16, _BF16 = torch.float16, torch.bfloat16
+_BLOCK_SIZES = (16, 32, 64, 128)
+_HEAD_DIMS = (16, 32, 64, 128, 256)
+_CODES = {_F16: _lib.DU_DTYPE_F16, _BF16: _lib.DU_DTYPE_BF16}
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _fit(t: torch.Tensor, dtype: torch.dtype, index: int) -> bool:
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
 def _validate_block_size(block_size: int) -> None:
-    if block_size not in (16, 32, 64, 128):
+    if block_size not in _BLOCK_SIZES:
         raise ValueError("block_size must be 16, 32, 64 or 128")
 
 
@@ -136,8 +149,8 @@ def _validate_tables_like(cos, sin, head_dim, device, dtype) -> None:
 _WS_SIZES = {}
 
 
-def _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, device) -> int:
-    key = (B, Hq, Hkv, D, block_size, max_blocks, device.index)
+def _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, index) -> int:
+    key = (B, Hq, Hkv, D, block_size, max_blocks, index)
     n = _WS_SIZES.get(key)
     if n is None:
         n = int(_lib.load().du_decode_paged_workspace_size(B, Hq, Hkv, D, block_size, max_blocks))
@@ -152,37 +165,52 @@ _SLABS = {}
 _SLAB_LOCK = threading.Lock()
 
 
-def _decode_scratch(nbytes: int, device: torch.device, stream: int):
+# Scratch of eager calls per (device, stream): [tickets, workspace], the workspace grown on demand.
+_SCRATCH = {}
+
+
+def _decode_scratch(nbytes: int, device: torch.device, index: int, stream: int):
     """(tickets, workspace, keep-alive tensors) of a paged decode on torch's current stream.
 
     Eager calls share a pair per (device, stream): calls on one stream run in order. A call that
     is being captured gets a workspace from the graph's own memory and tickets of its own.
     """
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    capturing = torch.cuda.is_current_stream_capturing()
-    if not capturing:
-        tickets, _ = _cached_workspace("decode_paged_tickets", 4 * _lib.DU_PAGED_TICKETS, device, stream)
-        ws, _ = _cached_workspace("decode_paged", nbytes, device, stream)
+    if not torch.cuda.is_current_stream_capturing():
+        pair = _SCRATCH.get((index, stream))
         slab = _SLABS.get(index)
-        if slab is None or slab[1] > _SLAB_WORDS // 2:
-            # (a copy from the host has ended when it returns: the zeros are there for any stream)
-            zeros = torch.zeros(_SLAB_WORDS, dtype=torch.int32).to(device)
-            with _SLAB_LOCK:
-                _SLABS[index] = [zeros, 0]
-                if slab is not None:
-                    _RETIRED.append(slab[0])
-        return tickets, ws, None
+        if pair is None or pair[2] < nbytes or slab is None or slab[1] > _SLAB_WORDS // 2:
+            pair = _grow_scratch(nbytes, device, index, stream)
+        return pair[0], pair[1], None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     with _SLAB_LOCK:
         slab = _SLABS.get(index)
         if slab is not None and slab[1] + _lib.DU_PAGED_TICKETS <= _SLAB_WORDS:
-            tickets = slab[0][slab[1] : slab[1] + _lib.DU_PAGED_TICKETS]
+            tickets = slab[0].data_ptr() + 4 * slab[1]
             slab[1] += _lib.DU_PAGED_TICKETS
-            return tickets.data_ptr(), ws.data_ptr(), ws
+            return tickets, ws.data_ptr(), ws
     # no slab yet (the process's first call), or more than half a slab of captures since the last
     # eager call: zeroed inside the graph, by a node of its own
     tickets = torch.zeros(_lib.DU_PAGED_TICKETS, dtype=torch.int32, device=device)
     return tickets.data_ptr(), ws.data_ptr(), (ws, tickets)
+
+
+def _grow_scratch(nbytes: int, device: torch.device, index: int, stream: int):
+    """A (device, stream)'s scratch of at least nbytes, and a ticket slab with room for captures."""
+    with _SLAB_LOCK:
+        slab = _SLABS.get(index)
+        if slab is None or slab[1] > _SLAB_WORDS // 2:
+            if slab is not None:
+                _RETIRED.append(slab[0])  # graphs count in it
+            # (a copy from the host has ended when it returns: the zeros are there for any stream)
+            _SLABS[index] = [torch.zeros(_SLAB_WORDS, dtype=torch.int32).to(device), 0]
+        pair = _SCRATCH.get((index, stream))
+        if pair is None or pair[2] < nbytes:
+            size = max(nbytes, 2 * pair[2] if pair is not None else 0)
+            tickets = pair[3] if pair is not None else torch.zeros(_lib.DU_PAGED_TICKETS, dtype=torch.int32, device=device)
+            ws = torch.empty(size, dtype=torch.uint8, device=device)
+            pair = (tickets.data_ptr(), ws.data_ptr(), size, tickets, ws)
+            _SCRATCH[(index, stream)] = pair
+    return pair
 
 
 def dominus_ultra_paged_tables(
@@ -224,6 +252,38 @@ def dominus_ultra_paged_tables(
             - seqlens: [batch] int32, the lengths that the requests have now
             - free_state: [2] int32
     """
+    shape = block_table.shape
+    index = block_table.get_device()
+    # One look at what every call has to have; where it fails, the checks by name.
+    if not (
+        len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and index >= 0
+        and block_size in _BLOCK_SIZES and max_new >= 0
+        and _fit(block_table, _I32, index) and _fit(free_blocks, _I32, index) and _fit(free_state, _I32, index)
+        and free_blocks.dim() == 1 and free_blocks.shape[0] > 0 and free_state.shape == (2,)
+        and _fit(cache_seqlens, _I32, index) and _fit(new_seqlens, _I32, index)
+        and cache_seqlens.shape == shape[:1] and new_seqlens.shape == shape[:1]
+    ):
+        cache_seqlens, new_seqlens = _check_tables(
+            block_table, cache_seqlens, new_seqlens, free_blocks, free_state, block_size, max_new
+        )
+    batch, max_blocks = shape
+    device = block_table.device
+    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
+        slots = block_table.new_empty((batch, max_new))
+        seqlens = torch.empty_like(cache_seqlens)
+        state = torch.empty_like(free_state)
+        rc = _lib.load().du_paged_tables(
+            block_table.data_ptr(), cache_seqlens.data_ptr(), new_seqlens.data_ptr(), free_blocks.data_ptr(),
+            free_state.data_ptr(), slots.data_ptr(), seqlens.data_ptr(), state.data_ptr(), batch, max_blocks,
+            free_blocks.shape[0], block_size, max_new, _stream(device),
+        )
+    if rc:
+        _lib.check(rc, "du_paged_tables")
+    return slots, seqlens, state
+
+
+def _check_tables(block_table, cache_seqlens, new_seqlens, free_blocks, free_state, block_size, max_new):
+    """The refusals of dominus_ultra_paged_tables; returns the lengths as int32 on the device."""
     if block_table.ndim != 2 or block_table.shape[0] <= 0 or block_table.shape[1] <= 0:
         raise ValueError("block_table must be a non-empty [batch, max_blocks] tensor")
     batch, max_blocks = block_table.shape
@@ -247,20 +307,8 @@ def dominus_ultra_paged_tables(
             _check_host_lengths(name, t, max_blocks * block_size)
         elif t.device != device:
             raise ValueError(f"{name} must be on the device of block_table (or on the CPU)")
-
-    lib = _lib.load()
     with _OnDevice(device):
-        old, new = _device_int32(cache_seqlens, device), _device_int32(new_seqlens, device)
-        slots = torch.empty((batch, max_new), dtype=torch.int32, device=device)
-        seqlens = torch.empty((batch,), dtype=torch.int32, device=device)
-        state = torch.empty((2,), dtype=torch.int32, device=device)
-        rc = lib.du_paged_tables(
-            _ptr(block_table), _ptr(old), _ptr(new), _ptr(free_blocks), _ptr(free_state),
-            _ptr(slots), _ptr(seqlens), _ptr(state), batch, max_blocks, free_blocks.shape[0],
-            block_size, max_new, _stream(device),
-        )
-    _lib.check(rc, "du_paged_tables")
-    return slots, seqlens, state
+        return _device_int32(cache_seqlens, device), _device_int32(new_seqlens, device)
 
 
 def dominus_ultra_paged_write(
@@ -295,6 +343,49 @@ def dominus_ultra_paged_write(
         cache_seqlens: [batch] integer lengths before these tokens (what the tables call took)
         cos, sin: tables from precompute_rope_cos_sin covering the new positions
     """
+    shape, cache = k_new.shape, k_cache.shape
+    index, dtype = k_new.get_device(), k_new.dtype
+    if not (
+        len(shape) == 4 and len(cache) == 4 and index >= 0 and dtype in _CODES
+        and k_new.is_contiguous() and _fit(v_new, dtype, index) and v_new.shape == shape
+        and _fit(cos, dtype, index) and _fit(sin, dtype, index)
+        and cos.dim() == 2 and sin.dim() == 2 and cos.shape[1] * 2 == shape[3] and sin.shape[1] * 2 == shape[3]
+        and cos.shape[0] > 0 and sin.shape[0] > 0
+        and shape[0] > 0 and shape[1] > 0 and shape[2] > 0 and shape[3] in _HEAD_DIMS
+        and _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index)
+        and cache[1] == shape[1] and cache[3] == shape[3]
+        and _fit(slots, _I32, index) and slots.shape == (shape[0], shape[2])
+        and _fit(cache_seqlens, _I32, index) and cache_seqlens.shape == shape[:1]
+    ):
+        cache_seqlens = _check_write(k_new, v_new, k_cache, v_cache, k_scale, v_scale, slots, cache_seqlens, cos, sin)
+    B, Hkv, T, D = shape
+    device = k_new.device
+    k, v, c, s = k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
+        if (k | v | c | s) & 15:
+            k_new, v_new, cos, sin = (_aligned(t) for t in (k_new, v_new, cos, sin))
+            k, v, c, s = k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+        rc = _lib.load().du_paged_write(
+            k, v, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(),
+            cache_seqlens.data_ptr(), c, s, B, Hkv, T, D, cache[0], cache[2], _CODES[dtype],
+            min(cos.shape[0], sin.shape[0]), _stream(device),
+        )
+    if rc:
+        _lib.check(rc, "du_paged_write")
+
+
+def _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index) -> bool:
+    return (
+        _fit(k_cache, _E4M3, index) and _fit(v_cache, _E4M3, index) and v_cache.shape == cache
+        and cache[0] > 0 and cache[1] > 0 and cache[2] in _BLOCK_SIZES
+        and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
+        and _fit(k_scale, _F32, index) and _fit(v_scale, _F32, index)
+        and k_scale.shape == cache[:2] and v_scale.shape == cache[:2]
+    )
+
+
+def _check_write(k_new, v_new, k_cache, v_cache, k_scale, v_scale, slots, cache_seqlens, cos, sin):
+    """The refusals of dominus_ultra_paged_write; returns the lengths as int32 on the device."""
     if k_new.ndim != 4 or v_new.ndim != 4 or k_cache.ndim != 4 or v_cache.ndim != 4:
         raise ValueError("k_new, v_new, k_cache, and v_cache must be rank-4 tensors")
     B, Hkv, T, D = k_new.shape
@@ -313,22 +404,12 @@ def dominus_ultra_paged_write(
     _validate_paged_cache(k_cache, v_cache, k_scale, v_scale, device)
     _validate_int32("slots", slots, device)
     _validate_tables_like(cos, sin, D, device, k_new.dtype)
-    positions = min(cos.shape[0], sin.shape[0])
     if cache_seqlens.device.type == "cpu":
-        _check_host_lengths("cache_seqlens", cache_seqlens, positions)
+        _check_host_lengths("cache_seqlens", cache_seqlens, min(cos.shape[0], sin.shape[0]))
     elif cache_seqlens.device != device:
         raise ValueError("cache_seqlens must be on the device of k_new (or on the CPU)")
-
-    lib = _lib.load()
     with _OnDevice(device):
-        k_new, v_new, cos, sin = (_aligned(t) for t in (k_new, v_new, cos, sin))
-        past = _device_int32(cache_seqlens, device)
-        rc = lib.du_paged_write(
-            _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-            _ptr(slots), _ptr(past), _ptr(cos), _ptr(sin), B, Hkv, T, D, k_cache.shape[0],
-            k_cache.shape[2], _dtype_code(k_new.dtype), positions, _stream(device),
-        )
-    _lib.check(rc, "du_paged_write")
+        return _device_int32(cache_seqlens, device)
 
 
 def dominus_ultra_decode_paged(
@@ -366,6 +447,48 @@ def dominus_ultra_decode_paged(
     Returns:
         Output tensor of shape [batch, num_heads, 1, head_dim]
     """
+    shape, cache, table = q_new.shape, k_cache.shape, block_table.shape
+    index, dtype = q_new.get_device(), q_new.dtype
+    if not (
+        len(shape) == 4 and len(cache) == 4 and len(table) == 2 and index >= 0 and dtype in _CODES
+        and q_new.is_contiguous() and _fit(cos, dtype, index) and _fit(sin, dtype, index)
+        and cos.dim() == 2 and sin.dim() == 2 and cos.shape[1] * 2 == shape[3] and sin.shape[1] * 2 == shape[3]
+        and cos.shape[0] > 0 and sin.shape[0] > 0
+        and shape[0] > 0 and shape[1] > 0 and shape[2] == 1 and shape[3] in _HEAD_DIMS
+        and _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index)
+        and shape[1] % cache[1] == 0 and cache[3] == shape[3]
+        and _fit(block_table, _I32, index) and table[0] == shape[0] and table[1] > 0
+        and _fit(cache_seqlens, _I32, index) and cache_seqlens.shape == shape[:1]
+    ):
+        block_table, cache_seqlens = _check_decode(
+            q_new, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, cos, sin
+        )
+    B, Hq, _, D = shape
+    num_blocks, Hkv, block_size, _ = cache
+    max_blocks = table[1]
+    device = q_new.device
+    q, c, s = q_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
+        if (q | c | s) & 15:
+            q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
+            q, c, s = q_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+        out = torch.empty_like(q_new)
+        stream = _stream(device)
+        nbytes = _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, index)
+        tickets, ws, keep = _decode_scratch(nbytes, device, index, stream)
+        rc = _lib.load().du_decode_paged(
+            q, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+            cache_seqlens.data_ptr(), c, s, out.data_ptr(), B, Hq, Hkv, D, num_blocks, block_size, max_blocks,
+            _CODES[dtype], D**-0.5, min(cos.shape[0], sin.shape[0]), tickets, ws, nbytes, stream,
+        )
+        del keep
+    if rc:
+        _lib.check(rc, "du_decode_paged")
+    return out
+
+
+def _check_decode(q_new, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, cos, sin):
+    """The refusals of dominus_ultra_decode_paged; returns the table and the lengths on the device."""
     if q_new.ndim != 4 or k_cache.ndim != 4 or v_cache.ndim != 4:
         raise ValueError("q_new, k_cache, and v_cache must be rank-4 tensors")
     B, Hq, _, D = q_new.shape
@@ -387,32 +510,15 @@ def dominus_ultra_decode_paged(
     _validate_paged_cache(k_cache, v_cache, k_scale, v_scale, device)
     _validate_tables_like(cos, sin, D, device, q_new.dtype)
     num_blocks, _, block_size, _ = k_cache.shape
-    max_blocks = block_table.shape[1]
     positions = min(cos.shape[0], sin.shape[0])
     if cache_seqlens.device.type == "cpu":
-        _check_host_lengths("cache_seqlens", cache_seqlens, min(max_blocks * block_size, positions))
+        _check_host_lengths("cache_seqlens", cache_seqlens, min(block_table.shape[1] * block_size, positions))
         if block_table.device.type == "cpu":
             _check_host_table(block_table, cache_seqlens, block_size, num_blocks)
     elif cache_seqlens.device != device:
         raise ValueError("cache_seqlens must be on the device of q_new (or on the CPU)")
-    if block_table.device.type == "cpu" and block_table.dtype == torch.int32:
-        block_table = block_table.to(device)
-    _validate_int32("block_table", block_table, device)
-
-    lib = _lib.load()
     with _OnDevice(device):
-        q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
-        lens = _device_int32(cache_seqlens, device)
-        out = torch.empty_like(q_new)
-        stream = _stream(device)
-        nbytes = _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, device)
-        tickets, ws, keep = _decode_scratch(nbytes, device, stream)
-        rc = lib.du_decode_paged(
-            _ptr(q_new), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-            _ptr(block_table), _ptr(lens), _ptr(cos), _ptr(sin), _ptr(out), B, Hq, Hkv, D,
-            num_blocks, block_size, max_blocks, _dtype_code(q_new.dtype), 1.0 / (D**0.5),
-            positions, tickets, ws, nbytes, stream,
-        )
-        del keep
-    _lib.check(rc, "du_decode_paged")
-    return out
+        if block_table.device.type == "cpu" and block_table.dtype == torch.int32:
+            block_table = block_table.to(device)
+        _validate_int32("block_table", block_table, device)
+        return block_table, _device_int32(cache_seqlens, device)
