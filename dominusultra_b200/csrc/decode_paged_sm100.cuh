@@ -168,14 +168,6 @@ struct DecodePagedShape {
   static_assert(OFF_SC % 16 == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
-// x / y for a quotient of at most 2^21 (x >= 0, y > 0): a float estimate, off by one at most, and a
-// step. (Here: chunks of a request, which the host keeps at 2^20, units of one, CTAs.)
-__device__ __forceinline__ int small_div(int x, int y) {
-  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
-  const int r = x - q * y;
-  return q + (r >= y) - (r < 0);
-}
-
 // This CTA's share of the flattened chunks, found by one warp. The host refuses batches whose block
 // tables could hold 2^31 chunks, so chunk numbers are ints.
 //

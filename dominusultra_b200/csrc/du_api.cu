@@ -1278,12 +1278,11 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 
 template <bool BF16, int WPI>
 int launch_paged_write_t(const du::PagedWriteParams& prm, cudaStream_t st) {
-  const long long items = static_cast<long long>(prm.pages) * prm.Hkv * 2;  // of a request
-  const long long ctas = WPI == 1 ? (items + 3) / 4 : items;
-  if (items > 0x7fffffffLL || prm.B > 65535)
-    return fail(DU_ERR_UNSUPPORTED, "more than 65535 requests or 2^31 - 1 (block, head) items of one");
-  cudaError_t e = launch_kernel(du::paged_write_kernel<BF16, WPI>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(prm.B)),
-                                WPI == 1 ? 128 : 32 * WPI, 0, st, true, prm);
+  constexpr int kWarps = WPI == 1 ? 4 : WPI;  // of a CTA
+  const long long need = WPI == 1 ? (static_cast<long long>(prm.items) + 3) / 4 : prm.items;
+  const long long most = static_cast<long long>(sm_count()) * (du::PAGED_WRITE_WARPS / kWarps);
+  cudaError_t e = launch_kernel(du::paged_write_kernel<BF16, WPI>, dim3(static_cast<unsigned>(need < most ? need : most)),
+                                32 * kWarps, 0, st, true, prm);
   if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
@@ -1473,6 +1472,10 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
   prm.N = num_blocks;
   prm.block = block_size;
   prm.pages = static_cast<int>((static_cast<long long>(T) + 2LL * block_size - 2) / block_size);
+  const long long items = static_cast<long long>(B) * prm.pages * Hkv * 2;
+  if (items > 0x7fffffffLL - (1 << 20) || T > (1 << 24) || B > (1 << 20))
+    return fail(DU_ERR_UNSUPPORTED, "more than 2^31 (request, block, head) items, 2^24 tokens of a request or 2^20 requests");
+  prm.items = static_cast<int>(items);
   prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
   prm.d_log2 = D == 16 ? 4 : (D == 32 ? 5 : (D == 64 ? 6 : (D == 128 ? 7 : 8)));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -24,6 +24,14 @@ __device__ __forceinline__ float2 e4m3x2_widen(uint32_t p) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// x / y for a quotient of at most 2^21 (x >= 0, y > 0): a float estimate, off by one at most, and a
+// step. (Chunks of a request, which the host keeps at 2^20, units of one, requests, CTAs.)
+__device__ __forceinline__ int small_div(int x, int y) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
+  const int r = x - q * y;
+  return q + (r >= y) - (r < 0);
+}
+
 // max(|a|, |b|, |c|), NaN if one of them is.
 __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
   float r;
@@ -229,6 +237,7 @@ struct PagedWriteParams {
   const void* sin;
   long long positions;
   int B, Hkv, T, N, block, pages;  // pages: blocks that one request's T tokens can touch
+  int items;         // B pages Hkv 2
   int d_log2, block_log2;  // head_dim = 2^d_log2, block = 2^block_log2
 };
 
@@ -250,6 +259,9 @@ __device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
   const int e = max((amax_bits & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7, -64);
   return __int_as_float((e + 127) << 23);
 }
+
+// Resident warps per SM that the writer's registers are kept to.
+constexpr int PAGED_WRITE_WARPS = 16;
 
 // Quantises the new tokens of a call into the cache: keys rotated at their positions, one scale
 // per (block, KV head) and per cache.
@@ -280,10 +292,16 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   const int r0 = pg == 0 ? row0 : 0;  // the block's first row that this call writes
   const int n = min(p.T - t0, p.block - r0);
   const int* slot_row = p.slots + static_cast<long long>(b) * p.T + t0;
-  const uint8_t* x = static_cast<const uint8_t*>(IS_V ? p.v : p.k) +
-                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0) * (2 * D);
+  // This thread's chunk pairs: chunk c of rows r, r + dr, ... (NT threads hold whole rows).
   const int pairs_log2 = p.d_log2 - 4;
-  const int units = n << pairs_log2;
+  const int r = lane_i >> pairs_log2, c = lane_i & ((1 << pairs_log2) - 1), dr = NT >> pairs_log2;
+  const uint8_t* x = static_cast<const uint8_t*>(IS_V ? p.v : p.k) +
+                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0 + r) * (2 * D) + c * 16;
+  const long long pos0 = static_cast<long long>(past) + t0 + r;
+  const uint8_t* cosp = static_cast<const uint8_t*>(p.cos) + pos0 * D + c * 16;
+  const uint8_t* sinp = static_cast<const uint8_t*>(p.sin) + pos0 * D + c * 16;
+  // Rows of this thread that the tables reach (values need none).
+  const int reach = IS_V ? n : (past < 0 ? 0 : static_cast<int>(min(static_cast<long long>(n), p.positions - past - t0)));
   // Everything whose address is known goes out at once: rows, slots and the rows of the tables.
   // (In prompts, where requests' padding makes whole blocks without tokens, those are left first.)
   uint4 xa[NP], xb[NP], cv[NP], sv[NP];
@@ -292,17 +310,16 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   if (p.T > p.block && slot0 < 0) return;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
-    const long long pos = static_cast<long long>(past) + t0 + r;
     xa[i] = xb[i] = cv[i] = sv[i] = make_uint4(0, 0, 0, 0);
     slots[i] = -1;
-    if (u < units) {
-      slots[i] = slot_row[r];
-      xa[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + c * 16);
-      xb[i] = ldg_stream_v4(x + static_cast<long long>(r) * (2 * D) + D + c * 16);
-      if (!IS_V && past >= 0 && pos < p.positions) {
-        cv[i] = ldg_v4(static_cast<const uint8_t*>(p.cos) + pos * D + c * 16);
-        sv[i] = ldg_v4(static_cast<const uint8_t*>(p.sin) + pos * D + c * 16);
+    if (r + i * dr < n) slots[i] = slot_row[r + i * dr];
+    if (r + i * dr < reach) {
+      // (rows dr apart: dr 2 D = 32 NT bytes, 16 NT in the tables)
+      xa[i] = ldg_stream_v4(x + i * 32 * NT);
+      xb[i] = ldg_stream_v4(x + i * 32 * NT + D);
+      if (!IS_V) {
+        cv[i] = ldg_v4(cosp + i * 16 * NT);
+        sv[i] = ldg_v4(sinp + i * 16 * NT);
       }
     }
   }
@@ -324,17 +341,17 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   float peak = 0.f;               // the largest magnitude (NaN stays)
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int u = lane_i + i * NT, r = u >> pairs_log2;
-    const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
-    const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
-    bool on = slots[i] == slot0 + r;
-    const bool far = on && !IS_V && static_cast<long long>(past) + t0 + r >= p.positions;
-    if (far || (!on && slots[i] >= 0)) {
-      wrong = far ? past + t0 + r : slots[i];
+    const int row = r + i * dr;
+    const bool on = slots[i] == slot0 + row && row < reach;
+    if (slots[i] >= 0 && !on) {
+      const bool far = slots[i] == slot0 + row;
+      wrong = far ? past + t0 + row : slots[i];
       code = far ? 6u : 7u;
     }
-    on = on && !far;
     live |= on ? 1u << i : 0u;
+    if (!on) xa[i] = xb[i] = make_uint4(0, 0, 0, 0);  // (zeros: no part in the magnitude)
+    const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
+    const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 v = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
@@ -352,9 +369,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
         y2[i][2 * e + 1] = fma_odd(w.y, cc.y, __fmul_rn(v.y, ss.y));
       }
     }
-    if (on)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) peak = max3_abs_nan(peak, y1[i][e], y2[i][e]);
+    for (int e = 0; e < 8; ++e) peak = max3_abs_nan(peak, y1[i][e], y2[i][e]);
   }
   if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
   uint32_t top = __float_as_uint(peak) & 0x7fffffffu;  // NaN above infinity above every number
@@ -370,10 +386,10 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   if (lane_i == 0) *scale = unit;
   const bool poison = unit != unit;
   const float inv = 1.0f / unit;
+  uint8_t* dst = out + (r0 + r) * D + 8 * c;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     if (!(live & (1u << i))) continue;
-    const int u = lane_i + i * NT, r = u >> pairs_log2, c = u & ((1 << pairs_log2) - 1);
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -383,9 +399,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
                  (e4m3x2(y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv) << 16);
     }
     if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
-    uint8_t* row = out + static_cast<long long>(r0 + r) * D;
-    *reinterpret_cast<uint2*>(row + 8 * c) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(row + D / 2 + 8 * c) = make_uint2(w[2], w[3]);
+    *reinterpret_cast<uint2*>(dst + i * 16 * NT) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(dst + i * 16 * NT + D / 2) = make_uint2(w[2], w[3]);
   }
   if (r0 > 0 && unit > had) {
     // The present rows under the larger scale.
@@ -405,18 +420,24 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
 }
 
 template <bool BF16, int WPI>
-__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) paged_write_kernel(const PagedWriteParams p) {
-  __shared__ uint32_t warp_max[WPI];
+__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, PAGED_WRITE_WARPS / (WPI == 1 ? 4 : WPI))
+    paged_write_kernel(const PagedWriteParams p) {
+  __shared__ uint32_t warp_max[2][WPI];
   griddep_launch_dependents();
   griddep_wait();
-  // With WPI = 1 a warp is an item; else the CTA is one, and its barrier is reached by all or none.
-  const unsigned item = WPI == 1 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;
-  const unsigned hh = item >> 1;
-  const int pg = static_cast<int>(hh / static_cast<unsigned>(p.Hkv));
-  if (pg >= p.pages) return;
-  const int h = static_cast<int>(hh) - pg * p.Hkv;
-  if (item & 1) paged_write_item<BF16, WPI, true>(p, blockIdx.y, pg, h, warp_max);
-  else paged_write_item<BF16, WPI, false>(p, blockIdx.y, pg, h, warp_max);
+  // A grid of resident CTAs walks the items (short CTAs, one per item, ended faster than new ones
+  // came: 13 of 64 warps per SM at any time). With WPI = 1 a warp is an item; else the CTA is one,
+  // and its barrier is reached by all or none.
+  const int per_page = 2 * p.Hkv, per_request = per_page * p.pages;
+  const int stride = static_cast<int>(gridDim.x) * (WPI == 1 ? 4 : 1);
+  int odd = 0;  // (the warps' maxima of one item are read while those of the next are written)
+  for (int item = WPI == 1 ? static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x) / 32 : static_cast<int>(blockIdx.x);
+       item < p.items; item += stride, odd ^= 1) {
+    const int b = small_div(item, per_request), in = item - b * per_request;
+    const int pg = small_div(in, per_page), kh = in - pg * per_page;
+    if (kh & 1) paged_write_item<BF16, WPI, true>(p, b, pg, kh >> 1, warp_max[odd]);
+    else paged_write_item<BF16, WPI, false>(p, b, pg, kh >> 1, warp_max[odd]);
+  }
 }
 
 }  // namespace du
