@@ -67,10 +67,18 @@ constexpr int DECODE_PAGED_PIECE_SLACK = 3;
 constexpr int DECODE_PAGED_MAX_CTAS = 12 * 36;
 __device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
 
-// cp.async of 4 bytes, and an arrival on `bar` once this thread's earlier cp.async have landed.
+// cp.async of 4 and of 16 bytes, and an arrival on `bar` once this thread's earlier cp.async have landed.
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
+// Brings a word into L1 and waits for nothing.
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("{\n\t.reg .b32 t;\n\tld.global.b32 t, [%0];\n\t}\n" ::"l"(p));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -129,7 +137,8 @@ struct DecodePagedShape {
   static constexpr int CB = DP < 64 ? DP : (DP == 128 && HPU == 8 ? 32 : 64);
   static constexpr int ROW = CB + 4;
   static constexpr int ML_BYTES = ((8 * HPU * 4) + 127) / 128 * 128;  // maxima and sums of the warps
-  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + 2560;
+  static constexpr int RAW_BYTES = (HPU + 1) * DP * 2;  // a unit's query rows and its cos and sin row
+  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + RAW_BYTES + 2560;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
   static constexpr int TILES = (BUDGET - FIXED) / TILE;
   static constexpr int NV = TILES / 2 > 8 ? 8 : TILES / 2;            // stages of V
@@ -138,7 +147,8 @@ struct DecodePagedShape {
   static constexpr int OFF_P = OFF_V + NV * TILE;
   static constexpr int OFF_Q = OFF_P + NPB * P_BYTES;
   static constexpr int OFF_ML = OFF_Q + 2 * Q_BYTES;
-  static constexpr int OFF_SC = OFF_ML + ML_BYTES;  // [NK][2][8] scales of a chunk's blocks
+  static constexpr int OFF_RAW = OFF_ML + ML_BYTES;
+  static constexpr int OFF_SC = OFF_RAW + RAW_BYTES;  // [NK][2][8] scales of a chunk's blocks
   static constexpr int NF = 4;                        // fragment entries in flight
   static constexpr int OFF_FRAG = OFF_SC + NK * 64;   // [NF] entries of 16 words
   static constexpr int OFF_OWED = OFF_FRAG + NF * 64; // [2] entries of units to join
@@ -382,36 +392,26 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   const int warp = tid >> 5;
   const int lane = tid & 31;
 
-  if (tid == 128) {
-    for (int s = 0; s < NK; ++s) {
-      mbar_init(KFULL(s), 1 + 32);
-      mbar_init(KEMPTY(s), 1 + 4);
+  if (warp == 4) {
+    for (int i = lane; i < S::N_BAR; i += 32) {
+      int n = 1;  // VFULL, VEMPTY, SFULL, PDONE, DRAIN, FFULL
+      if (i < S::B_KEMPTY) n = 1 + 32;                                              // KFULL
+      else if (i < S::B_VFULL) n = 1 + 4;                                           // KEMPTY
+      else if (i >= S::B_QFULL && i < S::B_QEMPTY) n = 32;                          // QFULL
+      else if (i >= S::B_QEMPTY && i < S::B_SFULL) n = 1 + 4;                       // QEMPTY
+      else if (i >= S::B_SEMPTY && i < S::B_PFULL) n = 4;                           // SEMPTY
+      else if ((i >= S::B_PFULL && i < S::B_PDONE) || i == S::B_MRG || i == S::B_FREE) n = 128;
+      else if (i >= S::B_FEMPTY) n = 7;                                             // FEMPTY
+      mbar_init(bar(i), n);
     }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(VFULL(s), 1);
-      mbar_init(VEMPTY(s), 1);
+    if (lane == 0) {
+      *failed = 0;
+      *emitted = 0;
+      *n_owed = 0;
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(QFULL(i), 32);
-      mbar_init(QEMPTY(i), 1 + 4);
-      mbar_init(SFULL(i), 1);
-      mbar_init(SEMPTY(i), 4);
-      mbar_init(PFULL(i), 128);
-      mbar_init(PDONE(i), 1);
-    }
-    for (int i = 0; i < S::NF; ++i) {
-      mbar_init(FFULL(i), 1);
-      mbar_init(FEMPTY(i), 7);
-    }
-    mbar_init(BAR_MRG, 128);
-    mbar_init(BAR_FREE, 128);
-    mbar_init(BAR_DRAIN, 1);
-    *failed = 0;
-    *emitted = 0;
-    *n_owed = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
   }
   if (warp == 5) {
     // (Only a predecessor whose CTAs all run or have ended lets this grid start early, and none of
@@ -422,6 +422,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   // Launched as a programmatic dependent: what is above runs beside the stream's previous kernel.
   griddep_wait();
   if (warp == 5) griddep_launch_dependents();  // (the columns are taken)
+  Walk walk;  // warp 6's
+  if (warp == 6) {
+    const PagedStart st = Walk::find(p, lane);
+    if (lane == 0) *start = st;
+    walk.init(st);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -558,17 +564,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     __syncwarp();
   } else if (warp == 6) {
     // ------------------------------------------------------------------ fragments and queries
-    Walk walk;
-    {
-      const PagedStart st = Walk::find(p, lane);
-      if (lane == 0) *start = st;
-      walk.init(st);
-    }
     const int D = p.D, half = D >> 1;
-    // A lane takes element pairs 2 lane + 64 e of each half. The 16-bit words of all heads are
-    // loaded before any is used, whatever their type.
+    // A unit's query rows and its rows of the tables come to shared memory; then head by head (a
+    // loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of each half.
     constexpr int EPL = DP >= 128 ? DP / 128 : 1;
-    const uint32_t* q32 = static_cast<const uint32_t*>(p.q);
+    const uint32_t raw = sbase + S::OFF_RAW;
+    const uint32_t* raw32 = reinterpret_cast<const uint32_t*>(sgen + S::OFF_RAW);
     auto widen = [&](uint32_t w) -> float2 { return p.bf16 ? unpack2<true>(w) : unpack2<false>(w); };
     // Rows of the query tiles beyond the parts stay zero.
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
@@ -588,6 +589,9 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         ended = !walk.next(p, f);
         if (ended) f.kind = 0;
         const int e = k % S::NF;
+        // The producers will ask for these entries of the block table.
+        if (!ended && f.kbeg + (lane << p.block_log2) < f.kbeg + f.keys)
+          prefetch_l1(p.table + static_cast<long long>(f.b) * p.width + (f.kbeg >> p.block_log2) + lane);
         if (k >= S::NF && !__all_sync(0xffffffffu, mbar_wait(FEMPTY(e), ((k / S::NF) - 1) & 1, failed, 821))) break;
         if (lane == 0) {
           *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + e * 64) = f;
@@ -604,40 +608,41 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       if (f.kind == 0) break;
       const bool busy = f.chunks > 0;
-      uint32_t c[EPL], sn[EPL], xa[HPU][EPL], xb[HPU][EPL];
       if (busy) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-          const int d = 2 * lane + 64 * e;
-          const bool on = d < half;
-          const long long tr = (static_cast<long long>(f.len - 1) * half + d) >> 1;
-          c[e] = on ? static_cast<const uint32_t*>(p.cos)[tr] : 0u;
-          sn[e] = on ? static_cast<const uint32_t*>(p.sin)[tr] : 0u;
+        const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (static_cast<long long>(f.b) * p.Hq + f.h0) * (2 * D);
+        const long long trow = static_cast<long long>(f.len - 1) * D;
+        for (int i = lane; i < f.nh * (D >> 3); i += 32) cp_async16(raw + 16 * i, qrow + 16 * i);
+        if (lane < 2 * (D >> 4)) {  // cos, then sin: D bytes each
+          const int half16 = D >> 4;
+          const bool is_sin = lane >= half16;
+          cp_async16(raw + HPU * 2 * D + 16 * lane,
+                     static_cast<const uint8_t*>(is_sin ? p.sin : p.cos) + trow + 16 * (is_sin ? lane - half16 : lane));
         }
-#pragma unroll
-        for (int h = 0; h < HPU; ++h)
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            const int d = 2 * lane + 64 * e;
-            const bool on = d < half && h < f.nh;
-            const long long qr = ((static_cast<long long>(f.b) * p.Hq + f.h0 + h) * D + d) >> 1;
-            xa[h][e] = on ? q32[qr] : 0u;
-            xb[h][e] = on ? q32[qr + (half >> 1)] : 0u;
-          }
+        cp_async_wait_all();
+        __syncwarp();
       }
       if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
       if (busy) {
         uint8_t* qt = sgen + S::OFF_Q + qb * S::Q_BYTES;
+        float2 cc[EPL], ss[EPL];
 #pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          const int d = 2 * lane + 64 * e;
+          cc[e] = widen(d < half ? raw32[(HPU * D + d) >> 1] : 0u);
+          ss[e] = widen(d < half ? raw32[(HPU * D + half + d) >> 1] : 0u);
+        }
+#pragma unroll 1
         for (int h = 0; h < HPU; ++h) {
           float2 y1[EPL], y2[EPL];
           float top = 0.f;
           bool fine = true;
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
-            const float2 a = widen(xa[h][e]), b = widen(xb[h][e]), cc = widen(c[e]), ss = widen(sn[e]);
-            y1[e] = make_float2(a.x * cc.x - b.x * ss.x, a.y * cc.y - b.y * ss.y);
-            y2[e] = make_float2(b.x * cc.x + a.x * ss.x, b.y * cc.y + a.y * ss.y);
+            const int d = 2 * lane + 64 * e;
+            const bool on = d < half && h < f.nh;
+            const float2 a = widen(on ? raw32[(h * D + d) >> 1] : 0u), b = widen(on ? raw32[(h * D + half + d) >> 1] : 0u);
+            y1[e] = make_float2(a.x * cc[e].x - b.x * ss[e].x, a.y * cc[e].y - b.y * ss[e].y);
+            y2[e] = make_float2(b.x * cc[e].x + a.x * ss[e].x, b.y * cc[e].y + a.y * ss[e].y);
             top = max3(top, fabsf(y1[e].x), fabsf(y1[e].y));
             top = max3(top, fabsf(y2[e].x), fabsf(y2[e].y));
             fine = fine && y1[e].x - y1[e].x == 0.f && y1[e].y - y1[e].y == 0.f && y2[e].x - y2[e].x == 0.f &&
@@ -671,7 +676,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
       }
       fence_proxy_async_smem();
-      __syncwarp();
+      __syncwarp();  // (and the raw rows have been read)
       mbar_arrive(QFULL(qb));
     }
   } else {
@@ -1008,7 +1013,6 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   if (*failed) {
     // A wait ran out (reported in the status words): NaN for what this CTA still owes, and its
     // tickets, so that the counters return to zero.
-    Walk walk;
     walk.init(*start);
     PagedFrag f;
     const float nan = __int_as_float(0x7fc00000);
