@@ -952,19 +952,26 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   // the weights are found, a warp per head, a lane per fragment.
   for (int e = 0; e < *n_owed; ++e) {
     const PagedFrag f = owed[e];
-    constexpr int KB = 16;
+    constexpr int KB = 8;
     auto slot_of = [&](int k) { return k == 0 ? 2 * f.c0 + 1 : 2 * (f.c0 + k); };
+    // `groups` threads of a warp share an output's fragments: k = group, group + groups, ...
     const int q4 = p.D >> 2, items = f.nh * q4;
+    int groups_log2 = 0;
+    while ((items << (groups_log2 + 1)) <= S::NTHREADS && (2 << groups_log2) <= f.nf && groups_log2 < 5) ++groups_log2;
+    const int groups = 1 << groups_log2;
     auto load = [&](float4 (&o)[KB], int i, int k0) {
       const int h = small_div(i, q4), d = 4 * (i - h * q4);
 #pragma unroll
-      for (int k = 0; k < KB; ++k)
-        if (i < items && k0 + k < f.nf)
+      for (int k = 0; k < KB; ++k) {
+        const int kk = k0 + (k << groups_log2);
+        if (i < items && kk < f.nf)
           o[k] = __ldcg(reinterpret_cast<const float4*>(
-              p.part + (static_cast<long long>(slot_of(k0 + k)) * HPU + h) * p.D + d));
+              p.part + (static_cast<long long>(slot_of(kk)) * HPU + h) * p.D + d));
+      }
     };
+    const int group = tid & (groups - 1);
     float4 o[KB];
-    load(o, tid, 0);
+    load(o, tid >> groups_log2, group);
     const float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
     float* wt = mrg;  // [HPU][nf]: nf <= gridDim.x <= DECODE_PAGED_MAX_CTAS
     for (int h = warp; h < f.nh; h += S::NTHREADS / 32) {
@@ -986,22 +993,33 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       for (int k = lane; k < f.nf; k += 32) wt[h * f.nf + k] *= inv;
     }
     __syncthreads();
-    for (int i = tid; i < items; i += S::NTHREADS) {
+    for (int i0 = 0; i0 < items; i0 += S::NTHREADS >> groups_log2) {
+      const int i = i0 + (tid >> groups_log2);
       const int h = small_div(i, q4), d = 4 * (i - h * q4);
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < items) {
 #pragma unroll 1
-      for (int k0 = 0; k0 < f.nf; k0 += KB) {
-        if (i != tid || k0 > 0) load(o, i, k0);
+        for (int k0 = group; k0 < f.nf; k0 += KB << groups_log2) {
+          if (i0 > 0 || k0 > group) load(o, i, k0);
 #pragma unroll
-        for (int k = 0; k < KB; ++k) {
-          if (k0 + k >= f.nf) break;
-          const float x = wt[h * f.nf + k0 + k];
-          A.x = fmaf(o[k].x, x, A.x);
-          A.y = fmaf(o[k].y, x, A.y);
-          A.z = fmaf(o[k].z, x, A.z);
-          A.w = fmaf(o[k].w, x, A.w);
+          for (int k = 0; k < KB; ++k) {
+            const int kk = k0 + (k << groups_log2);
+            if (kk >= f.nf) break;
+            const float x = wt[h * f.nf + kk];
+            A.x = fmaf(o[k].x, x, A.x);
+            A.y = fmaf(o[k].y, x, A.y);
+            A.z = fmaf(o[k].z, x, A.z);
+            A.w = fmaf(o[k].w, x, A.w);
+          }
         }
       }
+      for (int o2 = 1; o2 < groups; o2 <<= 1) {  // (an output's threads are neighbours in a warp)
+        A.x += __shfl_xor_sync(0xffffffffu, A.x, o2);
+        A.y += __shfl_xor_sync(0xffffffffu, A.y, o2);
+        A.z += __shfl_xor_sync(0xffffffffu, A.z, o2);
+        A.w += __shfl_xor_sync(0xffffffffu, A.w, o2);
+      }
+      if (i >= items || group != 0) continue;
       const long long at = (static_cast<long long>(f.b) * p.Hq + f.h0 + h) * p.D + d;
       uint2 w;
       if (p.bf16) w = make_uint2(pack2<true>(A.x, A.y), pack2<true>(A.z, A.w));

@@ -300,8 +300,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   const long long pos0 = static_cast<long long>(past) + t0 + r;
   const uint8_t* cosp = static_cast<const uint8_t*>(p.cos) + pos0 * D + c * 16;
   const uint8_t* sinp = static_cast<const uint8_t*>(p.sin) + pos0 * D + c * 16;
-  // Rows of this thread that the tables reach (values need none).
-  const int reach = IS_V ? n : (past < 0 ? 0 : static_cast<int>(min(static_cast<long long>(n), p.positions - past - t0)));
+  // Rows of the item that the tables reach (of values too: a token is written whole or not).
+  const int reach = past < 0 ? 0 : static_cast<int>(max(0LL, min(static_cast<long long>(n), p.positions - past - t0)));
   // Everything whose address is known goes out at once: rows, slots and the rows of the tables.
   // (In prompts, where requests' padding makes whole blocks without tokens, those are left first.)
   uint4 xa[NP], xb[NP], cv[NP], sv[NP];
@@ -373,7 +373,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
     for (int e = 0; e < 8; ++e) peak = max3_abs_nan(peak, y1[i][e], y2[i][e]);
   }
   if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
-  uint32_t top = __float_as_uint(peak) & 0x7fffffffu;  // NaN above infinity above every number
+  // Bits of the magnitude, NaN above infinity above every number; one more, 0: no row.
+  uint32_t top = live ? (__float_as_uint(peak) & 0x7fffffffu) + 1u : 0u;
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (WPI > 1) {
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
@@ -381,7 +382,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
 #pragma unroll
     for (int w = 0; w < WPI; ++w) top = max(top, warp_max[w]);
   }
-  float unit = paged_unit(top);
+  if (top == 0) return;  // the item's: nothing is written, the scale neither
+  float unit = paged_unit(top - 1);
   if (r0 > 0 && (unit <= had || had != had)) unit = had;  // (a NaN on either side stays)
   if (lane_i == 0) *scale = unit;
   const bool poison = unit != unit;

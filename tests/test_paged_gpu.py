@@ -237,10 +237,27 @@ def test_write_positions_beyond_the_rope_tables():
     past = [14]
     c = _write_case(1, 1, 64, 4, 16, past, [4], torch.bfloat16, 6)
     kn, vn, k8, v8, ks, vs, slots, cos, sin = c
-    _run_write(kn, vn, k8, v8, ks, vs, slots, past, cos[:16], sin[:16])
+    got = _run_write(kn, vn, k8, v8, ks, vs, slots, past, cos[:17], sin[:17])
+    assert _status()[:3] == [6, 0, 17]
+    same = _run_write(kn, vn, k8, v8, ks, vs, slots, [-2], cos, sin)
     assert _status()[0] == 6
-    _run_write(kn, vn, k8, v8, ks, vs, slots, [-2], cos, sin)
+    for a, w in zip(same, (k8, v8, ks, vs)):
+        assert _same(a, w)
+    slots[0, 3:] = -1  # the token at position 17, of keys and values both
+    plain.write(kn, vn, k8, v8, ks, vs, slots.tolist(), past, cos, sin)
+    for a, w in zip(got, (k8, v8, ks, vs)):
+        assert _same(a, w)
+
+
+def test_write_of_nothing_leaves_everything():
+    """Tokens beyond the tables in a fresh block: neither rows nor scales change."""
+    past = [16]
+    c = _write_case(1, 2, 64, 4, 16, past, [4], torch.bfloat16, 6)
+    kn, vn, k8, v8, ks, vs, slots, cos, sin = c
+    got = _run_write(kn, vn, k8, v8, ks, vs, slots, past, cos[:16], sin[:16])
     assert _status()[0] == 6
+    for a, w in zip(got, (k8, v8, ks, vs)):
+        assert _same(a, w)
 
 
 # ----------------------------------------------------------------------------------------- attend
