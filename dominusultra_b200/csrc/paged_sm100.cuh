@@ -17,6 +17,18 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return r;
 }
 
+// Four fp32 values to packed e4m3, a in the lowest byte.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}\n"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+
 // A packed e4m3 pair widened to fp32 (exact).
 __device__ __forceinline__ float2 e4m3x2_widen(uint32_t p) {
   uint32_t h;
@@ -297,36 +309,37 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   const int r = lane_i >> pairs_log2, c = lane_i & ((1 << pairs_log2) - 1), dr = NT >> pairs_log2;
   const uint8_t* x = static_cast<const uint8_t*>(IS_V ? p.v : p.k) +
                      ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0 + r) * (2 * D) + c * 16;
+  // Rows that the tables reach (of values too: a token is written whole or not).
+  const int reach = past < 0 ? 0 : static_cast<int>(max(0LL, min(static_cast<long long>(n), p.positions - past - t0)));
   const long long pos0 = static_cast<long long>(past) + t0 + r;
   const uint8_t* cosp = static_cast<const uint8_t*>(p.cos) + pos0 * D + c * 16;
   const uint8_t* sinp = static_cast<const uint8_t*>(p.sin) + pos0 * D + c * 16;
-  // Rows of the item that the tables reach (of values too: a token is written whole or not).
-  const int reach = past < 0 ? 0 : static_cast<int>(max(0LL, min(static_cast<long long>(n), p.positions - past - t0)));
-  // Everything whose address is known goes out at once: rows, slots and the rows of the tables.
-  // (In prompts, where requests' padding makes whole blocks without tokens, those are left first.)
+  // Everything whose address is known goes out at once: rows, slots and the rows of the tables. A
+  // row beyond the last is the last again, which changes no magnitude. (In prompts, where requests'
+  // padding makes whole blocks without tokens, those are left first.)
   uint4 xa[NP], xb[NP], cv[NP], sv[NP];
   int slots[NP];
   const int slot0 = slot_row[0];
-  if (p.T > p.block && slot0 < 0) return;
+  if (reach == 0 || (p.T > p.block && slot0 < 0)) {
+    if (lane_i == 0 && slot0 >= 0)
+      record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : past + t0));
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    xa[i] = xb[i] = cv[i] = sv[i] = make_uint4(0, 0, 0, 0);
-    slots[i] = -1;
-    if (r + i * dr < n) slots[i] = slot_row[r + i * dr];
-    if (r + i * dr < reach) {
-      // (rows dr apart: dr 2 D = 32 NT bytes, 16 NT in the tables)
-      xa[i] = ldg_stream_v4(x + i * 32 * NT);
-      xb[i] = ldg_stream_v4(x + i * 32 * NT + D);
-      if (!IS_V) {
-        cv[i] = ldg_v4(cosp + i * 16 * NT);
-        sv[i] = ldg_v4(sinp + i * 16 * NT);
-      }
+    const int row = r + i * dr, step = min(row, reach - 1) - r;
+    slots[i] = row < n ? slot_row[row] : -1;
+    xa[i] = ldg_stream_v4(x + step * (2 * D));
+    xb[i] = ldg_stream_v4(x + step * (2 * D) + D);
+    if (!IS_V) {
+      cv[i] = ldg_v4(cosp + step * D);
+      sv[i] = ldg_v4(sinp + step * D);
     }
   }
   if (slot0 < 0) return;  // no token here
   const int blk = slot0 >> p.block_log2;
-  if (past < 0 || blk >= p.N || (slot0 & (p.block - 1)) != r0) {
-    if (lane_i == 0) record_error(past < 0 ? 6u : 7u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : slot0));
+  if (blk >= p.N || (slot0 & (p.block - 1)) != r0) {
+    if (lane_i == 0) record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(slot0));
     return;
   }
   const long long cell = static_cast<long long>(blk) * p.Hkv + h;
@@ -349,9 +362,12 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
       code = far ? 6u : 7u;
     }
     live |= on ? 1u << i : 0u;
-    if (!on) xa[i] = xb[i] = make_uint4(0, 0, 0, 0);  // (zeros: no part in the magnitude)
     const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
-    const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
+    uint32_t cw[4], sw[4];
+    if constexpr (!IS_V) {
+      cw[0] = cv[i].x, cw[1] = cv[i].y, cw[2] = cv[i].z, cw[3] = cv[i].w;
+      sw[0] = sv[i].x, sw[1] = sv[i].y, sw[2] = sv[i].z, sw[3] = sv[i].w;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 v = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
@@ -369,8 +385,10 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
         y2[i][2 * e + 1] = fma_odd(w.y, cc.y, __fmul_rn(v.y, ss.y));
       }
     }
+    float high = peak;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) peak = max3_abs_nan(peak, y1[i][e], y2[i][e]);
+    for (int e = 0; e < 8; ++e) high = max3_abs_nan(high, y1[i][e], y2[i][e]);
+    peak = on ? high : peak;
   }
   if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
   // Bits of the magnitude, NaN above infinity above every number; one more, 0: no row.
@@ -395,10 +413,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      w[e] = e4m3x2(y1[i][4 * e] * inv, y1[i][4 * e + 1] * inv) |
-             (e4m3x2(y1[i][4 * e + 2] * inv, y1[i][4 * e + 3] * inv) << 16);
-      w[2 + e] = e4m3x2(y2[i][4 * e] * inv, y2[i][4 * e + 1] * inv) |
-                 (e4m3x2(y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv) << 16);
+      w[e] = e4m3x4(y1[i][4 * e] * inv, y1[i][4 * e + 1] * inv, y1[i][4 * e + 2] * inv, y1[i][4 * e + 3] * inv);
+      w[2 + e] = e4m3x4(y2[i][4 * e] * inv, y2[i][4 * e + 1] * inv, y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv);
     }
     if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
     *reinterpret_cast<uint2*>(dst + i * 16 * NT) = make_uint2(w[0], w[1]);
@@ -414,7 +430,7 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 lo = e4m3x2_widen(w[e] & 0xffffu), hi = e4m3x2_widen(w[e] >> 16);
-        w[e] = e4m3x2(lo.x * f, lo.y * f) | (e4m3x2(hi.x * f, hi.y * f) << 16);
+        w[e] = e4m3x4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
       }
       *q = make_uint4(w[0], w[1], w[2], w[3]);
     }
