@@ -1430,8 +1430,9 @@ int du_paged_tables(int* block_table, const int* cache_seqlens, const int* new_s
   // (an attribute of the largest batch, once per device: the kernel's shared memory is 64 KB then)
   cudaError_t e = ensure_smem_attr(du::paged_tables_kernel, 2 * du::PAGED_MAX_BATCH * static_cast<int>(sizeof(int)));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged tables)");
-  du::paged_tables_kernel<<<static_cast<unsigned>(grid), du::PAGED_TABLES_THREADS, smem,
-                            static_cast<cudaStream_t>(stream)>>>(prm);
+  e = launch_kernel(du::paged_tables_kernel, dim3(static_cast<unsigned>(grid)), du::PAGED_TABLES_THREADS,
+                    static_cast<size_t>(smem), static_cast<cudaStream_t>(stream), true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged tables launch");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged tables launch");
   return DU_OK;
@@ -1472,7 +1473,7 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
   prm.N = num_blocks;
   prm.block = block_size;
   prm.pages = static_cast<int>((static_cast<long long>(T) + 2LL * block_size - 2) / block_size);
-  const long long items = static_cast<long long>(B) * prm.pages * Hkv * 2;
+  const long long items = static_cast<long long>(B) * prm.pages * Hkv;
   if (items > 0x7fffffffLL - (1 << 20) || T > (1 << 24) || B > (1 << 20))
     return fail(DU_ERR_UNSUPPORTED, "more than 2^31 (request, block, head) items, 2^24 tokens of a request or 2^20 requests");
   prm.items = static_cast<int>(items);

@@ -17,6 +17,12 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return r;
 }
 
+// A packed pair of 16-bit values as two fp32 values (bf16: one shift and one mask).
+template <bool BF16>
+__device__ __forceinline__ float2 split2(uint32_t w) {
+  return f2_split(widen2<BF16>(w));
+}
+
 // Four fp32 values to packed e4m3, a in the lowest byte.
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   uint32_t r;
@@ -119,6 +125,7 @@ __global__ void __launch_bounds__(PAGED_TABLES_THREADS) paged_tables_kernel(cons
   int* give = sm_off + p.B;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int NW = PAGED_TABLES_THREADS / 32;
+  griddep_wait();
 
   const int head = p.state[0], count = p.state[1];
   bool ring_ok = head >= 0 && head < p.N && count >= 0 && count <= p.N;
@@ -249,7 +256,7 @@ struct PagedWriteParams {
   const void* sin;
   long long positions;
   int B, Hkv, T, N, block, pages;  // pages: blocks that one request's T tokens can touch
-  int items;         // B pages Hkv 2
+  int items;         // B pages Hkv
   int d_log2, block_log2;  // head_dim = 2^d_log2, block = 2^block_log2
 };
 
@@ -272,29 +279,31 @@ __device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
   return __int_as_float((e + 127) << 23);
 }
 
-// Resident warps per SM that the writer's registers are kept to.
+// Resident warps per SM that the writer's registers are kept to, and chunk pairs per thread of an item.
 constexpr int PAGED_WRITE_WARPS = 16;
+constexpr int PAGED_WRITE_PAIRS = 4;
 
 // Quantises the new tokens of a call into the cache: keys rotated at their positions, one scale
 // per (block, KV head) and per cache.
 //
-// A work item is (request, block that its tokens touch, KV head, key or value); WPI warps take it, a
-// thread at most four pairs of 16-byte chunks i, i + D/2 of a row, which is what a rotation pairs
-// up, held in registers from the load to the store. The largest magnitude of the item's rows
-// gives the scale: the smallest power of two with amax <= 448 scale, or the block's present scale
-// where that is larger and the block holds rows already. Products of two 16-bit values are exact
-// in fp32, their sum is rounded to odd and the scale is a power of two, so each byte is the e4m3
-// value nearest to the exact quotient. Where a block's scale grows, its present rows are scaled
-// down and rounded again; that is exact but for what falls below the format's normal range. A
-// block with a value that is not finite gets the scale NaN, which every attention over it then
+// A work item is (request, block that its tokens touch, KV head), its keys and then its values; WPI
+// warps take it, a thread at most four pairs of 16-byte chunks i, i + D/2 of a row, which is what a
+// rotation pairs up, held in registers from the load to the store. The largest magnitude of the
+// item's rows gives the scale: the smallest power of two with amax <= 448 scale, or the block's
+// present scale where that is larger and the block holds rows already. Products of two 16-bit values
+// are exact in fp32, their sum is rounded to odd and the scale is a power of two, so each byte is
+// the e4m3 value nearest to the exact quotient. Where a block's scale grows, its present rows are
+// scaled down and rounded again; that is exact but for what falls below the format's normal range.
+// A block with a value that is not finite gets the scale NaN, which every attention over it then
 // returns.
 //
-// Bound by HBM for prompts: 2 bytes read and 1 written per value; by the chain of loads (length,
-// rows and slots, scale) for single tokens.
-template <bool BF16, int WPI, bool IS_V>
-__device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int b, int pg, int h, uint32_t* warp_max) {
+// Bound by HBM for prompts (2 bytes read and 1 written per value), closely followed by the issue
+// slots: about 10 instructions per key value and 4 per value, besides some 400 per item and warp
+// for addresses and slots. By the chain of loads (length, rows and slots, scale) for single tokens.
+template <bool BF16, int WPI>
+__device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int b, int pg, int h, uint32_t (*warp_max)[WPI]) {
   constexpr int NT = 32 * WPI;  // threads per item
-  constexpr int NP = 4;         // chunk pairs per thread, at most
+  constexpr int NP = PAGED_WRITE_PAIRS;
   const int lane_i = threadIdx.x % NT;  // thread within the item
   const int D = 1 << p.d_log2;
   const int past = p.past[b];
@@ -307,8 +316,9 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   // This thread's chunk pairs: chunk c of rows r, r + dr, ... (NT threads hold whole rows).
   const int pairs_log2 = p.d_log2 - 4;
   const int r = lane_i >> pairs_log2, c = lane_i & ((1 << pairs_log2) - 1), dr = NT >> pairs_log2;
-  const uint8_t* x = static_cast<const uint8_t*>(IS_V ? p.v : p.k) +
-                     ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0 + r) * (2 * D) + c * 16;
+  const long long x0 = ((static_cast<long long>(b) * p.Hkv + h) * p.T + t0 + r) * (2 * D) + c * 16;
+  const uint8_t* kx = static_cast<const uint8_t*>(p.k) + x0;
+  const uint8_t* vx = static_cast<const uint8_t*>(p.v) + x0;
   // Rows that the tables reach (of values too: a token is written whole or not).
   const int reach = past < 0 ? 0 : static_cast<int>(max(0LL, min(static_cast<long long>(n), p.positions - past - t0)));
   const long long pos0 = static_cast<long long>(past) + t0 + r;
@@ -317,7 +327,7 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   // Everything whose address is known goes out at once: rows, slots and the rows of the tables. A
   // row beyond the last is the last again, which changes no magnitude. (In prompts, where requests'
   // padding makes whole blocks without tokens, those are left first.)
-  uint4 xa[NP], xb[NP], cv[NP], sv[NP];
+  uint4 xa[NP], xb[NP], cv[NP], sv[NP], va[NP], vb[NP];
   int slots[NP];
   const int slot0 = slot_row[0];
   if (reach == 0 || (p.T > p.block && slot0 < 0)) {
@@ -329,12 +339,12 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   for (int i = 0; i < NP; ++i) {
     const int row = r + i * dr, step = min(row, reach - 1) - r;
     slots[i] = row < n ? slot_row[row] : -1;
-    xa[i] = ldg_stream_v4(x + step * (2 * D));
-    xb[i] = ldg_stream_v4(x + step * (2 * D) + D);
-    if (!IS_V) {
-      cv[i] = ldg_v4(cosp + step * D);
-      sv[i] = ldg_v4(sinp + step * D);
-    }
+    xa[i] = ldg_stream_v4(kx + step * (2 * D));
+    xb[i] = ldg_stream_v4(kx + step * (2 * D) + D);
+    cv[i] = ldg_v4(cosp + step * D);
+    sv[i] = ldg_v4(sinp + step * D);
+    va[i] = ldg_stream_v4(vx + step * (2 * D));
+    vb[i] = ldg_stream_v4(vx + step * (2 * D) + D);
   }
   if (slot0 < 0) return;  // no token here
   const int blk = slot0 >> p.block_log2;
@@ -343,15 +353,10 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
     return;
   }
   const long long cell = static_cast<long long>(blk) * p.Hkv + h;
-  float* scale = (IS_V ? p.vs : p.ks) + cell;
-  uint8_t* out = (IS_V ? p.v8 : p.k8) + cell * p.block * D;
-  const float had = r0 > 0 ? *scale : 0.f;
-
-  float y1[NP][8], y2[NP][8];
-  unsigned live = 0;              // pairs of rows that hold a token
-  int wrong = -1;                 // a row whose slot or position is not fit, and its code
+  const float had_k = r0 > 0 ? p.ks[cell] : 0.f, had_v = r0 > 0 ? p.vs[cell] : 0.f;
+  unsigned live = 0;  // pairs of rows that hold a token
+  int wrong = -1;     // a row whose slot or position is not fit, and its code
   unsigned code = 0;
-  float peak = 0.f;               // the largest magnitude (NaN stays)
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int row = r + i * dr;
@@ -362,99 +367,115 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
       code = far ? 6u : 7u;
     }
     live |= on ? 1u << i : 0u;
-    const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
-    uint32_t cw[4], sw[4];
-    if constexpr (!IS_V) {
-      cw[0] = cv[i].x, cw[1] = cv[i].y, cw[2] = cv[i].z, cw[3] = cv[i].w;
-      sw[0] = sv[i].x, sw[1] = sv[i].y, sw[2] = sv[i].z, sw[3] = sv[i].w;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 v = unpack2<BF16>(aw[e]), w = unpack2<BF16>(dw[e]);
-      if constexpr (IS_V) {
-        y1[i][2 * e] = v.x;
-        y1[i][2 * e + 1] = v.y;
-        y2[i][2 * e] = w.x;
-        y2[i][2 * e + 1] = w.y;
-      } else {
-        // (products of two 16-bit values are exact)
-        const float2 cc = unpack2<BF16>(cw[e]), ss = unpack2<BF16>(sw[e]);
-        y1[i][2 * e] = fma_odd(v.x, cc.x, -__fmul_rn(w.x, ss.x));
-        y1[i][2 * e + 1] = fma_odd(v.y, cc.y, -__fmul_rn(w.y, ss.y));
-        y2[i][2 * e] = fma_odd(w.x, cc.x, __fmul_rn(v.x, ss.x));
-        y2[i][2 * e + 1] = fma_odd(w.y, cc.y, __fmul_rn(v.y, ss.y));
-      }
-    }
-    float high = peak;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) high = max3_abs_nan(high, y1[i][e], y2[i][e]);
-    peak = on ? high : peak;
   }
   if (wrong >= 0) record_error(code, static_cast<unsigned>(b), static_cast<unsigned>(wrong));
-  // Bits of the magnitude, NaN above infinity above every number; one more, 0: no row.
-  uint32_t top = live ? (__float_as_uint(peak) & 0x7fffffffu) + 1u : 0u;
-  top = __reduce_max_sync(0xffffffffu, top);
-  if constexpr (WPI > 1) {
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
-    __syncthreads();  // (and every thread has read the present scale)
+
+  // The rows' values y into the block of one cache.
+  auto put = [&](float (&y1)[NP][8], float (&y2)[NP][8], float* scale, uint8_t* cells, float had, uint32_t* maxima) {
+    float peak = 0.f;  // the largest magnitude (NaN stays)
 #pragma unroll
-    for (int w = 0; w < WPI; ++w) top = max(top, warp_max[w]);
-  }
-  if (top == 0) return;  // the item's: nothing is written, the scale neither
-  float unit = paged_unit(top - 1);
-  if (r0 > 0 && (unit <= had || had != had)) unit = had;  // (a NaN on either side stays)
-  if (lane_i == 0) *scale = unit;
-  const bool poison = unit != unit;
-  const float inv = 1.0f / unit;
-  uint8_t* dst = out + (r0 + r) * D + 8 * c;
+    for (int i = 0; i < NP; ++i) {
+      float high = peak;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) high = max3_abs_nan(high, y1[i][e], y2[i][e]);
+      peak = (live & (1u << i)) ? high : peak;
+    }
+    // Bits of the magnitude, NaN above infinity above every number; one more, 0: no row.
+    uint32_t top = live ? (__float_as_uint(peak) & 0x7fffffffu) + 1u : 0u;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if constexpr (WPI > 1) {
+      if ((threadIdx.x & 31) == 0) maxima[threadIdx.x >> 5] = top;
+      __syncthreads();  // (and every thread has read the present scales)
+#pragma unroll
+      for (int w = 0; w < WPI; ++w) top = max(top, maxima[w]);
+    }
+    if (top == 0) return;  // the item's: nothing is written, the scale neither
+    float unit = paged_unit(top - 1);
+    if (r0 > 0 && (unit <= had || had != had)) unit = had;  // (a NaN on either side stays)
+    if (lane_i == 0) scale[cell] = unit;
+    const bool poison = unit != unit;
+    const float inv = 1.0f / unit;
+    uint8_t* out = cells + cell * p.block * D;
+    uint8_t* dst = out + (r0 + r) * D + 8 * c;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if (!(live & (1u << i))) continue;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[e] = e4m3x4(y1[i][4 * e] * inv, y1[i][4 * e + 1] * inv, y1[i][4 * e + 2] * inv, y1[i][4 * e + 3] * inv);
+        w[2 + e] = e4m3x4(y2[i][4 * e] * inv, y2[i][4 * e + 1] * inv, y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv);
+      }
+      if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
+      *reinterpret_cast<uint2*>(dst + i * 16 * NT) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(dst + i * 16 * NT + D / 2) = make_uint2(w[2], w[3]);
+    }
+    if (r0 > 0 && unit > had) {
+      // The present rows under the larger scale.
+      const float f = had * inv;
+      for (int u = lane_i; u < r0 * (D / 16); u += NT) {
+        uint4* q = reinterpret_cast<uint4*>(out) + u;
+        const uint4 o = *q;
+        uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 lo = e4m3x2_widen(w[e] & 0xffffu), hi = e4m3x2_widen(w[e] >> 16);
+          w[e] = e4m3x4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+        }
+        *q = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+
+  float y1[NP][8], y2[NP][8];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    if (!(live & (1u << i))) continue;
-    uint32_t w[4];
+    const uint32_t aw[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, dw[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
+    const uint32_t cw[4] = {cv[i].x, cv[i].y, cv[i].z, cv[i].w}, sw[4] = {sv[i].x, sv[i].y, sv[i].z, sv[i].w};
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[e] = e4m3x4(y1[i][4 * e] * inv, y1[i][4 * e + 1] * inv, y1[i][4 * e + 2] * inv, y1[i][4 * e + 3] * inv);
-      w[2 + e] = e4m3x4(y2[i][4 * e] * inv, y2[i][4 * e + 1] * inv, y2[i][4 * e + 2] * inv, y2[i][4 * e + 3] * inv);
-    }
-    if (poison) w[0] = w[1] = w[2] = w[3] = 0x7f7f7f7fu;
-    *reinterpret_cast<uint2*>(dst + i * 16 * NT) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(dst + i * 16 * NT + D / 2) = make_uint2(w[2], w[3]);
-  }
-  if (r0 > 0 && unit > had) {
-    // The present rows under the larger scale.
-    const float f = had * inv;
-    for (int u = lane_i; u < r0 * (D / 16); u += NT) {
-      uint4* q = reinterpret_cast<uint4*>(out) + u;
-      const uint4 o = *q;
-      uint32_t w[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 lo = e4m3x2_widen(w[e] & 0xffffu), hi = e4m3x2_widen(w[e] >> 16);
-        w[e] = e4m3x4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
-      }
-      *q = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < 4; ++e) {
+      // (products of two 16-bit values are exact)
+      const float2 v = split2<BF16>(aw[e]), w = split2<BF16>(dw[e]);
+      const float2 cc = split2<BF16>(cw[e]), ss = split2<BF16>(sw[e]);
+      y1[i][2 * e] = fma_odd(v.x, cc.x, -__fmul_rn(w.x, ss.x));
+      y1[i][2 * e + 1] = fma_odd(v.y, cc.y, -__fmul_rn(w.y, ss.y));
+      y2[i][2 * e] = fma_odd(w.x, cc.x, __fmul_rn(v.x, ss.x));
+      y2[i][2 * e + 1] = fma_odd(w.y, cc.y, __fmul_rn(v.y, ss.y));
     }
   }
+  put(y1, y2, p.ks, p.k8, had_k, warp_max[0]);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const uint32_t aw[4] = {va[i].x, va[i].y, va[i].z, va[i].w}, dw[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = split2<BF16>(aw[e]), w = split2<BF16>(dw[e]);
+      y1[i][2 * e] = v.x;
+      y1[i][2 * e + 1] = v.y;
+      y2[i][2 * e] = w.x;
+      y2[i][2 * e + 1] = w.y;
+    }
+  }
+  put(y1, y2, p.vs, p.v8, had_v, warp_max[1]);
 }
 
 template <bool BF16, int WPI>
 __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, PAGED_WRITE_WARPS / (WPI == 1 ? 4 : WPI))
     paged_write_kernel(const PagedWriteParams p) {
+  // Warps' maxima of keys and of values: each is written again only after the other one's barrier.
   __shared__ uint32_t warp_max[2][WPI];
   griddep_launch_dependents();
   griddep_wait();
   // A grid of resident CTAs walks the items (short CTAs, one per item, ended faster than new ones
   // came: 13 of 64 warps per SM at any time). With WPI = 1 a warp is an item; else the CTA is one,
-  // and its barrier is reached by all or none.
-  const int per_page = 2 * p.Hkv, per_request = per_page * p.pages;
+  // and its barriers are reached by all or none.
+  const int per_request = p.Hkv * p.pages;
   const int stride = static_cast<int>(gridDim.x) * (WPI == 1 ? 4 : 1);
-  int odd = 0;  // (the warps' maxima of one item are read while those of the next are written)
   for (int item = WPI == 1 ? static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x) / 32 : static_cast<int>(blockIdx.x);
-       item < p.items; item += stride, odd ^= 1) {
+       item < p.items; item += stride) {
     const int b = small_div(item, per_request), in = item - b * per_request;
-    const int pg = small_div(in, per_page), kh = in - pg * per_page;
-    if (kh & 1) paged_write_item<BF16, WPI, true>(p, b, pg, kh >> 1, warp_max[odd]);
-    else paged_write_item<BF16, WPI, false>(p, b, pg, kh >> 1, warp_max[odd]);
+    const int pg = small_div(in, p.Hkv);
+    paged_write_item<BF16, WPI>(p, b, pg, in - pg * p.Hkv, warp_max);
   }
 }
 
