@@ -78,6 +78,8 @@ __device__ __forceinline__ void prefetch_l1(const void* p) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -138,7 +140,7 @@ struct DecodePagedShape {
   static constexpr int ROW = CB + 4;
   static constexpr int ML_BYTES = ((8 * HPU * 4) + 127) / 128 * 128;  // maxima and sums of the warps
   static constexpr int RAW_BYTES = (HPU + 1) * DP * 2;  // a unit's query rows and its cos and sin row
-  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + RAW_BYTES + 2560;
+  static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + 2 * RAW_BYTES + 2560;
   static constexpr int BUDGET = CTAS == 2 ? 113 * 1024 : 226 * 1024;
   static constexpr int TILES = (BUDGET - FIXED) / TILE;
   static constexpr int NV = TILES / 2 > 8 ? 8 : TILES / 2;            // stages of V
@@ -148,7 +150,7 @@ struct DecodePagedShape {
   static constexpr int OFF_Q = OFF_P + NPB * P_BYTES;
   static constexpr int OFF_ML = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_RAW = OFF_ML + ML_BYTES;
-  static constexpr int OFF_SC = OFF_RAW + RAW_BYTES;  // [NK][2][8] scales of a chunk's blocks
+  static constexpr int OFF_SC = OFF_RAW + 2 * RAW_BYTES;  // [NK][2][8] scales of a chunk's blocks
   static constexpr int NF = 4;                        // fragment entries in flight
   static constexpr int OFF_FRAG = OFF_SC + NK * 64;   // [NF] entries of 16 words
   static constexpr int OFF_OWED = OFF_FRAG + NF * 64; // [2] entries of units to join
@@ -565,11 +567,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   } else if (warp == 6) {
     // ------------------------------------------------------------------ fragments and queries
     const int D = p.D, half = D >> 1;
-    // A unit's query rows and its rows of the tables come to shared memory; then head by head (a
-    // loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of each half.
+    // A unit's query rows and its rows of the tables come to shared memory, a fragment ahead; then
+    // head by head (a loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of
+    // each half.
     constexpr int EPL = DP >= 128 ? DP / 128 : 1;
-    const uint32_t raw = sbase + S::OFF_RAW;
-    const uint32_t* raw32 = reinterpret_cast<const uint32_t*>(sgen + S::OFF_RAW);
     auto widen = [&](uint32_t w) -> float2 { return p.bf16 ? unpack2<true>(w) : unpack2<false>(w); };
     // Rows of the query tiles beyond the parts stay zero.
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
@@ -597,7 +598,22 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + e * 64) = f;
           mbar_arrive(FFULL(e));
         }
-        __syncwarp();
+        __syncwarp();  // (and every lane is done with the raw rows of entry k - 2)
+        if (!ended) {
+          if (f.chunks > 0) {
+            const uint32_t raw = sbase + S::OFF_RAW + (k & 1) * S::RAW_BYTES;
+            const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (static_cast<long long>(f.b) * p.Hq + f.h0) * (2 * D);
+            const long long trow = static_cast<long long>(f.len - 1) * D;
+            for (int i = lane; i < f.nh * (D >> 3); i += 32) cp_async16(raw + 16 * i, qrow + 16 * i);
+            if (lane < 2 * (D >> 4)) {  // cos, then sin: D bytes each
+              const int half16 = D >> 4;
+              const bool is_sin = lane >= half16;
+              cp_async16(raw + HPU * 2 * D + 16 * lane,
+                         static_cast<const uint8_t*>(is_sin ? p.sin : p.cos) + trow + 16 * (is_sin ? lane - half16 : lane));
+            }
+          }
+          cp_async_commit();
+        }
       }
       if (k == 0) {
         if (blockIdx.x == 0) report();
@@ -608,19 +624,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       if (f.kind == 0) break;
       const bool busy = f.chunks > 0;
-      if (busy) {
-        const uint8_t* qrow = static_cast<const uint8_t*>(p.q) + (static_cast<long long>(f.b) * p.Hq + f.h0) * (2 * D);
-        const long long trow = static_cast<long long>(f.len - 1) * D;
-        for (int i = lane; i < f.nh * (D >> 3); i += 32) cp_async16(raw + 16 * i, qrow + 16 * i);
-        if (lane < 2 * (D >> 4)) {  // cos, then sin: D bytes each
-          const int half16 = D >> 4;
-          const bool is_sin = lane >= half16;
-          cp_async16(raw + HPU * 2 * D + 16 * lane,
-                     static_cast<const uint8_t*>(is_sin ? p.sin : p.cos) + trow + 16 * (is_sin ? lane - half16 : lane));
-        }
-        cp_async_wait_all();
-        __syncwarp();
-      }
+      // (all but the newest group of copies: entry k - 1's)
+      if (ended) cp_async_wait_all(); else cp_async_wait_but_one();
+      __syncwarp();
+      const uint32_t* raw32 = reinterpret_cast<const uint32_t*>(sgen + S::OFF_RAW + (it & 1) * S::RAW_BYTES);
       if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
       if (busy) {
         uint8_t* qt = sgen + S::OFF_Q + qb * S::Q_BYTES;
