@@ -350,6 +350,25 @@ struct PagedWalk {
   }
 };
 
+// mbar_wait and mbar_wait_drain with everything but the first look in one place each: the kernel waits
+// at some thirty places, and what a fragment runs once is bound by the fetch of its code. The softmax
+// warps' waits stay inline at head_dim 128 and 256, where calls make them spill (8 x 32 heads of 2048
+// at head_dim 64: 17.9 -> 17.4 us with calls; a mixed batch at head_dim 128: 53.5 -> 55.6 us).
+__device__ __noinline__ bool paged_wait_on(uint32_t bar, uint32_t parity, volatile int* failed, unsigned int site) {
+  return mbar_wait(bar, parity, failed, site);
+}
+__device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int* failed, unsigned int site) {
+  return mbar_try_wait(bar, parity) || paged_wait_on(bar, parity, failed, site);
+}
+template <int DP>
+__device__ __forceinline__ bool softmax_wait(uint32_t bar, uint32_t parity, volatile int* failed, unsigned int site) {
+  if constexpr (DP <= 64) return paged_wait(bar, parity, failed, site);
+  else return mbar_wait(bar, parity, failed, site);
+}
+__device__ __noinline__ bool paged_wait_drain(uint32_t bar, uint32_t parity, unsigned int site) {
+  return mbar_wait_drain(bar, parity, site);
+}
+
 template <int DP, int HPU>
 __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePagedShape<DP, HPU>::CTAS)
     decode_paged_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -445,7 +464,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     int g = 0;
     bool ok = true;
     for (int it = 0; ok; ++it) {
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 800)))) break;
+      if (!(ok = __all_sync(0xffffffffu, paged_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 800)))) break;
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       __syncwarp();
       if (f.kind == 0) break;
@@ -473,7 +492,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (bad && is_k && lane < 8) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(mine));
         const long long cell = bad ? static_cast<long long>(p.N) * p.Hkv  // beyond the map: zeros
                                    : static_cast<long long>(mine) * p.Hkv + f.kvh;
-        if (g >= ns) ok = mbar_wait(is_k ? KEMPTY(s) : VEMPTY(s), ((g / ns) - 1) & 1, failed, 801);
+        if (g >= ns) ok = paged_wait(is_k ? KEMPTY(s) : VEMPTY(s), ((g / ns) - 1) & 1, failed, 801);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         if (lane == 0) mbar_expect_tx(full, static_cast<uint32_t>(here << p.block_log2) * DP);
         __syncwarp();
@@ -491,7 +510,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     }
     // The last copies land before the CTA may exit.
     for (int j = g > ns ? g - ns : 0; j < g; ++j)
-      mbar_wait_drain(is_k ? KFULL(j % ns) : VFULL(j % ns), (j / ns) & 1, 802);
+      paged_wait_drain(is_k ? KFULL(j % ns) : VFULL(j % ns), (j / ns) & 1, 802);
   } else if (warp == 5) {
     // ------------------------------------------------------------------ MMA issuer
     const bool leader = elect_one();
@@ -499,7 +518,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     int g = 0;
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 810)))) break;
+      if (!(ok = __all_sync(0xffffffffu, paged_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 810)))) break;
       const PagedFrag* f = reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       const int kind = f->kind, n = f->chunks;
       __syncwarp();
@@ -508,7 +527,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       __syncwarp();
       // (also without chunks: the queries of entry it are prepared once QEMPTY of entry it - 2 is
       // complete, so this warp's arrivals stay in their phases)
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 816)))) break;
+      if (!(ok = __all_sync(0xffffffffu, paged_wait(QFULL(qb), (it >> 1) & 1, failed, 816)))) break;
       if (n == 0) {
         if (leader) mbar_arrive(QEMPTY(qb));
         __syncwarp();
@@ -518,8 +537,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       for (int j = 0; j <= n; ++j) {
         if (j < n) {  // S of chunk j
           const int gj = g + j, s = gj % NK;
-          ok = mbar_wait(KFULL(s), (gj / NK) & 1, failed, 811);
-          if (ok && gj >= 2) ok = mbar_wait(SEMPTY(gj & 1), ((gj >> 1) - 1) & 1, failed, 812);
+          ok = paged_wait(KFULL(s), (gj / NK) & 1, failed, 811);
+          if (ok && gj >= 2) ok = paged_wait(SEMPTY(gj & 1), ((gj >> 1) - 1) & 1, failed, 812);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
           if (leader) {
@@ -539,8 +558,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         if (j > 0) {  // O of chunk j - 1
           const int gj = g + j - 1, s = gj % NV;
-          ok = mbar_wait(PFULL(gj % NPB), (gj / NPB) & 1, failed, 813);
-          if (ok) ok = mbar_wait(VFULL(s), (gj / NV) & 1, failed, 814);
+          ok = paged_wait(PFULL(gj % NPB), (gj / NPB) & 1, failed, 813);
+          if (ok) ok = paged_wait(VFULL(s), (gj / NV) & 1, failed, 814);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
           if (leader) {
@@ -561,7 +580,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     }
     if (leader) {
       umma_commit(BAR_DRAIN);
-      mbar_wait_drain(BAR_DRAIN, 0, 815);
+      paged_wait_drain(BAR_DRAIN, 0, 815);
     }
     __syncwarp();
   } else if (warp == 6) {
@@ -593,7 +612,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         // The producers will ask for these entries of the block table.
         if (!ended && f.kbeg + (lane << p.block_log2) < f.kbeg + f.keys)
           prefetch_l1(p.table + static_cast<long long>(f.b) * p.width + (f.kbeg >> p.block_log2) + lane);
-        if (k >= S::NF && !__all_sync(0xffffffffu, mbar_wait(FEMPTY(e), ((k / S::NF) - 1) & 1, failed, 821))) break;
+        if (k >= S::NF && !__all_sync(0xffffffffu, paged_wait(FEMPTY(e), ((k / S::NF) - 1) & 1, failed, 821))) break;
         if (lane == 0) {
           *reinterpret_cast<PagedFrag*>(sgen + S::OFF_FRAG + e * 64) = f;
           mbar_arrive(FFULL(e));
@@ -628,7 +647,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       if (ended) cp_async_wait_all(); else cp_async_wait_but_one();
       __syncwarp();
       const uint32_t* raw32 = reinterpret_cast<const uint32_t*>(sgen + S::OFF_RAW + (it & 1) * S::RAW_BYTES);
-      if (it >= 2 && !__all_sync(0xffffffffu, mbar_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
+      if (it >= 2 && !__all_sync(0xffffffffu, paged_wait(QEMPTY(qb), ((it >> 1) - 1) & 1, failed, 820))) break;
       if (busy) {
         uint8_t* qt = sgen + S::OFF_Q + qb * S::Q_BYTES;
         float2 cc[EPL], ss[EPL];
@@ -693,10 +712,10 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     int g = 0, mq = 0;  // chunks, combined column blocks
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
+      if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
       if (f.kind == 0) break;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(QFULL(qb), (it >> 1) & 1, failed, 830)))) break;
+      if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(QFULL(qb), (it >> 1) & 1, failed, 830)))) break;
       float qs[HPU];
 #pragma unroll
       for (int h = 0; h < HPU; ++h) qs[h] = reinterpret_cast<const float*>(sgen + S::OFF_QS)[qb * HPU + h];
@@ -717,7 +736,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       // A key's row of P has only its warp's bytes (a 16- or 32-byte part); the rest is zero, once
       // the last fragment's rows of O, which lie there too, have been read.
-      if (mq > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 838)))) break;
+      if (mq > 0 && !(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_FREE, (mq - 1) & 1, failed, 838)))) break;
 #pragma unroll
       for (int i = 0; i < NPB * S::PM / 16; ++i)
         st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + tid * S::PM + 16 * (i % (S::PM / 16)),
@@ -732,7 +751,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         const int gj = g + j, s = gj % NK;
         const int left = f.keys - j * CK;  // keys of this chunk and those behind it
         const bool valid = tid < left;
-        ok = mbar_wait(KFULL(s), (gj / NK) & 1, failed, 831);
+        ok = softmax_wait<DP>(KFULL(s), (gj / NK) & 1, failed, 831);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         const float* sc = reinterpret_cast<const float*>(sgen + S::OFF_SC + s * 64);
         const float ksc = valid ? sc[tid >> p.block_log2] : 1.0f;
@@ -741,7 +760,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         __syncwarp();
         if (lane == 0) mbar_arrive(KEMPTY(s));
         const float lv = lg2(vsc), rv = __fdividef(1.0f, vsc);
-        ok = mbar_wait(SFULL(gj & 1), (gj >> 1) & 1, failed, 832);
+        ok = softmax_wait<DP>(SFULL(gj & 1), (gj >> 1) & 1, failed, 832);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         float sv[NQ];
@@ -800,9 +819,9 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         // The P buffer was last read by PV(gj - NPB); a moved reference rescales O, which holds PV up
         // to gj - 1 of this fragment.
-        if (gj >= NPB) ok = mbar_wait(PDONE(gj % NPB), ((gj / NPB) - 1) & 1, failed, 833);
-        if (NPB > 1 && ok && moved && j > 0) ok = mbar_wait(PDONE((gj - 1) % NPB), ((gj - 1) / NPB) & 1, failed, 834);
-        if (ok && left < CK) ok = mbar_wait(VFULL(gj % NV), (gj / NV) & 1, failed, 835);
+        if (gj >= NPB) ok = softmax_wait<DP>(PDONE(gj % NPB), ((gj / NPB) - 1) & 1, failed, 833);
+        if (NPB > 1 && ok && moved && j > 0) ok = softmax_wait<DP>(PDONE((gj - 1) % NPB), ((gj - 1) / NPB) & 1, failed, 834);
+        if (ok && left < CK) ok = softmax_wait<DP>(VFULL(gj % NV), (gj / NV) & 1, failed, 835);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         if (moved && j > 0) {
@@ -858,7 +877,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h through shared
       // memory, then a thread sums the 12 of an output.
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(PDONE((g - 1) % NPB), ((g - 1) / NPB) & 1, failed, 836)))) break;
+      if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(PDONE((g - 1) % NPB), ((g - 1) / NPB) & 1, failed, 836)))) break;
       tc_fence_after();
       float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
       float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
@@ -870,7 +889,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
 #pragma unroll
           for (int c = 0; c < S::CB; c += 16) tmem_ld16(tmem + lane_off + S::TM_O + cb + c, o + c);
           // The columns combined before have been read.
-          if (cb > 0) ok = mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 837);
+          if (cb > 0) ok = softmax_wait<DP>(BAR_FREE, (mq - 1) & 1, failed, 837);
           tmem_wait_ld();
           if (lane < 3 * HPU) {
             float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW);
@@ -890,7 +909,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_before();
         mbar_arrive(BAR_MRG);
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(BAR_MRG, mq & 1, failed, 837)))) break;
+        if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_MRG, mq & 1, failed, 837)))) break;
         // Lane w HPU + h: the factor of warp w's rows of head h, 2^(m_w - M) / L.
         if (cb == 0) {
           const int i = lane % (4 * HPU);
@@ -937,7 +956,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           // A ticket on the unit's counter. The partial stores reach this thread through the barrier;
           // its acquire-release add makes them visible before the ticket and, after the last
           // ticket, the other fragments' partials visible to this CTA.
-          if (mbar_wait(BAR_FREE, (mq - 1) & 1, failed, 839)) {
+          if (softmax_wait<DP>(BAR_FREE, (mq - 1) & 1, failed, 839)) {
             if (atom_add_acq_rel_gpu(&p.cnt[f.c0], 1) == f.nf - 1) {
               p.cnt[f.c0] = 0;  // no other ticket is to come: ready for the next call
               owed[*n_owed] = f;
