@@ -37,6 +37,8 @@
 // others. Every wait is bounded.
 #pragma once
 
+#include <float.h>
+
 #include "paged_sm100.cuh"
 
 namespace du {
@@ -63,17 +65,14 @@ struct DecodePagedParams {
 // Chunks per CTA that whole pieces of units may cost over equal ranges of chunks: a CTA whose range
 // straddles two units combines twice, about three chunks' time.
 constexpr int DECODE_PAGED_PIECE_SLACK = 3;
-// The last fragment's CTA holds a weight per fragment and head where it combines rows otherwise.
+// The CTA that joins a unit holds a weight per fragment and head where P is otherwise.
 constexpr int DECODE_PAGED_MAX_CTAS = 12 * 36;
 __device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
 
-// cp.async of 4 and of 16 bytes, and an arrival on `bar` once this thread's earlier cp.async have landed.
+// cp.async of 4 and of 16 bytes, their groups, and an arrival on `bar` once this thread's earlier
+// cp.async have landed.
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// Brings a word into L1 and waits for nothing.
-__device__ __forceinline__ void prefetch_l1(const void* p) {
-  asm volatile("{\n\t.reg .b32 t;\n\tld.global.b32 t, [%0];\n\t}\n" ::"l"(p));
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -83,6 +82,10 @@ __device__ __forceinline__ void cp_async_wait_but_one() { asm volatile("cp.async
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Brings a word into L1 and waits for nothing.
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("{\n\t.reg .b32 t;\n\tld.global.b32 t, [%0];\n\t}\n" ::"l"(p));
 }
 // D[tmem] (+)= A[smem] * B[smem], e4m3 operands, fp32 accumulate, one CTA.
 __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -195,7 +198,7 @@ struct PagedStart {
   int pieces;
 };
 
-// One fragment, as warp 6 leaves it for the MMA and softmax warps (16 words).
+// One fragment, as warp 6 leaves it for the other warps (16 words).
 struct PagedFrag {
   int kind;       // 1 a fragment, 0 the end
   int b, h0, nh;  // request, first query head, heads
@@ -595,12 +598,6 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
       st_shared_v4(sbase + S::OFF_Q + 16 * i, make_uint4(0, 0, 0, 0));
     __syncwarp();
-    // Lengths out of range are reported once, by the first CTA.
-    auto report = [&]() {
-      for (int b = lane; b < p.B; b += 32)
-        if (static_cast<unsigned>(p.lens[b]) > static_cast<unsigned>(p.max_len))
-          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
-    };
     // Entry k is published before the queries of entry k - 1 are prepared.
     bool ended = false;
     for (int k = 0;; ++k) {
@@ -634,10 +631,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           cp_async_commit();
         }
       }
-      if (k == 0) {
-        if (blockIdx.x == 0) report();
-        continue;
-      }
+      if (k == 0) continue;
       const int it = k - 1, qb = it & 1;
       // (entry k - 1 stays until the softmax warps have read it, which wait for its queries)
       const PagedFrag f = *reinterpret_cast<const PagedFrag*>(sgen + S::OFF_FRAG + (it % S::NF) * 64);
@@ -705,6 +699,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       __syncwarp();  // (and the raw rows have been read)
       mbar_arrive(QFULL(qb));
     }
+    // Lengths out of range are reported by the first CTA, once its work is under way.
+    if (blockIdx.x == 0)
+      for (int b = lane; b < p.B; b += 32)
+        if (static_cast<unsigned>(p.lens[b]) > static_cast<unsigned>(p.max_len))
+          record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(p.lens[b]));
   } else {
     // ------------------------------------------------------------------ warps 0-3: softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
@@ -744,7 +743,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       float m[HPU], l[HPU];
 #pragma unroll
       for (int h = 0; h < HPU; ++h) {
-        m[h] = -1e30f;
+        m[h] = -FLT_MAX;  // (not infinite: a masked key's weight is 2^(-inf - m) = 0)
         l[h] = 0.f;
       }
       for (int j = 0; j < f.chunks; ++j) {

@@ -358,6 +358,24 @@ def test_attend_rising_scores():
     assert bool(((got.double() - want).abs() <= plain.tolerance(want, bound, torch.float16)).all())
 
 
+def test_attend_huge_negative_scores():
+    """Every score is far below any usual mask value; the largest still carries the weight."""
+    D, block, n = 64, 16, 40
+    q = torch.full((1, 2, 1, D), 2.0**60, dtype=torch.bfloat16)
+    k = -torch.ones(3, 2, block, D, dtype=torch.float64)
+    k[1, :, 3] = -0.5
+    k8, ks = plain.quantise_cache(k)
+    ks = ks * 2.0**50
+    v8, vs = plain.quantise_cache(torch.randn(k.shape, generator=_gen(1)).double())
+    cos, sin = torch.ones(n, D // 2, dtype=torch.bfloat16), torch.zeros(n, D // 2, dtype=torch.bfloat16)
+    table = [[0, 1, 2]]
+    d = lambda t, dt=torch.float8_e4m3fn: t.float().to(dt).to(DEV)  # noqa: E731
+    got = dominus_ultra_decode_paged(q.to(DEV), d(k8), d(v8), d(ks, torch.float32), d(vs, torch.float32), torch.tensor(table, dtype=torch.int32, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV), cos.to(DEV), sin.to(DEV)).cpu()
+    want = (v8[1, :, 3] * vs[1, :, None])[None, :, None]  # one key takes all
+    # the value is carried to 2^-11 (parts of the weight) and rounded to half a step
+    assert bool(((got.double() - want).abs() <= want.abs() * (2.0**-8 + 2.0**-10) + 1e-30).all())
+
+
 def _simple_call(B=2, Hq=4, Hkv=2, D=64, block=16, lens=(40, 100), dtype=torch.bfloat16, seed=1):
     q, k8, v8, ks, vs, table, cos, sin = _attend_case(B, Hq, Hkv, D, block, list(lens), dtype, seed)
     args = [q.to(DEV), k8.float().to(torch.float8_e4m3fn).to(DEV), v8.float().to(torch.float8_e4m3fn).to(DEV), ks.float().to(DEV),
