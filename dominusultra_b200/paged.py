@@ -16,7 +16,6 @@ and tables stay on the GPU: no call synchronises, and each can be captured into 
 
 from __future__ import annotations
 
-import contextlib
 import threading
 from typing import Tuple
 
@@ -24,6 +23,7 @@ import torch
 
 from . import _lib
 from .attention import (
+    _RAW_STREAM,
     _RETIRED,
     _aligned,
     _OnDevice,
@@ -47,11 +47,11 @@ _CODES = {_F16: _lib.DU_DTYPE_F16, _BF16: _lib.DU_DTYPE_BF16}
 _GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-_HERE = contextlib.nullcontext()
 
 
-def _fit(t: torch.Tensor, dtype: torch.dtype, index: int) -> bool:
-    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+def _stream_of(index: int) -> int:
+    """Handle of torch's current stream on the device of this index."""
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else _stream(torch.device("cuda", index))
 
 
 def _validate_block_size(block_size: int) -> None:
@@ -169,7 +169,7 @@ _SLAB_LOCK = threading.Lock()
 _SCRATCH = {}
 
 
-def _decode_scratch(nbytes: int, device: torch.device, index: int, stream: int):
+def _decode_scratch(nbytes: int, index: int, stream: int):
     """(tickets, workspace, keep-alive tensors) of a paged decode on torch's current stream.
 
     Eager calls share a pair per (device, stream): calls on one stream run in order. A call that
@@ -179,8 +179,9 @@ def _decode_scratch(nbytes: int, device: torch.device, index: int, stream: int):
         pair = _SCRATCH.get((index, stream))
         slab = _SLABS.get(index)
         if pair is None or pair[2] < nbytes or slab is None or slab[1] > _SLAB_WORDS // 2:
-            pair = _grow_scratch(nbytes, device, index, stream)
+            pair = _grow_scratch(nbytes, index, stream)
         return pair[0], pair[1], None
+    device = torch.device("cuda", index)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     with _SLAB_LOCK:
         slab = _SLABS.get(index)
@@ -194,8 +195,9 @@ def _decode_scratch(nbytes: int, device: torch.device, index: int, stream: int):
     return tickets.data_ptr(), ws.data_ptr(), (ws, tickets)
 
 
-def _grow_scratch(nbytes: int, device: torch.device, index: int, stream: int):
+def _grow_scratch(nbytes: int, index: int, stream: int):
     """A (device, stream)'s scratch of at least nbytes, and a ticket slab with room for captures."""
+    device = torch.device("cuda", index)
     with _SLAB_LOCK:
         slab = _SLABS.get(index)
         if slab is None or slab[1] > _SLAB_WORDS // 2:
@@ -254,29 +256,37 @@ def dominus_ultra_paged_tables(
     """
     shape = block_table.shape
     index = block_table.get_device()
-    # One look at what every call has to have; where it fails, the checks by name.
+    # One look at what every call has to have (written out: a call's host time is mostly this); where
+    # it fails, the checks by name.
     if not (
         len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and index >= 0
         and block_size in _BLOCK_SIZES and max_new >= 0
-        and _fit(block_table, _I32, index) and _fit(free_blocks, _I32, index) and _fit(free_state, _I32, index)
-        and free_blocks.dim() == 1 and free_blocks.shape[0] > 0 and free_state.shape == (2,)
-        and _fit(cache_seqlens, _I32, index) and _fit(new_seqlens, _I32, index)
-        and cache_seqlens.shape == shape[:1] and new_seqlens.shape == shape[:1]
+        and block_table.dtype is _I32 and block_table.is_contiguous()
+        and free_blocks.dtype is _I32 and free_blocks.get_device() == index and free_blocks.is_contiguous()
+        and free_state.dtype is _I32 and free_state.get_device() == index and free_state.is_contiguous()
+        and free_blocks.dim() == 1 and free_blocks.shape[0] > 0 and free_state.dim() == 1 and free_state.shape[0] == 2
+        and cache_seqlens.dtype is _I32 and cache_seqlens.get_device() == index and cache_seqlens.is_contiguous()
+        and new_seqlens.dtype is _I32 and new_seqlens.get_device() == index and new_seqlens.is_contiguous()
+        and cache_seqlens.dim() == 1 and cache_seqlens.shape[0] == shape[0]
+        and new_seqlens.dim() == 1 and new_seqlens.shape[0] == shape[0]
     ):
         cache_seqlens, new_seqlens = _check_tables(
             block_table, cache_seqlens, new_seqlens, free_blocks, free_state, block_size, max_new
         )
+    if _GET_DEVICE() != index:
+        with _OnDevice(block_table.device):
+            return dominus_ultra_paged_tables(
+                block_table, cache_seqlens, new_seqlens, free_blocks, free_state, block_size, max_new
+            )
     batch, max_blocks = shape
-    device = block_table.device
-    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
-        slots = block_table.new_empty((batch, max_new))
-        seqlens = torch.empty_like(cache_seqlens)
-        state = torch.empty_like(free_state)
-        rc = _lib.load().du_paged_tables(
-            block_table.data_ptr(), cache_seqlens.data_ptr(), new_seqlens.data_ptr(), free_blocks.data_ptr(),
-            free_state.data_ptr(), slots.data_ptr(), seqlens.data_ptr(), state.data_ptr(), batch, max_blocks,
-            free_blocks.shape[0], block_size, max_new, _stream(device),
-        )
+    slots = block_table.new_empty((batch, max_new))
+    seqlens = torch.empty_like(cache_seqlens)
+    state = torch.empty_like(free_state)
+    rc = _lib.load().du_paged_tables(
+        block_table.data_ptr(), cache_seqlens.data_ptr(), new_seqlens.data_ptr(), free_blocks.data_ptr(),
+        free_state.data_ptr(), slots.data_ptr(), seqlens.data_ptr(), state.data_ptr(), batch, max_blocks,
+        free_blocks.shape[0], block_size, max_new, _stream_of(index),
+    )
     if rc:
         _lib.check(rc, "du_paged_tables")
     return slots, seqlens, state
@@ -347,40 +357,55 @@ def dominus_ultra_paged_write(
     index, dtype = k_new.get_device(), k_new.dtype
     if not (
         len(shape) == 4 and len(cache) == 4 and index >= 0 and dtype in _CODES
-        and k_new.is_contiguous() and _fit(v_new, dtype, index) and v_new.shape == shape
-        and _fit(cos, dtype, index) and _fit(sin, dtype, index)
-        and cos.dim() == 2 and sin.dim() == 2 and cos.shape[1] * 2 == shape[3] and sin.shape[1] * 2 == shape[3]
-        and cos.shape[0] > 0 and sin.shape[0] > 0
+        and k_new.is_contiguous() and v_new.shape == shape
+        and v_new.dtype is dtype and v_new.get_device() == index and v_new.is_contiguous()
+        and _fit_rope(cos, sin, dtype, index, shape[3])
         and shape[0] > 0 and shape[1] > 0 and shape[2] > 0 and shape[3] in _HEAD_DIMS
         and _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index)
         and cache[1] == shape[1] and cache[3] == shape[3]
-        and _fit(slots, _I32, index) and slots.shape == (shape[0], shape[2])
-        and _fit(cache_seqlens, _I32, index) and cache_seqlens.shape == shape[:1]
+        and slots.dtype is _I32 and slots.get_device() == index and slots.is_contiguous()
+        and slots.dim() == 2 and slots.shape[0] == shape[0] and slots.shape[1] == shape[2]
+        and cache_seqlens.dtype is _I32 and cache_seqlens.get_device() == index and cache_seqlens.is_contiguous()
+        and cache_seqlens.dim() == 1 and cache_seqlens.shape[0] == shape[0]
     ):
         cache_seqlens = _check_write(k_new, v_new, k_cache, v_cache, k_scale, v_scale, slots, cache_seqlens, cos, sin)
-    B, Hkv, T, D = shape
-    device = k_new.device
+    if _GET_DEVICE() != index:
+        with _OnDevice(k_new.device):
+            return dominus_ultra_paged_write(
+                k_new, v_new, k_cache, v_cache, k_scale, v_scale, slots, cache_seqlens, cos, sin
+            )
     k, v, c, s = k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
-    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
-        if (k | v | c | s) & 15:
-            k_new, v_new, cos, sin = (_aligned(t) for t in (k_new, v_new, cos, sin))
-            k, v, c, s = k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
-        rc = _lib.load().du_paged_write(
-            k, v, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(),
-            cache_seqlens.data_ptr(), c, s, B, Hkv, T, D, cache[0], cache[2], _CODES[dtype],
-            min(cos.shape[0], sin.shape[0]), _stream(device),
-        )
+    if (k | v | c | s) & 15:
+        k_new, v_new, cos, sin = (_aligned(t) for t in (k_new, v_new, cos, sin))
+        k, v, c, s = k_new.data_ptr(), v_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    rc = _lib.load().du_paged_write(
+        k, v, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(),
+        cache_seqlens.data_ptr(), c, s, *shape, cache[0], cache[2], _CODES[dtype],
+        min(cos.shape[0], sin.shape[0]), _stream_of(index),
+    )
     if rc:
         _lib.check(rc, "du_paged_write")
 
 
-def _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index) -> bool:
+def _fit_rope(cos, sin, dtype, index, head_dim) -> bool:
+    c, s = cos.shape, sin.shape
     return (
-        _fit(k_cache, _E4M3, index) and _fit(v_cache, _E4M3, index) and v_cache.shape == cache
-        and cache[0] > 0 and cache[1] > 0 and cache[2] in _BLOCK_SIZES
+        cos.dtype is dtype and cos.get_device() == index and cos.is_contiguous()
+        and sin.dtype is dtype and sin.get_device() == index and sin.is_contiguous()
+        and len(c) == 2 and len(s) == 2 and c[1] * 2 == head_dim and s[1] * 2 == head_dim and c[0] > 0 and s[0] > 0
+    )
+
+
+def _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index) -> bool:
+    pair = cache[:2]
+    return (
+        k_cache.dtype is _E4M3 and k_cache.get_device() == index and k_cache.is_contiguous()
+        and v_cache.dtype is _E4M3 and v_cache.get_device() == index and v_cache.is_contiguous()
+        and v_cache.shape == cache and cache[0] > 0 and cache[1] > 0 and cache[2] in _BLOCK_SIZES
         and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
-        and _fit(k_scale, _F32, index) and _fit(v_scale, _F32, index)
-        and k_scale.shape == cache[:2] and v_scale.shape == cache[:2]
+        and k_scale.dtype is _F32 and k_scale.get_device() == index and k_scale.is_contiguous()
+        and v_scale.dtype is _F32 and v_scale.get_device() == index and v_scale.is_contiguous()
+        and k_scale.shape == pair and v_scale.shape == pair
     )
 
 
@@ -451,37 +476,40 @@ def dominus_ultra_decode_paged(
     index, dtype = q_new.get_device(), q_new.dtype
     if not (
         len(shape) == 4 and len(cache) == 4 and len(table) == 2 and index >= 0 and dtype in _CODES
-        and q_new.is_contiguous() and _fit(cos, dtype, index) and _fit(sin, dtype, index)
-        and cos.dim() == 2 and sin.dim() == 2 and cos.shape[1] * 2 == shape[3] and sin.shape[1] * 2 == shape[3]
-        and cos.shape[0] > 0 and sin.shape[0] > 0
+        and q_new.is_contiguous() and _fit_rope(cos, sin, dtype, index, shape[3])
         and shape[0] > 0 and shape[1] > 0 and shape[2] == 1 and shape[3] in _HEAD_DIMS
         and _fit_cache(k_cache, v_cache, k_scale, v_scale, cache, index)
         and shape[1] % cache[1] == 0 and cache[3] == shape[3]
-        and _fit(block_table, _I32, index) and table[0] == shape[0] and table[1] > 0
-        and _fit(cache_seqlens, _I32, index) and cache_seqlens.shape == shape[:1]
+        and block_table.dtype is _I32 and block_table.get_device() == index and block_table.is_contiguous()
+        and table[0] == shape[0] and table[1] > 0
+        and cache_seqlens.dtype is _I32 and cache_seqlens.get_device() == index and cache_seqlens.is_contiguous()
+        and cache_seqlens.dim() == 1 and cache_seqlens.shape[0] == shape[0]
     ):
         block_table, cache_seqlens = _check_decode(
             q_new, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, cos, sin
         )
+    if _GET_DEVICE() != index:
+        with _OnDevice(q_new.device):
+            return dominus_ultra_decode_paged(
+                q_new, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, cos, sin
+            )
     B, Hq, _, D = shape
     num_blocks, Hkv, block_size, _ = cache
     max_blocks = table[1]
-    device = q_new.device
     q, c, s = q_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
-    with _OnDevice(device) if _GET_DEVICE() != index else _HERE:
-        if (q | c | s) & 15:
-            q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
-            q, c, s = q_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
-        out = torch.empty_like(q_new)
-        stream = _stream(device)
-        nbytes = _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, index)
-        tickets, ws, keep = _decode_scratch(nbytes, device, index, stream)
-        rc = _lib.load().du_decode_paged(
-            q, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
-            cache_seqlens.data_ptr(), c, s, out.data_ptr(), B, Hq, Hkv, D, num_blocks, block_size, max_blocks,
-            _CODES[dtype], D**-0.5, min(cos.shape[0], sin.shape[0]), tickets, ws, nbytes, stream,
-        )
-        del keep
+    if (q | c | s) & 15:
+        q_new, cos, sin = (_aligned(t) for t in (q_new, cos, sin))
+        q, c, s = q_new.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    out = torch.empty_like(q_new)
+    stream = _stream_of(index)
+    nbytes = _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, index)
+    tickets, ws, keep = _decode_scratch(nbytes, index, stream)
+    rc = _lib.load().du_decode_paged(
+        q, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+        cache_seqlens.data_ptr(), c, s, out.data_ptr(), B, Hq, Hkv, D, num_blocks, block_size, max_blocks,
+        _CODES[dtype], D**-0.5, min(cos.shape[0], sin.shape[0]), tickets, ws, nbytes, stream,
+    )
+    del keep
     if rc:
         _lib.check(rc, "du_decode_paged")
     return out
