@@ -1276,12 +1276,12 @@ int check_paged(int Hkv, int num_blocks, int block_size) {
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
-template <bool BF16, int WPI>
+template <bool BF16, int WPI, int NP>
 int launch_paged_write_t(const du::PagedWriteParams& prm, cudaStream_t st) {
   constexpr int kWarps = WPI == 1 ? 4 : WPI;  // of a CTA
   const long long need = WPI == 1 ? (static_cast<long long>(prm.items) + 3) / 4 : prm.items;
-  const long long most = static_cast<long long>(sm_count()) * (du::PAGED_WRITE_WARPS / kWarps);
-  cudaError_t e = launch_kernel(du::paged_write_kernel<BF16, WPI>, dim3(static_cast<unsigned>(need < most ? need : most)),
+  const long long most = static_cast<long long>(sm_count()) * (du::paged_write_warps(NP) / kWarps);
+  cudaError_t e = launch_kernel(du::paged_write_kernel<BF16, WPI, NP>, dim3(static_cast<unsigned>(need < most ? need : most)),
                                 32 * kWarps, 0, st, true, prm);
   if (e != cudaSuccess) return cuda_fail(e, "paged write launch");
   e = cudaGetLastError();
@@ -1291,14 +1291,17 @@ int launch_paged_write_t(const du::PagedWriteParams& prm, cudaStream_t st) {
 
 template <bool BF16>
 int launch_paged_write(const du::PagedWriteParams& prm, cudaStream_t st) {
-  // Warps per item: enough for four chunk pairs per thread of the largest item.
+  // A warp per item while four chunk pairs per thread hold the largest one, with no more of them than
+  // it needs (rows repeated to fill a thread cost as much as rows); else warps enough for four.
   const int rows = prm.T < prm.block ? prm.T : prm.block;
   const long long pairs = static_cast<long long>(rows) << (prm.d_log2 - 4);
-  if (pairs <= 128) return launch_paged_write_t<BF16, 1>(prm, st);
-  if (pairs <= 256) return launch_paged_write_t<BF16, 2>(prm, st);
-  if (pairs <= 512) return launch_paged_write_t<BF16, 4>(prm, st);
-  if (pairs <= 1024) return launch_paged_write_t<BF16, 8>(prm, st);
-  return launch_paged_write_t<BF16, 16>(prm, st);
+  if (pairs <= 32) return launch_paged_write_t<BF16, 1, 1>(prm, st);
+  if (pairs <= 64) return launch_paged_write_t<BF16, 1, 2>(prm, st);
+  if (pairs <= 128) return launch_paged_write_t<BF16, 1, 4>(prm, st);
+  if (pairs <= 256) return launch_paged_write_t<BF16, 2, 4>(prm, st);
+  if (pairs <= 512) return launch_paged_write_t<BF16, 4, 4>(prm, st);
+  if (pairs <= 1024) return launch_paged_write_t<BF16, 8, 4>(prm, st);
+  return launch_paged_write_t<BF16, 16, 4>(prm, st);
 }
 
 // Query heads per unit of the paged decode: the group of a KV head in equal parts of at most 8.

@@ -279,15 +279,14 @@ __device__ __forceinline__ float paged_unit(uint32_t amax_bits) {
   return __int_as_float((e + 127) << 23);
 }
 
-// Resident warps per SM that the writer's registers are kept to, and chunk pairs per thread of an item.
-constexpr int PAGED_WRITE_WARPS = 16;
-constexpr int PAGED_WRITE_PAIRS = 4;
+// Resident warps per SM that the writer's registers are kept to, by the chunk pairs per thread.
+constexpr int paged_write_warps(int pairs) { return pairs == 4 ? 16 : (pairs == 2 ? 24 : 32); }
 
 // Quantises the new tokens of a call into the cache: keys rotated at their positions, one scale
 // per (block, KV head) and per cache.
 //
 // A work item is (request, block that its tokens touch, KV head), its keys and then its values; WPI
-// warps take it, a thread at most four pairs of 16-byte chunks i, i + D/2 of a row, which is what a
+// warps take it, a thread NP (at most four) pairs of 16-byte chunks i, i + D/2 of a row, which is what a
 // rotation pairs up, held in registers from the load to the store. The largest magnitude of the
 // item's rows gives the scale: the smallest power of two with amax <= 448 scale, or the block's
 // present scale where that is larger and the block holds rows already. Products of two 16-bit values
@@ -300,10 +299,9 @@ constexpr int PAGED_WRITE_PAIRS = 4;
 // Bound by HBM for prompts (2 bytes read and 1 written per value), closely followed by the issue
 // slots: about 10 instructions per key value and 4 per value, besides some 400 per item and warp
 // for addresses and slots. By the chain of loads (length, rows and slots, scale) for single tokens.
-template <bool BF16, int WPI>
+template <bool BF16, int WPI, int NP>
 __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int b, int pg, int h, uint32_t (*warp_max)[WPI]) {
   constexpr int NT = 32 * WPI;  // threads per item
-  constexpr int NP = PAGED_WRITE_PAIRS;
   const int lane_i = threadIdx.x % NT;  // thread within the item
   const int D = 1 << p.d_log2;
   const int past = p.past[b];
@@ -459,8 +457,8 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   put(y1, y2, p.vs, p.v8, had_v, warp_max[1]);
 }
 
-template <bool BF16, int WPI>
-__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, PAGED_WRITE_WARPS / (WPI == 1 ? 4 : WPI))
+template <bool BF16, int WPI, int NP>
+__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, paged_write_warps(NP) / (WPI == 1 ? 4 : WPI))
     paged_write_kernel(const PagedWriteParams p) {
   // Warps' maxima of keys and of values: each is written again only after the other one's barrier.
   __shared__ uint32_t warp_max[2][WPI];
@@ -475,7 +473,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, PAGED_WRITE_WARPS /
        item < p.items; item += stride) {
     const int b = small_div(item, per_request), in = item - b * per_request;
     const int pg = small_div(in, p.Hkv);
-    paged_write_item<BF16, WPI>(p, b, pg, in - pg * p.Hkv, warp_max);
+    paged_write_item<BF16, WPI, NP>(p, b, pg, in - pg * p.Hkv, warp_max);
   }
 }
 

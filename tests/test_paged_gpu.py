@@ -158,6 +158,13 @@ def _same(a, b):
     (3, 1, 32, 70, 64, [63, 1, 64], [70, 1, 64]),
     (2, 4, 64, 200, 32, [31, 17], [200, 0]),
     (1, 2, 16, 260, 128, [7], [259]),
+    # each number of warps and rows per thread that an item can take
+    (2, 2, 16, 70, 32, [3, 0], [70, 33]),
+    (3, 5, 64, 50, 16, [15, 0, 8], [50, 16, 49]),
+    (3, 3, 128, 90, 32, [31, 0, 40], [90, 31, 64]),
+    (2, 3, 128, 150, 64, [5, 64], [150, 64]),
+    (2, 1, 128, 300, 128, [127, 1], [300, 128]),
+    (2, 2, 256, 40, 16, [0, 9], [40, 23]),
 ])
 def test_write(B, Hkv, D, T, block, past, counts, dtype):
     c = _write_case(B, Hkv, D, T, block, past, counts, dtype, B + D + T)
@@ -313,7 +320,7 @@ def _check_attend(B, Hq, Hkv, D, block, lens, dtype, seed=0, spread=1.0):
     assert bool((off <= tol).all()), f"worst {(off / tol).max():.3f} of the tolerance"
 
 
-HEADS = [(1, 1, 16), (2, 2, 32), (8, 8, 64), (6, 2, 64), (4, 1, 128), (8, 2, 128), (16, 2, 128), (5, 1, 128), (24, 2, 64), (32, 1, 64), (4, 2, 256), (16, 1, 256), (12, 4, 32), (6, 3, 16)]
+HEADS = [(1, 1, 16), (2, 2, 32), (8, 8, 64), (6, 2, 64), (4, 1, 128), (8, 2, 128), (16, 2, 128), (5, 1, 128), (24, 2, 64), (32, 1, 64), (4, 2, 256), (16, 1, 256), (12, 4, 32), (6, 3, 16), (1, 1, 128), (2, 2, 256), (8, 1, 32), (8, 1, 16), (2, 1, 16), (7, 1, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
