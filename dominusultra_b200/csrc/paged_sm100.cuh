@@ -328,15 +328,23 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
   uint4 xa[NP], xb[NP], cv[NP], sv[NP], va[NP], vb[NP];
   int slots[NP];
   const int slot0 = slot_row[0];
+  int given = -1;  // a slot of this thread's rows
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int row = r + i * dr;
+    slots[i] = row < n ? slot_row[row] : -1;
+    given = max(given, slots[i]);
+  }
   if (reach == 0 || (p.T > p.block && slot0 < 0)) {
-    if (lane_i == 0 && slot0 >= 0)
-      record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : past + t0));
+    if (given >= 0) {  // beyond the tables, or behind a row without a token
+      if (reach == 0) record_error(6u, static_cast<unsigned>(b), static_cast<unsigned>(past < 0 ? past : past + t0));
+      else record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(given));
+    }
     return;
   }
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int row = r + i * dr, step = min(row, reach - 1) - r;
-    slots[i] = row < n ? slot_row[row] : -1;
+    const int step = min(r + i * dr, reach - 1) - r;
     xa[i] = ldg_stream_v4(kx + step * (2 * D));
     xb[i] = ldg_stream_v4(kx + step * (2 * D) + D);
     cv[i] = ldg_v4(cosp + step * D);
@@ -344,7 +352,10 @@ __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int 
     va[i] = ldg_stream_v4(vx + step * (2 * D));
     vb[i] = ldg_stream_v4(vx + step * (2 * D) + D);
   }
-  if (slot0 < 0) return;  // no token here
+  if (slot0 < 0) {  // no token here
+    if (given >= 0) record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(given));
+    return;
+  }
   const int blk = slot0 >> p.block_log2;
   if (blk >= p.N || (slot0 & (p.block - 1)) != r0) {
     if (lane_i == 0) record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(slot0));

@@ -286,7 +286,8 @@ int du_paged_tables(int* block_table, const int* cache_seqlens, const int* new_s
  * nearest to its quotient. Where the scale grows, the earlier rows are rescaled. A block that
  * gets a value that is not finite gets the scale NaN. Rows of other slots are left as they are.
  * Requests must not share a block that they write to. A token whose slot is not where its
- * position belongs, or whose position the tables do not reach, is not written (codes 7, 6).
+ * position belongs, or whose position the tables do not reach, is not written (codes 7, 6), nor is
+ * one whose block's first token in this call has no slot (code 7).
  */
 int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_cache,
                    float* k_scale, float* v_scale, const int* slots, const int* cache_seqlens,

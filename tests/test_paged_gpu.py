@@ -240,6 +240,22 @@ def test_write_damaged_slots_are_skipped():
         assert _same(a, w)
 
 
+@pytest.mark.parametrize("T,block,past", [(5, 16, 3), (40, 16, 3), (140, 128, 0), (6, 64, 0)])
+def test_write_slots_behind_a_row_without_one_are_reported(T, block, past):
+    """A block's new rows start with its first token; slots behind a hole there are not written."""
+    c = _write_case(2, 2, 64, T, block, [past, past], [T, T], torch.bfloat16, 12)
+    kn, vn, k8, v8, ks, vs, slots, cos, sin = c
+    t0 = 0 if T <= block else block - past  # the first token of the request's first or second block
+    n = min(T - t0, block)
+    slots[1, t0] = -1
+    got = _run_write(kn, vn, k8, v8, ks, vs, slots, [past, past], cos, sin)
+    assert _status()[:2] == [7, 1]
+    slots[1, t0 : t0 + n] = -1
+    plain.write(kn, vn, k8, v8, ks, vs, slots.tolist(), [past, past], cos, sin)
+    for a, w in zip(got, (k8, v8, ks, vs)):
+        assert _same(a, w)
+
+
 def test_write_positions_beyond_the_rope_tables():
     past = [14]
     c = _write_case(1, 1, 64, 4, 16, past, [4], torch.bfloat16, 6)
