@@ -116,7 +116,8 @@ __device__ __forceinline__ int paged_owner(const int* off, int n, int x) {
 // before every entry that is written, and a slot's new block is read from the ring, so no CTA
 // waits for another: every CTA repeats the scan of the lengths (two loads per request, L2) and
 // takes a share of the entries and slots. Bound by latency: the loads of the lengths, the scan,
-// the loads of ring or table.
+// the loads of ring or table. Measured (B200, calls in a CUDA graph): 64 requests of one new token
+// 3.6 us, 16 of 4096 each 6.1 us, 512 of up to 257 each 6.2 us.
 __global__ void __launch_bounds__(PAGED_TABLES_THREADS) paged_tables_kernel(const PagedTablesParams p) {
   extern __shared__ int sm_off[];  // take[B], give[B]: exclusive prefix sums
   __shared__ int warp_sum[2][PAGED_TABLES_THREADS / 32];
@@ -296,9 +297,12 @@ constexpr int paged_write_warps(int pairs) { return pairs == 4 ? 16 : (pairs == 
 // A block with a value that is not finite gets the scale NaN, which every attention over it then
 // returns.
 //
-// Bound by HBM for prompts (2 bytes read and 1 written per value), closely followed by the issue
-// slots: about 10 instructions per key value and 4 per value, besides some 400 per item and warp
+// Bound by the issue slots in prompts (57 % of them), then by HBM (2 bytes read and 1 written per
+// value): about 10 instructions per key value and 4 per value, besides some 400 per item and warp
 // for addresses and slots. By the chain of loads (length, rows and slots, scale) for single tokens.
+// Measured (B200, calls in a CUDA graph): 4 prompts of up to 8192 tokens, 8 KV heads of 128, blocks
+// of 16 33.8 us, 4.9 TB/s; 5 chunks of up to 777, 32 heads of 64 11.7 us, 3.3 TB/s; 64 single
+// tokens, 8 heads of 128 2.5 us. With four chunk pairs for every item the last one took 4.5 us.
 template <bool BF16, int WPI, int NP>
 __device__ __forceinline__ void paged_write_item(const PagedWriteParams& p, int b, int pg, int h, uint32_t (*warp_max)[WPI]) {
   constexpr int NT = 32 * WPI;  // threads per item
