@@ -932,10 +932,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         const int nd_log2 = p.D >= S::CB ? (S::CB == 64 ? 6 : 5) : 4;  // (4: head_dim 16)
         const int d = tid & ((1 << nd_log2) - 1), hg = tid >> nd_log2;
         const int hs = 128 >> nd_log2;
-        float A[HPU];
+        constexpr int NH = HPU * S::CB > 128 ? HPU * S::CB / 128 : 1;  // a thread's heads (less at head_dim 16)
+        float A[NH];
 #pragma unroll
-        for (int i = 0; i < HPU; ++i) {
-          const int h = (hg + i * hs) & (HPU - 1);  // (taken round where a thread has fewer heads)
+        for (int i = 0; i < NH; ++i) {
+          const int h = (hg + i * hs) & (HPU - 1);  // (taken round where there are fewer)
           A[i] = 0.f;
 #pragma unroll
           for (int w2 = 0; w2 < 4; ++w2) {
@@ -945,7 +946,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           }
         }
 #pragma unroll
-        for (int i = 0; i < HPU; ++i) {
+        for (int i = 0; i < NH; ++i) {
           const int h = hg + i * hs;
           if (h < f.nh) {
             if (f.nf == 1) store_out(row0 + h, cb + d, A[i]);
