@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     // ------------------------------------------------------------------ fragments and queries
     const int D = p.D, half = D >> 1;
     // A unit's query rows and its rows of the tables come to shared memory, a fragment ahead; then
-    // head by head (a loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of
+    // two heads at a time (a loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of
     // each half.
     constexpr int EPL = DP >= 128 ? DP / 128 : 1;
     auto widen = [&](uint32_t w) -> float2 { return p.bf16 ? unpack2<true>(w) : unpack2<false>(w); };
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           cc[e] = widen(d < half ? raw32[(HPU * D + d) >> 1] : 0u);
           ss[e] = widen(d < half ? raw32[(HPU * D + half + d) >> 1] : 0u);
         }
-#pragma unroll 1
+#pragma unroll 2
         for (int h = 0; h < HPU; ++h) {
           float2 y1[EPL], y2[EPL];
           float top = 0.f;
