@@ -744,8 +744,9 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       if (mq > 0 && !(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_FREE, (mq - 1) & 1, failed, 838)))) break;
 #pragma unroll
       for (int i = 0; i < NPB * S::PM / 16; ++i)
-        st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + tid * S::PM + 16 * (i % (S::PM / 16)),
+        st_shared_v4(sbase + S::OFF_P + (i / (S::PM / 16)) * S::P_BYTES + warp * 32 * S::PM + 512 * (i % (S::PM / 16)) + 16 * lane,
                      make_uint4(0, 0, 0, 0));
+      __syncwarp();  // (a warp's rows lie together, and only its own threads write them)
       float m[HPU], l[HPU];
 #pragma unroll
       for (int h = 0; h < HPU; ++h) {
@@ -851,9 +852,12 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           st_shared_v4(pbuf + swz_chunk_offset<S::PM>(CK, tid, 2 * warp + 1), make_uint4(w[4], w[5], w[6], w[7]));
         if (!valid) {
           // Rows behind the last key may hold anything, a NaN among it, and 0 x NaN is a NaN.
+          // (the lanes begin at different 16 bytes of their rows: no two in the same banks)
+          constexpr int PER = SPAN / 16;
+          const int turn = tid / (8 / PER) % PER;
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c)
-            st_shared_v4(sbase + S::OFF_V + (gj % NV) * S::TILE + ((c * 16) / SPAN) * CK * SPAN + tid * SPAN + (c * 16) % SPAN,
+            st_shared_v4(sbase + S::OFF_V + (gj % NV) * S::TILE + (c / PER) * CK * SPAN + tid * SPAN + 16 * (c % PER ^ turn),
                          make_uint4(0, 0, 0, 0));
         }
         fence_proxy_async_smem();
