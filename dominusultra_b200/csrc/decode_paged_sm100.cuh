@@ -595,10 +595,15 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   } else if (warp == 6) {
     // ------------------------------------------------------------------ fragments and queries
     const int D = p.D, half = D >> 1;
-    // A unit's query rows and its rows of the tables come to shared memory, a fragment ahead; then
-    // two heads at a time (a loop whose code is fetched once) a lane takes element pairs 2 lane + 64 e of
-    // each half.
+    // A unit's query rows and its rows of the tables come to shared memory, a fragment ahead; then a
+    // lane takes element pairs 2 l + 64 e of each half of a head, SETS heads (by lanes, and the
+    // same work of several side by side, its loads before all stores: a head's chain alone is some
+    // 600 clocks) in each turn of a loop whose code is fetched once.
     constexpr int EPL = DP >= 128 ? DP / 128 : 1;
+    constexpr int LPH = DP >= 128 ? 32 : DP / 4;  // lanes per head
+    constexpr int HPL = 32 / LPH;                 // heads by lanes
+    constexpr int SETS = HPU <= HPL ? 1 : (HPU / HPL < 4 / EPL ? HPU / HPL : 4 / EPL);
+    const int ql = lane % LPH, qh = lane / LPH;
     auto widen = [&](uint32_t w) -> float2 { return p.bf16 ? unpack2<true>(w) : unpack2<false>(w); };
     // Rows of the query tiles beyond the parts stay zero.
     for (int i = lane; i < 2 * S::Q_BYTES / 16; i += 32)
@@ -653,52 +658,82 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         float2 cc[EPL], ss[EPL];
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
-          const int d = 2 * lane + 64 * e;
+          const int d = 2 * ql + 64 * e;
           cc[e] = widen(d < half ? raw32[(HPU * D + d) >> 1] : 0u);
           ss[e] = widen(d < half ? raw32[(HPU * D + half + d) >> 1] : 0u);
         }
-#pragma unroll 2
-        for (int h = 0; h < HPU; ++h) {
-          float2 y1[EPL], y2[EPL];
-          float top = 0.f;
-          bool fine = true;
+#pragma unroll 1
+        for (int h0 = 0; h0 < HPU; h0 += SETS * HPL) {
+          float2 y1[SETS][EPL], y2[SETS][EPL];
+          uint32_t bits[SETS];
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            const int d = 2 * lane + 64 * e;
-            const bool on = d < half && h < f.nh;
-            const float2 a = widen(on ? raw32[(h * D + d) >> 1] : 0u), b = widen(on ? raw32[(h * D + half + d) >> 1] : 0u);
-            y1[e] = make_float2(a.x * cc[e].x - b.x * ss[e].x, a.y * cc[e].y - b.y * ss[e].y);
-            y2[e] = make_float2(b.x * cc[e].x + a.x * ss[e].x, b.y * cc[e].y + a.y * ss[e].y);
-            top = max3(top, fabsf(y1[e].x), fabsf(y1[e].y));
-            top = max3(top, fabsf(y2[e].x), fabsf(y2[e].y));
-            fine = fine && y1[e].x - y1[e].x == 0.f && y1[e].y - y1[e].y == 0.f && y2[e].x - y2[e].x == 0.f &&
-                   y2[e].y - y2[e].y == 0.f;
+          for (int i = 0; i < SETS; ++i) {
+            const int h = h0 + i * HPL + qh;
+            float top = 0.f;
+            bool fine = true;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+              const int d = 2 * ql + 64 * e;
+              const bool on = d < half && h < f.nh;
+              const float2 a = widen(on ? raw32[(h * D + d) >> 1] : 0u), b = widen(on ? raw32[(h * D + half + d) >> 1] : 0u);
+              y1[i][e] = make_float2(a.x * cc[e].x - b.x * ss[e].x, a.y * cc[e].y - b.y * ss[e].y);
+              y2[i][e] = make_float2(b.x * cc[e].x + a.x * ss[e].x, b.y * cc[e].y + a.y * ss[e].y);
+              top = max3(top, fabsf(y1[i][e].x), fabsf(y1[i][e].y));
+              top = max3(top, fabsf(y2[i][e].x), fabsf(y2[i][e].y));
+              fine = fine && y1[i][e].x - y1[i][e].x == 0.f && y1[i][e].y - y1[i][e].y == 0.f &&
+                     y2[i][e].x - y2[i][e].x == 0.f && y2[i][e].y - y2[i][e].y == 0.f;
+            }
+            bits[i] = fine ? __float_as_uint(top) : 0x7fc00000u;
           }
-          // a power of two: the row divided by it fits e4m3 (NaN for a row that is not finite)
-          const uint32_t bits = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(top) : 0x7fc00000u);
-          const float u = paged_unit(bits);
-          const float inv = 1.0f / u;
+          if constexpr (LPH == 32) {
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            const int d = 2 * lane + 64 * e;
-            float2 v1 = make_float2(y1[e].x * inv, y1[e].y * inv), v2 = make_float2(y2[e].x * inv, y2[e].y * inv);
+            for (int i = 0; i < SETS; ++i) bits[i] = __reduce_max_sync(0xffffffffu, bits[i]);
+          } else {
 #pragma unroll
-            for (int t = 0; t < 3; ++t) {
-              const uint32_t p1 = e4m3x2(v1.x, v1.y), p2 = e4m3x2(v2.x, v2.y);
-              const float2 w1 = e4m3x2_widen(p1), w2 = e4m3x2_widen(p2);
-              v1 = make_float2((v1.x - w1.x) * 16.0f, (v1.y - w1.y) * 16.0f);
-              v2 = make_float2((v2.x - w2.x) * 16.0f, (v2.y - w2.y) * 16.0f);
-              if (d < half) {
-                // row t HPU + h of the tile: swizzled, K-major
-                const int n = t * HPU + h, d2 = d + half;
-                *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d >> 4) + (d & 15)) =
-                    static_cast<uint16_t>(p1);
-                *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d2 >> 4) + (d2 & 15)) =
-                    static_cast<uint16_t>(p2);
+            for (int o = LPH / 2; o >= 1; o >>= 1)
+#pragma unroll
+              for (int i = 0; i < SETS; ++i) bits[i] = max(bits[i], __shfl_xor_sync(0xffffffffu, bits[i], o));
+          }
+#pragma unroll
+          for (int i = 0; i < SETS; ++i) {
+            // a power of two: the row divided by it fits e4m3 (NaN for a row that is not finite, whose
+            // scores the factor makes NaN)
+            const float u = paged_unit(bits[i]);
+            const float inv = __uint_as_float(0x7f000000u - __float_as_uint(u));  // 1 / u
+            const int h = h0 + i * HPL + qh;
+            if (ql == 0 && h < HPU) reinterpret_cast<float*>(sgen + S::OFF_QS)[qb * HPU + h] = u * p.scale_log2;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+              y1[i][e] = make_float2(y1[i][e].x * inv, y1[i][e].y * inv);
+              y2[i][e] = make_float2(y2[i][e].x * inv, y2[i][e].y * inv);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 3; ++t) {
+#pragma unroll
+            for (int i = 0; i < SETS; ++i) {
+              const int h = h0 + i * HPL + qh;
+#pragma unroll
+              for (int e = 0; e < EPL; ++e) {
+                const int d = 2 * ql + 64 * e;
+                float2 &v1 = y1[i][e], &v2 = y2[i][e];
+                const uint32_t p1 = e4m3x2(v1.x, v1.y), p2 = e4m3x2(v2.x, v2.y);
+                if (t < 2) {
+                  const float2 w1 = e4m3x2_widen(p1), w2 = e4m3x2_widen(p2);
+                  v1 = make_float2((v1.x - w1.x) * 16.0f, (v1.y - w1.y) * 16.0f);
+                  v2 = make_float2((v2.x - w2.x) * 16.0f, (v2.y - w2.y) * 16.0f);
+                }
+                if (d < half && h < HPU) {
+                  // row t HPU + h of the tile: swizzled, K-major
+                  const int n = t * HPU + h, d2 = d + half;
+                  *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d >> 4) + (d & 15)) =
+                      static_cast<uint16_t>(p1);
+                  *reinterpret_cast<uint16_t*>(qt + swz_chunk_offset<SPAN>(NQ, n, d2 >> 4) + (d2 & 15)) =
+                      static_cast<uint16_t>(p2);
+                }
               }
             }
           }
-          if (lane == 0) reinterpret_cast<float*>(sgen + S::OFF_QS)[qb * HPU + h] = u * p.scale_log2;
         }
       }
       fence_proxy_async_smem();
