@@ -424,13 +424,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
 
   if (warp == 4) {
     for (int i = lane; i < S::N_BAR; i += 32) {
-      int n = 1;  // VFULL, VEMPTY, SFULL, PDONE, DRAIN, FFULL
+      int n = 1;  // VFULL, VEMPTY, QFULL, SFULL, PDONE, DRAIN, FFULL
       if (i < S::B_KEMPTY) n = 1 + 32;                                              // KFULL
       else if (i < S::B_VFULL) n = 1 + 4;                                           // KEMPTY
-      else if (i >= S::B_QFULL && i < S::B_QEMPTY) n = 32;                          // QFULL
       else if (i >= S::B_QEMPTY && i < S::B_SFULL) n = 1 + 4;                       // QEMPTY
-      else if (i >= S::B_SEMPTY && i < S::B_PFULL) n = 4;                           // SEMPTY
-      else if ((i >= S::B_PFULL && i < S::B_PDONE) || i == S::B_MRG || i == S::B_FREE) n = 128;
+      else if ((i >= S::B_SEMPTY && i < S::B_PDONE) || i == S::B_MRG || i == S::B_FREE) n = 4;  // a warp each
       else if (i >= S::B_FEMPTY) n = 7;                                             // FEMPTY
       mbar_init(bar(i), n);
     }
@@ -738,7 +736,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       fence_proxy_async_smem();
       __syncwarp();  // (and the raw rows have been read)
-      mbar_arrive(QFULL(qb));
+      if (lane == 0) mbar_arrive(QFULL(qb));
     }
     // Lengths out of range are reported by the first CTA, once its work is under way.
     if (blockIdx.x == 0)
@@ -897,7 +895,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(PFULL(gj % NPB));
+        __syncwarp();  // (one arrival per warp: 32 on one barrier take their turns)
+        if (lane == 0) mbar_arrive(PFULL(gj % NPB));
       }
       if (!ok) break;
       g += f.chunks;
@@ -952,7 +951,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         }
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_before();
-        mbar_arrive(BAR_MRG);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR_MRG);
         if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_MRG, mq & 1, failed, 837)))) break;
         // Lane w HPU + h: the factor of warp w's rows of head h, 2^(m_w - M) / L.
         if (cb == 0) {
@@ -992,7 +992,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
             else part_o[h * p.D + cb + d] = A[i];
           }
         }
-        mbar_arrive(BAR_FREE);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR_FREE);
         ++mq;
       }
       if (!ok) break;
