@@ -169,7 +169,7 @@ struct DecodePagedShape {
                        B_QFULL = 2 * NK + 2 * NV, B_QEMPTY = B_QFULL + 2, B_SFULL = B_QFULL + 4,
                        B_SEMPTY = B_QFULL + 6, B_PFULL = B_QFULL + 8, B_PDONE = B_QFULL + 10,
                        B_MRG = B_QFULL + 12, B_DRAIN = B_QFULL + 13, B_FREE = B_QFULL + 14,
-                       B_FFULL = B_QFULL + 15,
+                       B_ML = B_QFULL + 15, B_FFULL = B_QFULL + 16,
                        B_FEMPTY = B_FFULL + NF;
   static constexpr int N_BAR = B_FEMPTY + NF;
   static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;  // 16 words
@@ -406,8 +406,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   auto SEMPTY = [&](int i) { return bar(S::B_SEMPTY + i); };
   auto PFULL = [&](int i) { return bar(S::B_PFULL + i); };
   auto PDONE = [&](int i) { return bar(S::B_PDONE + i); };    // PV of even / odd chunks complete
-  // rows of O in the combine area; rows read (and partials stored)
-  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_FREE = bar(S::B_FREE), BAR_DRAIN = bar(S::B_DRAIN);
+  // rows of O in the combine area; rows read (and partials stored); a fragment's maxima and sums
+  const uint32_t BAR_MRG = bar(S::B_MRG), BAR_FREE = bar(S::B_FREE), BAR_DRAIN = bar(S::B_DRAIN), BAR_ML = bar(S::B_ML);
   uint32_t* misc = reinterpret_cast<uint32_t*>(sgen + S::OFF_MISC);
   volatile int* failed = reinterpret_cast<volatile int*>(misc + 1);
   volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       if (i < S::B_KEMPTY) n = 1 + 32;                                              // KFULL
       else if (i < S::B_VFULL) n = 1 + 4;                                           // KEMPTY
       else if (i >= S::B_QEMPTY && i < S::B_SFULL) n = 1 + 4;                       // QEMPTY
-      else if ((i >= S::B_SEMPTY && i < S::B_PDONE) || i == S::B_MRG || i == S::B_FREE) n = 4;  // a warp each
+      else if ((i >= S::B_SEMPTY && i < S::B_PDONE) || i == S::B_MRG || i == S::B_FREE || i == S::B_ML) n = 4;  // a warp each
       else if (i >= S::B_FEMPTY) n = 7;                                             // FEMPTY
       mbar_init(bar(i), n);
     }
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
     // ------------------------------------------------------------------ warps 0-3: softmax
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     bool ok = true;
-    int g = 0, mq = 0;  // chunks, combined column blocks
+    int g = 0, mq = 0, nf = 0;  // chunks, combined column blocks, fragments with keys
     for (int it = 0; ok; ++it) {
       const int qb = it & 1;
       if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(FFULL(it % S::NF), (it / S::NF) & 1, failed, 829)))) break;
@@ -918,13 +918,40 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           }
         }
       }
-      // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h through shared
-      // memory, then a thread sums the 12 of an output.
+      // Maxima and sums of the warps, exchanged while the last PV runs.
+      {
+        // The head of a lane's sum: its top log2(HPU) lane bits.
+        constexpr int LANES = 32 / HPU;
+        if (lane % LANES == 0) mrg_l[warp * HPU + lane / LANES] = l[0];
+        float mm = m[0];
+#pragma unroll
+        for (int h = 1; h < HPU; ++h) mm = lane == h ? m[h] : mm;
+        if (lane < HPU) mrg_m[warp * HPU + lane] = mm;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(BAR_ML);
+      }
+      float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
+      if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_ML, nf++ & 1, failed, 837)))) break;
+      // Lane t HPU + h: the factor of this warp's row of it, 2^(m_w - M) / L 2^(-4 t).
+      float wt;
+      {
+        const int i = lane % (4 * HPU);  // warp w HPU + head
+        const float mi = mrg_m[i];
+        float top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2 * HPU));
+        float fac = ex2(mi - top);
+        float L = mrg_l[i] * fac;
+        L += __shfl_xor_sync(0xffffffffu, L, HPU);
+        L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
+        fac = fac / L;
+        if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + lg2(L);  // log2 of the sum
+        const int t = lane / HPU;
+        wt = __shfl_sync(0xffffffffu, fac, warp * HPU + lane % HPU) * (t == 0 ? 1.0f : (t == 1 ? 0x1p-4f : 0x1p-8f));
+      }
+      // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h under their factors
+      // through shared memory, then a thread sums the 12 of an output.
       if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(PDONE((g - 1) % NPB), ((g - 1) / NPB) & 1, failed, 836)))) break;
       tc_fence_after();
-      float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
-      float* part_l = p.part + 2LL * gridDim.x * HPU * p.D;
-      float fac = 0.f;
 #pragma unroll 1
       for (int cb = 0; cb < DP && ok; cb += S::CB) {
         {
@@ -937,16 +964,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           if (lane < 3 * HPU) {
             float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW);
 #pragma unroll
-            for (int i = 0; i < S::CB / 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-          if (cb == 0) {
-            // The head of a lane's sum: its top log2(HPU) lane bits.
-            constexpr int LANES = 32 / HPU;
-            if (lane % LANES == 0) mrg_l[warp * HPU + lane / LANES] = l[0];
-            float mm = m[0];
-#pragma unroll
-            for (int h = 1; h < HPU; ++h) mm = lane == h ? m[h] : mm;
-            if (lane < HPU) mrg_m[warp * HPU + lane] = mm;
+            for (int i = 0; i < S::CB / 4; ++i)
+              dst[i] = make_float4(o[4 * i] * wt, o[4 * i + 1] * wt, o[4 * i + 2] * wt, o[4 * i + 3] * wt);
           }
         }
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -954,19 +973,6 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         __syncwarp();
         if (lane == 0) mbar_arrive(BAR_MRG);
         if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_MRG, mq & 1, failed, 837)))) break;
-        // Lane w HPU + h: the factor of warp w's rows of head h, 2^(m_w - M) / L.
-        if (cb == 0) {
-          const int i = lane % (4 * HPU);
-          const float mi = mrg_m[i];
-          float top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2 * HPU));
-          fac = ex2(mi - top);
-          float L = mrg_l[i] * fac;
-          L += __shfl_xor_sync(0xffffffffu, L, HPU);
-          L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
-          fac = fac / L;
-          if (f.nf > 1 && tid < HPU) part_l[f.slot * HPU + tid] = top + lg2(L);  // log2 of the sum
-        }
         // A thread takes a column and every (128 / columns)-th head.
         const int nd_log2 = p.D >= S::CB ? (S::CB == 64 ? 6 : 5) : 4;  // (4: head_dim 16)
         const int d = tid & ((1 << nd_log2) - 1), hg = tid >> nd_log2;
@@ -979,9 +985,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           A[i] = 0.f;
 #pragma unroll
           for (int w2 = 0; w2 < 4; ++w2) {
-            const float wt = __shfl_sync(0xffffffffu, fac, w2 * HPU + h);
             const float* r = mrg + (w2 * 3 * HPU + h) * ROW + d;
-            A[i] = fmaf(fmaf(r[2 * HPU * ROW], 0x1p-8f, fmaf(r[HPU * ROW], 0x1p-4f, r[0])), wt, A[i]);
+            A[i] += (r[2 * HPU * ROW] + r[HPU * ROW]) + r[0];
           }
         }
 #pragma unroll
