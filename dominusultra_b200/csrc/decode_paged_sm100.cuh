@@ -178,9 +178,11 @@ struct DecodePagedShape {
   static constexpr int TM_O = 64;          // O: DP columns
   static constexpr int TMEM_COLS = TM_O + DP <= 128 ? 128 : (TM_O + DP <= 256 ? 256 : 512);
   static constexpr int NTHREADS = 256;
-  // Chunks that a unit's beginning is charged with (measured with 1, 2, 3, 4, 6: 64 requests of up
-  // to 4096, four heads 82, 75, 69, 68, 70 us; 16 of up to 20001, eight heads 86, 80, 77, 75, 73 us).
-  static constexpr int PEN = HPU == 8 ? 6 : 4;
+  // Chunks that a unit's beginning is charged with (measured with 2, 3, 4 and four heads or fewer: 64
+  // requests of up to 4096, 32 on 8 heads of 128 51.5, 51.9, 52.4 us; 48 of up to 3000, 16 heads of 64
+  // 35.7, 35.1, 36.2 us. With 3, 4, 5, 6 and eight heads: 16 of up to 20001, 64 on 8 heads of 128 66.9,
+  // 66.3, 66.9, 67.3 us; 100 of up to 2500, 32 on one of 64 27.1, 27.3, 27.9, 28.2 us).
+  static constexpr int PEN = HPU == 8 ? 4 : 3;
   static_assert(3 * HPU <= PM / 4, "a warp's rows of P");
   static_assert(12 * HPU * ROW * 4 <= NPB * P_BYTES, "rows of O where P is");
   static_assert(HPU * DECODE_PAGED_MAX_CTAS * 4 <= NPB * P_BYTES, "weights of a unit's fragments where P is");
