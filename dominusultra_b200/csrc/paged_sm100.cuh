@@ -297,7 +297,7 @@ constexpr int paged_write_warps(int pairs) { return pairs == 4 ? 16 : (pairs == 
 // A block with a value that is not finite gets the scale NaN, which every attention over it then
 // returns.
 //
-// Bound by the issue slots in prompts (57 % of them), then by HBM (2 bytes read and 1 written per
+// Bound by the issue slots in prompts (56 % of them), then by HBM (2 bytes read and 1 written per
 // value): about 10 instructions per key value and 4 per value, besides some 400 per item and warp
 // for addresses and slots. By the chain of loads (length, rows and slots, scale) for single tokens.
 // Measured (B200, calls in a CUDA graph): 4 prompts of up to 8192 tokens, 8 KV heads of 128, blocks
