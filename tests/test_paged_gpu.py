@@ -439,6 +439,20 @@ def test_attend_nan_scale_reaches_its_heads_only():
         assert bool(out[0, 2:].isnan().all()) and torch.equal(out[0, :2], good[0, :2]) and torch.equal(out[1], good[1])
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 1, 64), (16, 2, 128), (6, 2, 32), (4, 4, 256), (4, 1, 16)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attend_query_not_finite_reaches_its_head_only(Hq, Hkv, D, bad):
+    a = _simple_call(B=2, Hq=Hq, Hkv=Hkv, D=D, lens=(40, 300))
+    good = dominus_ultra_decode_paged(*a)
+    b = list(a)
+    b[0] = a[0].clone()
+    b[0][1, Hq - 2, 0, D - 3] = bad
+    out = dominus_ultra_decode_paged(*b)
+    assert bool(out[1, Hq - 2].isnan().all()) and torch.equal(out[0], good[0])
+    others = [h for h in range(Hq) if h != Hq - 2]
+    assert torch.equal(out[1, others], good[1, others])
+
+
 def test_attend_on_the_host_checked():
     a = _simple_call()
     good = dominus_ultra_decode_paged(*a)
