@@ -8,11 +8,15 @@
 // The call streams the cache once (1 byte per value) and should run at HBM speed: about 23 bytes
 // per clock and SM. Widening each byte on the CUDA cores would take most of their issue slots, so
 // the cached bytes go to the tensor cores as they are (kind::f8f6f4, e4m3 x e4m3 -> fp32) and the
-// few operands on the other side are carried as sums of e4m3 parts instead:
-//   x = x1 + x2 / 16 + x3 / 256,  x1 = e4m3(x), x2 = e4m3(16 (x - x1)), x3 = e4m3(16 (16 (x - x1) - x2))
-// Each part holds 4 significant bits of what the parts before it left, so three carry 12 bits: half
-// a step of 2^-12, as fp16 operands would. The parts are rows of their own in tiles that are
-// mostly empty otherwise, so they cost no tensor time:
+// few operands on the other side are carried as sums of e4m3 parts instead, each part what the parts
+// before it left, scaled up:
+//   query    x = x1 + x2 2^-4 + x3 2^-8,               x1 = e4m3(x), x2 = e4m3(2^4 (x - x1)), ...
+//   weight   w = w1 + w2 2^-5 + w3 2^-10 + w4 2^-15    (w rounded to fp16 first)
+// A query's part holds 4 significant bits, so three carry 12: half a step of 2^-12, as fp16 operands
+// would. A weight is at most 2^8, where a part leaves at most 2^3: the next one can be scaled by 2^5.
+// Three parts then hold any fp16 weight of normal size and the fourth those down to fp16's last
+// step, 2^-24 (e4m3's last step is 2^-9), so the four are the fp16 weight exactly. The parts are rows
+// of their own in tiles that are mostly empty otherwise, so they cost no tensor time:
 //   S^T = K8 Q^T     M = 128 keys of a chunk, N = 16 or 32 (three parts of the unit's heads),
 //                    K = head_dim. A = the K tile as TMA left it, B = the query parts.
 //   O  += P V8       M = 64 or 128, N = head_dim, K = 128 keys. A = P, B = the V tile as TMA left
@@ -22,9 +26,11 @@
 // reference maximum, a sum and rows of O of its own over its 32 keys of every chunk: no
 // reduction across warps per chunk. The value scale joins the weight before it is split: with
 // u_j = s_j + log2 vs_j (log2 domain) the carried weight is 2^(u_j - m) = w_j vs_j and the sum
-// takes it divided by vs_j. m moves only when some u exceeds it by 8 (then to 4 below that
-// maximum), so the weights stay within 2^8 < 448 and the largest one of a warp is at least 1;
-// a weight's last part ends at an absolute 2^-18.
+// takes it divided by vs_j. m moves only when some u exceeds it by 8 (then to 7 below that
+// maximum), so the weights stay within 2^8 and the largest one of a warp is at least 2^7. Half a step of
+// the smallest weights is 2^-25 then, 2^-32 of the largest: behind a key that takes nearly all of the
+// weight and has values of zero, a long tail keeps its part. (With three parts, a factor of 2^4
+// between them and the largest weight at 2^4 the floor was 2^-22, and a tail of that size 26 % off.)
 //
 // Work: the requests' chunks of 128 keys, unit by unit (unit: request, KV head, group of up to
 // HPU query heads), cut into equal ranges, one per CTA of a persistent grid. Lengths are read on
@@ -71,6 +77,8 @@ struct DecodePagedParams {
 // Chunks per CTA that whole pieces of units may cost over equal ranges of chunks: a CTA whose range
 // straddles two units combines twice, about three chunks' time.
 constexpr int DECODE_PAGED_PIECE_SLACK = 3;
+// What a warp's reference lies below its maximum when it moves, in octaves (see above).
+constexpr float DECODE_PAGED_BELOW = 7.0f;
 // The CTA that joins a unit holds a weight per fragment and head where P is otherwise.
 constexpr int DECODE_PAGED_MAX_CTAS = 12 * 36;
 __device__ float g_du_paged_nan = __builtin_nanf("");  // the scale of a block that does not exist
@@ -109,19 +117,19 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-// The three e4m3 parts of two values (packed fp16, |value| <= 256), each part packed as a pair.
-__device__ __forceinline__ void e4m3_parts2(uint32_t x, uint32_t (&t)[3]) {
+// The four e4m3 parts of two weights (packed fp16, 0 <= value <= 256), each part packed as a pair.
+__device__ __forceinline__ void e4m3_parts2(uint32_t x, uint32_t (&t)[4]) {
   uint32_t r = x;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 4; ++i) {
     uint16_t e;
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(e) : "r"(r));
     t[i] = e;
-    if (i < 2) {
+    if (i < 3) {
       uint32_t f;
       asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(e));
       const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&f));
-      const __half2 s = __hmul2(d, __float2half2_rn(16.0f));  // exact: d has at most 7 bits
+      const __half2 s = __hmul2(d, __float2half2_rn(32.0f));  // exact: d has at most 7 bits, and is at most 8
       r = *reinterpret_cast<const uint32_t*>(&s);
     }
   }
@@ -144,9 +152,8 @@ struct DecodePagedShape {
   static constexpr int P_BYTES = CK * PM;             // [key][PM rows] bytes, swizzled
   static constexpr int Q_BYTES = ((NQ * DP + 1023) / 1024) * 1024;
   // Rows of O are combined where P is, CB columns at a time (and P's zeros put back): 4 warps x
-  // 3 HPU rows of ROW floats.
+  // 4 HPU rows of CB floats, a row's 16-byte parts in an order that the row's number gives.
   static constexpr int CB = DP < 64 ? DP : (DP == 128 && HPU == 8 ? 32 : 64);
-  static constexpr int ROW = CB + 4;
   static constexpr int ML_BYTES = ((8 * HPU * 4) + 127) / 128 * 128;  // maxima and sums of the warps
   static constexpr int RAW_BYTES = (HPU + 1) * DP * 2;  // a unit's query rows and its cos and sin row
   static constexpr int FIXED = NPB * P_BYTES + 2 * Q_BYTES + ML_BYTES + 2 * RAW_BYTES + 2560;
@@ -183,8 +190,8 @@ struct DecodePagedShape {
   // 35.7, 35.1, 36.2 us. With 3, 4, 5, 6 and eight heads: 16 of up to 20001, 64 on 8 heads of 128 66.9,
   // 66.3, 66.9, 67.3 us; 100 of up to 2500, 32 on one of 64 27.1, 27.3, 27.9, 28.2 us).
   static constexpr int PEN = HPU == 8 ? 4 : 3;
-  static_assert(3 * HPU <= PM / 4, "a warp's rows of P");
-  static_assert(12 * HPU * ROW * 4 <= NPB * P_BYTES, "rows of O where P is");
+  static_assert(4 * HPU <= PM / 4, "a warp's rows of P");
+  static_assert(16 * HPU * CB * 4 <= NPB * P_BYTES, "rows of O where P is");
   static_assert(HPU * DECODE_PAGED_MAX_CTAS * 4 <= NPB * P_BYTES, "weights of a unit's fragments where P is");
   static_assert(NV >= 2 && NK >= 2, "at least two stages");
   static_assert(SMEM_BYTES <= (CTAS == 2 ? 115712 : 232448), "shared memory budget");
@@ -386,7 +393,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
                         const DecodePagedParams p) {
   using S = DecodePagedShape<DP, HPU>;
   using Walk = PagedWalk<S::PEN>;
-  constexpr int CK = S::CK, SPAN = S::SPAN, NK = S::NK, NV = S::NV, NPB = S::NPB, NQ = S::NQ, ROW = S::ROW;
+  constexpr int CK = S::CK, SPAN = S::SPAN, NK = S::NK, NV = S::NV, NPB = S::NPB, NQ = S::NQ, CB = S::CB;
   constexpr uint32_t SWZ = swizzle_code(SPAN);
   constexpr uint32_t IDESC_QK = idesc_f16(128, NQ, 0, 0, 0, 0);  // (format 0 of kind::f8f6f4: e4m3)
   constexpr uint32_t IDESC_PV = idesc_f16(S::PM, DP, 0, 0, 1, 1);
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   volatile int* emitted = reinterpret_cast<volatile int*>(misc + 2);  // fragments done with
   volatile int* n_owed = reinterpret_cast<volatile int*>(misc + 3);
   PagedStart* start = reinterpret_cast<PagedStart*>(misc + 4);
-  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_P);  // o [4][3 HPU][ROW]
+  float* mrg = reinterpret_cast<float*>(sgen + S::OFF_P);  // o [4][4 HPU][CB]
   float* mrg_m = reinterpret_cast<float*>(sgen + S::OFF_ML);  // m [4][HPU], l [4][HPU]
   float* mrg_l = mrg_m + 4 * HPU;
   PagedFrag* owed = reinterpret_cast<PagedFrag*>(sgen + S::OFF_OWED);  // units for this CTA to join
@@ -825,7 +832,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
 #pragma unroll
           for (int h = 0; h < HPU; ++h) {
             const float mx = warp_max(u[h]);
-            const float mn = mx > m[h] + 8.0f ? mx - 4.0f : m[h];
+            const float mn = mx > m[h] + 8.0f ? mx - DECODE_PAGED_BELOW : m[h];
             alpha[h] = ex2(m[h] - mn);
             l[h] *= alpha[h];
             m[h] = mn;
@@ -837,25 +844,25 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           pe[h] = ex2(u[h] - m[h]);
           l[h] = fmaf(pe[h], rv, l[h]);
         }
-        // Parts of the weights, rows t HPU + h of this warp: 3 HPU bytes of the key's row of P.
+        // Parts of the weights, rows t HPU + h of this warp: 4 HPU bytes of the key's row of P.
         uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if constexpr (HPU == 1) {
-          uint32_t t[3];
+          uint32_t t[4];
           e4m3_parts2(pack2<false>(pe[0], 0.f), t);
-          w[0] = (t[0] & 0xffu) | ((t[1] & 0xffu) << 8) | ((t[2] & 0xffu) << 16);
+          w[0] = (t[0] & 0xffu) | ((t[1] & 0xffu) << 8) | ((t[2] & 0xffu) << 16) | (t[3] << 24);
         } else if constexpr (HPU == 2) {
-          uint32_t t[3];
+          uint32_t t[4];
           e4m3_parts2(pack2<false>(pe[0], pe[1]), t);
           w[0] = t[0] | (t[1] << 16);
-          w[1] = t[2];
+          w[1] = t[2] | (t[3] << 16);
         } else {
 #pragma unroll
           for (int h = 0; h < HPU; h += 4) {
-            uint32_t a[3], b[3];
+            uint32_t a[4], b[4];
             e4m3_parts2(pack2<false>(pe[h], pe[h + 1]), a);
             e4m3_parts2(pack2<false>(pe[h + 2], pe[h + 3]), b);
 #pragma unroll
-            for (int t = 0; t < 3; ++t) w[t * (HPU / 4) + h / 4] = a[t] | (b[t] << 16);
+            for (int t = 0; t < 4; ++t) w[t * (HPU / 4) + h / 4] = a[t] | (b[t] << 16);
           }
         }
         // The P buffer was last read by PV(gj - NPB); a moved reference rescales O, which holds PV up
@@ -934,7 +941,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
       }
       float* part_o = p.part + static_cast<long long>(f.slot) * HPU * p.D;
       if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(BAR_ML, nf++ & 1, failed, 837)))) break;
-      // Lane t HPU + h: the factor of this warp's row of it, 2^(m_w - M) / L 2^(-4 t).
+      // Lane t HPU + h: the factor of this warp's row of it, 2^(m_w - M) / L 2^(-5 t).
       float wt;
       {
         const int i = lane % (4 * HPU);  // warp w HPU + head
@@ -947,11 +954,11 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
         fac = fac / L;
         if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + lg2(L);  // log2 of the sum
-        const int t = lane / HPU;
-        wt = __shfl_sync(0xffffffffu, fac, warp * HPU + lane % HPU) * (t == 0 ? 1.0f : (t == 1 ? 0x1p-4f : 0x1p-8f));
+        const int t = lane / HPU & 3;
+        wt = __shfl_sync(0xffffffffu, fac, warp * HPU + lane % HPU) * __int_as_float((127 - 5 * t) << 23);
       }
       // Combine the warps' rows of O, CB columns at a time: rows 32 w + t HPU + h under their factors
-      // through shared memory, then a thread sums the 12 of an output.
+      // through shared memory, then a thread sums the 16 of an output.
       if (!(ok = __all_sync(0xffffffffu, softmax_wait<DP>(PDONE((g - 1) % NPB), ((g - 1) / NPB) & 1, failed, 836)))) break;
       tc_fence_after();
 #pragma unroll 1
@@ -963,11 +970,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           // The columns combined before have been read.
           if (cb > 0) ok = softmax_wait<DP>(BAR_FREE, (mq - 1) & 1, failed, 837);
           tmem_wait_ld();
-          if (lane < 3 * HPU) {
-            float4* dst = reinterpret_cast<float4*>(mrg + (warp * 3 * HPU + lane) * ROW);
+          if (lane < 4 * HPU) {
+            // (part i of row r is at i ^ (r & 7): no two of eight rows in the same banks)
+            float4* dst = reinterpret_cast<float4*>(mrg + (warp * 4 * HPU + lane) * CB);
+            const int turn = (warp * 4 * HPU + lane) & 7;
 #pragma unroll
-            for (int i = 0; i < S::CB / 4; ++i)
-              dst[i] = make_float4(o[4 * i] * wt, o[4 * i + 1] * wt, o[4 * i + 2] * wt, o[4 * i + 3] * wt);
+            for (int i = 0; i < CB / 4; ++i)
+              dst[i ^ turn] = make_float4(o[4 * i] * wt, o[4 * i + 1] * wt, o[4 * i + 2] * wt, o[4 * i + 3] * wt);
           }
         }
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -987,8 +996,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           A[i] = 0.f;
 #pragma unroll
           for (int w2 = 0; w2 < 4; ++w2) {
-            const float* r = mrg + (w2 * 3 * HPU + h) * ROW + d;
-            A[i] += (r[2 * HPU * ROW] + r[HPU * ROW]) + r[0];
+            float part[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const int row = (w2 * 4 + t) * HPU + h;
+              part[t] = mrg[row * CB + 4 * ((d >> 2) ^ (row & 7)) + (d & 3)];
+            }
+            A[i] += ((part[3] + part[2]) + part[1]) + part[0];
           }
         }
 #pragma unroll
