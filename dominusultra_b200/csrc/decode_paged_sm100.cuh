@@ -25,8 +25,10 @@
 // One key per TMEM lane, so the softmax is one thread per key, and each of its four warps keeps a
 // reference maximum, a sum and rows of O of its own over its 32 keys of every chunk: no
 // reduction across warps per chunk. The value scale joins the weight before it is split: with
-// u_j = s_j + log2 vs_j (log2 domain) the carried weight is 2^(u_j - m) = w_j vs_j and the sum
-// takes it divided by vs_j. m moves only when some u exceeds it by 8 (then to 7 below that
+// u_j = s_j + log2 vs_j (log2 domain) the carried weight is 2^(u_j - m) = w_j vs_j. The sum takes
+// 2^(u_j - m - log2 vs_j), an exponential of its own: value scales may be 2^190 apart, and a key whose
+// carried weight is nothing beside another's can have all of the softmax's. (2^32 times that: its largest
+// term lies between 2^-121 and 2^72 without the factor, too near to the smallest float.) m moves only when some u exceeds it by 8 (then to 7 below that
 // maximum), so the weights stay within 2^8 and the largest one of a warp is at least 2^7. Half a step of
 // the smallest weights is 2^-25 then, 2^-32 of the largest: behind a key that takes nearly all of the
 // weight and has values of zero, a long tail keeps its part. (With three parts, a factor of 2^4
@@ -807,7 +809,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (vsc < 0x1p-64f) vsc = 0x1p-64f;  // (the writer's smallest; a NaN stays)
         __syncwarp();
         if (lane == 0) mbar_arrive(KEMPTY(s));
-        const float lv = lg2(vsc), rv = __fdividef(1.0f, vsc);
+        const float lv = lg2(vsc), lsum = lv - 32.0f;
         ok = softmax_wait<DP>(SFULL(gj & 1), (gj >> 1) & 1, failed, 832);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
@@ -833,16 +835,19 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
           for (int h = 0; h < HPU; ++h) {
             const float mx = warp_max(u[h]);
             const float mn = mx > m[h] + 8.0f ? mx - DECODE_PAGED_BELOW : m[h];
-            alpha[h] = ex2(m[h] - mn);
-            l[h] *= alpha[h];
+            // (in two halves: where the value scales jump the factor alone may be less than any float)
+            const float a = ex2(0.5f * (m[h] - mn));
+            alpha[h] = a * a;
+            l[h] = l[h] * a * a;
             m[h] = mn;
           }
         }
         float pe[HPU];
 #pragma unroll
         for (int h = 0; h < HPU; ++h) {
-          pe[h] = ex2(u[h] - m[h]);
-          l[h] = fmaf(pe[h], rv, l[h]);
+          const float x = u[h] - m[h];
+          pe[h] = ex2(x);
+          l[h] += ex2(x - lsum);
         }
         // Parts of the weights, rows t HPU + h of this warp: 4 HPU bytes of the key's row of P.
         uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -948,12 +953,13 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         const float mi = mrg_m[i];
         float top = fmaxf(mi, __shfl_xor_sync(0xffffffffu, mi, HPU));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2 * HPU));
-        float fac = ex2(mi - top);
-        float L = mrg_l[i] * fac;
+        const float half_fac = ex2(0.5f * (mi - top));  // (as above)
+        float fac = half_fac * half_fac;
+        float L = mrg_l[i] * half_fac * half_fac;
         L += __shfl_xor_sync(0xffffffffu, L, HPU);
         L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
-        fac = fac / L;
-        if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + lg2(L);  // log2 of the sum
+        fac = fac * 0x1p32f / L;
+        if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + (lg2(L) - 32.0f);  // log2 of the sum
         const int t = lane / HPU & 3;
         wt = __shfl_sync(0xffffffffu, fac, warp * HPU + lane % HPU) * __int_as_float((127 - 5 * t) << 23);
       }

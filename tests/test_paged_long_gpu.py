@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from dominusultra_b200 import _lib, dominus_ultra_decode_paged
+from dominusultra_b200 import _lib, dominus_ultra_decode_paged, dominus_ultra_paged_write
 from tests import _paged_exact as exact
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +51,59 @@ def test_long_tail_behind_a_sink(D, G, drop):
     want, bound = exact.attend(q[:1], k.to(exact.E4M3), v8, ks, vs, table[:1], [n], cos, sin)
     assert bool((bound <= 0.03 * want).all())
     assert bool(_within(got, want, bound).all()), f"off by {((got.double() - want).abs() / want).max():.4f}"
+
+
+def _scaled(Hq, Hkv, D, lens, dtype, seed, scales):
+    """Values whose blocks of 16 have the scales `scales(block of the request)`, magnitudes within the scale."""
+    block = 16
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    width = max(lens) // block + 1
+    N = len(lens) * width
+    table = torch.randperm(N, generator=g, device=DEV).int().reshape(len(lens), width)
+    k8, ks = exact.encode(torch.randn(N, Hkv, block, D, generator=g, device=DEV))
+    v8 = (torch.rand(N, Hkv, block, D, generator=g, device=DEV) + 0.5).to(exact.E4M3)
+    vs = torch.empty(N, Hkv, device=DEV)
+    for i in range(width):
+        vs[table[:, i].long()] = scales(i)
+    q = torch.randn(len(lens), Hq, 1, D, generator=g, device=DEV).to(dtype)
+    cos, sin = torch.ones(max(lens), D // 2, device=DEV).to(dtype), torch.zeros(max(lens), D // 2, device=DEV).to(dtype)
+    return q, k8, v8, ks, vs, table, lens, cos, sin
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,lens", [
+    (4, 1, 64, [32]), (8, 1, 128, [32, 300]), (2, 2, 256, [700]), (8, 2, 32, [3000]), (4, 1, 128, [2500] * 400), (1, 1, 16, [900] * 700),
+])
+@pytest.mark.parametrize("name,scales", [
+    ("zeros first", lambda i: 2.0**-64 if i == 0 else 2.0**67),
+    ("zeros last", lambda i: 2.0**119 if i == 0 else 2.0**-64),
+    ("alternating", lambda i: 2.0**-64 if i % 2 else 2.0**119),
+    ("largest", lambda i: 2.0**126 * 1.25),
+    ("largest among others", lambda i: (2.0**126, 2.0**-64, 2.0**-10, 2.0**40)[i % 4]),
+    ("rising by chunks", lambda i: 2.0 ** min(119, -64 + 10 * (i // 8))),
+])
+def test_value_scales_far_apart(Hq, Hkv, D, lens, name, scales):
+    """The softmax's sum has every key's weight, whatever the scales of the values."""
+    batch = _scaled(Hq, Hkv, D, lens, torch.bfloat16, D, scales)
+    q, k, v, ks, vs, table, _, cos, sin = batch
+    got = _call(*batch)
+    m = min(len(lens), 3)
+    want, bound = exact.attend(q[:m], k, v, ks, vs, table[:m], lens[:m], cos, sin)
+    assert bool((bound <= 0.02 * want).all())
+    assert bool(_within(got[:m], want, bound).all()), f"off by {((got[:m].double() - want).abs() / want).max():.4f}"
+
+
+def test_a_block_of_zeros_beside_huge_values_from_the_writer():
+    """A block whose values are all zero has the writer's smallest scale; its keys keep their weight."""
+    D, block = 64, 16
+    k = torch.zeros(1, 1, 32, D, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    v[:, :, 16:] = 2.0**80
+    k8, v8 = (torch.zeros(2, 1, block, D, device=DEV).to(exact.E4M3) for _ in range(2))
+    ks, vs = torch.zeros(2, 1, device=DEV), torch.zeros(2, 1, device=DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    cos, sin = torch.ones(32, D // 2, device=DEV).bfloat16(), torch.zeros(32, D // 2, device=DEV).bfloat16()
+    dominus_ultra_paged_write(k, v, k8, v8, ks, vs, torch.arange(32, **i32)[None], torch.zeros(1, **i32), cos, sin)
+    assert vs.flatten().tolist() == [2.0**-64, 2.0**72]
+    q = torch.randn(1, 2, 1, D, device=DEV).bfloat16()
+    got = _call(q, k8, v8, ks, vs, torch.arange(2, **i32)[None], [32], cos, sin)
+    assert bool((got == 2.0**79).all())
