@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
   }
   // Launched as a programmatic dependent: what is above runs beside the stream's previous kernel.
   griddep_wait();
+  if (warp == 4 || warp == 7) fence_proxy_async_global();  // the written blocks are read by TMA (async proxy)
   if (warp == 5) griddep_launch_dependents();  // (the columns are taken)
   Walk walk;  // warp 6's
   if (warp == 6) {

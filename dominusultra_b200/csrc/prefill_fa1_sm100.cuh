@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(256, 2)
       // it completes); nothing else this CTA reads is written by it. With krot there is no such
       // launch and the wait returns at once.
       griddep_wait();
+      fence_proxy_async_global();  // (written through the generic proxy, read by TMA)
       for (int j = 0; j < nk; ++j) {
         const int s = j % NSK;
         if (j >= NSK && !mbar_wait(BAR_KE(s), (j / NSK - 1) & 1, failed, 410)) break;

@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(384, 1)
       // The rotated keys come from the preceding rotary launch (this kernel may start before
       // it completes); nothing else this CTA reads is written by it.
       griddep_wait();
+      fence_proxy_async_global();  // (written through the generic proxy, read by TMA)
       for (int j = 0; j < nk_all; ++j) {
         const int s = j % NSK;
         if (j >= NSK && !mbar_wait(BAR_KE(s), (j / NSK - 1) & 1, failed, 310)) break;
