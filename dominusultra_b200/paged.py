@@ -170,17 +170,20 @@ _SCRATCH = {}
 
 
 def _decode_scratch(nbytes: int, index: int, stream: int):
-    """(tickets, workspace, keep-alive tensors) of a paged decode on torch's current stream.
+    """(tickets, workspace, what keeps them alive until the launch) of a paged decode on torch's
+    current stream.
 
-    Eager calls share a pair per (device, stream): calls on one stream run in order. A call that
-    is being captured gets a workspace from the graph's own memory and tickets of its own.
+    Eager calls share a pair per (device, stream): calls on one stream run in order. Another thread's
+    call on the stream may replace the pair before this one's launch, and a buffer that nothing
+    holds could then be another tensor's. A call that is being captured gets a workspace from the
+    graph's own memory and tickets of its own.
     """
     if not torch.cuda.is_current_stream_capturing():
         pair = _SCRATCH.get((index, stream))
         slab = _SLABS.get(index)
         if pair is None or pair[2] < nbytes or slab is None or slab[1] > _SLAB_WORDS // 2:
             pair = _grow_scratch(nbytes, index, stream)
-        return pair[0], pair[1], None
+        return pair[0], pair[1], pair
     device = torch.device("cuda", index)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     with _SLAB_LOCK:
