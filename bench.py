@@ -274,8 +274,8 @@ def rope_pass_ms(sets, cos, sin, cfg, steps, stream):
 
     lib = _lib.load()
     B, H, Hkv, S, D = cfg["B"], cfg["H"], cfg["Hkv"], cfg["S"], cfg["D"]
-    ws, _ = _cached_workspace("prefill", int(lib.du_prefill_workspace_size(B, H, Hkv, S, D)),
-                              cos.device, stream.cuda_stream)
+    ws, _, keep = _cached_workspace("prefill", int(lib.du_prefill_workspace_size(B, H, Hkv, S, D)),
+                                    cos.device, stream.cuda_stream)
 
     def one(i):
         k = sets[i % len(sets)][1]

@@ -10,6 +10,7 @@ There is no CPU path: CPU tensors are rejected exactly as the reference rejects 
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -168,6 +169,7 @@ class _OnDevice:
 # Workspace per (kind, device, stream): [buffer, used under a graph capture], reused across
 # calls, since kernels on one stream run in order; grown on demand.
 _WORKSPACES = {}
+_WORKSPACES_LOCK = threading.Lock()
 # Outgrown buffers that a captured CUDA graph may still reference: never freed.
 _RETIRED = []
 
@@ -226,7 +228,7 @@ def dominus_ultra_prefill(
     scale = 1.0 / (D**0.5)
     with _OnDevice(q.device):
         stream = _stream(q.device)
-        ws, ws_bytes = _cached_workspace(
+        ws, ws_bytes, keep = _cached_workspace(
             "prefill", _ws_size("du_prefill_workspace_size", B, Hq, KvH, T, D, q.device), q.device,
             stream,
         )
@@ -235,13 +237,15 @@ def dominus_ultra_prefill(
             B, Hq, KvH, T, D, _dtype_code(q.dtype), scale,
             min(cos.shape[0], sin.shape[0]), ws, ws_bytes, stream,
         )
+        del keep
     _lib.check(rc, "du_prefill")
     return out, lse
 
 
 def _cached_workspace(kind: str, nbytes: int, device, stream: int):
-    """(pointer, bytes) of a per-(kind, device, stream) scratch buffer of at least nbytes, grown on
-    demand. Calls on one stream are ordered, so reusing the buffer across them is safe.
+    """(pointer, bytes, buffer) of a per-(kind, device, stream) scratch buffer of at least nbytes, grown
+    on demand. Calls on one stream are ordered, so reusing the buffer across them is safe. The caller
+    holds the buffer until its launch: another thread's call on the stream may replace it before that.
 
     A buffer that a CUDA graph capture has used stays referenced by that graph's kernels, so
     when it is outgrown it is kept alive (``_RETIRED``) instead of being returned to the caching
@@ -250,21 +254,23 @@ def _cached_workspace(kind: str, nbytes: int, device, stream: int):
     safe). Growth is at least geometric, so few buffers are ever retired.
     """
     if nbytes == 0:
-        return 0, 0
+        return 0, 0, None
     key = (kind, device.index, stream)
-    entry = _WORKSPACES.get(key)
     capturing = torch.cuda.is_current_stream_capturing()
-    if entry is None or entry[0].numel() < nbytes:
-        if entry is not None and entry[1]:
-            _RETIRED.append(entry[0])
-        size = max(nbytes, 1 << 20, 2 * entry[0].numel() if entry is not None else 0)
-        # zero-filled: the decode split walk keeps its ticket counters at the front, and every
-        # call leaves them zero
-        entry = [torch.zeros(size, dtype=torch.uint8, device=device), capturing]
-        _WORKSPACES[key] = entry
-    elif capturing:
-        entry[1] = True
-    return entry[0].data_ptr(), entry[0].numel()
+    with _WORKSPACES_LOCK:
+        entry = _WORKSPACES.get(key)
+        if entry is None or entry[0].numel() < nbytes:
+            if entry is not None and entry[1]:
+                _RETIRED.append(entry[0])
+            size = max(nbytes, 1 << 20, 2 * entry[0].numel() if entry is not None else 0)
+            # zero-filled: the decode split walk keeps its ticket counters at the front, and every
+            # call leaves them zero
+            entry = [torch.zeros(size, dtype=torch.uint8, device=device), capturing]
+            _WORKSPACES[key] = entry
+        elif capturing:
+            entry[1] = True
+        buffer = entry[0]
+    return buffer.data_ptr(), buffer.numel(), buffer
 
 
 def _workspace(B: int, Hq: int, Hkv: int, L: int, D: int, device, stream: int):
@@ -325,12 +331,13 @@ def dominus_ultra_decode(
     scale = 1.0 / (D**0.5)
     with _OnDevice(q_new.device):
         stream = _stream(q_new.device)
-        ws, nbytes = _workspace(B, Hq, KvH, past_T, D, q_new.device, stream)
+        ws, nbytes, keep = _workspace(B, Hq, KvH, past_T, D, q_new.device, stream)
         rc = lib.du_decode(
             _ptr(q_new), _ptr(k_cache), _ptr(v_cache), _ptr(cos), _ptr(sin), _ptr(out),
             B, Hq, KvH, past_T, D, _dtype_code(q_new.dtype), scale,
             min(cos.shape[0], sin.shape[0]), ws, nbytes, stream,
         )
+        del keep
     _lib.check(rc, "du_decode")
     return out.unsqueeze(2)
 
@@ -434,7 +441,7 @@ def dominus_ultra_decode_kvcache(
     scale = 1.0 / (D**0.5)
     with _OnDevice(q_new.device):
         stream = _stream(q_new.device)
-        ws, nbytes = _cached_workspace(
+        ws, nbytes, keep = _cached_workspace(
             "decode_kvcache",
             _ws_size("du_decode_kvcache_workspace_size", B, Hq, KvH, max_len, D, q_new.device),
             q_new.device,
@@ -445,6 +452,7 @@ def dominus_ultra_decode_kvcache(
             _ptr(cos), _ptr(sin), _ptr(out), B, Hq, KvH, max_len, D, _dtype_code(q_new.dtype),
             scale, min(cos.shape[0], sin.shape[0]), ws, nbytes, stream,
         )
+        del keep
     _lib.check(rc, "du_decode_kvcache")
     return out.unsqueeze(2)
 
@@ -481,13 +489,14 @@ def decode_partial(
         lse = torch.empty((B, Hq), dtype=torch.float32, device=q_new.device)
     with _OnDevice(q_new.device):
         stream = _stream(q_new.device)
-        ws, nbytes = _workspace(B, Hq, KvH, L, D, q_new.device, stream)
+        ws, nbytes, keep = _workspace(B, Hq, KvH, L, D, q_new.device, stream)
         rc = lib.du_decode_partial(
             _ptr(q_new), _ptr(k_shard), _ptr(v_shard), _ptr(cos), _ptr(sin), _ptr(out), _ptr(lse),
             B, Hq, KvH, L, D, _dtype_code(q_new.dtype), 1.0 / (D**0.5),
             int(q_pos), int(kv_pos_offset), min(cos.shape[0], sin.shape[0]),
             ws, nbytes, stream,
         )
+        del keep
     _lib.check(rc, "du_decode_partial")
     return out, lse
 

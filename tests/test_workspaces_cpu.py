@@ -7,7 +7,7 @@ import weakref
 
 import torch
 
-from dominusultra_b200 import paged
+from dominusultra_b200 import attention, paged
 
 
 class _OnCpu:
@@ -43,3 +43,32 @@ def test_paged_scratch_outlives_its_replacement(monkeypatch):
     assert _alive(ws) and _alive(tickets)
     del first
     assert not _alive(ws) and _alive(tickets)
+
+
+def test_workspace_outlives_its_replacement(monkeypatch):
+    monkeypatch.setattr(attention, "torch", _OnCpu())
+    monkeypatch.setattr(attention, "_WORKSPACES", {})
+    cpu = torch.device("cpu")
+    first = attention._cached_workspace("prefill", 3 << 20, cpu, 7)
+    buf = weakref.ref(first[2])
+    assert first[:2] == (buf().data_ptr(), 3 << 20)
+    second = attention._cached_workspace("prefill", 4 << 20, cpu, 7)
+    assert second[1] == 6 << 20 and second[0] != first[0]
+    assert _alive(buf)
+    del first
+    assert not _alive(buf)
+    assert attention._cached_workspace("prefill", 0, cpu, 7) == (0, 0, None)
+
+
+def test_workspace_of_a_capture_is_never_dropped(monkeypatch):
+    fake = _OnCpu()
+    fake.cuda.is_current_stream_capturing = staticmethod(lambda: True)
+    monkeypatch.setattr(attention, "torch", fake)
+    monkeypatch.setattr(attention, "_WORKSPACES", {})
+    monkeypatch.setattr(attention, "_RETIRED", [])
+    cpu = torch.device("cpu")
+    first = attention._cached_workspace("decode", 3 << 20, cpu, 7)
+    buf = weakref.ref(first[2])
+    attention._cached_workspace("decode", 4 << 20, cpu, 7)
+    del first
+    assert _alive(buf)

@@ -9,7 +9,17 @@ import weakref
 import pytest
 import torch
 
-from dominusultra_b200 import _lib, dominus_ultra_decode_paged, paged, precompute_rope_cos_sin
+from dominusultra_b200 import (
+    _lib,
+    attention,
+    decode_partial,
+    dominus_ultra_decode,
+    dominus_ultra_decode_kvcache,
+    dominus_ultra_decode_paged,
+    dominus_ultra_prefill,
+    paged,
+    precompute_rope_cos_sin,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +97,40 @@ def test_paged_decode_from_threads(cuda_device):
         t.join()
     assert not bad
     assert _lib.read_status(reset=True)[0] == 0
+
+
+@pytest.mark.parametrize("name", ["prefill", "decode", "decode_partial", "decode_kvcache"])
+def test_calls_keep_their_workspace_until_the_launch(cuda_device, monkeypatch, name):
+    B, Hq, Hkv, L, D = 1, 8, 2, 20000, 64
+    T = 5000 if name == "prefill" else L
+    g = torch.Generator(device=DEV).manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    q, k, v = r(B, Hq, T if name == "prefill" else 1, D), r(B, Hkv, T, D), r(B, Hkv, T, D)
+    cos, sin = precompute_rope_cos_sin(T + 1, D, DEV, torch.bfloat16)
+    lens = torch.tensor([L], dtype=torch.int32, device=DEV)
+    call = {
+        "prefill": lambda: dominus_ultra_prefill(q, k, v, cos, sin, Hkv)[0],
+        "decode": lambda: dominus_ultra_decode(q, k, v, cos, sin, Hkv),
+        "decode_partial": lambda: decode_partial(q, k, v, cos, sin, Hkv, L, 0)[0],
+        "decode_kvcache": lambda: dominus_ultra_decode_kvcache(q, k, v, cos, sin, lens, num_kv_heads=Hkv),
+    }[name]
+    kind = "decode" if name == "decode_partial" else name
+    want = call()
+    key = (kind, torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
+    entry = attention._WORKSPACES[key]
+    entry[1] = False  # (a capture of an earlier test would keep the buffer)
+    held = weakref.ref(entry[0])
+    size = entry[0].numel()
+    del entry
+    seen = []
+
+    def replace():
+        attention._cached_workspace(kind, size + 1, q.device, key[2])
+        gc.collect()
+        seen.append(held() is not None)
+
+    monkeypatch.setattr(attention._lib, "load", lambda lib=_lib.load(): _Before(lib, "du_" + name, replace))
+    got = call()
+    gc.collect()
+    assert seen == [True] and held() is None
+    assert torch.equal(got, want)
