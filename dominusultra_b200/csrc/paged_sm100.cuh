@@ -208,7 +208,10 @@ __global__ void __launch_bounds__(PAGED_TABLES_THREADS) paged_tables_kernel(cons
   for (long long f = first; f < given; f += step) {
     const int b = paged_owner(give, p.B, static_cast<int>(f));
     const PagedAsk q = paged_ask(p, b, ring_ok);
-    p.ring[ring_at(count + f)] = p.table[static_cast<long long>(b) * p.width + q.new_pages + (f - give[b])];
+    const int id = p.table[static_cast<long long>(b) * p.width + q.new_pages + (f - give[b])];
+    // (it keeps its place in the ring: the ranks of the others are known before any entry is read)
+    if (id < 0 || id >= p.N) record_error(7u, static_cast<unsigned>(b), static_cast<unsigned>(id));
+    p.ring[ring_at(count + f)] = id;
   }
   const long long n_slots = static_cast<long long>(p.B) * p.T;
   for (long long i = first; i < n_slots; i += step) {

@@ -234,7 +234,8 @@ def dominus_ultra_paged_tables(
     ``max_new`` more), fewer (a rejected draft), or 0 (a request that ends). Requests that grow
     over a block's end take blocks from the ring of free ones, in order of ``b`` from its head, as
     long as the needs up to a request are covered; a request that is not served keeps its length.
-    Requests that shrink give blocks back behind the ring's tail, free from the next call on.
+    Requests that shrink give blocks back behind the ring's tail, free from the next call on; a block is
+    held by one request only (a block in two rows would be given back twice).
 
     ``block_table`` (new entries) and ``free_blocks`` (given-back ids) are updated in place; the
     lengths and ``free_state`` are not: pass the returned ones to the next call, or copy them
@@ -243,7 +244,8 @@ def dominus_ultra_paged_tables(
     Args:
         block_table: [batch, max_blocks] int32
         cache_seqlens: [batch] integer tokens cached (int32 or int64; on the CPU they are checked
-            here, on the GPU a bad request is left as it is and ``_lib.read_status()`` reports 6)
+            here, on the GPU a bad request is left as it is and ``_lib.read_status()`` reports 6;
+            a table entry that is not a block id is reported as 7 when it is used or given back)
         new_seqlens: [batch] integer tokens wanted
         free_blocks: [num_blocks] int32, a ring of free block ids
         free_state: [2] int32, {head, count} of the ring
@@ -345,7 +347,8 @@ def dominus_ultra_paged_write(
     and theirs is larger; when it grows, the earlier rows are rescaled. Values are rounded once, to
     the nearest e4m3 value. A value that is not finite makes its block's scale NaN.
 
-    Requests must not share a block that they write to; blocks that are only read may be shared.
+    Requests must not share a block that they write to. (Blocks that are only read may be shared by the
+    attention; ``dominus_ultra_paged_tables`` counts no references to them.)
 
     Args:
         k_new, v_new: [batch, num_kv_heads, T, head_dim], keys not rotated (one token each, or

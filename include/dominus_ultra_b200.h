@@ -269,7 +269,11 @@ int du_decode_noalloc(const void* q, const void* k_cache, const void* v_cache, c
  * free_state_out [2]; the inputs cache_seqlens, new_seqlens and free_state are not changed and
  * must not be the outputs. A request with a length below 0 or beyond the table's row, or with more
  * than max_new new tokens, is left as it is (code 6); a ring state that does not fit num_blocks
- * leaves every request as it is (code 7). B <= 8192; max_new may be 0 (slots is not used then).
+ * leaves every request as it is (code 7). A held entry that is not a block id is reported with its request
+ * (code 7) when one of its tokens needs a slot, which is -1 then, and when the request gives it back. It
+ * goes into the ring like a block; a request that is given it later has no slots in it and is reported
+ * too, so the ring has to be made anew. A block belongs to one request: this call counts no references,
+ * and a block in two rows would be given back twice. B <= 8192; max_new may be 0 (slots is not used then).
  */
 int du_paged_tables(int* block_table, const int* cache_seqlens, const int* new_seqlens,
                     int* free_blocks, const int* free_state, int* slots, int* seqlens_out,
