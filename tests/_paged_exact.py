@@ -1,5 +1,6 @@
 """The paged attention in 64 bits on the GPU (for batches that the plain loops of _paged.py take too
-long over), a bound on a kernel's error that has the weights' sum in it, and its parts of a weight."""
+long over), a bound on a kernel's error that has the weights' sum in it, the kernel's split of a batch
+over its CTAs, and its parts of a weight."""
 
 from __future__ import annotations
 
@@ -71,6 +72,58 @@ def tolerance(out, bound, dtype):
     """The bound and the output's own rounding, half a step, or half of its smallest one."""
     info = torch.finfo(dtype)
     return bound + (out.abs() + bound) * (info.eps / 2) + info.smallest_normal * info.eps
+
+
+# ------------------------------------------------------------------------------ split over CTAs
+
+
+def shape(Hq, Hkv, D):
+    """(heads per unit, units per request, stages of K, charge of a unit's beginning, CTAs per SM)."""
+    G = Hq // Hkv
+    parts = (G + 7) // 8
+    heads = -(-G // parts)
+    hpu = 1 if heads <= 1 else 2 if heads <= 2 else 4 if heads <= 4 else 8
+    return hpu, Hkv * parts, 4 if hpu == 8 else 3, 2 if D <= 128 else 1
+
+
+def split(lens, Hq, Hkv, D, block, width, sms=148):
+    """The kernel's fragments: a list per CTA of (unit, first chunk, end chunk, fragments of the unit),
+    and whether whole pieces of units were taken."""
+    _, ups, pen, per_sm = shape(Hq, Hkv, D)
+    chunks = [max(1, -(-n // 128)) for n in lens]
+    grid = min(sms * per_sm, 12 * 36, len(lens) * ups * -(-width * block // 128))
+    ctas = [[] for _ in range(grid)]
+    total = sum(chunks)
+    if len(lens) * ups <= grid:
+        per = -(-total * ups // grid)
+        for x in range(per, per + 4):
+            if sum(-(-c // x) for c in chunks) * ups <= grid:
+                at = unit = 0
+                for c in chunks:
+                    k = -(-c // x)
+                    for _ in range(ups):
+                        q, r = divmod(c, k)
+                        j = 0
+                        for i in range(k):
+                            e = j + q + (i < r)
+                            ctas[at + i].append((unit, j, e, k))
+                            j = e
+                        at += k
+                        unit += 1
+                return ctas, True
+    total = (total + len(lens) * pen) * ups
+    per = -(-total // grid)
+    base = unit = 0
+    for c in chunks:
+        for _ in range(ups):
+            first, last = base + pen, base + pen + c  # positions of the unit's chunks
+            nf = (last - 1) // per - first // per + 1
+            for cta in range(first // per, (last - 1) // per + 1):
+                lo, hi = max(first, cta * per), min(last, (cta + 1) * per)
+                ctas[cta].append((unit, lo - first, hi - first, nf))
+            base = last
+            unit += 1
+    return ctas, False
 
 
 def parts_of_weight(x: torch.Tensor, steps=(5, 5, 5)):

@@ -1,4 +1,6 @@
-"""Paged attention where a CTA runs through many chunks, against 64 bits."""
+"""Paged attention where a CTA runs through many chunks, against 64 bits: both ways of cutting a batch
+over the CTAs, references that move, sinks, value scales far apart, and results with a piece missing, which
+have to be told."""
 
 from __future__ import annotations
 
@@ -9,10 +11,12 @@ import torch
 
 from dominusultra_b200 import _lib, dominus_ultra_decode_paged, dominus_ultra_paged_write
 from tests import _paged_exact as exact
+from tests._paged_batches import EQUAL_RANGES, PIECES
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+CASES = {**EQUAL_RANGES, **PIECES}
 
 
 @pytest.fixture(autouse=True)
@@ -22,12 +26,85 @@ def _clean_status(cuda_device):
     assert _lib.read_status(reset=True)[0] == 0, "a test left a device status"
 
 
+def _batch(Hq, Hkv, D, block, lens, dtype, seed, rise=None):
+    """Random keys and values; the values of the request's chunk c have 8 more in column c mod D, so that
+    each chunk shows in the output. `rise`: the scores' spread instead, (from, to) along a request."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    width = max(1, -(-max(lens) // block))
+    N = sum(-(-n // block) for n in lens) + 2
+    perm = torch.randperm(N, generator=g, device=DEV).int()
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV)
+    k = torch.randn(N, Hkv, block, D, generator=g, device=DEV)
+    v = torch.randn(N, Hkv, block, D, generator=g, device=DEV) / 2
+    q = torch.randn(len(lens), Hq, 1, D, generator=g, device=DEV)
+    positions = max(1, max(lens))
+    if rise is None:
+        angle = torch.arange(positions, device=DEV).double()[:, None] / 10000.0 ** (torch.arange(0, D, 2, device=DEV) / D)
+        cos, sin = angle.cos().to(dtype), angle.sin().to(dtype)
+        q = q / 2
+    else:
+        cos, sin = torch.ones(positions, D // 2, device=DEV).to(dtype), torch.zeros(positions, D // 2, device=DEV).to(dtype)
+        q = torch.zeros_like(q)
+        q[..., 0] = math.sqrt(D)
+        k = k / 8
+    at = 0
+    for b, n in enumerate(lens):
+        m = -(-n // block)
+        ids = perm[at : at + m]
+        table[b, :m] = ids
+        at += m
+        page = torch.arange(m, device=DEV)
+        v[ids.long(), :, :, page * block // 128 % D] += 8
+        if rise is not None:
+            x = torch.linspace(*rise, m * block, device=DEV).reshape(m, 1, block)
+            k[ids.long(), :, :, 0] = x.expand(m, Hkv, block)
+    (k8, ks), (v8, vs) = exact.encode(k), exact.encode(v)
+    return q.to(dtype), k8, v8, ks, vs, table, lens, cos, sin
+
+
 def _call(q, k, v, ks, vs, table, lens, cos, sin):
     return dominus_ultra_decode_paged(q, k, v, ks, vs, table, torch.tensor(lens, dtype=torch.int32, device=DEV), cos, sin)
 
 
 def _within(got, want, bound):
     return (got.double() - want).abs() <= exact.tolerance(want, bound, got.dtype)
+
+
+def _check(batch, told=True):
+    got = _call(*batch)
+    want, bound = exact.attend(*batch)
+    ok = _within(got, want, bound)
+    assert bool(ok.all()), f"worst {((got.double() - want).abs() / exact.tolerance(want, bound, got.dtype)).max():.3f} of the tolerance"
+    if not told:
+        return
+    # The tolerance tells a wrong result: zeros, or one chunk of the longest request left out.
+    q, k, v, ks, vs, table, lens, cos, sin = batch
+    b = max(range(len(lens)), key=lambda i: lens[i])
+    one = (q[b : b + 1], k, v, ks, vs, table[b : b + 1], [lens[b]], cos, sin)
+    zero = ~_within(torch.zeros_like(want[b]).to(got.dtype), want[b], bound[b])
+    assert bool(zero.any(-1).all())
+    chunks = -(-lens[b] // 128)
+    for c in {0, 1, chunks // 2, chunks - 2}:
+        less, _ = exact.attend(*one, skip=(128 * c, 128 * c + 128))
+        assert not bool(_within(less.to(got.dtype), want[b : b + 1], bound[b : b + 1]).all(-1).any()), c
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_long(name):
+    Hq, Hkv, D, block, lens, dtype = CASES[name]
+    _check(_batch(Hq, Hkv, D, block, lens, dtype, len(lens) + D))
+
+
+@pytest.mark.parametrize("rise", [(-40.0, 40.0), (40.0, -40.0), (-3.0, 3.0)])
+@pytest.mark.parametrize("name", [
+    "64 requests, 32 heads on 8 of 128", "40 requests, 64 heads on 8 of 128", "50 requests, 8 heads of 64",
+    "45 requests, 16 heads on 8 of 64", "100 requests, 16 heads on one of 256", "200 requests, 6 heads on 2 of 16",
+])
+def test_long_with_moving_references(name, rise):
+    """Scores that rise (or fall) by 80 or 6 over a request: the weights' reference moves in most chunks
+    (or in none after the first)."""
+    Hq, Hkv, D, block, lens, dtype = CASES[name]
+    _check(_batch(Hq, Hkv, D, block, lens, dtype, 3, rise), told=False)
 
 
 @pytest.mark.parametrize("drop", [14.0, 18.5, 22.6, 25.0])
@@ -107,3 +184,28 @@ def test_a_block_of_zeros_beside_huge_values_from_the_writer():
     q = torch.randn(1, 2, 1, D, device=DEV).bfloat16()
     got = _call(q, k8, v8, ks, vs, torch.arange(2, **i32)[None], [32], cos, sin)
     assert bool((got == 2.0**79).all())
+
+
+@pytest.mark.parametrize("name", ["64 requests, 32 heads on 8 of 128", "36 uneven requests, 32 heads on 8 of 64", "one of 70000, 2 heads on one of 16"])
+def test_long_replayed_and_on_two_streams(name):
+    """A captured call replayed, and eager calls on two streams beside it, give the eager call's bits."""
+    Hq, Hkv, D, block, lens, dtype = CASES[name]
+    q, k, v, ks, vs, table, lens, cos, sin = _batch(Hq, Hkv, D, block, lens, dtype, 9)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    call = lambda: dominus_ultra_decode_paged(q, k, v, ks, vs, table, n, cos, sin)  # noqa: E731
+    want = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(call())
+        assert torch.equal(out, want)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got)
