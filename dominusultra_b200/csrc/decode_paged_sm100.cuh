@@ -14,9 +14,9 @@
 //   weight   w = w1 + w2 2^-5 + w3 2^-10 + w4 2^-15    (w rounded to fp16 first)
 // A query's part holds 4 significant bits, so three carry 12: half a step of 2^-12, as fp16 operands
 // would. A weight is at most 2^8, where a part leaves at most 2^3: the next one can be scaled by 2^5.
-// Three parts then hold any fp16 weight of normal size and the fourth those down to fp16's last
-// step, 2^-24 (e4m3's last step is 2^-9), so the four are the fp16 weight exactly. The parts are rows
-// of their own in tiles that are mostly empty otherwise, so they cost no tensor time:
+// Three parts then hold any fp16 weight of at least 2^-9 and the fourth the smaller ones down to fp16's
+// last step, 2^-24 (e4m3's last step is 2^-9), so the four are the fp16 weight exactly. The parts are
+// rows of their own in tiles that are mostly empty otherwise, so they cost no tensor time:
 //   S^T = K8 Q^T     M = 128 keys of a chunk, N = 16 or 32 (three parts of the unit's heads),
 //                    K = head_dim. A = the K tile as TMA left it, B = the query parts.
 //   O  += P V8       M = 64 or 128, N = head_dim, K = 128 keys. A = P, B = the V tile as TMA left
@@ -27,8 +27,9 @@
 // reduction across warps per chunk. The value scale joins the weight before it is split: with
 // u_j = s_j + log2 vs_j (log2 domain) the carried weight is 2^(u_j - m) = w_j vs_j. The sum takes
 // 2^(u_j - m - log2 vs_j), an exponential of its own: value scales may be 2^190 apart, and a key whose
-// carried weight is nothing beside another's can have all of the softmax's. (2^32 times that: its largest
-// term lies between 2^-121 and 2^72 without the factor, too near to the smallest float.) m moves only when some u exceeds it by 8 (then to 7 below that
+// carried weight is nothing beside another's can have all of the softmax's. (2^24 times that: without the
+// factor its largest term lies between 2^-121 and 2^72, too near to the smallest float; with it 2^27 terms
+// stay below 2^123.) m moves only when some u exceeds it by 8 (then to 7 below that
 // maximum), so the weights stay within 2^8 and the largest one of a warp is at least 2^7. Half a step of
 // the smallest weights is 2^-25 then, 2^-32 of the largest: behind a key that takes nearly all of the
 // weight and has values of zero, a long tail keeps its part. (With three parts, a factor of 2^4
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         if (vsc < 0x1p-64f) vsc = 0x1p-64f;  // (the writer's smallest; a NaN stays)
         __syncwarp();
         if (lane == 0) mbar_arrive(KEMPTY(s));
-        const float lv = lg2(vsc), lsum = lv - 32.0f;
+        const float lv = lg2(vsc), lsum = lv - 24.0f;
         ok = softmax_wait<DP>(SFULL(gj & 1), (gj >> 1) & 1, failed, 832);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
@@ -959,8 +960,8 @@ __global__ void __launch_bounds__(DecodePagedShape<DP, HPU>::NTHREADS, DecodePag
         float L = mrg_l[i] * half_fac * half_fac;
         L += __shfl_xor_sync(0xffffffffu, L, HPU);
         L += __shfl_xor_sync(0xffffffffu, L, 2 * HPU);
-        fac = fac * 0x1p32f / L;
-        if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + (lg2(L) - 32.0f);  // log2 of the sum
+        fac = fac * 0x1p24f / L;
+        if (f.nf > 1 && tid < HPU) p.part[(2LL * gridDim.x * p.D + f.slot) * HPU + tid] = top + (lg2(L) - 24.0f);  // log2 of the sum
         const int t = lane / HPU & 3;
         wt = __shfl_sync(0xffffffffu, fac, warp * HPU + lane % HPU) * __int_as_float((127 - 5 * t) << 23);
       }
