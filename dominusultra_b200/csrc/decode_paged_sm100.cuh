@@ -47,9 +47,10 @@
 //
 // Measured (B200, calls in a CUDA graph): 4 requests of 131072 tokens, 32 heads on 8 of 128 162-165 us, 6.5
 // TB/s, the rate of a copy; 16 of up to 20001, 64 on 8 of 128 66-68 us, 5.2 TB/s; 64 of up to 4096, 32 on
-// 8 of 128, blocks of 16 52 us, 5.3 TB/s; one of 32768, the same heads 21.6 us; 8 of 2048, 32 on 32 of 64
-// 17.2 us; one of 100, 8 heads of 64 5.5 us. Long contexts are bound by HBM; the others by the start (length,
-// table and first copies: some 4500 clocks before the first byte is asked for) and by the ends of fragments.
+// 8 of 128, blocks of 16 52.4 us, 5.2 TB/s; one of 32768, the same heads 21.8 us; 8 of 2048, 32 on 32 of 64
+// 17.6 us; 16 of 16384, 4 on 2 of 256 50.5 us, 5.3 TB/s; one of 100, 8 heads of 64 5.7 us. Long contexts are
+// bound by HBM; the others by the start (length, table and first copies: some 4500 clocks before the first
+// byte is asked for) and by the ends of fragments.
 #pragma once
 
 #include <float.h>

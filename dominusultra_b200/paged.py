@@ -11,7 +11,9 @@ as e4m3 with one scale per (block, KV head):
 
 A step is ``dominus_ultra_paged_tables`` (blocks and slots for the new tokens),
 ``dominus_ultra_paged_write`` (their keys and values) and ``dominus_ultra_decode_paged``. Lengths
-and tables stay on the GPU: no call synchronises, and each can be captured into a CUDA graph.
+and tables stay on the GPU: a step waits for nothing there, and each call can be captured into a CUDA
+graph. Two things do wait: lengths or a table given on the CPU are copied, and the first eager decode on
+a device (then the next one after every 512 captured ones) copies 4 MB of zeroed tickets from the host.
 """
 
 from __future__ import annotations
@@ -159,7 +161,9 @@ def _decode_workspace_size(B, Hq, Hkv, D, block_size, max_blocks, index) -> int:
 
 
 # Tickets for calls under a graph capture, handed out of zeroed slabs: [slab, words used] per device.
-# A graph's tickets and workspace are its own for good, so any two graphs may be replayed at once.
+# A captured call's tickets are its own for good; those of graphs that are gone are not taken back, 4 KB
+# each. Its workspace is memory of the capture's pool. So any two graphs may be replayed at once, unless
+# they were captured into one pool, which torch allows only for graphs that never run together.
 _SLAB_WORDS = 1024 * _lib.DU_PAGED_TICKETS
 _SLABS = {}
 _SLAB_LOCK = threading.Lock()

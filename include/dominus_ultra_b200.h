@@ -309,10 +309,11 @@ int du_paged_write(const void* k_new, const void* v_new, void* k_cache, void* v_
  * before the first call; every call leaves them zero). Calls that may overlap on the GPU, replayed
  * graphs among them, need tickets and a workspace each. A table row covers at most 2^27 tokens. The
  * scales may be any positive finite floats with which the scores, and a query's and a key's scale
- * together, stay within fp32's range (values of blocks whose value scale is below 2^-64 count as held at
- * 2^-64); a scale that is not a number makes the outputs over its block NaN. Precision: query elements are carried with 12 bits relative to the row's largest,
- * weights as fp16 values, so to 2^-11 of themselves, or to 2^-32 of the largest weight (times its value
- * scale) among the keys that one of the kernel's warps takes of a unit.
+ * together, stay within fp32's range (values of blocks whose value scale is below 2^-64 count as
+ * held at 2^-64); a scale that is not a number makes the outputs over its block NaN. Precision: query
+ * elements are carried with 12 bits relative to the row's largest, weights as fp16 values, so to
+ * 2^-11 of themselves, or to 2^-32 of the largest weight (times its value scale) among the keys that
+ * one of the kernel's warps takes of a unit.
  */
 #define DU_PAGED_TICKETS 1024
 size_t du_decode_paged_workspace_size(int B, int Hq, int Hkv, int D, int block_size, int max_blocks);
