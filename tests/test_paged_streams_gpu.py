@@ -166,3 +166,41 @@ def test_a_capture_that_forks_and_joins():
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
             o.zero_()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,block", [(16, 8, 64, 128), (32, 8, 128, 16), (8, 8, 256, 64)])
+def test_steps_back_to_back_equal_steps_apart(heads, kv_heads, dim, block):
+    """Steps whose scales grow nearly every time, launched without a pause and with the GPU idle between any
+    two calls: each kernel sees what the one before it wrote, neighbours' scales in one line among it."""
+    batch, steps, width = 48, 60, 128 // block + 2
+    g = torch.Generator(device=DEV).manual_seed(4)
+    cos, sin = precompute_rope_cos_sin(width * block, dim, DEV, torch.bfloat16)
+    grow = [2.0 ** (i * 0.6) for i in range(steps)]
+    q = [torch.randn(batch, heads, 1, dim, generator=g, device=DEV).bfloat16() for _ in range(steps)]
+    kv = [[(torch.randn(batch, kv_heads, 1, dim, generator=g, device=DEV) * x).bfloat16() for _ in range(2)] for x in grow]
+    first = torch.randint(1, block, (batch,), generator=g, device=DEV, dtype=torch.int32)
+
+    def run(pause):
+        n = batch * width
+        k8, v8 = (torch.zeros(n, kv_heads, block, dim, device=DEV).to(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = torch.zeros(n, kv_heads, device=DEV), torch.zeros(n, kv_heads, device=DEV)
+        table, ring, state = torch.full((batch, width), -1, **I32), torch.arange(n, **I32), torch.tensor([0, n], **I32)
+        lens, outs = torch.zeros(batch, **I32), []
+        for i in range(steps):
+            # (the first step brings a prompt of zeros, so that requests end in different rows)
+            new = first if i == 0 else lens + 1
+            k, v = kv[i] if i else (torch.zeros(batch, kv_heads, block, dim, device=DEV).bfloat16() for _ in range(2))
+            slots, grown, state = dominus_ultra_paged_tables(table, lens, new, ring, state, block, k.shape[2])
+            pause()
+            dominus_ultra_paged_write(k, v, k8, v8, ks, vs, slots, lens, cos, sin)
+            pause()
+            lens = grown
+            outs.append(dominus_ultra_decode_paged(q[i], k8, v8, ks, vs, table, lens, cos, sin))
+            pause()
+        return outs, (k8.view(torch.uint8), v8.view(torch.uint8), ks, vs, table, lens)
+
+    apart, state_apart = run(torch.cuda.synchronize)
+    for _ in range(3):
+        together, state_together = run(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(together, apart))
+        assert all(torch.equal(a, b) for a, b in zip(state_together, state_apart))

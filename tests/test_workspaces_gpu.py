@@ -134,3 +134,27 @@ def test_calls_keep_their_workspace_until_the_launch(cuda_device, monkeypatch, n
     gc.collect()
     assert seen == [True] and held() is None
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("slab", ["none yet", "used up"])
+def test_captures_without_a_ticket_slab(cuda_device, monkeypatch, slab):
+    """A process's first paged decode inside a capture, and captures beyond a slab's tickets: the graph zeroes
+    tickets of its own, on every replay."""
+    args = _paged_args(9000)
+    want = dominus_ultra_decode_paged(*args)
+    if slab == "none yet":
+        monkeypatch.setattr(paged, "_SLABS", {})
+    else:
+        index = torch.cuda.current_device()
+        monkeypatch.setattr(paged, "_SLABS", {index: [paged._SLABS[index][0], paged._SLAB_WORDS]})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [dominus_ultra_decode_paged(*args) for _ in range(3)]
+        outs.append(torch.full_like(outs[0], 3.0))  # (what may take the memory of tickets given back)
+        outs.append(dominus_ultra_decode_paged(*args))
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        assert all(torch.equal(o, want) for i, o in enumerate(outs) if i != 3)
+    assert _lib.read_status(reset=True)[0] == 0
