@@ -23,6 +23,12 @@ from dominusultra_b200.paged import (  # noqa: F401
     dominus_ultra_paged_tables,
     dominus_ultra_paged_write,
 )
+from dominusultra_b200.paged_blocks import (  # noqa: F401
+    dominus_ultra_paged_compact,
+    dominus_ultra_paged_copy,
+    dominus_ultra_paged_fork,
+)
+from dominusultra_b200.paged_extend import dominus_ultra_extend_paged  # noqa: F401
 
 __all__ = ["precompute_rope_cos_sin", "dominus_ultra_prefill", "dominus_ultra_decode"]
 

@@ -20,6 +20,8 @@
 #include "decode_sm100.cuh"
 #include "decode_tc_sm100.cuh"
 #include "exchange_sm100.cuh"
+#include "extend_paged_sm100.cuh"
+#include "paged_blocks_sm100.cuh"
 #include "paged_sm100.cuh"
 #include "prefill_fa1_sm100.cuh"
 #include "prefill_fa_sm100.cuh"
@@ -1550,6 +1552,219 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.heads = paged_unit_heads(prm.G);
   prm.scale_log2 = scale * 1.4426950408889634f;
   return launch_decode_paged(k_cache, v_cache, prm, grid, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+namespace {
+
+// What the fork and the compaction share: sizes, and shared memory for their sets.
+int check_paged_sets(int B, int max_blocks, int num_blocks, int block_size, long long set_words) {
+  int rc = check_paged(1, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (B <= 0 || max_blocks <= 0) return fail(DU_ERR_INVALID, "batch and max_blocks must be positive");
+  if (B > du::PAGED_MAX_BATCH) return fail(DU_ERR_UNSUPPORTED, "at most 8192 requests in one call");
+  if (static_cast<long long>(B) * max_blocks > 0x7fffffffLL ||
+      static_cast<long long>(max_blocks) * block_size > 0x7fffffffLL - 128)
+    return fail(DU_ERR_UNSUPPORTED, "the block table holds more than 2^31 - 1 entries, or a row more tokens");
+  if (4 * set_words > du::PAGED_SET_SMEM)
+    return fail(DU_ERR_UNSUPPORTED, "the sets of " + std::to_string(num_blocks) + " blocks and " + std::to_string(B) +
+                                        " requests do not fit the kernel's shared memory (200 KB: 3 bits a block and "
+                                        "36 a request in a fork, 2.1 bits a block in a compaction)");
+  return DU_OK;
+}
+
+template <typename Params>
+int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_words, void* stream, const char* what) {
+  // (an attribute of the largest sets, once per device)
+  cudaError_t e = ensure_smem_attr(kern, du::PAGED_SET_SMEM);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  e = launch_kernel(kern, dim3(du::PAGED_SET_CTAS), du::PAGED_SET_THREADS, static_cast<size_t>(4 * set_words),
+                    static_cast<cudaStream_t>(stream), true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return DU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* sources,
+                  const int* new_seqlens, int* free_blocks, const int* free_state, int* table_out,
+                  int* copies, int* seqlens_out, int* free_state_out, int B, int max_blocks,
+                  int num_blocks, int block_size, void* stream) {
+  g_last_error.clear();
+  const long long words = du::paged_fork_words(B, num_blocks);
+  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
+  if (rc != DU_OK) return rc;
+  const void* ins[] = {block_table, cache_seqlens, sources, new_seqlens, free_state, free_blocks};
+  const void* outs[] = {table_out, copies, seqlens_out, free_state_out};
+  for (const void* o : outs) {
+    if (!o) return fail(DU_ERR_INVALID, "null pointer argument");
+    for (const void* i : ins)
+      if (i == o) return fail(DU_ERR_INVALID, "the outputs must not be the inputs (every block of threads reads those)");
+  }
+  for (const void* i : ins)
+    if (!i) return fail(DU_ERR_INVALID, "null pointer argument");
+  for (const void* q : ins)
+    if (!aligned4(q)) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
+  for (const void* q : outs)
+    if (!aligned4(q)) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
+  du::PagedForkParams prm{};
+  prm.table = block_table;
+  prm.lens = cache_seqlens;
+  prm.sources = sources;
+  prm.wanted = new_seqlens;
+  prm.ring = free_blocks;
+  prm.state = free_state;
+  prm.table_out = table_out;
+  prm.copies = copies;
+  prm.lens_out = seqlens_out;
+  prm.state_out = free_state_out;
+  prm.B = B;
+  prm.width = max_blocks;
+  prm.N = num_blocks;
+  prm.block = block_size;
+  return launch_paged_sets(du::paged_fork_kernel, prm, words, stream, "paged fork launch");
+}
+
+int du_paged_compact(const int* block_table, const int* cache_seqlens, const int* free_blocks,
+                     const int* free_state, int* table_out, int* copies, int* free_blocks_out,
+                     int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
+                     void* stream) {
+  g_last_error.clear();
+  const long long words = du::paged_compact_words(num_blocks);
+  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
+  if (rc != DU_OK) return rc;
+  const void* ins[] = {block_table, cache_seqlens, free_blocks, free_state};
+  const void* outs[] = {table_out, free_blocks_out, free_state_out, copies};
+  for (int k = 0; k < 4; ++k) {
+    if (!outs[k] && (k < 3 || num_blocks > 1)) return fail(DU_ERR_INVALID, "null pointer argument");
+    for (const void* i : ins)
+      if (i == outs[k]) return fail(DU_ERR_INVALID, "the outputs must not be the inputs (every block of threads reads those)");
+    if (!aligned4(outs[k])) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
+  }
+  for (const void* i : ins) {
+    if (!i) return fail(DU_ERR_INVALID, "null pointer argument");
+    if (!aligned4(i)) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
+  }
+  du::PagedCompactParams prm{};
+  prm.table = block_table;
+  prm.lens = cache_seqlens;
+  prm.ring = free_blocks;
+  prm.state = free_state;
+  prm.table_out = table_out;
+  prm.copies = copies;
+  prm.ring_out = free_blocks_out;
+  prm.state_out = free_state_out;
+  prm.B = B;
+  prm.width = max_blocks;
+  prm.N = num_blocks;
+  prm.block = block_size;
+  return launch_paged_sets(du::paged_compact_kernel, prm, words, stream, "paged compact launch");
+}
+
+int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* copies, int n,
+                  int num_blocks, int Hkv, int block_size, int D, void* stream) {
+  g_last_error.clear();
+  int rc = check_paged(Hkv, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (!valid_head_dim(D)) return fail(DU_ERR_UNSUPPORTED, "head_dim must be a power of two between 16 and 256");
+  if (n < 0) return fail(DU_ERR_INVALID, "the number of copies must not be negative");
+  if (n == 0) return DU_OK;
+  if (!k_cache || !v_cache || !k_scale || !v_scale || !copies) return fail(DU_ERR_INVALID, "null pointer argument");
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(DU_ERR_INVALID, "the caches must be 16-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(copies))
+    return fail(DU_ERR_INVALID, "scales and copies must be 4-byte aligned");
+  du::PagedCopyParams prm{};
+  prm.k8 = static_cast<uint8_t*>(k_cache);
+  prm.v8 = static_cast<uint8_t*>(v_cache);
+  prm.ks = k_scale;
+  prm.vs = v_scale;
+  prm.copies = copies;
+  prm.n = n;
+  prm.N = num_blocks;
+  prm.Hkv = Hkv;
+  prm.bytes = static_cast<long long>(Hkv) * block_size * D;
+  if (prm.bytes > 0x7fffffffLL) return fail(DU_ERR_UNSUPPORTED, "a block holds more than 2^31 - 1 bytes");
+  prm.parts = static_cast<int>((prm.bytes + du::PAGED_COPY_PART - 1) / du::PAGED_COPY_PART);
+  constexpr int kWarps = du::PAGED_COPY_THREADS / 32;
+  const long long need = (2LL * n * prm.parts + kWarps - 1) / kWarps, most = 8LL * sm_count();
+  cudaError_t e = launch_kernel(du::paged_copy_kernel, dim3(static_cast<unsigned>(need < most ? need : most)),
+                                du::PAGED_COPY_THREADS, 0, static_cast<cudaStream_t>(stream), true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged copy launch");
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged copy launch");
+  return DU_OK;
+}
+
+size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size, int max_blocks) {
+  if (check_common(B, Hq, Hkv, T, D, DU_DTYPE_BF16) != DU_OK || check_paged(Hkv, 1, block_size) != DU_OK || max_blocks <= 0)
+    return 0;
+  return 0;
+}
+
+int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                    const float* v_scale, const int* block_table, const int* past_seqlens,
+                    const int* cache_seqlens, const void* cos, const void* sin, void* out, int B, int Hq,
+                    int Hkv, int T, int D, int num_blocks, int block_size, int max_blocks, int dtype,
+                    float scale, long long rope_positions, int* tickets, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  int rc = check_common(B, Hq, Hkv, T, D, dtype);
+  if (rc != DU_OK) return rc;
+  rc = check_paged(Hkv, num_blocks, block_size);
+  if (rc != DU_OK) return rc;
+  if (max_blocks <= 0) return fail(DU_ERR_INVALID, "max_blocks must be positive");
+  if (static_cast<long long>(max_blocks) * block_size > (1LL << 27))
+    return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^27 tokens");
+  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !past_seqlens || !cache_seqlens || !cos ||
+      !sin || !out)
+    return fail(DU_ERR_INVALID, "null pointer argument");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(cos) || !aligned16(sin) || !aligned16(out))
+    return fail(DU_ERR_INVALID, "q, out, the caches and the rope tables must be 16-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(past_seqlens) || !aligned4(cache_seqlens))
+    return fail(DU_ERR_INVALID, "scales, block_table and the lengths must be 4-byte aligned");
+  if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
+  if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
+  if (Hq > 65536 || T > (1 << 24) || B > (1 << 20))
+    return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads, 2^24 new tokens of a request and 2^20 requests");
+  du::ExtendPagedParams prm{};
+  prm.q = q;
+  prm.k8 = static_cast<const uint8_t*>(k_cache);
+  prm.v8 = static_cast<const uint8_t*>(v_cache);
+  prm.ks = k_scale;
+  prm.vs = v_scale;
+  prm.table = block_table;
+  prm.past = past_seqlens;
+  prm.lens = cache_seqlens;
+  prm.cos = cos;
+  prm.sin = sin;
+  prm.out = out;
+  const long long cover = static_cast<long long>(max_blocks) * block_size;
+  prm.max_len = static_cast<int>(cover < rope_positions ? cover : rope_positions);
+  prm.D = D;
+  prm.bf16 = dtype == DU_DTYPE_BF16;
+  prm.B = B;
+  prm.Hq = Hq;
+  prm.Hkv = Hkv;
+  prm.G = Hq / Hkv;
+  prm.T = T;
+  prm.N = num_blocks;
+  prm.width = max_blocks;
+  prm.block = block_size;
+  prm.scale_log2 = scale * 1.4426950408889634f;
+  const long long rows = static_cast<long long>(B) * Hq * T;
+  const long long most = 16LL * sm_count();
+  const long long need = (rows + 3) / 4;
+  cudaError_t e = launch_kernel(du::extend_paged_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 128, 0,
+                                static_cast<cudaStream_t>(stream), true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
+  return DU_OK;
 }
 
 }  // extern "C"

@@ -325,6 +325,71 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
                     void* stream);
 
 /*
+ * Attention of several new tokens per request over the cache: a prompt's chunk behind cached tokens,
+ * or a draft. q [B, Hq, T, D] (rotated here), out [B, Hq, T, D]. Request b has past_seqlens[b] tokens
+ * before its new ones and cache_seqlens[b] with them, all cached (du_paged_write before this call); its
+ * new token t, at position past_seqlens[b] + t, sees the keys up to its own. Rows behind the last new
+ * token are zeros. Lengths that are out of range (0 <= past <= cached <= past + T, and cached at most
+ * the table's row and rope_positions) give zeros and code 6; a block id out of range gives NaN in the
+ * rows that see its keys, and code 7. tickets and workspace (du_extend_paged_workspace_size bytes,
+ * 16-byte aligned, any contents) as in du_decode_paged, with which they may be shared by calls that
+ * do not overlap. A table row covers at most 2^27 tokens. The caches are as du_paged_write leaves them:
+ * no value that is not a number under a finite scale.
+ */
+size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size,
+                                      int max_blocks);
+int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                    const float* v_scale, const int* block_table, const int* past_seqlens,
+                    const int* cache_seqlens, const void* cos, const void* sin, void* out, int B,
+                    int Hq, int Hkv, int T, int D, int num_blocks, int block_size, int max_blocks,
+                    int dtype, float scale, long long rope_positions, int* tickets, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/*
+ * Blocks that several requests share. Request b of the new state holds the first new_seqlens[b]
+ * tokens (0: none; it ends) of request sources[b] of the old one, all requests at once: row b of
+ * table_out [B, max_blocks] is row sources[b] of block_table, up to its pages, then -1. Whole blocks are
+ * shared. A last block that is partly filled is going to be written, so it must be b's own: of the
+ * requests that end in it the lowest keeps it, unless some request holds it whole; each of the others
+ * takes a block from the ring's head, in order of b, and leaves the pair {its source, its own} in
+ * copies [B, 2] for du_paged_copy ({-1, -1}: none). A request for which no block is left is cut to its
+ * whole blocks: seqlens_out[b] says so. Blocks that were held before and are not held any more go
+ * behind the ring's tail in order of their ids, free from the next call on. free_blocks is updated in
+ * place, nothing else is: outputs must not be inputs. A request whose lengths or source are out of
+ * range keeps its row and its blocks (code 6); if more is given back than the ring has room for, or its
+ * state is out of range, nothing changes (code 7). num_blocks and B are bounded by the kernel's 200 KB of
+ * sets: 3 bits a block and 36 a request (up to 8192 requests and 436000 blocks).
+ */
+int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* sources,
+                  const int* new_seqlens, int* free_blocks, const int* free_state, int* table_out,
+                  int* copies, int* seqlens_out, int* free_state_out, int B, int max_blocks,
+                  int num_blocks, int block_size, void* stream);
+
+/*
+ * Copies blocks of the cache, keys, values and scales: for each of the n pairs {source, destination} of
+ * copies [n, 2]; {-1, -1} is no copy. A block must not be the destination of two pairs, nor the
+ * source of one and the destination of another. A pair with a block id out of range is left out
+ * (code 7).
+ */
+int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* copies,
+                  int n, int num_blocks, int Hkv, int block_size, int D, void* stream);
+
+/*
+ * Moves the blocks in use to the lowest ids. Of the blocks that these requests hold and the free ones
+ * (others are not touched), the lowest ids become the ones in use: blocks above them move into the free
+ * ones among them, in ascending order, and their pairs are left in copies [num_blocks / 2, 2] for
+ * du_paged_copy, the rest {-1, -1}. table_out [B, max_blocks] has the new ids up to each request's pages,
+ * then -1; free_blocks_out [num_blocks] the free ids in ascending order, then -1, with free_state_out
+ * {0, count}. Outputs must not be inputs. A request whose length is out of range keeps its row, and its
+ * blocks stay (code 6). A ring that does not hold `count` different block ids, none of them in use,
+ * leaves everything as it is (code 7). At most 770000 blocks.
+ */
+int du_paged_compact(const int* block_table, const int* cache_seqlens, const int* free_blocks,
+                     const int* free_state, int* table_out, int* copies, int* free_blocks_out,
+                     int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
+                     void* stream);
+
+/*
  * Failure-detection self-test (no counterpart in the reference): launches one CTA whose
  * bounded wait can never complete -- an mbarrier nothing arrives at -- with a limit of
  * timeout_us microseconds (1..1000000). The kernel records DU_ERR_TIMEOUT in the status words
