@@ -1587,6 +1587,50 @@ int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_wor
   return DU_OK;
 }
 
+// How the extension's rows are laid out: row tiles of an item, and parts of a tile that share its keys.
+struct ExtendPlan {
+  int nt, cs, grid;
+};
+
+ExtendPlan extend_plan(int T, int G, int D) {
+  const long long rows = static_cast<long long>(T) * G;
+  ExtendPlan pl{};
+  pl.nt = rows > 128 && D <= 128 ? 2 : 1;
+  pl.cs = rows <= 32 ? 4 : 1;
+  pl.grid = sm_count();
+  if (pl.grid > DU_PAGED_TICKETS - 1) pl.grid = DU_PAGED_TICKETS - 1;
+  return pl;
+}
+
+// Two partial slots per CTA: rows of an item, fp32, and the log2 of a sum in two parts.
+size_t extend_ws_bytes(const ExtendPlan& pl, int D) {
+  return 2 * static_cast<size_t>(pl.grid) * (pl.nt * 128 / pl.cs) * (D + 2) * sizeof(float);
+}
+
+template <int D, int NT, int CS>
+int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st) {
+  using S = du::ExtendShape<D, NT, CS>;
+  auto kern = du::extend_paged_kernel<D, NT, CS>;
+  if (launch_registers(kern) * du::EXTEND_THREADS < S::REGS * 128)
+    return fail(DU_ERR_CUDA, "paged extend kernel built with too few registers for its split");
+  cudaError_t e = ensure_smem_attr(kern, S::SMEM_BYTES);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged extend)");
+  e = launch_kernel(kern, dim3(static_cast<unsigned>(grid)), du::EXTEND_THREADS, S::SMEM_BYTES, st, true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
+  return DU_OK;
+}
+
+template <int D>
+int launch_extend(const du::ExtendPagedParams& prm, const ExtendPlan& pl, cudaStream_t st) {
+  if constexpr (D <= 128) {
+    if (pl.nt == 2) return launch_extend_t<D, 2, 1>(prm, pl.grid, st);
+  }
+  if (pl.cs == 4) return launch_extend_t<D, 1, 4>(prm, pl.grid, st);
+  return launch_extend_t<D, 1, 1>(prm, pl.grid, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1703,7 +1747,7 @@ int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
 size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size, int max_blocks) {
   if (check_common(B, Hq, Hkv, T, D, DU_DTYPE_BF16) != DU_OK || check_paged(Hkv, 1, block_size) != DU_OK || max_blocks <= 0)
     return 0;
-  return 0;
+  return extend_ws_bytes(extend_plan(T, Hq / Hkv, D), D);
 }
 
 int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -1721,16 +1765,20 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   if (static_cast<long long>(max_blocks) * block_size > (1LL << 27))
     return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^27 tokens");
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !past_seqlens || !cache_seqlens || !cos ||
-      !sin || !out)
+      !sin || !out || !tickets)
     return fail(DU_ERR_INVALID, "null pointer argument");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(cos) || !aligned16(sin) || !aligned16(out))
     return fail(DU_ERR_INVALID, "q, out, the caches and the rope tables must be 16-byte aligned");
-  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(past_seqlens) || !aligned4(cache_seqlens))
-    return fail(DU_ERR_INVALID, "scales, block_table and the lengths must be 4-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(past_seqlens) ||
+      !aligned4(cache_seqlens) || !aligned4(tickets))
+    return fail(DU_ERR_INVALID, "scales, block_table, the lengths and tickets must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
-  if (Hq > 65536 || T > (1 << 24) || B > (1 << 20))
-    return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads, 2^24 new tokens of a request and 2^20 requests");
+  if (Hq > 65536 || static_cast<long long>(T) * (Hq / Hkv) > (1 << 30) || B > (1 << 20))
+    return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads, 2^30 query rows of a KV head and 2^20 requests");
+  const ExtendPlan plan = extend_plan(T, Hq / Hkv, D);
+  if (!workspace || workspace_bytes < extend_ws_bytes(plan, D) || !aligned16(workspace))
+    return fail(DU_ERR_WORKSPACE, "workspace missing, misaligned or smaller than du_extend_paged_workspace_size");
   du::ExtendPagedParams prm{};
   prm.q = q;
   prm.k8 = static_cast<const uint8_t*>(k_cache);
@@ -1743,9 +1791,11 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.cos = cos;
   prm.sin = sin;
   prm.out = out;
+  prm.cnt = tickets;
+  prm.part = static_cast<float*>(workspace);
+  prm.done = DU_PAGED_TICKETS - 1;
   const long long cover = static_cast<long long>(max_blocks) * block_size;
   prm.max_len = static_cast<int>(cover < rope_positions ? cover : rope_positions);
-  prm.D = D;
   prm.bf16 = dtype == DU_DTYPE_BF16;
   prm.B = B;
   prm.Hq = Hq;
@@ -1755,16 +1805,16 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.N = num_blocks;
   prm.width = max_blocks;
   prm.block = block_size;
+  prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
   prm.scale_log2 = scale * 1.4426950408889634f;
-  const long long rows = static_cast<long long>(B) * Hq * T;
-  const long long most = 16LL * sm_count();
-  const long long need = (rows + 3) / 4;
-  cudaError_t e = launch_kernel(du::extend_paged_kernel, dim3(static_cast<unsigned>(need < most ? need : most)), 128, 0,
-                                static_cast<cudaStream_t>(stream), true, prm);
-  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
-  return DU_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (D) {
+    case 16: return launch_extend<16>(prm, plan, st);
+    case 32: return launch_extend<32>(prm, plan, st);
+    case 64: return launch_extend<64>(prm, plan, st);
+    case 128: return launch_extend<128>(prm, plan, st);
+    default: return launch_extend<256>(prm, plan, st);
+  }
 }
 
 }  // extern "C"
