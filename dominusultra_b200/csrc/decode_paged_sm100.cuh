@@ -101,10 +101,6 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-// Brings a word into L1 and waits for nothing.
-__device__ __forceinline__ void prefetch_l1(const void* p) {
-  asm volatile("{\n\t.reg .b32 t;\n\tld.global.b32 t, [%0];\n\t}\n" ::"l"(p));
-}
 // D[tmem] (+)= A[smem] * B[smem], e4m3 operands, fp32 accumulate, one CTA.
 __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                            uint32_t idesc, uint32_t accumulate) {

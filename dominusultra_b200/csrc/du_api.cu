@@ -1587,16 +1587,14 @@ int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_wor
   return DU_OK;
 }
 
-// How the extension's rows are laid out: row tiles of an item, and parts of a tile that share its keys.
+// How the extension's rows are laid out: row tiles of 128 in an item.
 struct ExtendPlan {
-  int nt, cs, grid;
+  int nt, grid;
 };
 
 ExtendPlan extend_plan(int T, int G, int D) {
-  const long long rows = static_cast<long long>(T) * G;
   ExtendPlan pl{};
-  pl.nt = rows > 128 && D <= 128 ? 2 : 1;
-  pl.cs = rows <= 32 ? 4 : 1;
+  pl.nt = static_cast<long long>(T) * G > 128 && D <= 128 ? 2 : 1;
   pl.grid = sm_count();
   if (pl.grid > DU_PAGED_TICKETS - 1) pl.grid = DU_PAGED_TICKETS - 1;
   return pl;
@@ -1604,14 +1602,14 @@ ExtendPlan extend_plan(int T, int G, int D) {
 
 // Two partial slots per CTA: rows of an item, fp32, and the log2 of a sum in two parts.
 size_t extend_ws_bytes(const ExtendPlan& pl, int D) {
-  return 2 * static_cast<size_t>(pl.grid) * (pl.nt * 128 / pl.cs) * (D + 2) * sizeof(float);
+  return 2 * static_cast<size_t>(pl.grid) * (pl.nt * 128) * (D + 2) * sizeof(float);
 }
 
-template <int D, int NT, int CS>
+template <int D, int NT>
 int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st) {
-  using S = du::ExtendShape<D, NT, CS>;
-  auto kern = du::extend_paged_kernel<D, NT, CS>;
-  if (launch_registers(kern) * du::EXTEND_THREADS < S::REGS * 128)
+  using S = du::ExtendShape<D, NT>;
+  auto kern = du::extend_paged_kernel<D, NT>;
+  if (launch_registers(kern) < 128)
     return fail(DU_ERR_CUDA, "paged extend kernel built with too few registers for its split");
   cudaError_t e = ensure_smem_attr(kern, S::SMEM_BYTES);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(paged extend)");
@@ -1625,10 +1623,9 @@ int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st)
 template <int D>
 int launch_extend(const du::ExtendPagedParams& prm, const ExtendPlan& pl, cudaStream_t st) {
   if constexpr (D <= 128) {
-    if (pl.nt == 2) return launch_extend_t<D, 2, 1>(prm, pl.grid, st);
+    if (pl.nt == 2) return launch_extend_t<D, 2>(prm, pl.grid, st);
   }
-  if (pl.cs == 4) return launch_extend_t<D, 1, 4>(prm, pl.grid, st);
-  return launch_extend_t<D, 1, 1>(prm, pl.grid, st);
+  return launch_extend_t<D, 1>(prm, pl.grid, st);
 }
 
 }  // namespace
@@ -1774,9 +1771,15 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
     return fail(DU_ERR_INVALID, "scales, block_table, the lengths and tickets must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
-  if (Hq > 65536 || static_cast<long long>(T) * (Hq / Hkv) > (1 << 30) || B > (1 << 20))
-    return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads, 2^30 query rows of a KV head and 2^20 requests");
+  if (Hq > 65536 || T > (1 << 20) || static_cast<long long>(T) * (Hq / Hkv) > (1 << 24) || B > (1 << 20))
+    return fail(DU_ERR_UNSUPPORTED, "at most 65536 query heads, 2^20 new tokens, 2^24 query rows of a KV head and 2^20 requests");
   const ExtendPlan plan = extend_plan(T, Hq / Hkv, D);
+  // Positions of the kernel's walk, and what its divisions by estimate take.
+  const int rows_item = plan.nt * 128;
+  const int items = (T * (Hq / Hkv) + rows_item - 1) / rows_item;
+  if (static_cast<double>(B) * items * Hkv * (static_cast<double>(max_blocks) * block_size / 64 + 8) > 2147480000.0 ||
+      static_cast<double>(B) * items > 2097152.0)
+    return fail(DU_ERR_UNSUPPORTED, "the call's rows and block tables can hold 2^31 key tiles of 64 or more, or 2^21 row tiles");
   if (!workspace || workspace_bytes < extend_ws_bytes(plan, D) || !aligned16(workspace))
     return fail(DU_ERR_WORKSPACE, "workspace missing, misaligned or smaller than du_extend_paged_workspace_size");
   du::ExtendPagedParams prm{};
@@ -1804,6 +1807,7 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.T = T;
   prm.N = num_blocks;
   prm.width = max_blocks;
+  prm.items = items;
   prm.block = block_size;
   prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
   prm.scale_log2 = scale * 1.4426950408889634f;

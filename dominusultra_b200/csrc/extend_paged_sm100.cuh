@@ -12,31 +12,33 @@
 // products are kind::f16: the cached bytes are widened to fp16 (exactly, by one conversion per pair) in
 // shared memory once per tile for all rows of an item, unscaled. Scales are per block of at least 16
 // keys, so they cost a multiplication per 16 scores: with x = s + log2 vs (log2 domain, s = S kq, kq the
-// key scale, the softmax scale and the query row's own factor) the carried weight is 2^(x - m + 11) =
-// w vs up to a row's constant, an fp16 value of at most 2^15 since m moves when some x exceeds it by 4,
+// key scale, the softmax scale and the query row's own factor) the carried weight is 2^(x - m + 8) =
+// w vs up to a row's constant, an fp16 value of at most 2^15 since m moves when some x exceeds it by 7,
 // and the sum takes 2^(vr - log2 vs) times the sum of a group's weights, vr being the log2 of the first
 // value scale of the fragment. Where a value scale is beyond 2^30 of that (then, and for the rest of the
 // fragment) the sum has exponentials and a reference of its own: a key whose carried weight is nothing
-// beside another's can have all of the softmax's. fp16 holds weights down to 2^-25 of a row's largest at
-// full precision and to 2^-36 at all. Query rows are carried as fp16 with a power of two for each row.
+// beside another's can have all of the softmax's. fp16 holds weights down to 2^-22 of a row's largest at
+// full precision, and half its smallest step is 2^-33 of that. Query rows are carried as fp16 with a power of two for each row.
 //
 // Work: the items' key tiles, item by item, cut into equal ranges, one per CTA of a persistent grid (an
 // item's beginning is charged with PEN tiles). Lengths are read on the device; every CTA repeats the sum
 // over them. An item within one CTA is written at once; the fragments of others leave fp32 partials, and
 // the CTA that leaves the last one joins them.
 //
-// NT = 2 (more than 128 rows in an item, head_dim up to 128): two tiles of 128 rows, whose softmax
-// warpgroups alternate with the tensor core. At head_dim 128 P overwrites S in tensor memory, and O_x += P_x V
-// comes before the next S_x, so that S_x being there means that O_x is (products of the same shape
-// complete in order); below that P has columns of its own, and the next S_x is computed as soon as S_x
-// is read. NT = 1: one tile, two buffers of S, P over S. With CS = 4 (up to 32 rows) the rows stand in all four 32-lane parts of the tile, and each warp takes a quarter of
-// a key tile's columns (P is zero in the others): the softmax of few rows is done by all four warps. Each
-// part has a maximum, sum and O of its own, joined at the fragment's end.
+// Streams: two softmax warpgroups (one at head_dim 256, where tensor memory holds one O), each with an S, an O
+// and a warp that issues its products. P overwrites S, and O += P V comes before the next S. With NT = 2
+// (more than 128 rows in an item) a stream is a tile of 128 rows. With NT = 1 the streams share the one row
+// tile and take every other key tile each; a row then has two parts, each with a maximum, sum and O of its
+// own, joined at the fragment's end.
 //
-// Warps (512 threads): 0-3 softmax (of the first row tile); 4-7 softmax of the second, or widening K;
-// 8-11 widening (of both, or of V); 12 and 13 bulk copies of K and of V; 14 TMEM and MMA; 15 walks the
-// fragments and fetches the scales. Every wait is bounded.
+// Warps (512 threads): 0-3 and 4-7 softmax; 8-11 widen K and V (4-11 at head_dim 256); 12 bulk copies of K;
+// 13 walks the fragments, fetches the scales and copies V; 14 and 15 the products of a stream each (14: and
+// TMEM). Every wait is bounded.
 #pragma once
+
+#include <float.h>
+
+#include <type_traits>
 
 #include "paged_sm100.cuh"
 
@@ -60,35 +62,37 @@ struct ExtendPagedParams {
   int max_len;        // tokens that the table's row and the rope tables cover
   int bf16;
   int B, Hq, Hkv, G, T, N, width;
+  int items;          // of a request with T new tokens
   int block, block_log2;
   float scale_log2;
 };
 
 constexpr int EXTEND_THREADS = 512;
-constexpr float EXTEND_TOP = 11.0f;   // log2 of the weight at a row's reference
-constexpr float EXTEND_MOVE = 4.0f;   // how far beyond its reference a row's maximum may be
+constexpr float EXTEND_TOP = 8.0f;   // log2 of the weight at a row's reference
+constexpr float EXTEND_MOVE = 7.0f;   // how far beyond its reference a row's maximum may be
 constexpr float EXTEND_LARGE = 1024.0f;  // references beyond this are kept in two parts
 constexpr float EXTEND_FAR = 30.0f;   // how far a value scale may be from the fragment's first
 
-template <int D_, int NT_, int CS_>
+template <int D_, int NT_>
 struct ExtendShape {
-  static constexpr int D = D_, NT = NT_, CS = CS_;
-  static constexpr int R = 128 / CS;             // rows of a tile
-  static constexpr int RP = NT * R;              // rows of an item
+  static constexpr int D = D_, NT = NT_;
+  static constexpr int NS = D <= 128 ? 2 : 1;    // streams
+  static constexpr bool ALT = NT < NS;           // that take key tiles in turn
+  static constexpr int RP = NT * 128;            // rows of an item
   static constexpr int KT = D == 256 ? 64 : 128; // keys of a tile
-  static constexpr int NC = KT / CS;             // columns of a key tile that a softmax thread takes
   static constexpr int SPAN = 2 * D >= 128 ? 128 : 2 * D;  // bytes per row of a swizzled block
-  static constexpr int NBLK = 2 * D / SPAN;
   static constexpr int GPT = KT / 16;            // groups of 16 keys in a tile
   static constexpr int NB = 32 / GPT;            // tiles of a batch of scales
   static constexpr int Q_BYTES = 128 * D * 2;
   static constexpr int T_BYTES = KT * D * 2;     // a widened tile
-  static constexpr int RAW = KT * D;             // a tile as it is cached
+  static constexpr int RK = 64;                  // keys of a copied piece
+  static constexpr int RPT = KT / RK;            // pieces of a tile
+  static constexpr int RAW = RK * D;
   static constexpr int NK = 2, NV = D == 256 ? 1 : 2;  // widened tiles
-  static constexpr int MISC = CS > 1 ? 2560 : 2048;
-  static constexpr int TILES = (231424 - MISC - NT * Q_BYTES - (NK + NV) * T_BYTES) / RAW;
-  static constexpr int NRV = TILES / 2 > 8 ? 8 : TILES / 2;            // cached tiles of V in flight
-  static constexpr int NRK = TILES - NRV > 8 ? 8 : TILES - NRV;        // and of K
+  static constexpr int MISC = 2048;
+  static constexpr int RAWS = (231424 - MISC - NT * Q_BYTES - (NK + NV) * T_BYTES) / RAW;
+  static constexpr int NRV = RAWS / 2 > 8 ? 8 : RAWS / 2;             // copied pieces of V in flight
+  static constexpr int NRK = RAWS - NRV > 8 ? 8 : RAWS - NRV;         // and of K
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + NT * Q_BYTES;
   static constexpr int OFF_V = OFF_K + NK * T_BYTES;
@@ -99,37 +103,30 @@ struct ExtendShape {
   static constexpr int OFF_SC = OFF_MISC;              // [2] batches of scales
   static constexpr int SC_BYTES = 3 * 128 + 4 * NB + 16;  // kq, log2 vs, factor [32]; zero mask [NB]; vr, far
   static constexpr int OFF_FRAG = OFF_SC + 2 * SC_BYTES;
-  static constexpr int OFF_LSE = OFF_FRAG + NF * 64;   // [128] sums of the parts of a row, in two parts (CS > 1)
-  static constexpr int OFF_BAR = OFF_LSE + (CS > 1 ? 1024 : 0);
+  static constexpr int OFF_BAR = OFF_FRAG + NF * 64;
   static constexpr int B_RKF = 0, B_RKE = B_RKF + NRK, B_RVF = B_RKE + NRK, B_RVE = B_RVF + NRV, B_KF = B_RVE + NRV,
                        B_KE = B_KF + NK, B_VF = B_KE + NK, B_VE = B_VF + NV, B_SCF = B_VE + NV, B_SCE = B_SCF + 2,
-                       B_QF = B_SCE + 2, B_SF = B_QF + 2, B_SR = B_SF + 2, B_PF = B_SR + 2, B_OD = B_PF + 2, B_FF = B_OD + 2,
-                       B_FE = B_FF + NF, B_GS = B_FE + NF, B_DR = B_GS + 1, N_BAR = B_DR + 1;
+                       B_QF = B_SCE + 2, B_SF = B_QF + 2, B_PF = B_SF + 2, B_OF = B_PF + 4, B_OD = B_OF + 2,
+                       B_FF = B_OD + 2, B_FE = B_FF + NF, B_DR = B_FE + NF, N_BAR = B_DR + 2;
   static constexpr int OFF_WORDS = OFF_BAR + 8 * N_BAR;  // TMEM address, failed, flag
   static constexpr int SMEM_BYTES = OFF_WORDS + 16 + 1024;
-  static constexpr int TM_S = 0;       // + x KT, x the row tile or the buffer
-  static constexpr int TM_O = 2 * KT;  // + x D
-  static constexpr bool SEP = NT == 2 && D < 128;            // P in columns of its own
-  static constexpr int TM_P = SEP ? TM_O + NT * D : TM_S;    // + x KT / 2, or where S is
-  static constexpr int TMEM_COLS = TM_O + NT * D + (SEP ? KT : 0) <= 256 ? 256 : 512;
-  // Softmax warps, and the warps that widen K and V.
-  static constexpr int SW = 4 * NT;
-  static constexpr int CK = NT == 2 ? 2 : 4, CV = CK;
-  static constexpr int REG_SOFTMAX = NT == 2 ? 192 : 216;
-  static constexpr int REG_WIDEN = NT == 2 ? 80 : 104;
-  static constexpr int REG_REST = NT == 2 ? 48 : 88;
-  static constexpr int REGS = NT == 2 ? 2 * REG_SOFTMAX + REG_WIDEN + REG_REST : REG_SOFTMAX + 2 * REG_WIDEN + REG_REST;
-  static constexpr int PEN = 3;
-  static_assert(NT == 1 || (CS == 1 && 2 * KT + 2 * D <= 512), "two row tiles");
-  static_assert(TM_O + NT * D + (SEP ? KT : 0) <= 512, "tensor memory");
-  static_assert(NRV >= 1 && NRK >= 1 && NRK >= NRV, "cached tiles in flight");
-  static_assert(OFF_WORDS + 16 - OFF_MISC <= MISC, "the small things' shared memory");
-  static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static constexpr int TM_S = 0;         // + x KT, x the stream
+  static constexpr int TM_O = NS * KT;   // + x D
+  static constexpr int TMEM_COLS = TM_O + NS * D <= 256 ? 256 : 512;
+  static constexpr int SW = 4 * NS;      // softmax warps
+  static constexpr int WC = NS == 2 ? 2 : 4;  // warps that widen K, and as many V
+  static constexpr int REG_SOFTMAX = 200, REG_WIDEN = NS == 2 ? 64 : 112, REG_ISSUE = NS == 2 ? 48 : 88;
+  // Tiles that an item's beginning is charged with.
+  static constexpr int PEN = NT == 2 ? 3 : 4;
+  static_assert(NT <= NS, "a row tile needs a stream");
+  static_assert(TM_O + NS * D <= 512, "tensor memory");
+  static_assert(NRV >= 1 && NRK >= NRV && NB * RPT == 8, "copied pieces in flight");
+  static_assert(OFF_WORDS + 16 - OFF_MISC <= MISC && SMEM_BYTES <= 232448, "shared memory budget");
   static_assert(OFF_FRAG % 16 == 0 && OFF_BAR % 8 == 0 && SC_BYTES % 16 == 0 && OFF_MISC % 16 == 0, "alignment");
-  static_assert(REGS * 128 <= 65536, "register split");
+  static_assert((NS * REG_SOFTMAX + (3 - NS) * REG_WIDEN + REG_ISSUE) * 128 <= EXTEND_THREADS * 128, "register split");
 };
 
-// One fragment, as warp 15 leaves it for the other warps (16 words).
+// One fragment, as warp 13 leaves it for the other warps (16 words).
 struct ExtendFrag {
   int kind;         // 1 a fragment, 0 the end
   int b, kvh;
@@ -150,108 +147,100 @@ __device__ __forceinline__ int extend_new(const ExtendPagedParams& p, int b, int
 }
 
 // Walks a CTA's share of the flattened tiles fragment by fragment (one warp; all lanes hold the same).
+// Positions run over requests, items of a request and KV heads, in that order; a KV head's item takes PEN
+// positions and one per key tile. The host keeps them below 2^31.
 template <typename S>
 struct ExtendWalk {
-  long long cur, hi, base, per;  // base: position of the current item's beginning
-  int b, kvh, item, past, len, items;
-  // Key tiles of an item's rows up to `row` of (b, kvh).
-  __device__ __forceinline__ static int tiles(const ExtendPagedParams& p, int past, int row) { return (past + row / p.G) / S::KT + 1; }
-  __device__ __forceinline__ static int item_tiles(const ExtendPagedParams& p, int past, int n, int i) {
-    return tiles(p, past, min(n * p.G, (i + 1) * S::RP) - 1);
-  }
-  __device__ __forceinline__ static int items_of(const ExtendPagedParams& p, int n) { return (n * p.G + S::RP - 1) / S::RP; }
-  // Positions of one KV head of request b (a lane's own b).
-  __device__ __forceinline__ static int span(const ExtendPagedParams& p, int b) {
+  int cur, hi, base, per, grid;  // base: position of the current item's beginning
+  int b, kvh, item, past, len, items, cost;
+  // Key tiles of rows up to `row` of (b, kvh).
+  __device__ __forceinline__ static int tiles(const ExtendPagedParams& p, int past, int row) { return (past + small_div(row, p.G)) / S::KT + 1; }
+  // Positions of an item of request b for one KV head; 0: the request has no such item.
+  __device__ __forceinline__ static int span(const ExtendPagedParams& p, int b, int item) {
     int past, len;
-    const int n = extend_new(p, b, past, len);
-    if (n <= 0) return 0;
-    int sum = 0;
-    const int k = items_of(p, n);
-    for (int i = 0; i < k; ++i) sum += item_tiles(p, past, n, i) + S::PEN;
-    return sum;
+    const int rows = max(extend_new(p, b, past, len), 0) * p.G;
+    return item * S::RP < rows ? tiles(p, past, min(rows, (item + 1) * S::RP) - 1) + S::PEN : 0;
   }
+  // The request's lengths, and the item's cost.
   __device__ __forceinline__ void enter(const ExtendPagedParams& p) {
-    const int n = extend_new(p, b, past, len);
-    items = n > 0 ? items_of(p, n) : 0;
+    const int rows = max(extend_new(p, b, past, len), 0) * p.G;
+    items = (rows + S::RP - 1) / S::RP;
   }
   __device__ __forceinline__ void init(const ExtendPagedParams& p, int lane) {
-    long long total = 0;
-    for (int i = lane; i < p.B; i += 32) total += span(p, i);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= p.Hkv;
-    const long long grid = gridDim.x;
-    per = (total + grid - 1) / grid;
-    cur = min(per * blockIdx.x, total);
-    hi = min(cur + per, total);
-    base = 0;
-    b = kvh = item = items = 0;
+    grid = static_cast<int>(gridDim.x);
+    const int most = p.items, pairs = p.B * most;  // items of a request with T new tokens; (request, item)
+    auto span_of = [&](int e) {
+      if (e >= pairs) return 0;
+      const int bb = most == 1 ? e : small_div(e, most);
+      return span(p, bb, e - bb * most);
+    };
+    const int span0 = span_of(lane);  // (most batches have no more)
+    int total = span0;
+    for (int e = 32 + lane; e < pairs; e += 32) total += span_of(e);
+    total = static_cast<int>(__reduce_add_sync(0xffffffffu, total)) * p.Hkv;
+    per = max((total + grid - 1) / grid, S::PEN);  // (no cuts so fine that joining costs more)
+    cur = static_cast<int>(min(static_cast<long long>(per) * blockIdx.x, static_cast<long long>(total)));
+    hi = min(total - cur, per) + cur;
+    base = b = kvh = item = items = 0;
     if (cur >= hi) return;
-    // The request that holds `cur`.
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const long long own = b0 + lane < p.B ? static_cast<long long>(span(p, b0 + lane)) * p.Hkv : 0;
-      long long in = own;
+    // The item that holds `cur`.
+    for (int e0 = 0; e0 < pairs; e0 += 32) {
+      const int own = e0 == 0 ? span0 : span_of(e0 + lane);
+      int in = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, in, o);
+        const int t = __shfl_up_sync(0xffffffffu, in, o);
         if (lane >= o) in += t;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, cur < base + in);
+      const unsigned hit = __ballot_sync(0xffffffffu, cur - base < in * p.Hkv);
       if (hit) {
         const int l = __ffs(static_cast<int>(hit)) - 1;
-        b = b0 + l;
-        base += __shfl_sync(0xffffffffu, in - own, l);
-        const long long one = __shfl_sync(0xffffffffu, own, l) / p.Hkv;
-        kvh = static_cast<int>((cur - base) / one);
-        base += kvh * one;
+        cost = __shfl_sync(0xffffffffu, own, l);
+        b = most == 1 ? e0 + l : small_div(e0 + l, most);
+        item = e0 + l - b * most;
+        base += __shfl_sync(0xffffffffu, in - own, l) * p.Hkv;
+        kvh = small_div(cur - base, cost);
+        base += kvh * cost;
         break;
       }
-      base += __shfl_sync(0xffffffffu, in, 31);
+      base += __shfl_sync(0xffffffffu, in, 31) * p.Hkv;
     }
     enter(p);
-    while (true) {
-      const int cost = item_tiles(p, past, len - past, item) + S::PEN;
-      if (cur < base + cost) break;
-      base += cost;
-      ++item;
-    }
   }
   __device__ __forceinline__ bool next(const ExtendPagedParams& p, ExtendFrag& f) {
     while (true) {
       if (cur >= hi) return false;
-      while (item >= items) {  // on to the next KV head, or the next request that has items
-        item = 0;
-        if (items == 0 || ++kvh == p.Hkv) {
-          kvh = 0;
-          ++b;
-          enter(p);
-        }
-      }
-      const int n = len - past;
-      const int nk = item_tiles(p, past, n, item);
-      const long long first = base + S::PEN, end = first + nk;
-      const int j0 = static_cast<int>(max(cur - first, 0LL));
-      const int j1 = static_cast<int>(min(hi, end) - first);
+      const int first = base + S::PEN, end = base + cost;
+      const int j0 = max(cur - first, 0), j1 = min(hi, end) - first;
       cur = min(hi, end);
       if (j1 > 0) {
         f.kind = 1;
         f.b = b;
         f.kvh = kvh;
         f.row0 = item * S::RP;
-        f.rows = min(n * p.G - f.row0, S::RP);
+        f.rows = min((len - past) * p.G - f.row0, S::RP);
         f.past = past;
         f.len = len;
         f.j0 = j0;
         f.j1 = j1;
-        f.nk0 = tiles(p, past, f.row0 + min(f.rows, S::R) - 1);
-        f.nk1 = f.rows > S::R ? nk : 0;
-        f.c0 = static_cast<int>(first / per);
-        f.nf = static_cast<int>((end - 1) / per) - f.c0 + 1;
+        f.nk0 = tiles(p, past, f.row0 + min(f.rows, 128) - 1);
+        f.nk1 = f.rows > 128 ? end - first : 0;
+        f.c0 = small_div(first, per);
+        f.nf = small_div(end - 1, per) - f.c0 + 1;
         f.slot = 2 * static_cast<int>(blockIdx.x) + (j0 > 0 ? 0 : 1);
       }
-      if (cur == end) {
+      if (cur == end && cur < hi) {
         base = end;
-        ++item;
+        if (++kvh == p.Hkv) {
+          kvh = 0;
+          ++item;
+          while (item >= items) {  // the next request that has any (there is one: cur < hi)
+            item = 0;
+            ++b;
+            enter(p);
+          }
+          cost = span(p, b, item);
+        }
       }
       if (j1 > 0) return true;
     }
@@ -281,59 +270,97 @@ __device__ __forceinline__ void widen16(const uint4& x, uint4& lo, uint4& hi) {
   hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
-// One more part of a row's sum, y, beside those that `sum` counts relative to `top` (logarithms in two
-// parts; -inf: nothing); `share` is the caller's own part relative to `top`, y if `mine`.
-__device__ __forceinline__ void join_sums(float2& top, float& sum, float& share, float2 y, bool mine) {
-  if (y.x == -INFINITY) return;
-  float scale = 1.f, w = 1.f;
-  if (top.x == -INFINITY) {
-    top = y;
+// Four consecutive columns of tensor memory.
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float* v) {
+  uint32_t r[4];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <int N>
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, float* v) {
+  if constexpr (N % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 16) tmem_ld16(taddr + i, v + i);
   } else {
-    const float d = (y.x - top.x) + (y.y - top.y);
-    if (d > 0.f) {
-      scale = exp2f(-d);
-      top = y;
-    } else {
-      w = exp2f(d);  // (NaN where one is)
-    }
+#pragma unroll
+    for (int i = 0; i < N; i += 4) tmem_ld4(taddr + i, v + i);
   }
-  sum = sum * scale + w;
-  share = mine ? w : share * scale;
 }
 
-template <int D, int NT, int CS>
+// A barrier of the softmax warps, and one that says whether `bad` is set in any of their threads.
+template <int THREADS>
+__device__ __forceinline__ void softmax_sync() {
+  asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ bool softmax_any(bool bad) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, 1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(bad)), "n"(THREADS)
+      : "memory");
+  return r != 0u;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// A bounded wait of few instructions: a number of suspended looks of up to 20 us each, after which the
+// site is left in `failed` for the CTA's end to report, and every later wait gives up at once.
+constexpr uint32_t EXTEND_LOOKS = 1u << 17;
+__device__ __forceinline__ bool extend_wait(uint32_t bar, uint32_t parity, volatile int* failed, int site) {
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+#pragma unroll 1
+  for (uint32_t i = 0; i < EXTEND_LOOKS; ++i) {
+    if (mbar_try_wait_sleep(bar, parity, DU_WAIT_SLEEP_NS)) return true;
+    if (*failed) return false;
+  }
+  *failed = site;
+  return false;
+}
+
+template <int D, int NT>
 __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const ExtendPagedParams p) {
-  using S = ExtendShape<D, NT, CS>;
-  constexpr int KT = S::KT, NC = S::NC, R = S::R, RP = S::RP, SPAN = S::SPAN, GPT = S::GPT, NB = S::NB;
+  using S = ExtendShape<D, NT>;
+  constexpr int KT = S::KT, RP = S::RP, SPAN = S::SPAN, GPT = S::GPT, NB = S::NB, NS = S::NS, RPT = S::RPT;
+  constexpr bool ALT = S::ALT;
   constexpr int NK = S::NK, NV = S::NV, NRK = S::NRK, NRV = S::NRV, NF = S::NF;
   constexpr uint32_t SWZ = swizzle_code(SPAN);
   constexpr uint32_t IDESC_QK = idesc_f16(128, KT, 0, 0, 0, 0);
   constexpr uint32_t IDESC_PV = idesc_f16(128, D, 0, 0, 0, 1);
+  // The products of one thread are known to complete in order if they are of one shape; else the end of
+  // P V is waited for before its P is overwritten by the next S.
+  constexpr bool ORDERED = D == KT;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
   const uint32_t sbase = (raw_u32 + 1023u) & ~1023u;
   uint8_t* sgen = smem_raw + (sbase - raw_u32);
   auto bar = [&](int i) -> uint32_t { return sbase + S::OFF_BAR + 8u * static_cast<uint32_t>(i); };
-  auto RKF = [&](int s) { return bar(S::B_RKF + s); };  // cached tile of K landed
+  auto RKF = [&](int s) { return bar(S::B_RKF + s); };  // cached piece of K landed
   auto RKE = [&](int s) { return bar(S::B_RKE + s); };  // and widened
   auto RVF = [&](int s) { return bar(S::B_RVF + s); };
   auto RVE = [&](int s) { return bar(S::B_RVE + s); };
   auto KF = [&](int s) { return bar(S::B_KF + s); };    // widened K written
-  auto KE = [&](int s) { return bar(S::B_KE + s); };    // and multiplied
+  auto KE = [&](int s) { return bar(S::B_KE + s); };    // and multiplied, by each stream that has it
   auto VF = [&](int s) { return bar(S::B_VF + s); };
   auto VE = [&](int s) { return bar(S::B_VE + s); };
   auto SCF = [&](int s) { return bar(S::B_SCF + s); };  // batch of scales written
   auto SCE = [&](int s) { return bar(S::B_SCE + s); };  // read by the softmax warps and those that widen V
   auto QF = [&](int x) { return bar(S::B_QF + x); };    // query rows written
-  auto SF = [&](int x) { return bar(S::B_SF + x); };    // S (of row tile x, or in buffer x) complete
-  auto SR = [&](int x) { return bar(S::B_SR + x); };    // S_x read (SEP)
-  auto PF = [&](int x) { return bar(S::B_PF + x); };    // P written
-  auto OD = [&](int x) { return bar(S::B_OD + x); };    // P V of a tile done; with P over two S: O_x final
+  auto SF = [&](int x) { return bar(S::B_SF + x); };    // S of stream x complete, and its O of the tile before
+  auto PF = [&](int x, int half) { return bar(S::B_PF + 2 * x + half); };  // half of P written
+  auto OD = [&](int x) { return bar(S::B_OD + x); };    // P V of a tile done (not ORDERED)
+  auto OF = [&](int x) { return bar(S::B_OF + x); };    // O of stream x final
   auto FF = [&](int i) { return bar(S::B_FF + i); };    // fragment entry written
-  auto FE = [&](int i) { return bar(S::B_FE + i); };    // and read by every warp but the walker
-  const uint32_t BAR_GS = bar(S::B_GS);                 // the softmax warps among themselves
-  const uint32_t BAR_DR = bar(S::B_DR);
+  auto FE = [&](int i) { return bar(S::B_FE + i); };    // and read by every warp that takes it
+  auto DR = [&](int i) { return bar(S::B_DR + i); };    // all products of an issuing warp done
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(sgen + S::OFF_WORDS);
@@ -344,35 +371,35 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
   if (tid == 0) {
     for (int s = 0; s < NRK; ++s) {
       mbar_init(RKF(s), 1);
-      mbar_init(RKE(s), S::CK);
+      mbar_init(RKE(s), S::WC);
     }
     for (int s = 0; s < NRV; ++s) {
       mbar_init(RVF(s), 1);
-      mbar_init(RVE(s), S::CV);
+      mbar_init(RVE(s), S::WC);
     }
     for (int s = 0; s < NK; ++s) {
-      mbar_init(KF(s), S::CK);
-      mbar_init(KE(s), 1);
+      mbar_init(KF(s), S::WC);
+      mbar_init(KE(s), NT);
     }
     for (int s = 0; s < NV; ++s) {
-      mbar_init(VF(s), S::CV);
-      mbar_init(VE(s), 1);
+      mbar_init(VF(s), S::WC);
+      mbar_init(VE(s), NT);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(SCF(s), 1);
-      mbar_init(SCE(s), S::SW + S::CV);
-      mbar_init(QF(s), 4);
+      mbar_init(SCE(s), S::SW + S::WC);
+      mbar_init(QF(s), ALT ? 8 : 4);
       mbar_init(SF(s), 1);
-      mbar_init(SR(s), 4);
-      mbar_init(PF(s), 4);
+      mbar_init(PF(s, 0), 4);
+      mbar_init(PF(s, 1), 4);
       mbar_init(OD(s), 1);
+      mbar_init(OF(s), 1);
+      mbar_init(DR(s), 1);
     }
     for (int s = 0; s < NF; ++s) {
       mbar_init(FF(s), 1);
-      mbar_init(FE(s), 15);
+      mbar_init(FE(s), S::SW + 2 * S::WC + 1 + NS);
     }
-    mbar_init(BAR_GS, S::SW);
-    mbar_init(BAR_DR, 1);
     *failed = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
@@ -388,15 +415,14 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // The next fragment, for every warp but the walker; kind 0: none (or a wait expired).
+  // The next fragment; kind 0: there is none, -1: a wait expired.
   int n_frag = 0;
   auto take = [&]() -> ExtendFrag {
     ExtendFrag f;
     const int s = n_frag % NF;
-    bool ok = mbar_wait(FF(s), (n_frag / NF) & 1, failed, 500);
-    ok = __all_sync(0xffffffffu, ok);
+    const bool ok = __all_sync(0xffffffffu, extend_wait(FF(s), (n_frag / NF) & 1, failed, 500));
     const volatile int* e = frags + 16 * s;
-    f.kind = ok ? e[0] : 0;
+    f.kind = ok ? e[0] : -1;
     f.b = e[1];
     f.kvh = e[2];
     f.row0 = e[3];
@@ -415,101 +441,137 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     ++n_frag;
     return f;
   };
+  // Key tiles of a fragment that stream x has.
+  auto tiles_of = [&](const ExtendFrag& f, int x) -> int {
+    const int nt = f.j1 - f.j0;
+    if (ALT) return (nt - x + 1) >> 1;
+    return max(0, min(f.j1, x ? f.nk1 : f.nk0) - f.j0);
+  };
 
   if (warp < S::SW) {
     // ------------------------------------------------------------------ softmax
     regs_inc<S::REG_SOFTMAX>();
-    const int x = warp >> 2, w4 = warp & 3;
-    const int lane128 = 32 * w4 + lane;   // TMEM lane
-    const int row = lane128 % R;          // row of the tile
-    const int col0 = (lane128 / R) * NC;  // first column of a key tile that this thread takes
+    const int x = warp >> 2, w4 = warp & 3;  // stream
+    const int xr = ALT ? 0 : x;              // row tile
+    const int row = 32 * w4 + lane;          // row of the tile = TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>(w4 * 32) << 16;
-    const uint32_t q_tile = sbase + S::OFF_Q + x * S::Q_BYTES;
-    const int stid = tid;                 // thread among the softmax warps
-    constexpr int ST = 32 * S::SW;
-    int n_tile = 0, n_batch = 0, n_of = 0, n_gs = 0;
-    auto group_sync = [&]() -> bool {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(BAR_GS);
-      const bool w = mbar_wait(BAR_GS, n_gs++ & 1, failed, 501);
-      return __all_sync(0xffffffffu, w);
-    };
-    bool ok = true;
-    while (ok) {
+    const uint32_t q_tile = sbase + S::OFF_Q + xr * S::Q_BYTES;
+    const uint32_t s_addr = tmem + lane_off + S::TM_S + x * KT, o_addr = tmem + lane_off + S::TM_O + x * D;
+    constexpr int ST = 32 * S::SW;           // softmax threads
+    int n_tile = 0, n_batch = 0, n_of = 0;
+    while (true) {
       const ExtendFrag f = take();
-      if (f.kind == 0) break;
-      const int nt = f.j1 - f.j0;                                     // key tiles of the fragment
-      const int n = max(0, min(f.j1, x ? f.nk1 : f.nk0) - f.j0);      // and of this row tile
-      const int r_item = x * R + row;                                 // row of the item
+      if (f.kind <= 0) {
+        softmax_any<ST>(f.kind < 0);
+        break;
+      }
+      const int nt = f.j1 - f.j0, n = tiles_of(f, x);
+      const int r_item = xr * 128 + row;                               // row of the item
       const bool row_ok = r_item < f.rows;
       const int r_all = f.row0 + min(r_item, f.rows - 1);
-      const int t = r_all / p.G;                                      // its token and head
+      const int t = small_div(r_all, p.G);                             // its token and head
       const int h = f.kvh * p.G + (r_all - t * p.G);
       const long long q_row = (static_cast<long long>(f.b) * p.Hq + h) * p.T + t;
-      const int kmax = f.past + t;                                    // the last key that it sees
-      const int kmin = f.past + (f.row0 + x * R) / p.G;               // that every row of the tile sees
+      const int kmax = f.past + t;                                     // the last key that it sees
+      const int kmin = f.past + small_div(f.row0 + min(xr * 128, f.rows - 1), p.G);  // that every row of the tile sees
+      const bool warp_rows = xr * 128 + 32 * w4 < f.rows;              // some row of the warp is one
       float qs = 0.f;  // the row's factor
-      if (n > 0) {
+      bool ok = true;
+      if (ALT || n > 0) {
         // The query row: rotated in fp32, times a power of two that brings its largest input to
-        // [2^8, 2^9), as fp16.
+        // [2^8, 2^9), as fp16. (Streams that share the rows rotate half of a row each.)
+        constexpr int PQ = ALT && D >= 32 ? D / 32 : D / 16;  // pairs of 16-byte pieces of this thread
+        constexpr int PL = PQ < 2 ? PQ : 2;                   // at a time (more would be code fetched once)
         const uint8_t* src = static_cast<const uint8_t*>(p.q) + q_row * (2 * D);
+        const int c0 = ALT && D >= 32 ? x * PQ : 0;
         const uint8_t* cp = static_cast<const uint8_t*>(p.cos) + static_cast<long long>(kmax) * D;
         const uint8_t* sp = static_cast<const uint8_t*>(p.sin) + static_cast<long long>(kmax) * D;
-        uint4 v[D / 8];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) v[i] = ldg_v4(src + 16 * i);
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = __vmaxu2(top, u[k] & 0x7fff7fffu);
-        }
-        const float2 tops = p.bf16 ? split2<true>(top) : split2<false>(top);
-        const uint32_t top_bits = __float_as_uint(fmaxf(tops.x, tops.y));
-        int e = static_cast<int>(top_bits >> 23) - 127;
-        if (e == -127 || e == 128) e = 8;  // (zero, or not finite)
-        e = min(max(e - 8, -100), 100);
-        const float up = __int_as_float((127 - e) << 23);
-        qs = __int_as_float((127 + e) << 23);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint4 c = ldg_v4(cp + 16 * i), s = ldg_v4(sp + 16 * i);
-          const uint4 a = v[i], b = v[i + D / 16];
-          const uint32_t ca[4] = {c.x, c.y, c.z, c.w}, sa[4] = {s.x, s.y, s.z, s.w};
-          const uint32_t aa[4] = {a.x, a.y, a.z, a.w}, ba[4] = {b.x, b.y, b.z, b.w};
-          uint32_t lo[4], hi[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 fc = p.bf16 ? split2<true>(ca[k]) : split2<false>(ca[k]);
-            const float2 fs = p.bf16 ? split2<true>(sa[k]) : split2<false>(sa[k]);
-            float2 fa = p.bf16 ? split2<true>(aa[k]) : split2<false>(aa[k]);
-            float2 fb = p.bf16 ? split2<true>(ba[k]) : split2<false>(ba[k]);
-            fa.x *= up;
-            fa.y *= up;
-            fb.x *= up;
-            fb.y *= up;
-            lo[k] = pack2<false>(fa.x * fc.x - fb.x * fs.x, fa.y * fc.y - fb.y * fs.y);
-            hi[k] = pack2<false>(fb.x * fc.x + fa.x * fs.x, fb.y * fc.y + fa.y * fs.y);
+        if (warp_rows) {
+          for (int i = 0; i < D; i += 128) {
+            prefetch_l1(cp + i);
+            prefetch_l1(sp + i);
           }
-          st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, lane128, i), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-          st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, lane128, i + D / 16), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          // The row's pieces, this thread's first; they wait in their places for their rotation.
+          uint32_t top = 0u;
+          uint4 v[D / 8];
+#pragma unroll
+          for (int i = 0; i < PQ; ++i) {
+            v[i] = ldg_v4(src + 16 * (c0 + i));
+            v[PQ + i] = ldg_v4(src + 16 * (c0 + i + D / 16));
+          }
+          if constexpr (2 * PQ < D / 8) {
+#pragma unroll
+            for (int i = 0; i < PQ; ++i) {
+              v[2 * PQ + i] = ldg_v4(src + 16 * (PQ - c0 + i));
+              v[3 * PQ + i] = ldg_v4(src + 16 * (PQ - c0 + i + D / 16));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+          if (!(ALT && D < 32) || x == 0) {
+#pragma unroll
+            for (int i = 0; i < PQ; ++i) {
+              st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, c0 + i), v[i]);
+              st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, c0 + i + D / 16), v[PQ + i]);
+            }
+          }
+          const float2 tops = p.bf16 ? split2<true>(top) : split2<false>(top);
+          const uint32_t top_bits = __float_as_uint(fmaxf(tops.x, tops.y));
+          int e = static_cast<int>(top_bits >> 23) - 127;
+          if (e == -127 || e == 128) e = 8;  // (zero, or not finite)
+          e = min(max(e - 8, -100), 100);
+          const float up = __int_as_float((127 - e) << 23);
+          qs = __int_as_float((127 + e) << 23);
+          auto rotate = [&](auto bf16) {
+            constexpr bool BF = decltype(bf16)::value;
+#pragma unroll 1
+            for (int i0 = c0; i0 < c0 + PQ; i0 += PL) {
+              uint4 a[PL], b[PL], c[PL], s[PL];
+#pragma unroll
+              for (int i = 0; i < PL; ++i) {
+                a[i] = ld_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i));
+                b[i] = ld_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i + D / 16));
+                c[i] = ldg_v4(cp + 16 * (i0 + i));
+                s[i] = ldg_v4(sp + 16 * (i0 + i));
+              }
+#pragma unroll
+              for (int i = 0; i < PL; ++i) {
+                const uint32_t aa[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, ba[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+                const uint32_t ca[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, sa[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+                uint32_t lo[4], hi[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint64_t U = f2(up, up), C = widen2<BF>(ca[k]), N = widen2<BF>(sa[k]);
+                  const uint64_t A = f2_mul(widen2<BF>(aa[k]), U), B = f2_mul(widen2<BF>(ba[k]), U);
+                  const float2 l2 = f2_split(f2_fma(B, f2_mul(N, f2(-1.f, -1.f)), f2_mul(A, C))), h2 = f2_split(f2_fma(A, N, f2_mul(B, C)));
+                  lo[k] = pack2<false>(l2.x, l2.y);
+                  hi[k] = pack2<false>(h2.x, h2.y);
+                }
+                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i + D / 16), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+              }
+            }
+          };
+          if (!(ALT && D < 32) || x == 0) {
+            if (p.bf16) rotate(std::true_type{});
+            else rotate(std::false_type{});
+          }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(QF(x));
+        if (lane == 0) mbar_arrive(QF(xr));
       }
-      const uint32_t o_addr = tmem + lane_off + S::TM_O + x * D;
       // The reference of the weights is m + mlo (log2 domain); mlo is 0 but for references so large that
-      // a sum with log2 vs would round away. l: the sum of 2^(s + vr - m - mlo + 11), with `far` of
+      // a sum with log2 vs would round away. l: the sum of 2^(s + vr - m - mlo + 8), with `far` of
       // 2^(s - m - eo).
       float m = -INFINITY, mlo = 0.f, l = 0.f, eo = -INFINITY, vr = 0.f;
       bool far = false;
-      for (int jj = 0; ok && jj < nt; ++jj) {
+      for (int jj = 0; jj < nt; ++jj) {
         const int bs = n_batch & 1;
         const uint8_t* sc = sgen + S::OFF_SC + bs * S::SC_BYTES;
         if (jj % NB == 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(SCF(bs), (n_batch >> 1) & 1, failed, 502));
+          ok = __all_sync(0xffffffffu, extend_wait(SCF(bs), (n_batch >> 1) & 1, failed, 502));
           if (!ok) break;
           const bool now = *reinterpret_cast<const int*>(sc + 384 + 4 * NB + 4) != 0;
           if (jj == 0) vr = *reinterpret_cast<const float*>(sc + 384 + 4 * NB);
@@ -518,176 +580,155 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
             eo = l == 0.f ? -INFINITY : mlo - EXTEND_TOP - vr;
           }
         }
-        if (jj < n) {
-          const int sb = NT == 2 ? x : n_tile & 1;
-          const uint32_t s_addr = tmem + lane_off + S::TM_S + sb * KT;
-          const uint32_t p_addr = S::SEP ? tmem + lane_off + S::TM_P + x * (KT / 2) : s_addr;
-          ok = mbar_wait(SF(sb), (NT == 2 ? n_tile : n_tile >> 1) & 1, failed, 503);
-          ok = __all_sync(0xffffffffu, ok);
+        if (ALT ? (jj & 1) == x : jj < n) {
+          ok = __all_sync(0xffffffffu, extend_wait(SF(x), n_tile & 1, failed, 503));
           if (!ok) break;
           tc_fence_after();
-          float s[NC];
-          const int k0 = (f.j0 + jj) * KT + col0;
-          const bool diag = (f.j0 + jj) * KT + KT - 1 > kmin;  // some key of the tile is hidden from some row
+          const bool first = ALT ? jj < 2 : jj == 0;                 // this stream has no O yet
+          const int lim = kmax - (f.j0 + jj) * KT;                   // columns beyond it are hidden from this row
+          const bool diag = (f.j0 + jj) * KT + KT - 1 > kmin;        // some key of the tile is hidden from some row
+          const float* scq = reinterpret_cast<const float*>(sc) + (jj % NB) * GPT;  // (log2 vs 32 words behind, factors 64)
+          if (warp_rows) {
+            // S in two halves: the first is reduced while the second loads.
+            constexpr int HALF = KT / 2, NG = KT / 16;
+            float s[KT], kq[NG], ga[NG];
+            tmem_ldn<HALF>(s_addr, s);
 #pragma unroll
-          for (int c = 0; c < NC; c += 16) tmem_ld16(s_addr + col0 + c, s + c);
-          float kq[NC / 16], lv[NC / 16];
-          const int g0 = (jj % NB) * GPT + col0 / 16;
-#pragma unroll
-          for (int g = 0; g < NC / 16; ++g) {
-            kq[g] = reinterpret_cast<const float*>(sc)[g0 + g] * qs;
-            lv[g] = reinterpret_cast<const float*>(sc + 128)[g0 + g];
-          }
-          tmem_wait_ld();
-          if (diag) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-              if (k0 + c > kmax) s[c] = -INFINITY;
-          }
-          if constexpr (S::SEP) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(SR(x));  // S is in registers: the next one may overwrite it
-          }
-          float mx = -INFINITY, ga[NC / 16];
-#pragma unroll
-          for (int g = 0; g < NC / 16; ++g) {
-            float a = fmaxf(s[16 * g], s[16 * g + 1]), b = fmaxf(s[16 * g + 2], s[16 * g + 3]);
-#pragma unroll
-            for (int c = 4; c < 16; c += 4) {
-              a = max3(a, s[16 * g + c], s[16 * g + c + 1]);
-              b = max3(b, s[16 * g + c + 2], s[16 * g + c + 3]);
+            for (int g = 0; g < NG; g += 4) {
+              const float4 a4 = *reinterpret_cast<const float4*>(scq + g);
+              kq[g] = a4.x * qs;
+              kq[g + 1] = a4.y * qs;
+              kq[g + 2] = a4.z * qs;
+              kq[g + 3] = a4.w * qs;
             }
-            ga[g] = fmaxf(a, b);
-            mx = fmaxf(mx, fmaf(ga[g], kq[g], lv[g]));
-          }
-          const float m_old = m, mlo_old = mlo;
-          bool moved = mx > m + mlo + EXTEND_MOVE;
-          float base = 0.f;  // what is subtracted from log2 vs
-          const bool large = (fabsf(m) > EXTEND_LARGE && m != -INFINITY) || (fabsf(mx) > EXTEND_LARGE && mx != -INFINITY);
-          if (!far && !__any_sync(0xffffffffu, large)) {
-            if (moved) {
-              m = mx;
-              mlo = 0.f;
-            }
-            if (m != -INFINITY) base = m + mlo;
-          } else {
-            // Scores relative to the reference first, then the rest: nothing is rounded away beside a
-            // large score. The product is rounded before the difference is taken, so that scores that are
-            // alike have the same weight whatever their size.
-            auto less = [](float a, float k, float r) { return __fadd_rn(__fmul_rn(a, k), -r); };
-            float hi = -INFINITY, lo = -INFINITY;
+            float mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < NC / 16; ++g) hi = fmaxf(hi, ga[g] * kq[g]);
-            const float h0 = hi == -INFINITY ? 0.f : hi;
-#pragma unroll
-            for (int g = 0; g < NC / 16; ++g) lo = fmaxf(lo, less(ga[g], kq[g], h0) + lv[g]);
-            moved = m == -INFINITY ? hi != -INFINITY : (hi - m) + (lo - mlo) > EXTEND_MOVE;
-            if (moved) {
-              m = hi;
-              mlo = lo;
-            }
-            const float mr = m == -INFINITY ? 0.f : m;
-            base = m == -INFINITY ? 0.f : mlo;
-            float es = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < NC / 16; ++g) es = fmaxf(es, less(ga[g], kq[g], mr));
-#pragma unroll
-            for (int c = 0; c < NC; ++c) s[c] = less(s[c], kq[c / 16], mr);
-#pragma unroll
-            for (int g = 0; g < NC / 16; ++g) kq[g] = 1.f;
-            if (far) {
-              // value scales far apart: the sum has a reference of its own
-              if (moved && m_old != -INFINITY) eo += m_old - m;
-              const float en = fmaxf(l == 0.f ? -INFINITY : eo, es), e0 = en == -INFINITY ? 0.f : en;
-              l = l == 0.f ? 0.f : l * exp2f(eo - e0);
-              eo = en;
-#pragma unroll
-              for (int c = 0; c < NC; ++c) {
-                const float w = exp2f(s[c] - e0);
-                if (!diag || k0 + c <= kmax) l += w;
-              }
-            }
-          }
-          uint64_t acc = f2(0.f, 0.f);
-          uint32_t pk[NC / 2];
-#pragma unroll
-          for (int g = 0; g < NC / 16; ++g) {
-            const float add = lv[g] - base + EXTEND_TOP;
-            const uint64_t A = f2(add, add), K = f2(kq[g], kq[g]);
-            uint64_t sum = f2(0.f, 0.f);
-#pragma unroll
-            for (int c = 16 * g; c < 16 * g + 16; c += 2) {
-              const float2 xx = f2_split(f2_fma(f2(s[c], s[c + 1]), K, A));
-              float2 pp = make_float2(ex2(xx.x), ex2(xx.y));
-              if (diag) {
-                if (k0 + c > kmax) pp.x = 0.f;
-                if (k0 + c + 1 > kmax) pp.y = 0.f;
-              }
-              sum = f2_add(sum, f2(pp.x, pp.y));
-              pk[c / 2] = pack2<false>(pp.x, pp.y);
-            }
-            const float iv = reinterpret_cast<const float*>(sc + 256)[g0 + g];
-            acc = f2_fma(sum, f2(iv, iv), acc);
-          }
-          if ((NT == 1 || S::SEP) && jj > 0) {
-            // The product before must be done with O, and with P where that is not over S. (Waited for in
-            // every tile: a parity tells only two phases apart.)
-            ok = __all_sync(0xffffffffu, mbar_wait(OD(x), (n_tile - 1) & 1, failed, 504));
-            if (!ok) break;
-            tc_fence_after();
-          }
-          if (jj > 0 && __any_sync(0xffffffffu, moved)) {
-            const float alpha = moved && m_old != -INFINITY ? ex2((m_old - m) + (mlo_old - mlo)) : 1.0f;
-            if (!far) l *= alpha;
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-              float o[16];
-              tmem_ld16(o_addr + c, o);
+            for (int c0 = 0; c0 < KT; c0 += HALF) {
               tmem_wait_ld();
+              if (c0 == 0) tmem_ldn<HALF>(s_addr + HALF, s + HALF);
+              if (__builtin_expect(diag, 0)) {
+                // Hidden keys have a score of -inf, and where a whole group is hidden its scales do not count.
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] *= alpha;
-              tmem_st16(o_addr + c, o);
-            }
-          }
-          if (!far) {
-            const float2 rs = f2_split(acc);
-            l += rs.x + rs.y;
-          }
-          if constexpr (CS == 1) {
+                for (int c = c0; c < c0 + HALF; ++c)
+                  if (c > lim) s[c] = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < NC / 2; c += 16) tmem_st16u(p_addr + c, pk + c);
-          } else {
-            // this thread's columns of P, zeros in the others
-            uint32_t z[16];
+                for (int g = c0 / 16; g < (c0 + HALF) / 16; ++g)
+                  if (kq[g] == 0.f || 16 * g > lim) kq[g] = FLT_MIN;  // (times -inf it has to be -inf)
+              }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) z[i] = 0u;
-            if constexpr (NC >= 32) {
+              for (int g = c0 / 16; g < (c0 + HALF) / 16; ++g) {
+                float a = fmaxf(s[16 * g], s[16 * g + 1]), b = fmaxf(s[16 * g + 2], s[16 * g + 3]);
 #pragma unroll
-              for (int c = 0; c < KT / 2; c += 16) {
-                const int mine = c - col0 / 2;
-                if (mine >= 0 && mine < NC / 2) {
-                  if constexpr (NC == 32) tmem_st16u(p_addr + c, pk);
-                  else if (mine == 0) tmem_st16u(p_addr + c, pk);
-                  else tmem_st16u(p_addr + c, pk + 16);
-                } else {
-                  tmem_st16u(p_addr + c, z);
+                for (int c = 16 * g + 4; c < 16 * g + 16; c += 4) {
+                  a = max3(a, s[c], s[c + 1]);
+                  b = max3(b, s[c + 2], s[c + 3]);
                 }
-              }
-            } else {  // (NC = 16: eight columns)
-#pragma unroll
-              for (int c = 0; c < KT / 2; c += 16) {
-                uint32_t y[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = (c + i) / 8 == col0 / 16 ? pk[i % 8] : 0u;
-                tmem_st16u(p_addr + c, y);
+                ga[g] = fmaxf(a, b);
+                mx = fmaxf(mx, fmaf(ga[g], kq[g], scq[32 + g]));
               }
             }
+            const float m_old = m, mlo_old = mlo;
+            bool moved = mx > m + mlo + EXTEND_MOVE;
+            float base = 0.f;  // what is taken off log2 vs
+            // (infinities: a row without keys so far, or one that will be NaN)
+            const bool large = (fabsf(m) > EXTEND_LARGE && fabsf(m) < INFINITY) || (fabsf(mx) > EXTEND_LARGE && fabsf(mx) < INFINITY);
+            const bool any = far || __any_sync(0xffffffffu, moved || large);
+            if (__builtin_expect(!any || (!far && !__any_sync(0xffffffffu, large)), 1)) {
+              if (moved) {
+                m = mx;
+                mlo = 0.f;
+              }
+              if (m != -INFINITY) base = m + mlo;
+            } else {
+              // Scores relative to the reference first, then the rest: nothing is rounded away beside a
+              // large score. The product is rounded before the reference is taken off, so that scores that are
+              // alike have the same weight whatever their size.
+              auto less = [](float a, float k, float r) { return __fadd_rn(__fmul_rn(a, k), -r); };
+              float hi = -INFINITY, lo = -INFINITY;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) hi = fmaxf(hi, ga[g] * kq[g]);
+              const float h0 = hi == -INFINITY ? 0.f : hi;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) lo = fmaxf(lo, less(ga[g], kq[g], h0) + scq[32 + g]);
+              moved = m == -INFINITY ? hi != -INFINITY : (hi - m) + (lo - mlo) > EXTEND_MOVE;
+              if (moved) {
+                m = hi;
+                mlo = lo;
+              }
+              const float mr = m == -INFINITY ? 0.f : m;
+              base = m == -INFINITY ? 0.f : mlo;
+#pragma unroll
+              for (int c = 0; c < KT; ++c) s[c] = less(s[c], kq[c / 16], mr);
+#pragma unroll
+              for (int g = 0; g < NG; ++g) kq[g] = 1.f;
+              if (far) {
+                // Value scales far apart: the sum has a reference of its own, eo beyond m.
+                if (moved && m_old != -INFINITY) eo += m_old - m;
+                const float en = fmaxf(l == 0.f ? -INFINITY : eo, hi == -INFINITY ? -INFINITY : hi - mr);
+                const float e0 = en == -INFINITY ? 0.f : en;
+                l = l == 0.f ? 0.f : l * ex2(eo - e0);
+                eo = en;
+#pragma unroll
+                for (int c = 0; c < KT; ++c) l += ex2(s[c] - e0);
+              }
+            }
+            if (__builtin_expect(any && !first && __any_sync(0xffffffffu, moved), 0)) {
+              // (S being there says that O has the products of the tiles before)
+              const float alpha = moved && m_old != -INFINITY ? ex2((m_old - m) + (mlo_old - mlo)) : 1.0f;
+              if (!far) l *= alpha;
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                tmem_ld16(o_addr + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] *= alpha;
+                tmem_st16(o_addr + c, o);
+              }
+            }
+            uint64_t acc = f2(0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < NG; g += 2) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int q = g; q < g + 2; ++q) {
+                // (a group that is hidden from the row has scores of -inf, whatever its scales)
+                float lv = scq[32 + q], iv = scq[64 + q];
+                if (__builtin_expect(diag, 0) && 16 * q > lim) {
+                  lv = vr;
+                  iv = 1.f;
+                }
+                const float add = lv - base + EXTEND_TOP;
+                const uint64_t A = f2(add, add), K = f2(kq[q], kq[q]);
+                uint64_t sum = f2(0.f, 0.f);
+#pragma unroll
+                for (int c = 16 * q; c < 16 * q + 16; c += 2) {
+                  const float2 xx = f2_split(f2_fma(f2(s[c], s[c + 1]), K, A));
+                  const float2 pp = make_float2(ex2(xx.x), ex2(xx.y));
+                  sum = f2_add(sum, f2(pp.x, pp.y));
+                  pk[c / 2 - 8 * g] = pack2<false>(pp.x, pp.y);
+                }
+                acc = f2_fma(sum, f2(iv, iv), acc);
+              }
+              tmem_st16u(s_addr + 8 * g, pk);
+              if (g + 2 == NG / 2) {
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(PF(x, 0));
+              }
+            }
+            if (!far) {
+              const float2 rs = f2_split(acc);
+              l += rs.x + rs.y;
+            }
+            tmem_wait_st();
+          } else if (lane == 0) {
+            mbar_arrive(PF(x, 0));
           }
-          tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(PF(sb));
+          if (lane == 0) mbar_arrive(PF(x, 1));
           ++n_tile;
         }
         if (jj % NB == NB - 1 || jj == nt - 1) {
@@ -696,157 +737,173 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           ++n_batch;
         }
       }
-      if (!ok) break;
-      if (n > 0) {
-        ok = mbar_wait(OD(x), (NT == 2 && !S::SEP ? n_of++ : n_tile - 1) & 1, failed, 505);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-      }
+      if (ok && n > 0) ok = __all_sync(0xffffffffu, extend_wait(OF(x), n_of++ & 1, failed, 505));
+      // Every softmax warp comes here once per fragment, whatever happened to it, and all go on or none.
+      if (softmax_any<ST>(!ok)) break;
+      tc_fence_after();
       // The log2 of the row's (or its part's) sum, in two parts; and what brings O to the fragment's output,
-      // O 2^(m + mlo - 11) over the sum, in two factors since the exponent may be large.
-      const float2 lse = l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m, lg2(l) + (far ? eo : mlo - EXTEND_TOP - vr));
+      // O 2^(m + mlo - 8) over the sum, in two factors since the exponent may be large.
+      float2 lse = l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m, lg2(l) + (far ? eo : mlo - EXTEND_TOP - vr));
       float w1 = 0.f, w2 = 0.f;
       if (l != 0.f) {
         const float ex = far ? mlo - EXTEND_TOP - eo : vr, half = rintf(0.5f * ex);
-        w2 = exp2f(half);
-        w1 = exp2f(ex - half) / l;
+        w2 = ex2(half);
+        w1 = ex2(ex - half) / l;
       }
-      float* part_o = p.part;
+      float* part_o = p.part + (static_cast<long long>(f.slot) * RP + r_item) * D;
       float2* part_l = reinterpret_cast<float2*>(p.part + 2LL * gridDim.x * RP * D);
-      if constexpr (CS == 1) {
-        if (f.nf > 1 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = lse;
-        if (n > 0) {
-          float* dst = part_o + (static_cast<long long>(f.slot) * RP + r_item) * D;
-          uint8_t* out = static_cast<uint8_t*>(p.out) + q_row * (2 * D);
+      uint8_t* out = static_cast<uint8_t*>(p.out) + q_row * (2 * D);
+      // Four columns of the row from `col` on.
+      auto put = [&](int col, float4 a) {
+        if (f.nf > 1) {
+          *reinterpret_cast<float4*>(part_o + col) = a;
+        } else {
+          uint2 u;
+          u.x = p.bf16 ? pack2<true>(a.x, a.y) : pack2<false>(a.x, a.y);
+          u.y = p.bf16 ? pack2<true>(a.z, a.w) : pack2<false>(a.z, a.w);
+          *reinterpret_cast<uint2*>(out + 2 * col) = u;
+        }
+      };
+      if constexpr (ALT) {
+        // The two parts of a row joined: weights by their sums, then each stream finishes half of the columns,
+        // a quarter of D at a time, the other's share of which comes through shared memory where the query
+        // rows were (a row's 16-byte pieces turned by the row's number).
+        float2* lses = reinterpret_cast<float2*>(sgen + S::OFF_Q);
+        lses[x * 128 + row] = lse;
+        softmax_sync<ST>();
+        const float2 other = lses[(1 - x) * 128 + row];
+        softmax_sync<ST>();
+        if (other.x != -INFINITY) {
+          if (lse.x == -INFINITY) {
+            lse = other;
+          } else {
+            const float d = (other.x - lse.x) + (other.y - lse.y);  // (NaN where one is)
+            const float e = ex2(-fabsf(d)), total = 1.f + e;
+            w1 *= (d > 0.f ? e : 1.f) / total;
+            if (d > 0.f) lse = other;
+            lse.y += lg2(total);
+          }
+        }
+        if (f.nf > 1 && x == 0 && row_ok) part_l[static_cast<long long>(f.slot) * RP + row] = lse;
+        constexpr int CB = D / 4, PC = CB / 4;
+        float4* buf = reinterpret_cast<float4*>(sgen + S::OFF_Q);
+        // `CB` of this stream's columns, weighted.
+        auto mine = [&](int c0, float (&o)[CB]) {
+          if (n > 0) {
+            tmem_ldn<CB>(o_addr + c0, o);
+            tmem_wait_ld();
 #pragma unroll
+            for (int i = 0; i < CB; ++i) o[i] = o[i] * w1 * w2;
+          } else {
+#pragma unroll
+            for (int i = 0; i < CB; ++i) o[i] = 0.f;
+          }
+        };
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          if (warp_rows) {
+            float o[CB];
+            mine((1 - x) * (D / 2) + pass * CB, o);
+            if (row_ok) {
+#pragma unroll
+              for (int i = 0; i < PC; ++i) buf[((1 - x) * 128 + row) * PC + (i + row) % PC] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          }
+          softmax_sync<ST>();
+          if (warp_rows) {
+            float o[CB];
+            const int c0 = x * (D / 2) + pass * CB;
+            mine(c0, o);
+            if (row_ok) {
+#pragma unroll
+              for (int i = 0; i < PC; ++i) {
+                const float4 a = buf[(x * 128 + row) * PC + (i + row) % PC];
+                put(c0 + 4 * i, make_float4(o[4 * i] + a.x, o[4 * i + 1] + a.y, o[4 * i + 2] + a.z, o[4 * i + 3] + a.w));
+              }
+            }
+          }
+          softmax_sync<ST>();
+        }
+      } else {
+        if (f.nf > 1 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = lse;
+        if (n > 0 && warp_rows) {
+#pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             float o[16];
             tmem_ld16(o_addr + c, o);
             tmem_wait_ld();
             if (row_ok) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = o[i] * w1 * w2;
-              if (f.nf > 1) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(dst + c)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-              } else {
-                uint32_t u[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] = p.bf16 ? pack2<true>(o[2 * i], o[2 * i + 1]) : pack2<false>(o[2 * i], o[2 * i + 1]);
-                reinterpret_cast<uint4*>(out + 2 * c)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-                reinterpret_cast<uint4*>(out + 2 * c)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-              }
+              for (int i = 0; i < 16; i += 4)
+                put(c + i, make_float4(o[i] * w1 * w2, o[i + 1] * w1 * w2, o[i + 2] * w1 * w2, o[i + 3] * w1 * w2));
             }
           }
         }
-      } else {
-        // The parts of a row joined: their weights by their sums, O half the columns at a time where
-        // the query rows were (a row's 16-byte pieces turned by the row's number).
-        float2* lses = reinterpret_cast<float2*>(sgen + S::OFF_LSE);
-        lses[lane128] = lse;
-        if (!(ok = group_sync())) break;
-        float2 top = lses[row];
-        float sum = 1.f, share = lane128 < R ? 1.f : 0.f;  // relative to `top`
-        if (top.x == -INFINITY) sum = share = 0.f;
-#pragma unroll
-        for (int c = 1; c < CS; ++c) {
-          const float2 y = lses[c * R + row];
-          join_sums(top, sum, share, y, lane128 / R == c);
-        }
-        w1 *= share / sum;
-        if (sum == 0.f) w1 = 0.f;
-        if (sum != sum) w1 = sum;  // (a part that is not a number)
-        if (f.nf > 1 && lane128 < R && row_ok)
-          part_l[static_cast<long long>(f.slot) * RP + row] = sum == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(top.x, top.y + lg2(sum));
-        constexpr int PC = D / 8;  // 16-byte pieces of half a row
-        float4* buf = reinterpret_cast<float4*>(sgen + S::OFF_Q);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int c = 0; c < D / 2; c += 8) {
-            float o[8];
-            uint32_t u[8];
-            asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
-                         : "r"(o_addr + half * (D / 2) + c)
-                         : "memory");
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(u[i]) * w1 * w2;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              buf[lane128 * PC + (c / 4 + i + lane128) % PC] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-          if (!(ok = group_sync())) break;
-          for (int i = stid; i < min(f.rows, R) * PC; i += ST) {
-            const int rr = i / PC, k = i - rr * PC;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < CS; ++c) {
-              const float4 o = buf[(c * R + rr) * PC + (k + c * R + rr) % PC];
-              a.x += o.x;
-              a.y += o.y;
-              a.z += o.z;
-              a.w += o.w;
-            }
-            const int col = half * (D / 2) + 4 * k;
-            if (f.nf > 1) {
-              *reinterpret_cast<float4*>(part_o + (static_cast<long long>(f.slot) * RP + rr) * D + col) = a;
-            } else {
-              const int ra = f.row0 + rr, tt = ra / p.G;
-              const long long orow = (static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt;
-              uint2 u;
-              u.x = p.bf16 ? pack2<true>(a.x, a.y) : pack2<false>(a.x, a.y);
-              u.y = p.bf16 ? pack2<true>(a.z, a.w) : pack2<false>(a.z, a.w);
-              *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (orow * D + col) * 2) = u;
-            }
-          }
-          if (!(ok = group_sync())) break;
-        }
-        if (!ok) break;
       }
       if (f.nf > 1) {
-        // The last of the item's fragments joins them.
-        if (!(ok = group_sync())) break;
-        if (stid == 0) *joins = atom_add_acq_rel_gpu(p.cnt + f.c0, 1) == f.nf - 1;
-        if (!(ok = group_sync())) break;
+        // The last of the item's fragments joins them: four 16-byte pieces of rows per thread at a time, two
+        // fragments of each in flight.
+        softmax_sync<ST>();
+        if (tid == 0) *joins = atom_add_acq_rel_gpu(p.cnt + f.c0, 1) == f.nf - 1;
+        softmax_sync<ST>();
         if (*joins) {
-          for (int i = stid; i < f.rows * (D / 4); i += ST) {
-            const int rr = i / (D / 4), col = 4 * (i - rr * (D / 4));
-            float2 top = make_float2(-INFINITY, 0.f);
-            float sum = 0.f;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = 0; c < f.nf; ++c) {
-              const int slot = 2 * (f.c0 + c) + (c == 0 ? 1 : 0);
-              const float2 ls = __ldcg(part_l + static_cast<long long>(slot) * RP + rr);
-              const float4 o = __ldcg(reinterpret_cast<const float4*>(part_o + (static_cast<long long>(slot) * RP + rr) * D + col));
-              if (ls.x == -INFINITY) continue;
-              float scale = 1.f, w = 1.f;
-              if (top.x == -INFINITY) {
-                top = ls;
-              } else {
-                const float d = (ls.x - top.x) + (ls.y - top.y);
-                if (d > 0.f) {
-                  scale = exp2f(-d);
-                  top = ls;
-                } else {
-                  w = exp2f(d);
+          const float* all_o = p.part;
+          constexpr int U = 4, F = 2, PR = D / 4;
+#pragma unroll 1
+          for (int i0 = tid; i0 < f.rows * PR; i0 += U * ST) {
+            float2 top[U];
+            float sum[U];
+            float4 a[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              top[u] = make_float2(-INFINITY, 0.f);
+              sum[u] = 0.f;
+              a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll 1
+            for (int c0 = 0; c0 < f.nf; c0 += F) {
+              float2 ls[F][U];
+              float4 o[F][U];
+#pragma unroll
+              for (int c = 0; c < F; ++c) {
+                const int slot = 2 * (f.c0 + min(c0 + c, f.nf - 1)) + (c0 + c == 0 ? 1 : 0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                  const int i = min(i0 + u * ST, f.rows * PR - 1);
+                  const long long at = static_cast<long long>(slot) * RP + i / PR;
+                  ls[c][u] = __ldcg(part_l + at);
+                  o[c][u] = __ldcg(reinterpret_cast<const float4*>(all_o + at * D) + i % PR);
                 }
               }
-              a.x = a.x * scale + o.x * w;
-              a.y = a.y * scale + o.y * w;
-              a.z = a.z * scale + o.z * w;
-              a.w = a.w * scale + o.w * w;
-              sum = sum * scale + w;
+#pragma unroll
+              for (int c = 0; c < F; ++c) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                  if (c0 + c >= f.nf || ls[c][u].x == -INFINITY) continue;
+                  float d = (ls[c][u].x - top[u].x) + (ls[c][u].y - top[u].y);
+                  if (top[u].x == -INFINITY) d = INFINITY;
+                  const float e = ex2(-fabsf(d)), scale = d > 0.f ? e : 1.f, w = d > 0.f ? 1.f : e;
+                  if (d > 0.f) top[u] = ls[c][u];
+                  a[u].x = a[u].x * scale + o[c][u].x * w;
+                  a[u].y = a[u].y * scale + o[c][u].y * w;
+                  a[u].z = a[u].z * scale + o[c][u].z * w;
+                  a[u].w = a[u].w * scale + o[c][u].w * w;
+                  sum[u] = sum[u] * scale + w;
+                }
+              }
             }
-            const float inv = 1.0f / sum;
-            const int ra = f.row0 + rr, tt = ra / p.G;
-            const long long orow = (static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt;
-            uint2 u;
-            u.x = p.bf16 ? pack2<true>(a.x * inv, a.y * inv) : pack2<false>(a.x * inv, a.y * inv);
-            u.y = p.bf16 ? pack2<true>(a.z * inv, a.w * inv) : pack2<false>(a.z * inv, a.w * inv);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (orow * D + col) * 2) = u;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int i = i0 + u * ST;
+              if (i >= f.rows * PR) continue;
+              const float inv = 1.0f / sum[u];
+              const int ra = f.row0 + i / PR, tt = small_div(ra, p.G);
+              const long long orow = (static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt;
+              uint2 v;
+              v.x = p.bf16 ? pack2<true>(a[u].x * inv, a[u].y * inv) : pack2<false>(a[u].x * inv, a[u].y * inv);
+              v.y = p.bf16 ? pack2<true>(a[u].z * inv, a[u].w * inv) : pack2<false>(a[u].z * inv, a[u].w * inv);
+              *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (orow * D + 4 * (i % PR)) * 2) = v;
+            }
           }
         }
       }
@@ -855,8 +912,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     // ------------------------------------------------------------------ rows behind the last token
     regs_dec<S::REG_WIDEN>();
     {
-      const int first = warp - S::SW, warps = 12 - S::SW;
-      const int G16 = D / 8;  // 16-byte pieces of a row
+      const int first = warp - S::SW;
+      constexpr int warps = 12 - S::SW, P16 = D / 8;  // 16-byte pieces of a row
       for (int b0 = 0; b0 < p.B; b0 += 32) {
         int n = p.T;
         if (b0 + lane < p.B) {
@@ -871,42 +928,52 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           const int l = __ffs(static_cast<int>(todo)) - 1, b = b0 + l;
           const int from = __shfl_sync(0xffffffffu, n, l);
           // every gridDim.x-th row set (b, h), each warp a share of its rows
-          const long long s0 = static_cast<long long>(b) * p.Hq;
-          const long long skip = (blockIdx.x + gridDim.x - s0 % gridDim.x) % gridDim.x;
-          for (long long h = skip; h < p.Hq; h += gridDim.x) {
-            uint4* dst = reinterpret_cast<uint4*>(p.out) + ((s0 + h) * p.T + from) * G16;
-            const long long pieces = static_cast<long long>(p.T - from) * G16;
+          const unsigned g = gridDim.x, at = ((static_cast<unsigned>(b) % g) * (static_cast<unsigned>(p.Hq) % g)) % g;
+          for (int h = static_cast<int>((blockIdx.x + g - at) % g); h < p.Hq; h += static_cast<int>(g)) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out) + ((static_cast<long long>(b) * p.Hq + h) * p.T + from) * P16;
+            const long long pieces = static_cast<long long>(p.T - from) * P16;
             for (long long i = 32 * first + lane; i < pieces; i += 32 * warps) dst[i] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
       }
     }
     // ------------------------------------------------------------------ widening
-    const bool values = NT == 2 ? warp >= 10 : warp >= 8;
-    const int wt = (NT == 2 ? (warp & 1) : (warp & 3)) * 32 + lane;  // thread of this cache's warps
-    constexpr int WT = 32 * S::CK;
-    constexpr int CPR = D / 16;        // 16-byte pieces of a cached row
-    constexpr int PIECES = KT * CPR;
-    constexpr int PER = PIECES / WT;   // of a thread
+    const bool values = warp >= S::SW + S::WC;
+    const int wt = (warp - S::SW) % S::WC * 32 + lane;  // thread of this cache's warps
+    constexpr int CPR = D / 16;             // 16-byte parts of a cached row
+    constexpr int PARTS = S::RK * CPR;      // of a copied piece
+    constexpr int WT = PARTS < 32 * S::WC ? PARTS : 32 * S::WC;  // threads that have any
+    constexpr int PER = PARTS / WT;
+    // A thread's parts are RS rows apart, a multiple of the swizzle's period, so their offsets in the
+    // widened tile are RS SPAN apart. Where a row has eight parts or more, a quarter-warp takes four of
+    // one row and the next four of the row below: then neither its loads nor its stores meet in a bank.
+    constexpr int RS = WT / CPR;
+    static_assert(RS % 8 == 0 && PARTS % WT == 0, "a thread's parts");
+    int r0 = wt / CPR, k0 = wt % CPR;
+    if constexpr (CPR >= 8) {
+      const int in = wt % (2 * CPR), below = (in >> 2) & 1;
+      r0 = wt / (2 * CPR) * 2 + below;
+      k0 = (in & 3) + 4 * ((in >> 3) ^ below);
+    }
+    const uint32_t from = 16 * (r0 * CPR + k0);
+    const uint32_t to0 = swz_chunk_offset<SPAN>(KT, r0, 2 * k0), to1 = swz_chunk_offset<SPAN>(KT, r0, 2 * k0 + 1);
     const int n_raw = values ? NRV : NRK, n_wide = values ? NV : NK;
-    const int off_raw = values ? S::OFF_RV : S::OFF_RK, off_wide = values ? S::OFF_V : S::OFF_K;
-    auto raw_full = [&](int s) { return values ? RVF(s) : RKF(s); };
-    auto raw_empty = [&](int s) { return values ? RVE(s) : RKE(s); };
-    auto wide_full = [&](int s) { return values ? VF(s) : KF(s); };
-    auto wide_empty = [&](int s) { return values ? VE(s) : KE(s); };
+    const uint32_t raw0 = sbase + (values ? S::OFF_RV : S::OFF_RK) + from, wide0 = sbase + (values ? S::OFF_V : S::OFF_K);
+    const uint32_t raw_full = values ? RVF(0) : RKF(0), raw_empty = values ? RVE(0) : RKE(0);
+    const uint32_t wide_full = values ? VF(0) : KF(0), wide_empty = values ? VE(0) : KE(0);
     int rs = 0, rp = 0, ws = 0, wp = 1, n_batch = 0;  // stages and parities
     bool ok = true;
     while (ok) {
       const ExtendFrag f = take();
-      if (f.kind == 0) break;
+      if (f.kind <= 0) break;
       const int nt = f.j1 - f.j0;
-      for (int jj = 0; jj < nt; ++jj) {
+      for (int jj = 0; ok && jj < nt; ++jj) {
         uint32_t zero = 0u;   // groups of V that are not to be used
         int rows_left = KT;   // rows up to the request's end
         if (values) {
           const int bs = n_batch & 1;
           if (jj % NB == 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(SCF(bs), (n_batch >> 1) & 1, failed, 510));
+            ok = __all_sync(0xffffffffu, extend_wait(SCF(bs), (n_batch >> 1) & 1, failed, 510));
             if (!ok) break;
           }
           zero = *reinterpret_cast<const uint32_t*>(sgen + S::OFF_SC + bs * S::SC_BYTES + 384 + 4 * (jj % NB));
@@ -917,33 +984,50 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
             ++n_batch;
           }
         }
-        ok = mbar_wait(raw_full(rs), rp, failed, 511) && mbar_wait(wide_empty(ws), wp, failed, 512);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, extend_wait(wide_empty + 8 * ws, wp, failed, 512));
         if (!ok) break;
-        const uint32_t src = sbase + off_raw + rs * S::RAW, dst = sbase + off_wide + ws * S::T_BYTES;
         const bool clear = zero != 0u || (values && rows_left < KT);
-#pragma unroll 4
-        for (int i = 0; i < PER; ++i) {
-          const int c = wt + i * WT, r = c / CPR, k = c % CPR;
-          const uint4 b = ld_shared_v4(src + 16 * c);
-          uint4 lo, hi;
-          widen16(b, lo, hi);
-          if (clear && (r >= rows_left || ((zero >> (r / 16)) & 1u))) lo = hi = make_uint4(0u, 0u, 0u, 0u);
-          // (lanes of a quarter-warp that would meet in a bank write their halves in the other order)
-          const bool turn = CPR >= 8 && (k & 4);
-          st_shared_v4(dst + swz_chunk_offset<SPAN>(KT, r, 2 * k + turn), turn ? hi : lo);
-          st_shared_v4(dst + swz_chunk_offset<SPAN>(KT, r, 2 * k + !turn), turn ? lo : hi);
+        uint32_t dst = wide0 + ws * S::T_BYTES;
+#pragma unroll 1
+        for (int piece = 0; piece < RPT; ++piece) {
+          ok = __all_sync(0xffffffffu, extend_wait(raw_full + 8 * rs, rp, failed, 511));
+          if (!ok) break;
+          if (WT == 32 * S::WC || wt < WT) {
+            const uint32_t src = raw0 + rs * S::RAW;
+            constexpr int UN = PER < 4 ? PER : 4;
+#pragma unroll 1
+            for (int i0 = 0; i0 < PER; i0 += UN) {
+              uint4 b[UN];
+#pragma unroll
+              for (int i = 0; i < UN; ++i) b[i] = ld_shared_v4(src + 16 * RS * CPR * (i0 + i));
+              if (__builtin_expect(clear, 0)) {
+#pragma unroll
+                for (int i = 0; i < UN; ++i) {
+                  const int r = piece * S::RK + r0 + RS * (i0 + i);
+                  if (r >= rows_left || ((zero >> (r / 16)) & 1u)) b[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < UN; ++i) {
+                uint4 lo, hi;
+                widen16(b[i], lo, hi);
+                st_shared_v4(dst + to0 + RS * SPAN * (i0 + i), lo);
+                st_shared_v4(dst + to1 + RS * SPAN * (i0 + i), hi);
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(raw_empty + 8 * rs);
+          if (++rs == n_raw) {
+            rs = 0;
+            rp ^= 1;
+          }
+          dst += S::RK * SPAN;
         }
+        if (!ok) break;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(raw_empty(rs));
-          mbar_arrive(wide_full(ws));
-        }
-        if (++rs == n_raw) {
-          rs = 0;
-          rp ^= 1;
-        }
+        if (lane == 0) mbar_arrive(wide_full + 8 * ws);
         if (++ws == n_wide) {
           ws = 0;
           wp ^= 1;
@@ -951,175 +1035,148 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       }
     }
   } else {
-    regs_dec<S::REG_REST>();
-    if (warp == 12 || warp == 13) {
-      // ------------------------------------------------------------------ copies of K or V
-      const bool values = warp == 13;
-      const uint8_t* cache = values ? p.v8 : p.k8;
-      const int n_raw = values ? NRV : NRK, off_raw = values ? S::OFF_RV : S::OFF_RK;
-      auto full = [&](int s) { return values ? RVF(s) : RKF(s); };
-      auto empty = [&](int s) { return values ? RVE(s) : RKE(s); };
-      const int piece = min(p.block, KT);          // keys of a copy
-      const uint32_t bytes = static_cast<uint32_t>(piece) * D;
-      int st = 0, ph = 1;
-      long long issued = 0;
-      bool ok = true;
+    regs_dec<S::REG_ISSUE>();
+    const int keys = min(p.block, S::RK);        // of a copy
+    const uint32_t bytes = static_cast<uint32_t>(keys) * D;
+    constexpr int GPP = S::RK / 16;              // groups of 16 keys in a piece
+    int st = 0, ph = 1, used = 0;                // a copying warp's stage, parity, stages that were used
+    bool ok = true;
+    // Up to eight pieces of a cache, of which a lane has the block id of a group of 16 keys from `key` on.
+    auto copy = [&](const ExtendFrag& f, const uint8_t* cache, int id, int key, int pieces, int n_raw, uint32_t raw0, uint32_t full, uint32_t empty, int site) {
+      const bool first = (16 * lane) % keys == 0 && static_cast<unsigned>(id) < static_cast<unsigned>(p.N);
+      const uint8_t* src = cache + ((static_cast<long long>(id) * p.Hkv + f.kvh) * p.block + (key & (p.block - 1))) * D;
+      const unsigned firsts = __ballot_sync(0xffffffffu, first);
+#pragma unroll 1
+      for (int i = 0; i < pieces; ++i) {
+        ok = __all_sync(0xffffffffu, extend_wait(empty + 8 * st, ph, failed, site));
+        if (!ok) break;
+        const unsigned mine = firsts & (((1u << GPP) - 1u) << (i * GPP));
+        if (lane == 0) mbar_expect_tx(full + 8 * st, __popc(mine) * bytes);
+        __syncwarp();
+        if ((mine >> lane) & 1u) bulk_load(raw0 + st * S::RAW + (lane % GPP) * 16 * D, src, bytes, full + 8 * st);
+        used = max(used, st + 1);
+        if (++st == n_raw) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    };
+    if (warp == 12) {
+      // ------------------------------------------------------------------ copies of K
       while (ok) {
         const ExtendFrag f = take();
-        if (f.kind == 0) break;
-        const int nt = f.j1 - f.j0;
+        if (f.kind <= 0) break;
+        const int np = (f.j1 - f.j0) * RPT, key0 = f.j0 * KT;
         const int* row = p.table + static_cast<long long>(f.b) * p.width;
-        // A lane has a group of 16 keys of NB tiles; the ids of the next ones are fetched ahead.
-        auto fetch = [&](int t0) {
-          const int key = (f.j0 + t0) * KT + 16 * lane;
+        // A lane has a group of 16 keys of eight pieces; the ids of the next ones are fetched ahead.
+        auto fetch = [&](int p0) {
+          const int key = key0 + p0 * S::RK + 16 * lane;
           return key < f.len ? row[key >> p.block_log2] : -1;
         };
         int id = fetch(0);
-        for (int t0 = 0; ok && t0 < nt; t0 += NB) {
-          const int next = t0 + NB < nt ? fetch(t0 + NB) : -1;
-          const bool first = (16 * lane) % piece == 0 && static_cast<unsigned>(id) < static_cast<unsigned>(p.N);
-          const int key = (f.j0 + t0) * KT + 16 * lane;
-          const uint8_t* src = cache + ((static_cast<long long>(id) * p.Hkv + f.kvh) * p.block + (key & (p.block - 1))) * D;
-          const unsigned firsts = __ballot_sync(0xffffffffu, first);
-          for (int i = 0; i < NB && t0 + i < nt; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(empty(st), ph, failed, 520));
-            if (!ok) break;
-            const unsigned mine = firsts & (((GPT == 32 ? 0u : (1u << GPT)) - 1u) << (i * GPT));
-            if (lane == 0) mbar_expect_tx(full(st), __popc(mine) * bytes);
-            __syncwarp();
-            if ((mine >> lane) & 1u) bulk_load(sbase + off_raw + st * S::RAW + (lane % GPT) * 16 * D, src, bytes, full(st));
-            ++issued;
-            if (++st == n_raw) {
-              st = 0;
-              ph ^= 1;
-            }
-          }
+        for (int p0 = 0; ok && p0 < np; p0 += 8) {
+          const int next = p0 + 8 < np ? fetch(p0 + 8) : -1;
+          copy(f, p.k8, id, key0 + p0 * S::RK + 16 * lane, min(8, np - p0), NRK, sbase + S::OFF_RK, RKF(0), RKE(0), 520);
           id = next;
         }
       }
       // Every copy lands before the CTA ends.
-      for (long long i = issued > n_raw ? issued - n_raw : 0; i < issued; ++i)
-        mbar_wait_drain(full(static_cast<int>(i % n_raw)), static_cast<uint32_t>((i / n_raw) & 1), 521);
-    } else if (warp == 14) {
-      // ------------------------------------------------------------------ MMA issuer
-      const uint64_t dq0 = smem_desc(sbase + S::OFF_Q, 16, 8 * SPAN, SWZ);
+      for (int s = 0; s < used; ++s) mbar_wait_drain(RKF(s), static_cast<uint32_t>(s < st ? ph ^ 1 : ph), 521);
+    } else if (warp >= 14 && warp < 14 + NS) {
+      // ------------------------------------------------------------------ products of stream x
+      const int x = warp - 14;
+      const uint64_t dq = smem_desc(sbase + S::OFF_Q + (ALT ? 0 : x) * S::Q_BYTES, 16, 8 * SPAN, SWZ);
       const uint64_t dk0 = smem_desc(sbase + S::OFF_K, 16, 8 * SPAN, SWZ);
       const uint64_t dv0 = smem_desc(sbase + S::OFF_V, KT * SPAN, 8 * SPAN, SWZ);
+      const uint32_t s_tmem = tmem + S::TM_S + x * KT, o_tmem = tmem + S::TM_O + x * D;
       const bool leader = elect_one();
-      int ks = 0, kp = 0, vs = 0, vp = 0;      // stages and parities of widened K and V
-      int n_q[2] = {0, 0}, n_s[2] = {0, 0}, n_p[2] = {0, 0};  // fragments, S and P tiles per row tile
-      bool ok = true;
-      auto wait = [&](uint32_t b, int parity, unsigned site) {
-        return __all_sync(0xffffffffu, mbar_wait(b, parity, failed, site)) != 0;
+      int kt = 0;                        // key tiles of the fragments before
+      int n_q = 0, n_p = 0, n_d = 0;     // query tiles, tiles of P, waits for the end of P V
+      auto wait = [&](uint32_t b, int parity, int site) {
+        return __all_sync(0xffffffffu, extend_wait(b, parity, failed, site)) != 0;
+      };
+      // S of tile jj of the fragment, once its widened K is there.
+      auto scores = [&](int jj) {
+        const int st = (kt + jj) % NK;
+        if (!(ok = wait(KF(st), ((kt + jj) / NK) & 1, 533))) return;
+        tc_fence_after();
+        if (leader) {
+          const uint64_t dk = dk0 + static_cast<uint64_t>((st * S::T_BYTES) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off_q = ((kk * 32) / SPAN) * 128 * SPAN + (kk * 32) % SPAN;
+            const uint32_t off_k = ((kk * 32) / SPAN) * KT * SPAN + (kk * 32) % SPAN;
+            umma_f16_ss(s_tmem, dq + (off_q >> 4), dk + (off_k >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(SF(x));
+          umma_commit(KE(st));
+        }
+        __syncwarp();
       };
       while (ok) {
         const ExtendFrag f = take();
-        if (f.kind == 0) break;
-        const int nt = f.j1 - f.j0;
-        int n[2] = {max(0, min(f.j1, f.nk0) - f.j0), NT == 2 ? max(0, min(f.j1, f.nk1) - f.j0) : 0};
-        for (int x = 0; x < NT && ok; ++x)
-          if (n[x] > 0) ok = wait(QF(x), n_q[x]++ & 1, 530);
-        if (!ok) break;
-        auto qk = [&](int x, int jj) {  // S of key tile jj (its widened K is there)
-          if (jj >= n[x]) return;
-          const int sb = NT == 2 ? x : n_s[0] & 1;
-          // S may be written over: P there is multiplied (NT = 1; the shapes differ, so the order of the
-          // products alone does not say so), or S is read
-          if (NT == 1 && jj >= 2) ok = wait(OD(0), n_s[0] & 1, 535);  // (before: known from the query rows)
-          if (S::SEP && n_s[x] >= 1) ok = wait(SR(x), (n_s[x] - 1) & 1, 536);
-          if (!ok) return;
-          tc_fence_after();
-          if (leader) {
-            const uint64_t dq = dq0 + static_cast<uint64_t>((x * S::Q_BYTES) >> 4);
-            const uint64_t dk = dk0 + static_cast<uint64_t>((ks * S::T_BYTES) >> 4);
+        if (f.kind <= 0) break;
+        const int nt = f.j1 - f.j0, n = tiles_of(f, x);
+        const int step = ALT ? 2 : 1, first = ALT ? x : 0;
+        if (ALT || n > 0) ok = wait(QF(ALT ? 0 : x), n_q++ & 1, 530);
+        if (ok && n > 0) scores(first);
+        for (int i = 0; ok && i < n; ++i) {
+          const int jj = first + i * step, st = (kt + jj) % NV;
+          if (!(ok = wait(VF(st), ((kt + jj) / NV) & 1, 532))) break;
+          const uint64_t dv = dv0 + static_cast<uint64_t>((st * S::T_BYTES) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off_q = ((kk * 32) / SPAN) * 128 * SPAN + (kk * 32) % SPAN;
-              const uint32_t off_k = ((kk * 32) / SPAN) * KT * SPAN + (kk * 32) % SPAN;
-              umma_f16_ss(tmem + S::TM_S + sb * KT, dq + (off_q >> 4), dk + (off_k >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
-            }
-            umma_commit(SF(sb));
-          }
-          __syncwarp();
-          ++n_s[x];
-        };
-        bool v_there = false;
-        auto pv = [&](int x, int jj) -> bool {  // O of key tile jj
-          if (jj < 0 || jj >= n[x]) return true;
-          const int sb = NT == 2 ? x : n_p[0] & 1;
-          if (!wait(PF(sb), (NT == 2 ? n_p[x] : n_p[0] >> 1) & 1, 531)) return false;
-          if (!v_there && !wait(VF(vs), vp, 532)) return false;
-          v_there = true;
-          tc_fence_after();
-          if (leader) {
-            const uint64_t dv = dv0 + static_cast<uint64_t>((vs * S::T_BYTES) >> 4);
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = wait(PF(x, half), n_p & 1, 531))) break;
+            tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk)
-              umma_f16_ts(tmem + S::TM_O + x * D, tmem + (S::SEP ? S::TM_P + x * (KT / 2) : S::TM_S + sb * KT) + kk * 8,
-                          dv + static_cast<uint64_t>((kk * 16 * SPAN) >> 4), IDESC_PV, (jj > 0 || kk > 0) ? 1u : 0u);
-            if (NT == 1 || S::SEP || jj == n[x] - 1) umma_commit(OD(x));
-          }
-          __syncwarp();
-          ++n_p[x];
-          return true;
-        };
-        for (int jj = 0; ok && jj <= nt; ++jj) {
-          const bool has_k = jj < nt;
-          if (has_k && !(ok = wait(KF(ks), kp, 533))) break;
-          v_there = false;
-          if constexpr (NT == 1) {
-            if (has_k) {
-              qk(0, jj);
-              if (leader) umma_commit(KE(ks));  // (before P V: the next K may be widened meanwhile)
+              for (int kk = half * (KT / 32); kk < (half + 1) * (KT / 32); ++kk)
+                umma_f16_ts(o_tmem, s_tmem + kk * 8, dv + static_cast<uint64_t>((kk * 16 * SPAN) >> 4), IDESC_PV, (i > 0 || kk > 0) ? 1u : 0u);
             }
-            ok = ok && pv(0, jj - 1);
-          } else if constexpr (S::SEP) {
-            if (has_k) {
-              qk(0, jj);
-              if (ok) qk(1, jj);
-            }
-            ok = ok && pv(0, jj - 1) && pv(1, jj - 1);
-          } else {
-            ok = pv(0, jj - 1);
-            if (ok && has_k) qk(0, jj);
-            ok = ok && pv(1, jj - 1);
-            if (ok && has_k) qk(1, jj);
+            __syncwarp();
           }
           if (!ok) break;
-          if (has_k) {
-            if (NT == 2 && leader) umma_commit(KE(ks));
-            if (++ks == NK) {
-              ks = 0;
-              kp ^= 1;
-            }
-          }
-          if (jj > 0) {
-            if (leader) umma_commit(VE(vs));
-            if (++vs == NV) {
-              vs = 0;
-              vp ^= 1;
-            }
+          ++n_p;
+          if (leader) {
+            umma_commit(VE(st));
+            if (i == n - 1) umma_commit(OF(x));
+            else if (!ORDERED) umma_commit(OD(x));
           }
           __syncwarp();
+          if (i + 1 < n) {
+            if (!ORDERED && !(ok = wait(OD(x), n_d++ & 1, 534))) break;
+            scores(jj + step);
+          }
         }
+        if (NT == 2) {
+          // Tiles that only the other stream has: released as they come.
+          for (int jj = n; ok && jj < nt; ++jj) {
+            const int st = (kt + jj) % NK, sv = (kt + jj) % NV;
+            if (!(ok = wait(KF(st), ((kt + jj) / NK) & 1, 537))) break;
+            if (lane == 0) mbar_arrive(KE(st));
+            if (!(ok = wait(VF(sv), ((kt + jj) / NV) & 1, 538))) break;
+            if (lane == 0) mbar_arrive(VE(sv));
+          }
+        }
+        kt += nt;
       }
+      // Every product is done before tensor memory is released.
       if (leader) {
-        umma_commit(BAR_DR);
-        mbar_wait_drain(BAR_DR, 0, 534);
+        umma_commit(DR(x));
+        mbar_wait_drain(DR(x), 0, 535);
       }
       __syncwarp();
-    } else {
-      // ------------------------------------------------------------------ fragments and scales
+    } else if (warp == 13) {
+      // ------------------------------------------------------------------ fragments, scales, copies of V
       ExtendWalk<S> walk;
       walk.init(p, lane);
       int nfr = 0, n_batch = 0;
-      bool ok = true;
       while (true) {
         ExtendFrag f{};
         const bool more = walk.next(p, f);
         if (!more) f.kind = 0;
         const int slot = nfr % NF;
-        if (nfr >= NF) ok = __all_sync(0xffffffffu, mbar_wait(FE(slot), (nfr / NF - 1) & 1, failed, 540));
+        if (nfr >= NF) ok = __all_sync(0xffffffffu, extend_wait(FE(slot), (nfr / NF - 1) & 1, failed, 540));
         if (!ok) break;
         if (lane == 0) {
           volatile int* e = frags + 16 * slot;
@@ -1142,27 +1199,41 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         __syncwarp();
         ++nfr;
         if (!more) break;
+        // The query rows on their way into L2 (the softmax gets to them a fragment later).
+        for (int r = lane; r < f.rows; r += 32) {
+          const int t = small_div(f.row0 + r, p.G), h = f.kvh * p.G + (f.row0 + r - t * p.G);
+          const uint8_t* src = static_cast<const uint8_t*>(p.q) + ((static_cast<long long>(f.b) * p.Hq + h) * p.T + t) * (2 * D);
+#pragma unroll 1
+          for (int i = 0; i < 2 * D; i += 128) prefetch_l2(src + i);
+        }
         const int nt = f.j1 - f.j0;
         const int* row = p.table + static_cast<long long>(f.b) * p.width;
         float vr = 0.f;
         bool far = false;
-        for (int t0 = 0; t0 < nt; t0 += NB) {
+        // A lane has a group of 16 keys of NB tiles; the ids and scales of the next ones are fetched ahead.
+        int id = -1;
+        float ks = 0.f, vs = 1.f;
+        bool live = false;
+        auto fetch = [&](int t0) {
           const int key = (f.j0 + t0) * KT + 16 * lane;
-          const bool live = key < f.len && key < f.j1 * KT;
-          float ks = 0.f, vs = 1.f;
-          bool good = true;
+          live = key < f.len && key < f.j1 * KT;
+          ks = 0.f;
+          vs = 1.f;
+          id = -1;
           if (live) {
-            const int id = row[key >> p.block_log2];
-            good = static_cast<unsigned>(id) < static_cast<unsigned>(p.N);
-            if (good) {
+            id = row[key >> p.block_log2];
+            if (static_cast<unsigned>(id) < static_cast<unsigned>(p.N)) {
               const long long cell = static_cast<long long>(id) * p.Hkv + f.kvh;
-              ks = p.ks[cell] * p.scale_log2;
+              ks = p.ks[cell];
               vs = p.vs[cell];
-            } else {
-              ks = __int_as_float(0x7fc00000);
-              record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(id));
             }
           }
+        };
+        fetch(0);
+        for (int t0 = 0; t0 < nt; t0 += NB) {
+          const bool good = !live || static_cast<unsigned>(id) < static_cast<unsigned>(p.N);
+          if (!good) record_error(7u, static_cast<unsigned>(f.b), static_cast<unsigned>(id));
+          ks = good ? ks * p.scale_log2 : __int_as_float(0x7fc00000);
           float lv = log2_scale(vs);
           if (t0 == 0) {
             vr = __shfl_sync(0xffffffffu, lv, 0);
@@ -1174,7 +1245,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           far = far || __any_sync(0xffffffffu, fabsf(d) > EXTEND_FAR);
           const unsigned bad = __ballot_sync(0xffffffffu, !good || nan || ks != ks);
           const int bs = n_batch & 1;
-          if (n_batch >= 2) ok = __all_sync(0xffffffffu, mbar_wait(SCE(bs), ((n_batch >> 1) - 1) & 1, failed, 541));
+          if (n_batch >= 2) ok = __all_sync(0xffffffffu, extend_wait(SCE(bs), ((n_batch >> 1) - 1) & 1, failed, 541));
           if (!ok) break;
           uint8_t* sc = sgen + S::OFF_SC + bs * S::SC_BYTES;
           reinterpret_cast<float*>(sc)[lane] = ks;
@@ -1188,9 +1259,14 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           __syncwarp();
           if (lane == 0) mbar_arrive(SCF(bs));
           ++n_batch;
+          const int at = id, key = (f.j0 + t0) * KT + 16 * lane;
+          if (t0 + NB < nt) fetch(t0 + NB);
+          copy(f, p.v8, at, key, min(8, (nt - t0) * RPT), NRV, sbase + S::OFF_RV, RVF(0), RVE(0), 522);
+          if (!ok) break;
         }
         if (!ok) break;
       }
+      for (int s = 0; s < used; ++s) mbar_wait_drain(RVF(s), static_cast<uint32_t>(s < st ? ph ^ 1 : ph), 523);
     }
     __syncwarp();
   }
@@ -1201,6 +1277,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     tc_fence_after();
     tmem_dealloc(tmem, S::TMEM_COLS);
   }
+  if (tid == 0 && *failed) record_timeout(static_cast<unsigned>(*failed));
   // The CTA that ends last leaves the tickets as they were.
   if (tid == 0 && atom_add_acq_rel_gpu(p.cnt + p.done, 1) == static_cast<int>(gridDim.x) - 1) {
     for (int i = 0; i < static_cast<int>(gridDim.x); ++i) p.cnt[i] = 0;

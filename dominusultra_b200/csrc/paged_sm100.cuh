@@ -57,6 +57,11 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
   return r;
 }
 
+// Brings a word into L1 and waits for nothing.
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("{\n\t.reg .b32 t;\n\tld.global.b32 t, [%0];\n\t}\n" ::"l"(p));
+}
+
 // ---------------------------------------------------------------------------------------------
 // Block tables and slot maps
 // ---------------------------------------------------------------------------------------------
