@@ -57,7 +57,9 @@ struct ExtendPagedParams {
   const void* sin;
   void* out;          // [B, Hq, T, D]
   int* cnt;           // tickets, zero between calls; the last one counts the CTAs that are done
-  float* part;        // [2 gridDim.x][rows][D] partial outs, then [2 gridDim.x][rows] log2 of their sums, in two parts
+  // Partial outs [2 gridDim.x][D / 4][rows] by four columns (neighbouring lanes have neighbouring rows), then
+  // the log2 of their sums, in two parts, [2 gridDim.x][rows].
+  float* part;
   int done;           // index of the last ticket
   int max_len;        // tokens that the table's row and the rope tables cover
   int bf16;
@@ -750,18 +752,27 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         w2 = ex2(half);
         w1 = ex2(ex - half) / l;
       }
-      float* part_o = p.part + (static_cast<long long>(f.slot) * RP + r_item) * D;
-      float2* part_l = reinterpret_cast<float2*>(p.part + 2LL * gridDim.x * RP * D);
+      float4* const part_o = reinterpret_cast<float4*>(p.part);
+      float2* const part_l = reinterpret_cast<float2*>(p.part + 2LL * gridDim.x * RP * D);
+      auto part_at = [&](int slot, int col, int r) { return (static_cast<long long>(slot) * (D / 4) + col / 4) * RP + r; };
       uint8_t* out = static_cast<uint8_t*>(p.out) + q_row * (2 * D);
-      // Four columns of the row from `col` on.
-      auto put = [&](int col, float4 a) {
+      // N columns of the row (four or eight) from `col` on.
+      auto pack4 = [&](const float* a) {
+        return p.bf16 ? make_uint2(pack2<true>(a[0], a[1]), pack2<true>(a[2], a[3])) : make_uint2(pack2<false>(a[0], a[1]), pack2<false>(a[2], a[3]));
+      };
+      auto put = [&](int col, const auto& a) {
+        constexpr int N = sizeof(a) / sizeof(float);
         if (f.nf > 1) {
-          *reinterpret_cast<float4*>(part_o + col) = a;
+#pragma unroll
+          for (int i = 0; i < N; i += 4) part_o[part_at(f.slot, col + i, r_item)] = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
         } else {
-          uint2 u;
-          u.x = p.bf16 ? pack2<true>(a.x, a.y) : pack2<false>(a.x, a.y);
-          u.y = p.bf16 ? pack2<true>(a.z, a.w) : pack2<false>(a.z, a.w);
-          *reinterpret_cast<uint2*>(out + 2 * col) = u;
+          const uint2 u = pack4(a);
+          if constexpr (N == 8) {
+            const uint2 v = pack4(a + 4);
+            *reinterpret_cast<uint4*>(out + 2 * col) = make_uint4(u.x, u.y, v.x, v.y);
+          } else {
+            *reinterpret_cast<uint2*>(out + 2 * col) = u;
+          }
         }
       };
       if constexpr (ALT) {
@@ -815,10 +826,19 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
             const int c0 = x * (D / 2) + pass * CB;
             mine(c0, o);
             if (row_ok) {
+              constexpr int N = CB < 8 ? CB : 8;
 #pragma unroll
-              for (int i = 0; i < PC; ++i) {
-                const float4 a = buf[(x * 128 + row) * PC + (i + row) % PC];
-                put(c0 + 4 * i, make_float4(o[4 * i] + a.x, o[4 * i + 1] + a.y, o[4 * i + 2] + a.z, o[4 * i + 3] + a.w));
+              for (int c = 0; c < CB; c += N) {
+                float a[N];
+#pragma unroll
+                for (int i = 0; i < N; i += 4) {
+                  const float4 b = buf[(x * 128 + row) * PC + ((c + i) / 4 + row) % PC];
+                  a[i] = o[c + i] + b.x;
+                  a[i + 1] = o[c + i + 1] + b.y;
+                  a[i + 2] = o[c + i + 2] + b.z;
+                  a[i + 3] = o[c + i + 3] + b.w;
+                }
+                put(c0 + c, a);
               }
             }
           }
@@ -834,75 +854,81 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
             tmem_wait_ld();
             if (row_ok) {
 #pragma unroll
-              for (int i = 0; i < 16; i += 4)
-                put(c + i, make_float4(o[i] * w1 * w2, o[i + 1] * w1 * w2, o[i + 2] * w1 * w2, o[i + 3] * w1 * w2));
+              for (int k = 0; k < 16; k += 8) {
+                float a[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = o[k + i] * w1 * w2;
+                put(c + k, a);
+              }
             }
           }
         }
       }
       if (f.nf > 1) {
-        // The last of the item's fragments joins them: four 16-byte pieces of rows per thread at a time, two
-        // fragments of each in flight.
+        // The last of the item's fragments joins them: a thread has a row, and twice eight columns of it at
+        // a time, the loads of four fragments in flight.
         softmax_sync<ST>();
         if (tid == 0) *joins = atom_add_acq_rel_gpu(p.cnt + f.c0, 1) == f.nf - 1;
         softmax_sync<ST>();
         if (*joins) {
-          const float* all_o = p.part;
-          constexpr int U = 4, F = 2, PR = D / 4;
+          const int lg = 32 - __clz(f.rows - 1), r = min(tid & ((1 << lg) - 1), f.rows - 1);
+          auto slot_of = [&](int c) { return 2 * (f.c0 + min(c, f.nf - 1)) + (c == 0 ? 1 : 0); };
+          float2 top = make_float2(-INFINITY, 0.f);
+          float sum = 0.f;
 #pragma unroll 1
-          for (int i0 = tid; i0 < f.rows * PR; i0 += U * ST) {
-            float2 top[U];
-            float sum[U];
-            float4 a[U];
+          for (int c0 = 0; c0 < f.nf; c0 += 4) {
+            float2 ls[4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              top[u] = make_float2(-INFINITY, 0.f);
-              sum[u] = 0.f;
-              a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < 4; ++c) ls[c] = __ldcg(part_l + static_cast<long long>(slot_of(c0 + c)) * RP + r);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (c0 + c >= f.nf || ls[c].x == -INFINITY) continue;
+              const float d = top.x == -INFINITY ? INFINITY : (ls[c].x - top.x) + (ls[c].y - top.y);
+              const float e = ex2(-fabsf(d));
+              if (d > 0.f) top = ls[c];
+              sum = d > 0.f ? sum * e + 1.f : sum + e;  // (NaN where one is)
             }
+          }
+          const float inv = 1.0f / sum;
+          const int ra = f.row0 + r, tt = small_div(ra, p.G);
+          uint8_t* to = static_cast<uint8_t*>(p.out) + ((static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt) * (2 * D);
+          const int step = ST >> lg;
 #pragma unroll 1
-            for (int c0 = 0; c0 < f.nf; c0 += F) {
-              float2 ls[F][U];
-              float4 o[F][U];
+          for (int c8 = tid >> lg; c8 < D / 8; c8 += 2 * step) {
+            float a[2][8] = {};
+#pragma unroll 1
+            for (int c0 = 0; c0 < f.nf; c0 += 4) {
+              float2 ls[4];
+              float4 o[4][2][2];
 #pragma unroll
-              for (int c = 0; c < F; ++c) {
-                const int slot = 2 * (f.c0 + min(c0 + c, f.nf - 1)) + (c0 + c == 0 ? 1 : 0);
+              for (int c = 0; c < 4; ++c) {
+                const int slot = slot_of(c0 + c);
+                ls[c] = __ldcg(part_l + static_cast<long long>(slot) * RP + r);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                  const int i = min(i0 + u * ST, f.rows * PR - 1);
-                  const long long at = static_cast<long long>(slot) * RP + i / PR;
-                  ls[c][u] = __ldcg(part_l + at);
-                  o[c][u] = __ldcg(reinterpret_cast<const float4*>(all_o + at * D) + i % PR);
+                for (int u = 0; u < 2; ++u) {
+                  const int col = 8 * min(c8 + u * step, D / 8 - 1);
+                  o[c][u][0] = __ldcg(part_o + part_at(slot, col, r));
+                  o[c][u][1] = __ldcg(part_o + part_at(slot, col + 4, r));
                 }
               }
 #pragma unroll
-              for (int c = 0; c < F; ++c) {
+              for (int c = 0; c < 4; ++c) {
+                if (c0 + c >= f.nf || ls[c].x == -INFINITY) continue;
+                const float w = ex2((ls[c].x - top.x) + (ls[c].y - top.y)) * inv;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                  if (c0 + c >= f.nf || ls[c][u].x == -INFINITY) continue;
-                  float d = (ls[c][u].x - top[u].x) + (ls[c][u].y - top[u].y);
-                  if (top[u].x == -INFINITY) d = INFINITY;
-                  const float e = ex2(-fabsf(d)), scale = d > 0.f ? e : 1.f, w = d > 0.f ? 1.f : e;
-                  if (d > 0.f) top[u] = ls[c][u];
-                  a[u].x = a[u].x * scale + o[c][u].x * w;
-                  a[u].y = a[u].y * scale + o[c][u].y * w;
-                  a[u].z = a[u].z * scale + o[c][u].z * w;
-                  a[u].w = a[u].w * scale + o[c][u].w * w;
-                  sum[u] = sum[u] * scale + w;
+                for (int u = 0; u < 2; ++u) {
+                  const float4 v0 = o[c][u][0], v1 = o[c][u][1];
+                  const float b[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) a[u][i] = fmaf(b[i], w, a[u][i]);
                 }
               }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int i = i0 + u * ST;
-              if (i >= f.rows * PR) continue;
-              const float inv = 1.0f / sum[u];
-              const int ra = f.row0 + i / PR, tt = small_div(ra, p.G);
-              const long long orow = (static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt;
-              uint2 v;
-              v.x = p.bf16 ? pack2<true>(a[u].x * inv, a[u].y * inv) : pack2<false>(a[u].x * inv, a[u].y * inv);
-              v.y = p.bf16 ? pack2<true>(a[u].z * inv, a[u].w * inv) : pack2<false>(a[u].z * inv, a[u].w * inv);
-              *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + (orow * D + 4 * (i % PR)) * 2) = v;
+            for (int u = 0; u < 2; ++u) {
+              if ((tid & ((1 << lg) - 1)) >= f.rows || c8 + u * step >= D / 8) continue;
+              const uint2 lo = pack4(a[u]), hi = pack4(a[u] + 4);
+              *reinterpret_cast<uint4*>(to + 16 * (c8 + u * step)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
           }
         }
