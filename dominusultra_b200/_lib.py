@@ -85,7 +85,7 @@ SIGNATURES = {
     "du_decode_paged_workspace_size": (_sz, [_i] * 6),
     "du_decode_paged": (_i, [_vp] * 10 + [_i] * 8 + [_f, _ll, _vp, _vp, _sz, _vp]),
     "du_extend_paged_workspace_size": (_sz, [_i] * 7),
-    "du_extend_paged": (_i, [_vp] * 11 + [_i] * 9 + [_f, _ll, _vp, _vp, _sz, _vp]),
+    "du_extend_paged": (_i, [_vp] * 11 + [_i] * 9 + [_f, _ll, _vp, _sz, _vp]),
     "du_paged_fork": (_i, [_vp] * 10 + [_i] * 4 + [_vp]),
     "du_paged_copy": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
     "du_paged_compact": (_i, [_vp] * 8 + [_i] * 4 + [_vp]),

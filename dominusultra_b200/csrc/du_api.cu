@@ -1596,14 +1596,15 @@ ExtendPlan extend_plan(int T, int G, int D) {
   ExtendPlan pl{};
   pl.nt = static_cast<long long>(T) * G > 128 && D <= 128 ? 2 : 1;
   pl.grid = sm_count();
-  if (pl.grid > DU_PAGED_TICKETS - 1) pl.grid = DU_PAGED_TICKETS - 1;
   return pl;
 }
 
-// Two partial slots per CTA: rows of an item, fp32, and the log2 of a sum in two parts.
-size_t extend_ws_bytes(const ExtendPlan& pl, int D) {
+// Two partial slots per CTA: rows of an item, fp32, and the log2 of a sum in two parts; then eight words
+// per CTA about an item that was cut.
+size_t extend_part_bytes(const ExtendPlan& pl, int D) {
   return 2 * static_cast<size_t>(pl.grid) * (pl.nt * 128) * (D + 2) * sizeof(float);
 }
+size_t extend_ws_bytes(const ExtendPlan& pl, int D) { return extend_part_bytes(pl, D) + static_cast<size_t>(pl.grid) * 8 * sizeof(int); }
 
 template <int D, int NT>
 int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st) {
@@ -1617,6 +1618,14 @@ int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st)
   if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "paged extend launch");
+  // Where no request's row can hold two key tiles, no item is cut.
+  if (prm.max_len <= S::KT) return DU_OK;
+  constexpr int kShares = (S::RP * (D / 8) + 2 * du::EXTEND_JOIN_THREADS - 1) / (2 * du::EXTEND_JOIN_THREADS);
+  e = launch_kernel(du::extend_join_kernel<D, NT>, dim3(static_cast<unsigned>(grid * kShares)), du::EXTEND_JOIN_THREADS, 0, st, true,
+                    prm, grid, kShares);
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend join launch");
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged extend join launch");
   return DU_OK;
 }
 
@@ -1751,8 +1760,8 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
                     const float* v_scale, const int* block_table, const int* past_seqlens,
                     const int* cache_seqlens, const void* cos, const void* sin, void* out, int B, int Hq,
                     int Hkv, int T, int D, int num_blocks, int block_size, int max_blocks, int dtype,
-                    float scale, long long rope_positions, int* tickets, void* workspace,
-                    size_t workspace_bytes, void* stream) {
+                    float scale, long long rope_positions, void* workspace, size_t workspace_bytes,
+                    void* stream) {
   g_last_error.clear();
   int rc = check_common(B, Hq, Hkv, T, D, dtype);
   if (rc != DU_OK) return rc;
@@ -1762,13 +1771,12 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   if (static_cast<long long>(max_blocks) * block_size > (1LL << 27))
     return fail(DU_ERR_UNSUPPORTED, "a block table row covers more than 2^27 tokens");
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !past_seqlens || !cache_seqlens || !cos ||
-      !sin || !out || !tickets)
+      !sin || !out)
     return fail(DU_ERR_INVALID, "null pointer argument");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(cos) || !aligned16(sin) || !aligned16(out))
     return fail(DU_ERR_INVALID, "q, out, the caches and the rope tables must be 16-byte aligned");
-  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(past_seqlens) ||
-      !aligned4(cache_seqlens) || !aligned4(tickets))
-    return fail(DU_ERR_INVALID, "scales, block_table, the lengths and tickets must be 4-byte aligned");
+  if (!aligned4(k_scale) || !aligned4(v_scale) || !aligned4(block_table) || !aligned4(past_seqlens) || !aligned4(cache_seqlens))
+    return fail(DU_ERR_INVALID, "scales, block_table and the lengths must be 4-byte aligned");
   if (rope_positions <= 0) return fail(DU_ERR_INVALID, "rope tables must hold at least one position");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
   if (Hq > 65536 || T > (1 << 20) || static_cast<long long>(T) * (Hq / Hkv) > (1 << 24) || B > (1 << 20))
@@ -1794,9 +1802,8 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.cos = cos;
   prm.sin = sin;
   prm.out = out;
-  prm.cnt = tickets;
   prm.part = static_cast<float*>(workspace);
-  prm.done = DU_PAGED_TICKETS - 1;
+  prm.split = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + extend_part_bytes(plan, D));
   const long long cover = static_cast<long long>(max_blocks) * block_size;
   prm.max_len = static_cast<int>(cover < rope_positions ? cover : rope_positions);
   prm.bf16 = dtype == DU_DTYPE_BF16;

@@ -22,8 +22,9 @@
 //
 // Work: the items' key tiles, item by item, cut into equal ranges, one per CTA of a persistent grid (an
 // item's beginning is charged with PEN tiles). Lengths are read on the device; every CTA repeats the sum
-// over them. An item within one CTA is written at once; the fragments of others leave fp32 partials, and
-// the CTA that leaves the last one joins them.
+// over them. An item within one CTA is written at once; the fragments of others leave fp32 partials, which
+// a second kernel joins with all SMs (a CTA that joined its item's five fragments of 256 rows took 20-30 us
+// for it at the end of a call, when the others were done).
 //
 // Streams: two softmax warpgroups (one at head_dim 256, where tensor memory holds one O), each with an S, an O
 // and a warp that issues its products. P overwrites S, and O += P V comes before the next S. With NT = 2
@@ -56,11 +57,10 @@ struct ExtendPagedParams {
   const void* cos;    // [positions, D/2]
   const void* sin;
   void* out;          // [B, Hq, T, D]
-  int* cnt;           // tickets, zero between calls; the last one counts the CTAs that are done
   // Partial outs [2 gridDim.x][D / 4][rows] by four columns (neighbouring lanes have neighbouring rows), then
   // the log2 of their sums, in two parts, [2 gridDim.x][rows].
   float* part;
-  int done;           // index of the last ticket
+  int* split;         // [gridDim.x][8]: the item that this CTA has the first of several fragments of
   int max_len;        // tokens that the table's row and the rope tables cover
   int bf16;
   int B, Hq, Hkv, G, T, N, width;
@@ -110,7 +110,7 @@ struct ExtendShape {
                        B_KE = B_KF + NK, B_VF = B_KE + NK, B_VE = B_VF + NV, B_SCF = B_VE + NV, B_SCE = B_SCF + 2,
                        B_QF = B_SCE + 2, B_SF = B_QF + 2, B_PF = B_SF + 2, B_OF = B_PF + 4, B_OD = B_OF + 2,
                        B_FF = B_OD + 2, B_FE = B_FF + NF, B_DR = B_FE + NF, N_BAR = B_DR + 2;
-  static constexpr int OFF_WORDS = OFF_BAR + 8 * N_BAR;  // TMEM address, failed, flag
+  static constexpr int OFF_WORDS = OFF_BAR + 8 * N_BAR;  // TMEM address, failed
   static constexpr int SMEM_BYTES = OFF_WORDS + 16 + 1024;
   static constexpr int TM_S = 0;         // + x KT, x the stream
   static constexpr int TM_O = NS * KT;   // + x D
@@ -367,7 +367,6 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(sgen + S::OFF_WORDS);
   volatile int* failed = reinterpret_cast<volatile int*>(sgen + S::OFF_WORDS + 4);
-  volatile int* joins = reinterpret_cast<volatile int*>(sgen + S::OFF_WORDS + 8);
   volatile int* frags = reinterpret_cast<volatile int*>(sgen + S::OFF_FRAG);
 
   if (tid == 0) {
@@ -864,75 +863,6 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           }
         }
       }
-      if (f.nf > 1) {
-        // The last of the item's fragments joins them: a thread has a row, and twice eight columns of it at
-        // a time, the loads of four fragments in flight.
-        softmax_sync<ST>();
-        if (tid == 0) *joins = atom_add_acq_rel_gpu(p.cnt + f.c0, 1) == f.nf - 1;
-        softmax_sync<ST>();
-        if (*joins) {
-          const int lg = 32 - __clz(f.rows - 1), r = min(tid & ((1 << lg) - 1), f.rows - 1);
-          auto slot_of = [&](int c) { return 2 * (f.c0 + min(c, f.nf - 1)) + (c == 0 ? 1 : 0); };
-          float2 top = make_float2(-INFINITY, 0.f);
-          float sum = 0.f;
-#pragma unroll 1
-          for (int c0 = 0; c0 < f.nf; c0 += 4) {
-            float2 ls[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) ls[c] = __ldcg(part_l + static_cast<long long>(slot_of(c0 + c)) * RP + r);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c0 + c >= f.nf || ls[c].x == -INFINITY) continue;
-              const float d = top.x == -INFINITY ? INFINITY : (ls[c].x - top.x) + (ls[c].y - top.y);
-              const float e = ex2(-fabsf(d));
-              if (d > 0.f) top = ls[c];
-              sum = d > 0.f ? sum * e + 1.f : sum + e;  // (NaN where one is)
-            }
-          }
-          const float inv = 1.0f / sum;
-          const int ra = f.row0 + r, tt = small_div(ra, p.G);
-          uint8_t* to = static_cast<uint8_t*>(p.out) + ((static_cast<long long>(f.b) * p.Hq + f.kvh * p.G + (ra - tt * p.G)) * p.T + tt) * (2 * D);
-          const int step = ST >> lg;
-#pragma unroll 1
-          for (int c8 = tid >> lg; c8 < D / 8; c8 += 2 * step) {
-            float a[2][8] = {};
-#pragma unroll 1
-            for (int c0 = 0; c0 < f.nf; c0 += 4) {
-              float2 ls[4];
-              float4 o[4][2][2];
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const int slot = slot_of(c0 + c);
-                ls[c] = __ldcg(part_l + static_cast<long long>(slot) * RP + r);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  const int col = 8 * min(c8 + u * step, D / 8 - 1);
-                  o[c][u][0] = __ldcg(part_o + part_at(slot, col, r));
-                  o[c][u][1] = __ldcg(part_o + part_at(slot, col + 4, r));
-                }
-              }
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if (c0 + c >= f.nf || ls[c].x == -INFINITY) continue;
-                const float w = ex2((ls[c].x - top.x) + (ls[c].y - top.y)) * inv;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  const float4 v0 = o[c][u][0], v1 = o[c][u][1];
-                  const float b[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) a[u][i] = fmaf(b[i], w, a[u][i]);
-                }
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if ((tid & ((1 << lg) - 1)) >= f.rows || c8 + u * step >= D / 8) continue;
-              const uint2 lo = pack4(a[u]), hi = pack4(a[u] + 4);
-              *reinterpret_cast<uint4*>(to + 16 * (c8 + u * step)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
-          }
-        }
-      }
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------------ rows behind the last token
@@ -1196,6 +1126,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       // ------------------------------------------------------------------ fragments, scales, copies of V
       ExtendWalk<S> walk;
       walk.init(p, lane);
+      int* split = p.split + 8 * blockIdx.x;
+      if (lane == 0) split[0] = 0;
       int nfr = 0, n_batch = 0;
       while (true) {
         ExtendFrag f{};
@@ -1221,6 +1153,13 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           e[12] = f.c0;
           e[13] = f.slot;
           mbar_arrive(FF(slot));
+          if (more && f.nf > 1 && f.j0 == 0) {
+            split[1] = f.b;
+            split[2] = f.kvh;
+            split[3] = f.row0;
+            split[4] = f.rows;
+            split[0] = f.nf;
+          }
         }
         __syncwarp();
         ++nfr;
@@ -1304,10 +1243,58 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     tmem_dealloc(tmem, S::TMEM_COLS);
   }
   if (tid == 0 && *failed) record_timeout(static_cast<unsigned>(*failed));
-  // The CTA that ends last leaves the tickets as they were.
-  if (tid == 0 && atom_add_acq_rel_gpu(p.cnt + p.done, 1) == static_cast<int>(gridDim.x) - 1) {
-    for (int i = 0; i < static_cast<int>(gridDim.x); ++i) p.cnt[i] = 0;
-    p.cnt[p.done] = 0;
+}
+
+// Joins the fragments of items that lie across CTAs. Block (c, k) takes the k-th share of the item that CTA c
+// of the kernel before has the first fragment of, if it has one: a thread has a row, and eight columns of it.
+// Bound by the partials' reads from L2 (and, where there are none, by the launch).
+constexpr int EXTEND_JOIN_THREADS = 256;
+template <int D, int NT>
+__global__ void __launch_bounds__(EXTEND_JOIN_THREADS) extend_join_kernel(const ExtendPagedParams p, int ctas, int shares) {
+  constexpr int RP = ExtendShape<D, NT>::RP;
+  griddep_wait();
+  const int c0 = static_cast<int>(blockIdx.x) / shares, share = static_cast<int>(blockIdx.x) - c0 * shares;
+  const int4 s = __ldcg(reinterpret_cast<const int4*>(p.split) + 2 * c0);
+  const int nf = s.x, b = s.y, kvh = s.z, row0 = s.w;
+  if (nf < 2) return;
+  const int rows = __ldcg(p.split + 8 * c0 + 4);
+  const float4* part_o = reinterpret_cast<const float4*>(p.part);
+  const float2* part_l = reinterpret_cast<const float2*>(p.part + 2LL * ctas * RP * D);
+  auto slot_of = [&](int c) { return 2 * (c0 + min(c, nf - 1)) + (c == 0 ? 1 : 0); };
+  for (int i = share * EXTEND_JOIN_THREADS + static_cast<int>(threadIdx.x); i < rows * (D / 8); i += shares * EXTEND_JOIN_THREADS) {
+    const int c8 = small_div(i, rows), r = i - c8 * rows;
+    float2 top = make_float2(-INFINITY, 0.f);
+    float sum = 0.f, a[8] = {};
+#pragma unroll 1
+    for (int f0 = 0; f0 < nf; f0 += 4) {
+      float2 ls[4];
+      float4 o[4][2];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const long long slot = slot_of(f0 + f);
+        ls[f] = __ldcg(part_l + slot * RP + r);
+        o[f][0] = __ldcg(part_o + (slot * (D / 4) + 2 * c8) * RP + r);
+        o[f][1] = __ldcg(part_o + (slot * (D / 4) + 2 * c8 + 1) * RP + r);
+      }
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        if (f0 + f >= nf || ls[f].x == -INFINITY) continue;  // (of the latter nothing was left but this)
+        const float d = top.x == -INFINITY ? INFINITY : (ls[f].x - top.x) + (ls[f].y - top.y);
+        const float e = ex2(-fabsf(d)), scale = d > 0.f ? e : 1.f, w = d > 0.f ? 1.f : e;  // (NaN where one is)
+        if (d > 0.f) top = ls[f];
+        const float v[8] = {o[f][0].x, o[f][0].y, o[f][0].z, o[f][0].w, o[f][1].x, o[f][1].y, o[f][1].z, o[f][1].w};
+        sum = sum * scale + w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] = a[k] * scale + v[k] * w;
+      }
+    }
+    const float inv = 1.0f / sum;
+    const int ra = row0 + r, t = small_div(ra, p.G);
+    const long long row = (static_cast<long long>(b) * p.Hq + kvh * p.G + (ra - t * p.G)) * p.T + t;
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = p.bf16 ? pack2<true>(a[2 * k] * inv, a[2 * k + 1] * inv) : pack2<false>(a[2 * k] * inv, a[2 * k + 1] * inv);
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (row * D + 8 * c8) * 2) = make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
 

@@ -17,11 +17,12 @@ from .paged import (
     _CODES,
     _GET_DEVICE,
     _HEAD_DIMS,
+    _SCRATCH,
     _check_host_table,
-    _decode_scratch,
     _device_int32,
     _fit_cache,
     _fit_rope,
+    _grow_scratch,
     _lengths,
     _stream_of,
     _validate_int32,
@@ -40,6 +41,18 @@ def _workspace_size(*key) -> int:
     if n is None:
         n = _WS_SIZES[key] = int(_lib.load().du_extend_paged_workspace_size(*key[:-1]))
     return n
+
+
+def _workspace(nbytes: int, index: int, stream: int):
+    """(workspace, what keeps it alive until the launch): the paged decode's of this (device, stream), whose
+    calls run in order; a call that is being captured gets memory of its graph."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        return ws.data_ptr(), ws
+    pair = _SCRATCH.get((index, stream))
+    if pair is None or pair[2] < nbytes:
+        pair = _grow_scratch(nbytes, index, stream)
+    return pair[1], pair
 
 
 def dominus_ultra_extend_paged(
@@ -112,11 +125,11 @@ def dominus_ultra_extend_paged(
     out = torch.empty_like(q_new)
     stream = _stream_of(index)
     nbytes = _workspace_size(B, Hq, Hkv, T, D, block_size, max_blocks, index)
-    tickets, ws, keep = _decode_scratch(nbytes, index, stream)
+    ws, keep = _workspace(nbytes, index, stream)
     rc = _lib.load().du_extend_paged(
         q, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
         past_seqlens.data_ptr(), cache_seqlens.data_ptr(), c, s, out.data_ptr(), B, Hq, Hkv, T, D, num_blocks,
-        block_size, max_blocks, _CODES[dtype], D**-0.5, min(cos.shape[0], sin.shape[0]), tickets, ws, nbytes, stream,
+        block_size, max_blocks, _CODES[dtype], D**-0.5, min(cos.shape[0], sin.shape[0]), ws, nbytes, stream,
     )
     del keep
     if rc:

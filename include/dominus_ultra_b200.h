@@ -331,9 +331,9 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
  * new token t, at position past_seqlens[b] + t, sees the keys up to its own. Rows behind the last new
  * token are zeros. Lengths that are out of range (0 <= past <= cached <= past + T, and cached at most
  * the table's row and rope_positions) give zeros and code 6; a block id out of range gives NaN in the
- * rows that see its keys, and code 7. tickets and workspace (du_extend_paged_workspace_size bytes,
- * 16-byte aligned, any contents) as in du_decode_paged, with which they may be shared by calls that
- * do not overlap. A table row covers at most 2^27 tokens. The caches are as du_paged_write leaves them:
+ * rows that see its keys, and code 7. workspace: du_extend_paged_workspace_size bytes, 16-byte
+ * aligned, any contents; calls that may overlap on the GPU, replayed graphs among them, need one each.
+ * A table row covers at most 2^27 tokens. The caches are as du_paged_write leaves them:
  * no value that is not a number under a finite scale.
  */
 size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size,
@@ -342,7 +342,7 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
                     const float* v_scale, const int* block_table, const int* past_seqlens,
                     const int* cache_seqlens, const void* cos, const void* sin, void* out, int B,
                     int Hq, int Hkv, int T, int D, int num_blocks, int block_size, int max_blocks,
-                    int dtype, float scale, long long rope_positions, int* tickets, void* workspace,
+                    int dtype, float scale, long long rope_positions, void* workspace,
                     size_t workspace_bytes, void* stream);
 
 /*

@@ -151,7 +151,7 @@ def test_c_entry_points_refuse():
 
     def extend(**kw):
         a = dict(q=fake, kc=fake, vc=fake, ks=fake, vs=fake, t=fake, p=fake, ln=fake, c=fake, s=fake, o=fake, B=1, Hq=4, Hkv=2, T=3,
-                 D=64, N=8, bs=16, w=4, dt=_lib.DU_DTYPE_BF16, sc=0.125, rp=64, tk=fake, ws=fake, wsb=1 << 32)
+                 D=64, N=8, bs=16, w=4, dt=_lib.DU_DTYPE_BF16, sc=0.125, rp=64, ws=fake, wsb=1 << 32)
         a.update(kw)
         return lib.du_extend_paged(*a.values(), null)
 
@@ -167,6 +167,9 @@ def test_c_entry_points_refuse():
     assert extend(rp=0) == _lib.DU_ERR_INVALID
     assert extend(sc=0.0) == _lib.DU_ERR_INVALID
     assert extend(dt=_lib.DU_DTYPE_F32) == _lib.DU_ERR_INVALID
+    assert extend(wsb=0) == _lib.DU_ERR_WORKSPACE and extend(ws=null) == _lib.DU_ERR_WORKSPACE
+    assert lib.du_extend_paged_workspace_size(1, 4, 2, 3, 64, 16, 4) > 0
+    assert lib.du_extend_paged_workspace_size(1, 3, 2, 3, 64, 16, 4) == 0
 
 
 class TestPlain:
