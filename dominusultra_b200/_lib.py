@@ -88,7 +88,8 @@ SIGNATURES = {
     "du_extend_paged": (_i, [_vp] * 11 + [_i] * 9 + [_f, _ll, _vp, _sz, _vp]),
     "du_paged_fork": (_i, [_vp] * 10 + [_i] * 4 + [_vp]),
     "du_paged_copy": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
-    "du_paged_compact": (_i, [_vp] * 8 + [_i] * 4 + [_vp]),
+    "du_paged_compact_workspace_size": (_sz, [_i]),
+    "du_paged_compact": (_i, [_vp] * 8 + [_i] * 4 + [_vp, _sz, _vp]),
     "du_selftest_wait_timeout": (_i, [_i, _vp]),
     "du_read_status": (_i, [ctypes.POINTER(ctypes.c_uint), _i]),
 }

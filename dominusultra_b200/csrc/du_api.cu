@@ -1570,17 +1570,16 @@ int check_paged_sets(int B, int max_blocks, int num_blocks, int block_size, long
   if (4 * set_words > du::PAGED_SET_SMEM)
     return fail(DU_ERR_UNSUPPORTED, "the sets of " + std::to_string(num_blocks) + " blocks and " + std::to_string(B) +
                                         " requests do not fit the kernel's shared memory (200 KB: 3 bits a block and "
-                                        "36 a request in a fork, 2.1 bits a block in a compaction)");
+                                        "36 a request in a fork, 2 bits a block in a compaction)");
   return DU_OK;
 }
 
 template <typename Params>
-int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_words, void* stream, const char* what) {
+int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_words, cudaStream_t st, const char* what) {
   // (an attribute of the largest sets, once per device)
   cudaError_t e = ensure_smem_attr(kern, du::PAGED_SET_SMEM);
   if (e != cudaSuccess) return cuda_fail(e, what);
-  e = launch_kernel(kern, dim3(du::PAGED_SET_CTAS), du::PAGED_SET_THREADS, static_cast<size_t>(4 * set_words),
-                    static_cast<cudaStream_t>(stream), true, prm);
+  e = launch_kernel(kern, dim3(du::PAGED_SET_CTAS), du::PAGED_SET_THREADS, static_cast<size_t>(4 * set_words), st, true, prm);
   if (e != cudaSuccess) return cuda_fail(e, what);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, what);
@@ -1677,13 +1676,13 @@ int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* s
   prm.width = max_blocks;
   prm.N = num_blocks;
   prm.block = block_size;
-  return launch_paged_sets(du::paged_fork_kernel, prm, words, stream, "paged fork launch");
+  return launch_paged_sets(du::paged_fork_kernel, prm, words, static_cast<cudaStream_t>(stream), "paged fork launch");
 }
 
 int du_paged_compact(const int* block_table, const int* cache_seqlens, const int* free_blocks,
                      const int* free_state, int* table_out, int* copies, int* free_blocks_out,
                      int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
-                     void* stream) {
+                     void* workspace, size_t workspace_bytes, void* stream) {
   g_last_error.clear();
   const long long words = du::paged_compact_words(num_blocks);
   int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
@@ -1700,7 +1699,12 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
     if (!i) return fail(DU_ERR_INVALID, "null pointer argument");
     if (!aligned4(i)) return fail(DU_ERR_INVALID, "the integer tensors must be 4-byte aligned");
   }
+  const size_t need = du::paged_compact_ws(num_blocks);
+  if (!workspace || workspace_bytes < need)
+    return fail(DU_ERR_WORKSPACE, "workspace of " + std::to_string(need) + " bytes required");
+  if (!aligned16(workspace)) return fail(DU_ERR_INVALID, "workspace must be 16-byte aligned");
   du::PagedCompactParams prm{};
+  prm.map = static_cast<int4*>(workspace);
   prm.table = block_table;
   prm.lens = cache_seqlens;
   prm.ring = free_blocks;
@@ -1713,7 +1717,22 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
   prm.width = max_blocks;
   prm.N = num_blocks;
   prm.block = block_size;
-  return launch_paged_sets(du::paged_compact_kernel, prm, words, stream, "paged compact launch");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  rc = launch_paged_sets(du::paged_compact_kernel, prm, words, st, "paged compact launch");
+  if (rc != DU_OK) return rc;
+  // a thread per entry of the table and per block
+  const long long entries = static_cast<long long>(B) * max_blocks, threads = entries > num_blocks ? entries : num_blocks;
+  const long long ctas = (threads + du::PAGED_APPLY_THREADS - 1) / du::PAGED_APPLY_THREADS, most = 8LL * sm_count();
+  cudaError_t e = launch_kernel(du::paged_compact_rows_kernel, dim3(static_cast<unsigned>(ctas < most ? ctas : most)),
+                                du::PAGED_APPLY_THREADS, 0, st, true, prm);
+  if (e != cudaSuccess) return cuda_fail(e, "paged compact launch");
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "paged compact launch");
+  return DU_OK;
+}
+
+size_t du_paged_compact_workspace_size(int num_blocks) {
+  return num_blocks > 0 && 4 * du::paged_compact_words(num_blocks) <= du::PAGED_SET_SMEM ? du::paged_compact_ws(num_blocks) : 0;
 }
 
 int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* copies, int n,

@@ -202,6 +202,18 @@ def _decode_scratch(nbytes: int, index: int, stream: int):
     return tickets.data_ptr(), ws.data_ptr(), (ws, tickets)
 
 
+def _workspace(nbytes: int, index: int, stream: int):
+    """(workspace, what keeps it alive until the launch): the paged decode's of this (device, stream), whose
+    calls run in order; a call that is being captured gets memory of its graph."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        return ws.data_ptr(), ws
+    pair = _SCRATCH.get((index, stream))
+    if pair is None or pair[2] < nbytes:
+        pair = _grow_scratch(nbytes, index, stream)
+    return pair[1], pair
+
+
 def _grow_scratch(nbytes: int, index: int, stream: int):
     """A (device, stream)'s scratch of at least nbytes, and a ticket slab with room for captures."""
     device = torch.device("cuda", index)

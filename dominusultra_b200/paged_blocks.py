@@ -31,6 +31,7 @@ from .paged import (
     _validate_block_size,
     _validate_int32,
     _validate_paged_cache,
+    _workspace,
 )
 
 __all__ = [
@@ -267,10 +268,13 @@ def dominus_ultra_paged_compact(
     copies = block_table.new_empty((num_blocks // 2, 2))
     ring = torch.empty_like(free_blocks)
     state = torch.empty_like(free_state)
+    stream = _stream_of(index)
+    nbytes = 16 * (1 + (num_blocks + 31) // 32)  # (du_paged_compact_workspace_size, which a test compares)
+    ws, keep = _workspace(nbytes, index, stream)
     rc = _lib.load().du_paged_compact(
         block_table.data_ptr(), cache_seqlens.data_ptr(), free_blocks.data_ptr(), free_state.data_ptr(),
         table.data_ptr(), copies.data_ptr(), ring.data_ptr(), state.data_ptr(), batch, max_blocks, num_blocks,
-        block_size, _stream_of(index),
+        block_size, ws, nbytes, stream,
     )
     if rc:
         _lib.check(rc, "du_paged_compact")

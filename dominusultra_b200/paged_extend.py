@@ -17,16 +17,15 @@ from .paged import (
     _CODES,
     _GET_DEVICE,
     _HEAD_DIMS,
-    _SCRATCH,
     _check_host_table,
     _device_int32,
     _fit_cache,
     _fit_rope,
-    _grow_scratch,
     _lengths,
     _stream_of,
     _validate_int32,
     _validate_paged_cache,
+    _workspace,
     _validate_tables_like,
 )
 
@@ -41,18 +40,6 @@ def _workspace_size(*key) -> int:
     if n is None:
         n = _WS_SIZES[key] = int(_lib.load().du_extend_paged_workspace_size(*key[:-1]))
     return n
-
-
-def _workspace(nbytes: int, index: int, stream: int):
-    """(workspace, what keeps it alive until the launch): the paged decode's of this (device, stream), whose
-    calls run in order; a call that is being captured gets memory of its graph."""
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        return ws.data_ptr(), ws
-    pair = _SCRATCH.get((index, stream))
-    if pair is None or pair[2] < nbytes:
-        pair = _grow_scratch(nbytes, index, stream)
-    return pair[1], pair
 
 
 def dominus_ultra_extend_paged(

@@ -382,12 +382,15 @@ int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
  * then -1; free_blocks_out [num_blocks] the free ids in ascending order, then -1, with free_state_out
  * {0, count}. Outputs must not be inputs. A request whose length is out of range keeps its row, and its
  * blocks stay (code 6). A ring that does not hold `count` different block ids, none of them in use,
- * leaves everything as it is (code 7). At most 770000 blocks.
+ * leaves everything as it is (code 7). At most 819200 blocks. workspace:
+ * du_paged_compact_workspace_size bytes, 16-byte aligned, any contents; calls that may overlap on the
+ * GPU, replayed graphs among them, need one each.
  */
+size_t du_paged_compact_workspace_size(int num_blocks);
 int du_paged_compact(const int* block_table, const int* cache_seqlens, const int* free_blocks,
                      const int* free_state, int* table_out, int* copies, int* free_blocks_out,
                      int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
-                     void* stream);
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Failure-detection self-test (no counterpart in the reference): launches one CTA whose

@@ -119,7 +119,7 @@ def test_c_entry_points_refuse():
         return lib.du_paged_fork(*a.values(), null)
 
     def compact(**kw):
-        a = dict(t=fake, ln=fake, r=fake, st=fake, to=other[0], c=other[1], ro=other[2], so=other[3], B=2, width=4, N=8, bs=16)
+        a = dict(t=fake, ln=fake, r=fake, st=fake, to=other[0], c=other[1], ro=other[2], so=other[3], B=2, width=4, N=8, bs=16, ws=fake, wsb=1 << 20)
         a.update(kw)
         return lib.du_paged_compact(*a.values(), null)
 
@@ -135,6 +135,11 @@ def test_c_entry_points_refuse():
         assert call(ln=odd) == _lib.DU_ERR_INVALID and "4-byte" in _lib.last_error()
         assert call(so=odd) == _lib.DU_ERR_INVALID and "4-byte" in _lib.last_error()
         assert call(to=fake) == _lib.DU_ERR_INVALID and "must not be the inputs" in _lib.last_error()
+    assert compact(ws=null) == _lib.DU_ERR_WORKSPACE and compact(wsb=31) == _lib.DU_ERR_WORKSPACE
+    assert compact(ws=ctypes.c_void_p(0x10008)) == _lib.DU_ERR_INVALID and "workspace" in _lib.last_error()
+    # (what the Python call passes)
+    assert all(lib.du_paged_compact_workspace_size(n) == 16 * (1 + (n + 31) // 32) for n in (1, 32, 33, 819200))
+    assert lib.du_paged_compact_workspace_size(0) == lib.du_paged_compact_workspace_size(819201) == 0
 
     def copy(**kw):
         a = dict(k=fake, v=fake, ks=fake, vs=fake, c=fake, n=3, N=8, H=2, bs=16, D=64)
