@@ -1570,8 +1570,14 @@ int check_paged_sets(int B, int max_blocks, int num_blocks, int block_size, long
   if (4 * set_words > du::PAGED_SET_SMEM)
     return fail(DU_ERR_UNSUPPORTED, "the sets of " + std::to_string(num_blocks) + " blocks and " + std::to_string(B) +
                                         " requests do not fit the kernel's shared memory (200 KB: 3 bits a block and "
-                                        "36 a request in a fork, 2 bits a block in a compaction)");
+                                        "112 a request in a fork, 2.1 bits a block in a compaction)");
   return DU_OK;
+}
+
+int log2_of(int power) {
+  int n = 0;
+  while (power >> (n + 1)) ++n;
+  return n;
 }
 
 template <typename Params>
@@ -1645,8 +1651,11 @@ int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* s
                   int* copies, int* seqlens_out, int* free_state_out, int B, int max_blocks,
                   int num_blocks, int block_size, void* stream) {
   g_last_error.clear();
-  const long long words = du::paged_fork_words(B, num_blocks);
-  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
+  // (the sizes are checked before the sums over them are taken)
+  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, 0);
+  if (rc != DU_OK) return rc;
+  const long long words = num_blocks <= du::PAGED_FORK_BLOCKS ? du::paged_fork_words(B, num_blocks) : du::PAGED_SET_SMEM;
+  rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
   if (rc != DU_OK) return rc;
   const void* ins[] = {block_table, cache_seqlens, sources, new_seqlens, free_state, free_blocks};
   const void* outs[] = {table_out, copies, seqlens_out, free_state_out};
@@ -1676,6 +1685,7 @@ int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* s
   prm.width = max_blocks;
   prm.N = num_blocks;
   prm.block = block_size;
+  prm.shift = log2_of(block_size);
   return launch_paged_sets(du::paged_fork_kernel, prm, words, static_cast<cudaStream_t>(stream), "paged fork launch");
 }
 
@@ -1684,8 +1694,10 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
                      int* free_state_out, int B, int max_blocks, int num_blocks, int block_size,
                      void* workspace, size_t workspace_bytes, void* stream) {
   g_last_error.clear();
-  const long long words = du::paged_compact_words(num_blocks);
-  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
+  int rc = check_paged_sets(B, max_blocks, num_blocks, block_size, 0);
+  if (rc != DU_OK) return rc;
+  const long long words = num_blocks <= du::PAGED_COMPACT_BLOCKS ? du::paged_compact_words(num_blocks) : du::PAGED_SET_SMEM;
+  rc = check_paged_sets(B, max_blocks, num_blocks, block_size, words);
   if (rc != DU_OK) return rc;
   const void* ins[] = {block_table, cache_seqlens, free_blocks, free_state};
   const void* outs[] = {table_out, free_blocks_out, free_state_out, copies};
@@ -1717,6 +1729,7 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
   prm.width = max_blocks;
   prm.N = num_blocks;
   prm.block = block_size;
+  prm.shift = log2_of(block_size);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   rc = launch_paged_sets(du::paged_compact_kernel, prm, words, st, "paged compact launch");
   if (rc != DU_OK) return rc;
@@ -1732,7 +1745,7 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
 }
 
 size_t du_paged_compact_workspace_size(int num_blocks) {
-  return num_blocks > 0 && 4 * du::paged_compact_words(num_blocks) <= du::PAGED_SET_SMEM ? du::paged_compact_ws(num_blocks) : 0;
+  return num_blocks > 0 && num_blocks <= du::PAGED_COMPACT_BLOCKS ? du::paged_compact_ws(num_blocks) : 0;
 }
 
 int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* copies, int n,

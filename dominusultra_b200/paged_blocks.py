@@ -269,7 +269,7 @@ def dominus_ultra_paged_compact(
     ring = torch.empty_like(free_blocks)
     state = torch.empty_like(free_state)
     stream = _stream_of(index)
-    nbytes = 16 * (1 + (num_blocks + 31) // 32)  # (du_paged_compact_workspace_size, which a test compares)
+    nbytes = 16 * (1 + (num_blocks + 127) // 128 * 4)  # (du_paged_compact_workspace_size, which a test compares)
     ws, keep = _workspace(nbytes, index, stream)
     rc = _lib.load().du_paged_compact(
         block_table.data_ptr(), cache_seqlens.data_ptr(), free_blocks.data_ptr(), free_state.data_ptr(),

@@ -358,7 +358,8 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
  * place, nothing else is: outputs must not be inputs. A request whose lengths or source are out of
  * range keeps its row and its blocks (code 6); if more is given back than the ring has room for, or its
  * state is out of range, nothing changes (code 7). num_blocks and B are bounded by the kernel's 200 KB of
- * sets: 3 bits a block and 36 a request (up to 8192 requests and 436000 blocks).
+ * sets: 3 bits a block and 112 a request (at most 8192 requests, and 524287 blocks or, with 8192 requests,
+ * 240000).
  */
 int du_paged_fork(const int* block_table, const int* cache_seqlens, const int* sources,
                   const int* new_seqlens, int* free_blocks, const int* free_state, int* table_out,
@@ -382,7 +383,7 @@ int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
  * then -1; free_blocks_out [num_blocks] the free ids in ascending order, then -1, with free_state_out
  * {0, count}. Outputs must not be inputs. A request whose length is out of range keeps its row, and its
  * blocks stay (code 6). A ring that does not hold `count` different block ids, none of them in use,
- * leaves everything as it is (code 7). At most 819200 blocks. workspace:
+ * leaves everything as it is (code 7). At most 770000 blocks. workspace:
  * du_paged_compact_workspace_size bytes, 16-byte aligned, any contents; calls that may overlap on the
  * GPU, replayed graphs among them, need one each.
  */

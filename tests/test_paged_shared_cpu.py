@@ -137,9 +137,11 @@ def test_c_entry_points_refuse():
         assert call(to=fake) == _lib.DU_ERR_INVALID and "must not be the inputs" in _lib.last_error()
     assert compact(ws=null) == _lib.DU_ERR_WORKSPACE and compact(wsb=31) == _lib.DU_ERR_WORKSPACE
     assert compact(ws=ctypes.c_void_p(0x10008)) == _lib.DU_ERR_INVALID and "workspace" in _lib.last_error()
+    assert fork(N=2**19) == _lib.DU_ERR_UNSUPPORTED and "shared memory" in _lib.last_error()
+    assert fork(N=250000, B=8192) == _lib.DU_ERR_UNSUPPORTED and "shared memory" in _lib.last_error()
     # (what the Python call passes)
-    assert all(lib.du_paged_compact_workspace_size(n) == 16 * (1 + (n + 31) // 32) for n in (1, 32, 33, 819200))
-    assert lib.du_paged_compact_workspace_size(0) == lib.du_paged_compact_workspace_size(819201) == 0
+    assert all(lib.du_paged_compact_workspace_size(n) == 16 * (1 + (n + 127) // 128 * 4) for n in (1, 128, 129, 770000))
+    assert lib.du_paged_compact_workspace_size(0) == lib.du_paged_compact_workspace_size(770001) == 0
 
     def copy(**kw):
         a = dict(k=fake, v=fake, ks=fake, vs=fake, c=fake, n=3, N=8, H=2, bs=16, D=64)
