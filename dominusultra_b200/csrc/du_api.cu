@@ -1592,14 +1592,16 @@ int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_wor
   return DU_OK;
 }
 
-// How the extension's rows are laid out: row tiles of 128 in an item.
+// How the extension's rows are laid out: row tiles of 128 in an item, or copies of its rows in the one tile.
 struct ExtendPlan {
-  int nt, grid;
+  int nt, copies, grid;
 };
 
 ExtendPlan extend_plan(int T, int G, int D) {
   ExtendPlan pl{};
-  pl.nt = static_cast<long long>(T) * G > 128 && D <= 128 ? 2 : 1;
+  const long long rows = static_cast<long long>(T) * G;
+  pl.nt = rows > 128 && D <= 128 ? 2 : 1;
+  pl.copies = rows > 64 ? 1 : (rows > 32 || D == 256 ? 2 : 4);
   pl.grid = sm_count();
   return pl;
 }
@@ -1611,10 +1613,10 @@ size_t extend_part_bytes(const ExtendPlan& pl, int D) {
 }
 size_t extend_ws_bytes(const ExtendPlan& pl, int D) { return extend_part_bytes(pl, D) + static_cast<size_t>(pl.grid) * 8 * sizeof(int); }
 
-template <int D, int NT>
+template <int D, int NT, int CP>
 int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st) {
-  using S = du::ExtendShape<D, NT>;
-  auto kern = du::extend_paged_kernel<D, NT>;
+  using S = du::ExtendShape<D, NT, CP>;
+  auto kern = du::extend_paged_kernel<D, NT, CP>;
   if (launch_registers(kern) < 128)
     return fail(DU_ERR_CUDA, "paged extend kernel built with too few registers for its split");
   cudaError_t e = ensure_smem_attr(kern, S::SMEM_BYTES);
@@ -1637,9 +1639,11 @@ int launch_extend_t(const du::ExtendPagedParams& prm, int grid, cudaStream_t st)
 template <int D>
 int launch_extend(const du::ExtendPagedParams& prm, const ExtendPlan& pl, cudaStream_t st) {
   if constexpr (D <= 128) {
-    if (pl.nt == 2) return launch_extend_t<D, 2>(prm, pl.grid, st);
+    if (pl.nt == 2) return launch_extend_t<D, 2, 1>(prm, pl.grid, st);
+    if (pl.copies == 4) return launch_extend_t<D, 1, 4>(prm, pl.grid, st);
   }
-  return launch_extend_t<D, 1>(prm, pl.grid, st);
+  if (pl.copies == 2) return launch_extend_t<D, 1, 2>(prm, pl.grid, st);
+  return launch_extend_t<D, 1, 1>(prm, pl.grid, st);
 }
 
 }  // namespace

@@ -30,7 +30,10 @@
 // and a warp that issues its products. P overwrites S, and O += P V comes before the next S. With NT = 2
 // (more than 128 rows in an item) a stream is a tile of 128 rows. With NT = 1 the streams share the one row
 // tile and take every other key tile each; a row then has two parts, each with a maximum, sum and O of its
-// own, joined at the fragment's end.
+// own, joined at the fragment's end. A softmax warp has 32 of the row tile's rows, so with 64 rows or fewer
+// most would idle while one has all the keys of a tile to do: there the tile holds two (or, with 32 rows, four)
+// copies of the rows, and a copy's warps take half (a quarter) of each tile's keys, P being zero for the others.
+// Each copy is a part of its rows of its own.
 //
 // Warps (512 threads): 0-3 and 4-7 softmax; 8-11 widen K and V (4-11 at head_dim 256); 12 bulk copies of K;
 // 13 walks the fragments, fetches the scales and copies V; 14 and 15 the products of a stream each (14: and
@@ -75,9 +78,10 @@ constexpr float EXTEND_MOVE = 7.0f;   // how far beyond its reference a row's ma
 constexpr float EXTEND_LARGE = 1024.0f;  // references beyond this are kept in two parts
 constexpr float EXTEND_FAR = 30.0f;   // how far a value scale may be from the fragment's first
 
-template <int D_, int NT_>
+template <int D_, int NT_, int CP_ = 1>
 struct ExtendShape {
   static constexpr int D = D_, NT = NT_;
+  static constexpr int CP = CP_;                 // copies of the row tile's rows
   static constexpr int NS = D <= 128 ? 2 : 1;    // streams
   static constexpr bool ALT = NT < NS;           // that take key tiles in turn
   static constexpr int RP = NT * 128;            // rows of an item
@@ -120,7 +124,11 @@ struct ExtendShape {
   static constexpr int REG_SOFTMAX = 200, REG_WIDEN = NS == 2 ? 64 : 112, REG_ISSUE = NS == 2 ? 48 : 88;
   // Tiles that an item's beginning is charged with.
   static constexpr int PEN = NT == 2 ? 3 : 4;
+  static constexpr int KC = KT / CP;             // keys of a tile that a softmax warp takes
+  static constexpr int RW = 4 / CP;              // softmax warps of a copy
+  static constexpr int PARTS = CP * (ALT ? NS : 1);  // of a row, to be joined
   static_assert(NT <= NS, "a row tile needs a stream");
+  static_assert(CP == 1 || (NT == 1 && (CP == 2 || CP == 4) && KC % 32 == 0), "copies");
   static_assert(TM_O + NS * D <= 512, "tensor memory");
   static_assert(NRV >= 1 && NRK >= NRV && NB * RPT == 8, "copied pieces in flight");
   static_assert(OFF_WORDS + 16 - OFF_MISC <= MISC && SMEM_BYTES <= 232448, "shared memory budget");
@@ -327,9 +335,9 @@ __device__ __forceinline__ bool extend_wait(uint32_t bar, uint32_t parity, volat
   return false;
 }
 
-template <int D, int NT>
+template <int D, int NT, int CP>
 __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const ExtendPagedParams p) {
-  using S = ExtendShape<D, NT>;
+  using S = ExtendShape<D, NT, CP>;
   constexpr int KT = S::KT, RP = S::RP, SPAN = S::SPAN, GPT = S::GPT, NB = S::NB, NS = S::NS, RPT = S::RPT;
   constexpr bool ALT = S::ALT;
   constexpr int NK = S::NK, NV = S::NV, NRK = S::NRK, NRV = S::NRV, NF = S::NF;
@@ -455,6 +463,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     const int x = warp >> 2, w4 = warp & 3;  // stream
     const int xr = ALT ? 0 : x;              // row tile
     const int row = 32 * w4 + lane;          // row of the tile = TMEM lane
+    const int part = w4 / S::RW;             // the copy that the row belongs to
     const uint32_t lane_off = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t q_tile = sbase + S::OFF_Q + xr * S::Q_BYTES;
     const uint32_t s_addr = tmem + lane_off + S::TM_S + x * KT, o_addr = tmem + lane_off + S::TM_O + x * D;
@@ -467,7 +476,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         break;
       }
       const int nt = f.j1 - f.j0, n = tiles_of(f, x);
-      const int r_item = xr * 128 + row;                               // row of the item
+      const int r_item = CP > 1 ? row % (128 / CP) : xr * 128 + row;   // row of the item
       const bool row_ok = r_item < f.rows;
       const int r_all = f.row0 + min(r_item, f.rows - 1);
       const int t = small_div(r_all, p.G);                             // its token and head
@@ -475,7 +484,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       const long long q_row = (static_cast<long long>(f.b) * p.Hq + h) * p.T + t;
       const int kmax = f.past + t;                                     // the last key that it sees
       const int kmin = f.past + small_div(f.row0 + min(xr * 128, f.rows - 1), p.G);  // that every row of the tile sees
-      const bool warp_rows = xr * 128 + 32 * w4 < f.rows;              // some row of the warp is one
+      const bool warp_rows = r_item - lane < f.rows;                   // some row of the warp is one
       float qs = 0.f;  // the row's factor
       bool ok = true;
       if (ALT || n > 0) {
@@ -586,27 +595,25 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           if (!ok) break;
           tc_fence_after();
           const bool first = ALT ? jj < 2 : jj == 0;                 // this stream has no O yet
-          const int lim = kmax - (f.j0 + jj) * KT;                   // columns beyond it are hidden from this row
+          const int lim = kmax - (f.j0 + jj) * KT - part * S::KC;    // columns beyond it are hidden from this row
           const bool diag = (f.j0 + jj) * KT + KT - 1 > kmin;        // some key of the tile is hidden from some row
-          const float* scq = reinterpret_cast<const float*>(sc) + (jj % NB) * GPT;  // (log2 vs 32 words behind, factors 64)
+          const float* scq = reinterpret_cast<const float*>(sc) + (jj % NB) * GPT + part * (S::KC / 16);  // (log2 vs 32 words behind, factors 64)
           if (warp_rows) {
             // S in two halves: the first is reduced while the second loads.
-            constexpr int HALF = KT / 2, NG = KT / 16;
-            float s[KT], kq[NG], ga[NG];
-            tmem_ldn<HALF>(s_addr, s);
+            constexpr int KC = S::KC, HALF = KC / 2, NG = KC / 16;
+            float s[KC], kq[NG], ga[NG];
+            tmem_ldn<HALF>(s_addr + part * KC, s);
 #pragma unroll
-            for (int g = 0; g < NG; g += 4) {
-              const float4 a4 = *reinterpret_cast<const float4*>(scq + g);
-              kq[g] = a4.x * qs;
-              kq[g + 1] = a4.y * qs;
-              kq[g + 2] = a4.z * qs;
-              kq[g + 3] = a4.w * qs;
+            for (int g = 0; g < NG; g += 2) {
+              const float2 a2 = *reinterpret_cast<const float2*>(scq + g);
+              kq[g] = a2.x * qs;
+              kq[g + 1] = a2.y * qs;
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int c0 = 0; c0 < KT; c0 += HALF) {
+            for (int c0 = 0; c0 < KC; c0 += HALF) {
               tmem_wait_ld();
-              if (c0 == 0) tmem_ldn<HALF>(s_addr + HALF, s + HALF);
+              if (c0 == 0) tmem_ldn<HALF>(s_addr + part * KC + HALF, s + HALF);
               if (__builtin_expect(diag, 0)) {
                 // Hidden keys have a score of -inf, and where a whole group is hidden its scales do not count.
 #pragma unroll
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               const float mr = m == -INFINITY ? 0.f : m;
               base = m == -INFINITY ? 0.f : mlo;
 #pragma unroll
-              for (int c = 0; c < KT; ++c) s[c] = less(s[c], kq[c / 16], mr);
+              for (int c = 0; c < KC; ++c) s[c] = less(s[c], kq[c / 16], mr);
 #pragma unroll
               for (int g = 0; g < NG; ++g) kq[g] = 1.f;
               if (far) {
@@ -670,7 +677,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 l = l == 0.f ? 0.f : l * ex2(eo - e0);
                 eo = en;
 #pragma unroll
-                for (int c = 0; c < KT; ++c) l += ex2(s[c] - e0);
+                for (int c = 0; c < KC; ++c) l += ex2(s[c] - e0);
               }
             }
             if (__builtin_expect(any && !first && __any_sync(0xffffffffu, moved), 0)) {
@@ -686,6 +693,12 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 for (int i = 0; i < 16; ++i) o[i] *= alpha;
                 tmem_st16(o_addr + c, o);
               }
+            }
+            if constexpr (CP > 1) {  // nothing for the keys of the other copies
+              const uint32_t none[16] = {};
+#pragma unroll
+              for (int c = 0; c < KT / 2; c += 16)
+                if (c / (KC / 2) != part) tmem_st16u(s_addr + c, none);
             }
             uint64_t acc = f2(0.f, 0.f);
 #pragma unroll
@@ -711,8 +724,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 }
                 acc = f2_fma(sum, f2(iv, iv), acc);
               }
-              tmem_st16u(s_addr + 8 * g, pk);
-              if (g + 2 == NG / 2) {
+              tmem_st16u(s_addr + part * (KC / 2) + 8 * g, pk);
+              if (CP == 1 && g + 2 == NG / 2) {
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -724,12 +737,15 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               l += rs.x + rs.y;
             }
             tmem_wait_st();
-          } else if (lane == 0) {
+          } else if (CP == 1 && lane == 0) {
             mbar_arrive(PF(x, 0));
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(PF(x, 1));
+          if (lane == 0) {
+            if (CP > 1) mbar_arrive(PF(x, 0));
+            mbar_arrive(PF(x, 1));
+          }
           ++n_tile;
         }
         if (jj % NB == NB - 1 || jj == nt - 1) {
@@ -774,7 +790,66 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           }
         }
       };
-      if constexpr (ALT) {
+      if constexpr (CP > 1) {
+        // The parts of a row joined: weights by their sums, then a quarter of the columns at a time, weighted,
+        // through shared memory where the query rows were (a row's 16-byte pieces turned by the row's number). A
+        // thread adds up its own row, of every so many columns.
+        constexpr int PARTS = S::PARTS, ROWS = 128 / CP, CB = D / 4, PC = CB / 4, GROUPS = S::SW / S::RW;
+        const int mine = (ALT ? x * CP : 0) + part;
+        float2* lses = reinterpret_cast<float2*>(sgen + S::OFF_Q);
+        float4* buf = reinterpret_cast<float4*>(sgen + S::OFF_Q);
+        lses[mine * ROWS + r_item] = lse;
+        softmax_sync<ST>();
+        float2 top = make_float2(-INFINITY, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const float2 a = lses[i * ROWS + r_item];
+          if (a.x == -INFINITY) continue;
+          const float d = top.x == -INFINITY ? INFINITY : (a.x - top.x) + (a.y - top.y);
+          const float e = ex2(-fabsf(d));
+          sum = d > 0.f ? sum * e + 1.f : sum + e;  // (NaN where one is)
+          if (d > 0.f || top.x == -INFINITY) top = a;
+        }
+        softmax_sync<ST>();
+        if (lse.x != -INFINITY) w1 *= ex2((lse.x - top.x) + (lse.y - top.y)) / sum;
+        if (top.x != -INFINITY) top.y += lg2(sum);
+        if (f.nf > 1 && mine == 0 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = top;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += CB) {
+          if (warp_rows) {
+            float o[CB];
+            if (n > 0) {
+              tmem_ldn<CB>(o_addr + c0, o);
+              tmem_wait_ld();
+            }
+            if (row_ok) {
+#pragma unroll
+              for (int i = 0; i < PC; ++i)
+                buf[(mine * ROWS + r_item) * PC + (i + row) % PC] =
+                    n > 0 ? make_float4(o[4 * i] * w1 * w2, o[4 * i + 1] * w1 * w2, o[4 * i + 2] * w1 * w2, o[4 * i + 3] * w1 * w2) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+          softmax_sync<ST>();
+          if (row_ok) {
+#pragma unroll 1
+            for (int c = mine; c < PC; c += GROUPS) {
+              float a[4] = {};
+#pragma unroll
+              for (int i = 0; i < PARTS; ++i) {
+                // (the turn is by the writer's row of the tile)
+                const float4 b = buf[(i * ROWS + r_item) * PC + (c + (i % CP) * ROWS + r_item) % PC];
+                a[0] += b.x;
+                a[1] += b.y;
+                a[2] += b.z;
+                a[3] += b.w;
+              }
+              put(c0 + 4 * c, a);
+            }
+          }
+          softmax_sync<ST>();
+        }
+      } else if constexpr (ALT) {
         // The two parts of a row joined: weights by their sums, then each stream finishes half of the columns,
         // a quarter of D at a time, the other's share of which comes through shared memory where the query
         // rows were (a row's 16-byte pieces turned by the row's number).
