@@ -1601,7 +1601,7 @@ ExtendPlan extend_plan(int T, int G, int D) {
   ExtendPlan pl{};
   const long long rows = static_cast<long long>(T) * G;
   pl.nt = rows > 128 && D <= 128 ? 2 : 1;
-  pl.copies = rows > 64 ? 1 : (rows > 32 || D == 256 ? 2 : 4);
+  pl.copies = rows > 64 || D == 256 ? 1 : (rows > 32 ? 2 : 4);
   pl.grid = sm_count();
   return pl;
 }

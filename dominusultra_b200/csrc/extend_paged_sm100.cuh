@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     while (true) {
       const ExtendFrag f = take();
       if (f.kind <= 0) {
-        softmax_any<ST>(f.kind < 0);
+        if (S::PARTS > 1) softmax_any<ST>(f.kind < 0);
         break;
       }
       const int nt = f.j1 - f.j0, n = tiles_of(f, x);
@@ -488,42 +488,50 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       float qs = 0.f;  // the row's factor
       bool ok = true;
       if (ALT || n > 0) {
-        // The query row: rotated in fp32, times a power of two that brings its largest input to
-        // [2^8, 2^9), as fp16. (Streams that share the rows rotate half of a row each.)
-        constexpr int PQ = ALT && D >= 32 ? D / 32 : D / 16;  // pairs of 16-byte pieces of this thread
-        constexpr int PL = PQ < 2 ? PQ : 2;                   // at a time (more would be code fetched once)
-        const uint8_t* src = static_cast<const uint8_t*>(p.q) + q_row * (2 * D);
-        const int c0 = ALT && D >= 32 ? x * PQ : 0;
-        const uint8_t* cp = static_cast<const uint8_t*>(p.cos) + static_cast<long long>(kmax) * D;
-        const uint8_t* sp = static_cast<const uint8_t*>(p.sin) + static_cast<long long>(kmax) * D;
+        // The warp's query rows: rotated in fp32, times a power of two (of each row) that brings its largest input
+        // to [2^8, 2^9), as fp16. LPR lanes share a row, each with a pair of 16-byte pieces at a time: a row per
+        // lane would touch 32 lines with each load, 4 us for 256 rows. First the rows as they are, where they
+        // belong, and the largest of each; then the rotation in place. Streams that share the rows take turns.
+        constexpr int LPR = D / 16, RPS = 32 / LPR;
+        constexpr int UN = LPR < 8 ? LPR : 8;  // steps in flight
+        const int piece = lane % LPR, in_step = lane / LPR;
+        const int steps = min(LPR, (f.rows - (r_item - lane) + RPS - 1) / RPS);  // that have rows
         if (warp_rows) {
+          const uint8_t* cp = static_cast<const uint8_t*>(p.cos) + static_cast<long long>(kmax) * D;
+          const uint8_t* sp = static_cast<const uint8_t*>(p.sin) + static_cast<long long>(kmax) * D;
           for (int i = 0; i < D; i += 128) {
             prefetch_l1(cp + i);
             prefetch_l1(sp + i);
           }
-          // The row's pieces, this thread's first; they wait in their places for their rotation.
           uint32_t top = 0u;
-          uint4 v[D / 8];
+          const int q_row_lo = static_cast<int>(q_row), q_row_hi = static_cast<int>(q_row >> 32);
+          auto row_of = [&](int from) {
+            return static_cast<long long>(__shfl_sync(0xffffffffu, q_row_hi, from)) << 32 | static_cast<uint32_t>(__shfl_sync(0xffffffffu, q_row_lo, from));
+          };
+#pragma unroll 1
+          for (int s0 = 0; s0 < steps; s0 += UN) {
+            uint4 a[UN], b[UN];
 #pragma unroll
-          for (int i = 0; i < PQ; ++i) {
-            v[i] = ldg_v4(src + 16 * (c0 + i));
-            v[PQ + i] = ldg_v4(src + 16 * (c0 + i + D / 16));
-          }
-          if constexpr (2 * PQ < D / 8) {
-#pragma unroll
-            for (int i = 0; i < PQ; ++i) {
-              v[2 * PQ + i] = ldg_v4(src + 16 * (PQ - c0 + i));
-              v[3 * PQ + i] = ldg_v4(src + 16 * (PQ - c0 + i + D / 16));
+            for (int i = 0; i < UN; ++i) {
+              const uint8_t* src = static_cast<const uint8_t*>(p.q) + row_of((s0 + i) * RPS + in_step) * (2 * D) + 16 * piece;
+              a[i] = ldg_v4(src);
+              b[i] = ldg_v4(src + D);
             }
-          }
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
-          if (!(ALT && D < 32) || x == 0) {
+            for (int i = 0; i < UN; ++i) {
+              const int at = 32 * w4 + (s0 + i) * RPS + in_step;
+              if (!ALT || (i & 1) == x) {  // (s0 is even, or 0)
+                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, at, piece), a[i]);
+                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, at, piece + LPR), b[i]);
+              }
+              uint32_t big = 0u;
+              const uint32_t w[8] = {a[i].x, a[i].y, a[i].z, a[i].w, b[i].x, b[i].y, b[i].z, b[i].w};
 #pragma unroll
-            for (int i = 0; i < PQ; ++i) {
-              st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, c0 + i), v[i]);
-              st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, c0 + i + D / 16), v[PQ + i]);
+              for (int k = 0; k < 8; ++k) big = __vmaxu2(big, w[k] & 0x7fff7fffu);
+#pragma unroll
+              for (int o = 1; o < LPR; o <<= 1) big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
+              big = __shfl_sync(0xffffffffu, big, lane % RPS * LPR);
+              if (lane / RPS == s0 + i) top = big;
             }
           }
           const float2 tops = p.bf16 ? split2<true>(top) : split2<false>(top);
@@ -531,19 +539,28 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           int e = static_cast<int>(top_bits >> 23) - 127;
           if (e == -127 || e == 128) e = 8;  // (zero, or not finite)
           e = min(max(e - 8, -100), 100);
-          const float up = __int_as_float((127 - e) << 23);
+          const float up_own = __int_as_float((127 - e) << 23);
           qs = __int_as_float((127 + e) << 23);
+          __syncwarp();
           auto rotate = [&](auto bf16) {
             constexpr bool BF = decltype(bf16)::value;
+            constexpr int TURN = ALT ? 2 : 1, PL = LPR < 2 * TURN ? 1 : 2;  // (more at a time would be code fetched once)
 #pragma unroll 1
-            for (int i0 = c0; i0 < c0 + PQ; i0 += PL) {
+            for (int s0 = ALT ? x : 0; s0 < steps; s0 += TURN * PL) {
               uint4 a[PL], b[PL], c[PL], s[PL];
+              uint32_t lo_at[PL], hi_at[PL];
+              float up[PL];
 #pragma unroll
               for (int i = 0; i < PL; ++i) {
-                a[i] = ld_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i));
-                b[i] = ld_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i + D / 16));
-                c[i] = ldg_v4(cp + 16 * (i0 + i));
-                s[i] = ldg_v4(sp + 16 * (i0 + i));
+                const int from = (s0 + i * TURN) * RPS + in_step, at = 32 * w4 + from;  // (rows past the last step's: below 32)
+                up[i] = __shfl_sync(0xffffffffu, up_own, from);
+                const int pos = __shfl_sync(0xffffffffu, kmax, from);
+                lo_at[i] = q_tile + swz_chunk_offset<SPAN>(128, at, piece);
+                hi_at[i] = q_tile + swz_chunk_offset<SPAN>(128, at, piece + LPR);
+                a[i] = ld_shared_v4(lo_at[i]);
+                b[i] = ld_shared_v4(hi_at[i]);
+                c[i] = ldg_v4(static_cast<const uint8_t*>(p.cos) + static_cast<long long>(pos) * D + 16 * piece);
+                s[i] = ldg_v4(static_cast<const uint8_t*>(p.sin) + static_cast<long long>(pos) * D + 16 * piece);
               }
 #pragma unroll
               for (int i = 0; i < PL; ++i) {
@@ -552,21 +569,19 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 uint32_t lo[4], hi[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  const uint64_t U = f2(up, up), C = widen2<BF>(ca[k]), N = widen2<BF>(sa[k]);
+                  const uint64_t U = f2(up[i], up[i]), C = widen2<BF>(ca[k]), N = widen2<BF>(sa[k]);
                   const uint64_t A = f2_mul(widen2<BF>(aa[k]), U), B = f2_mul(widen2<BF>(ba[k]), U);
                   const float2 l2 = f2_split(f2_fma(B, f2_mul(N, f2(-1.f, -1.f)), f2_mul(A, C))), h2 = f2_split(f2_fma(A, N, f2_mul(B, C)));
                   lo[k] = pack2<false>(l2.x, l2.y);
                   hi[k] = pack2<false>(h2.x, h2.y);
                 }
-                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, i0 + i + D / 16), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                st_shared_v4(lo_at[i], make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                st_shared_v4(hi_at[i], make_uint4(hi[0], hi[1], hi[2], hi[3]));
               }
             }
           };
-          if (!(ALT && D < 32) || x == 0) {
-            if (p.bf16) rotate(std::true_type{});
-            else rotate(std::false_type{});
-          }
+          if (p.bf16) rotate(std::true_type{});
+          else rotate(std::false_type{});
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -755,8 +770,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         }
       }
       if (ok && n > 0) ok = __all_sync(0xffffffffu, extend_wait(OF(x), n_of++ & 1, failed, 505));
-      // Every softmax warp comes here once per fragment, whatever happened to it, and all go on or none.
-      if (softmax_any<ST>(!ok)) break;
+      // Where a row has parts, every softmax warp comes here once per fragment, whatever happened to it, and all
+      // go on or none. Else each goes its own way (the others' waits expire with its own).
+      if (S::PARTS > 1 ? softmax_any<ST>(!ok) : !ok) break;
       tc_fence_after();
       // The log2 of the row's (or its part's) sum, in two parts; and what brings O to the fragment's output,
       // O 2^(m + mlo - 8) over the sum, in two factors since the exponent may be large.
@@ -815,30 +831,33 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         if (lse.x != -INFINITY) w1 *= ex2((lse.x - top.x) + (lse.y - top.y)) / sum;
         if (top.x != -INFINITY) top.y += lg2(sum);
         if (f.nf > 1 && mine == 0 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = top;
+        // (two quarters, or all, where half or a quarter of the rows are there)
+        const int at_once = f.rows > ROWS / 2 ? 1 : (f.rows > ROWS / 4 ? 2 : 4), rows_p = ROWS / at_once;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += CB) {
-          if (warp_rows) {
+        for (int c0 = 0; c0 < D; c0 += at_once * CB) {
+#pragma unroll 1
+          for (int q = 0; q < at_once; ++q) {
+            if (!warp_rows) continue;
             float o[CB];
             if (n > 0) {
-              tmem_ldn<CB>(o_addr + c0, o);
+              tmem_ldn<CB>(o_addr + c0 + q * CB, o);
               tmem_wait_ld();
             }
             if (row_ok) {
 #pragma unroll
               for (int i = 0; i < PC; ++i)
-                buf[(mine * ROWS + r_item) * PC + (i + row) % PC] =
+                buf[((q * PARTS + mine) * rows_p + r_item) * PC + (i + r_item) % PC] =
                     n > 0 ? make_float4(o[4 * i] * w1 * w2, o[4 * i + 1] * w1 * w2, o[4 * i + 2] * w1 * w2, o[4 * i + 3] * w1 * w2) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
           }
           softmax_sync<ST>();
           if (row_ok) {
 #pragma unroll 1
-            for (int c = mine; c < PC; c += GROUPS) {
+            for (int c = mine; c < at_once * PC; c += GROUPS) {
               float a[4] = {};
 #pragma unroll
               for (int i = 0; i < PARTS; ++i) {
-                // (the turn is by the writer's row of the tile)
-                const float4 b = buf[(i * ROWS + r_item) * PC + (c + (i % CP) * ROWS + r_item) % PC];
+                const float4 b = buf[((c / PC * PARTS + i) * rows_p + r_item) * PC + (c + r_item) % PC];
                 a[0] += b.x;
                 a[1] += b.y;
                 a[2] += b.z;
@@ -921,20 +940,41 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       } else {
         if (f.nf > 1 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = lse;
         if (n > 0 && warp_rows) {
+          // Whole items' rows go out through shared memory, where the query rows were, so that lanes share lines.
+          const uint32_t mine = q_tile + row * (2 * D);
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             float o[16];
             tmem_ld16(o_addr + c, o);
             tmem_wait_ld();
-            if (row_ok) {
 #pragma unroll
-              for (int k = 0; k < 16; k += 8) {
-                float a[8];
+            for (int i = 0; i < 16; ++i) o[i] = o[i] * w1 * w2;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = o[k + i] * w1 * w2;
-                put(c + k, a);
+            for (int k = 0; k < 16; k += 8) {
+              if (f.nf > 1) {
+                if (row_ok) {
+                  part_o[part_at(f.slot, c + k, r_item)] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                  part_o[part_at(f.slot, c + k + 4, r_item)] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
+                }
+              } else {
+                const uint2 u = pack4(o + k), v = pack4(o + k + 4);
+                st_shared_v4(mine + 16 * (((c + k) / 8 + row) % (D / 8)), make_uint4(u.x, u.y, v.x, v.y));
               }
             }
+          }
+          if (f.nf == 1) {
+            constexpr int LPO = D / 8, RPO = 32 / LPO;  // lanes that share a row, rows of a step
+            const int q_row_lo = static_cast<int>(q_row), q_row_hi = static_cast<int>(q_row >> 32);
+            __syncwarp();
+#pragma unroll 2
+            for (int i = 0; i < LPO; ++i) {
+              const int from = i * RPO + lane / LPO, at = 32 * w4 + from;
+              const long long to = static_cast<long long>(__shfl_sync(0xffffffffu, q_row_hi, from)) << 32 |
+                                   static_cast<uint32_t>(__shfl_sync(0xffffffffu, q_row_lo, from));
+              const uint4 v = ld_shared_v4(q_tile + at * (2 * D) + 16 * ((lane % LPO + at) % LPO));
+              if (r_item - lane + from < f.rows) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + to * (2 * D) + 16 * (lane % LPO)) = v;
+            }
+            __syncwarp();
           }
         }
       }
