@@ -26,14 +26,19 @@
 // a second kernel joins with all SMs (a CTA that joined its item's five fragments of 256 rows took 20-30 us
 // for it at the end of a call, when the others were done).
 //
-// Streams: two softmax warpgroups (one at head_dim 256, where tensor memory holds one O), each with an S, an O
-// and a warp that issues its products. P overwrites S, and O += P V comes before the next S. With NT = 2
-// (more than 128 rows in an item) a stream is a tile of 128 rows. With NT = 1 the streams share the one row
-// tile and take every other key tile each; a row then has two parts, each with a maximum, sum and O of its
-// own, joined at the fragment's end. A softmax warp has 32 of the row tile's rows, so with 64 rows or fewer
-// most would idle while one has all the keys of a tile to do: there the tile holds two (or, with 32 rows, four)
-// copies of the rows, and a copy's warps take half (a quarter) of each tile's keys, P being zero for the others.
-// Each copy is a part of its rows of its own.
+// Streams: two softmax warpgroups (one at head_dim 256, where tensor memory holds one O), each with an O and a
+// warp that issues its products. P overwrites its S.
+//  - NT = 2 (more than 128 rows in an item): a stream is a tile of 128 rows. It has two tiles of S of 64 keys, so
+//    that a warpgroup goes from tile to tile without waiting for products (also at head_dim 256, with one row tile).
+//  - NT = 1: the streams share the one row tile and take every other key tile of 128 each; a row then has two
+//    parts, each with a maximum, sum and O of its own, joined at the fragment's end. What bounds these is shared
+//    memory: of the bytes that widening and products move per key there, the query rows' are per tile, so tiles are
+//    long (with 64 keys 117 -> 122 us for 16 requests of 128 rows behind 10000 keys), and the other stream's
+//    softmax fills the time in which one waits.
+//  - Copies: a softmax warp has 32 of the row tile's rows, so with 64 rows or fewer most would idle while one has all
+//    the keys of a tile to do: there the tile holds two (or, with 32 rows, four) copies of the rows, and a copy's
+//    warps take half (a quarter) of each tile's keys, P being zero for the others. Each copy is a part of its
+//    rows of its own. (At head_dim 256 joining the copies cost as much as they gave.)
 //
 // Warps (512 threads): 0-3 and 4-7 softmax; 8-11 widen K and V (4-11 at head_dim 256); 12 bulk copies of K;
 // 13 walks the fragments, fetches the scales and copies V; 14 and 15 the products of a stream each (14: and
@@ -85,7 +90,8 @@ struct ExtendShape {
   static constexpr int NS = D <= 128 ? 2 : 1;    // streams
   static constexpr bool ALT = NT < NS;           // that take key tiles in turn
   static constexpr int RP = NT * 128;            // rows of an item
-  static constexpr int KT = D == 256 ? 64 : 128; // keys of a tile
+  static constexpr int SB = NT == 2 || D == 256 ? 2 : 1;  // tiles of S of a stream
+  static constexpr int KT = SB == 2 ? 64 : 128;  // keys of a tile
   static constexpr int SPAN = 2 * D >= 128 ? 128 : 2 * D;  // bytes per row of a swizzled block
   static constexpr int GPT = KT / 16;            // groups of 16 keys in a tile
   static constexpr int NB = 32 / GPT;            // tiles of a batch of scales
@@ -94,7 +100,7 @@ struct ExtendShape {
   static constexpr int RK = 64;                  // keys of a copied piece
   static constexpr int RPT = KT / RK;            // pieces of a tile
   static constexpr int RAW = RK * D;
-  static constexpr int NK = 2, NV = D == 256 ? 1 : 2;  // widened tiles
+  static constexpr int NK = D == 256 || SB == 1 ? 2 : 3, NV = D == 256 ? 1 : NK;  // widened tiles
   static constexpr int MISC = 2048;
   static constexpr int RAWS = (231424 - MISC - NT * Q_BYTES - (NK + NV) * T_BYTES) / RAW;
   static constexpr int NRV = RAWS / 2 > 8 ? 8 : RAWS / 2;             // copied pieces of V in flight
@@ -112,23 +118,23 @@ struct ExtendShape {
   static constexpr int OFF_BAR = OFF_FRAG + NF * 64;
   static constexpr int B_RKF = 0, B_RKE = B_RKF + NRK, B_RVF = B_RKE + NRK, B_RVE = B_RVF + NRV, B_KF = B_RVE + NRV,
                        B_KE = B_KF + NK, B_VF = B_KE + NK, B_VE = B_VF + NV, B_SCF = B_VE + NV, B_SCE = B_SCF + 2,
-                       B_QF = B_SCE + 2, B_SF = B_QF + 2, B_PF = B_SF + 2, B_OF = B_PF + 4, B_OD = B_OF + 2,
+                       B_QF = B_SCE + 2, B_SF = B_QF + 2, B_PF = B_SF + 4, B_OF = B_PF + 4, B_OD = B_OF + 2,
                        B_FF = B_OD + 2, B_FE = B_FF + NF, B_DR = B_FE + NF, N_BAR = B_DR + 2;
   static constexpr int OFF_WORDS = OFF_BAR + 8 * N_BAR;  // TMEM address, failed
   static constexpr int SMEM_BYTES = OFF_WORDS + 16 + 1024;
-  static constexpr int TM_S = 0;         // + x KT, x the stream
-  static constexpr int TM_O = NS * KT;   // + x D
+  static constexpr int TM_S = 0;             // + (SB x + tile % SB) KT, x the stream
+  static constexpr int TM_O = NS * SB * KT;  // + x D
   static constexpr int TMEM_COLS = TM_O + NS * D <= 256 ? 256 : 512;
   static constexpr int SW = 4 * NS;      // softmax warps
   static constexpr int WC = NS == 2 ? 2 : 4;  // warps that widen K, and as many V
   static constexpr int REG_SOFTMAX = 200, REG_WIDEN = NS == 2 ? 64 : 112, REG_ISSUE = NS == 2 ? 48 : 88;
   // Tiles that an item's beginning is charged with.
-  static constexpr int PEN = NT == 2 ? 3 : 4;
+  static constexpr int PEN = KT == 64 ? 6 : 5;
   static constexpr int KC = KT / CP;             // keys of a tile that a softmax warp takes
   static constexpr int RW = 4 / CP;              // softmax warps of a copy
   static constexpr int PARTS = CP * (ALT ? NS : 1);  // of a row, to be joined
   static_assert(NT <= NS, "a row tile needs a stream");
-  static_assert(CP == 1 || (NT == 1 && (CP == 2 || CP == 4) && KC % 32 == 0), "copies");
+  static_assert(CP == 1 || (NT == 1 && (CP == 2 || CP == 4) && KC % 16 == 0), "copies");
   static_assert(TM_O + NS * D <= 512, "tensor memory");
   static_assert(NRV >= 1 && NRK >= NRV && NB * RPT == 8, "copied pieces in flight");
   static_assert(OFF_WORDS + 16 - OFF_MISC <= MISC && SMEM_BYTES <= 232448, "shared memory budget");
@@ -301,6 +307,19 @@ __device__ __forceinline__ void tmem_ldn(uint32_t taddr, float* v) {
   }
 }
 
+// Eight or sixteen columns of tensor memory, written.
+template <int N>
+__device__ __forceinline__ void tmem_stn(uint32_t taddr, const uint32_t* v) {
+  static_assert(N == 8 || N == 16, "columns");
+  if constexpr (N == 16) {
+    tmem_st16u(taddr, v);
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  }
+}
+
 // A barrier of the softmax warps, and one that says whether `bad` is set in any of their threads.
 template <int THREADS>
 __device__ __forceinline__ void softmax_sync() {
@@ -344,9 +363,13 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
   constexpr uint32_t SWZ = swizzle_code(SPAN);
   constexpr uint32_t IDESC_QK = idesc_f16(128, KT, 0, 0, 0, 0);
   constexpr uint32_t IDESC_PV = idesc_f16(128, D, 0, 0, 0, 1);
-  // The products of one thread are known to complete in order if they are of one shape; else the end of
-  // P V is waited for before its P is overwritten by the next S.
-  constexpr bool ORDERED = D == KT;
+
+  // The place of a stream's n-th tile of S, and the parity of its barriers.
+  auto place = [](int n) { return S::SB == 2 ? n & 1 : 0; };
+  auto turn = [](int n) { return S::SB == 2 ? (n >> 1) & 1 : n & 1; };
+  // With one tile of S, P V begins with half of P. The products of one thread are known to complete in order if
+  // they are of one shape; else the end of P V is waited for before its P is overwritten by a later S.
+  constexpr bool HALVES = S::SB == 1 && CP == 1, ORDERED = S::SB == 1 && D == KT;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -364,9 +387,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
   auto SCF = [&](int s) { return bar(S::B_SCF + s); };  // batch of scales written
   auto SCE = [&](int s) { return bar(S::B_SCE + s); };  // read by the softmax warps and those that widen V
   auto QF = [&](int x) { return bar(S::B_QF + x); };    // query rows written
-  auto SF = [&](int x) { return bar(S::B_SF + x); };    // S of stream x complete, and its O of the tile before
-  auto PF = [&](int x, int half) { return bar(S::B_PF + 2 * x + half); };  // half of P written
-  auto OD = [&](int x) { return bar(S::B_OD + x); };    // P V of a tile done (not ORDERED)
+  auto SF = [&](int x, int i) { return bar(S::B_SF + 2 * x + i); };  // S of stream x complete, in place i
+  auto PF = [&](int x, int i) { return bar(S::B_PF + 2 * x + i); };  // P written, in place i (HALVES: its i-th half)
+  auto OD = [&](int x) { return bar(S::B_OD + x); };    // P V of a tile done
   auto OF = [&](int x) { return bar(S::B_OF + x); };    // O of stream x final
   auto FF = [&](int i) { return bar(S::B_FF + i); };    // fragment entry written
   auto FE = [&](int i) { return bar(S::B_FE + i); };    // and read by every warp that takes it
@@ -398,9 +421,10 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       mbar_init(SCF(s), 1);
       mbar_init(SCE(s), S::SW + S::WC);
       mbar_init(QF(s), ALT ? 8 : 4);
-      mbar_init(SF(s), 1);
-      mbar_init(PF(s, 0), 4);
-      mbar_init(PF(s, 1), 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(SF(s, i), 1);
+        mbar_init(PF(s, i), 4);
+      }
       mbar_init(OD(s), 1);
       mbar_init(OF(s), 1);
       mbar_init(DR(s), 1);
@@ -466,7 +490,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
     const int part = w4 / S::RW;             // the copy that the row belongs to
     const uint32_t lane_off = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t q_tile = sbase + S::OFF_Q + xr * S::Q_BYTES;
-    const uint32_t s_addr = tmem + lane_off + S::TM_S + x * KT, o_addr = tmem + lane_off + S::TM_O + x * D;
+    const uint32_t s_addr0 = tmem + lane_off + S::TM_S + S::SB * x * KT, o_addr = tmem + lane_off + S::TM_O + x * D;
     constexpr int ST = 32 * S::SW;           // softmax threads
     int n_tile = 0, n_batch = 0, n_of = 0;
     while (true) {
@@ -606,24 +630,21 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           }
         }
         if (ALT ? (jj & 1) == x : jj < n) {
-          ok = __all_sync(0xffffffffu, extend_wait(SF(x), n_tile & 1, failed, 503));
+          ok = __all_sync(0xffffffffu, extend_wait(SF(x, place(n_tile)), turn(n_tile), failed, 503));
           if (!ok) break;
           tc_fence_after();
+          const uint32_t s_addr = s_addr0 + place(n_tile) * KT;
           const bool first = ALT ? jj < 2 : jj == 0;                 // this stream has no O yet
           const int lim = kmax - (f.j0 + jj) * KT - part * S::KC;    // columns beyond it are hidden from this row
           const bool diag = (f.j0 + jj) * KT + KT - 1 > kmin;        // some key of the tile is hidden from some row
           const float* scq = reinterpret_cast<const float*>(sc) + (jj % NB) * GPT + part * (S::KC / 16);  // (log2 vs 32 words behind, factors 64)
           if (warp_rows) {
             // S in two halves: the first is reduced while the second loads.
-            constexpr int KC = S::KC, HALF = KC / 2, NG = KC / 16;
+            constexpr int KC = S::KC, HALF = KC / 2, NG = KC / 16, GS = NG < 2 ? 1 : 2;
             float s[KC], kq[NG], ga[NG];
             tmem_ldn<HALF>(s_addr + part * KC, s);
 #pragma unroll
-            for (int g = 0; g < NG; g += 2) {
-              const float2 a2 = *reinterpret_cast<const float2*>(scq + g);
-              kq[g] = a2.x * qs;
-              kq[g + 1] = a2.y * qs;
-            }
+            for (int g = 0; g < NG; ++g) kq[g] = scq[g] * qs;
             float mx = -INFINITY;
 #pragma unroll
             for (int c0 = 0; c0 < KC; c0 += HALF) {
@@ -696,7 +717,11 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               }
             }
             if (__builtin_expect(any && !first && __any_sync(0xffffffffu, moved), 0)) {
-              // (S being there says that O has the products of the tiles before)
+              // (O has to have the products of the tile before; the one tile of S is there after them)
+              if (S::SB == 2) {
+                ok = __all_sync(0xffffffffu, extend_wait(OD(x), (n_tile - 1) & 1, failed, 504));
+                tc_fence_after();
+              }
               const float alpha = moved && m_old != -INFINITY ? ex2((m_old - m) + (mlo_old - mlo)) : 1.0f;
               if (!far) l *= alpha;
 #pragma unroll 1
@@ -710,17 +735,18 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               }
             }
             if constexpr (CP > 1) {  // nothing for the keys of the other copies
-              const uint32_t none[16] = {};
+              constexpr int W = KC / 2 < 16 ? KC / 2 : 16;
+              const uint32_t none[W] = {};
 #pragma unroll
-              for (int c = 0; c < KT / 2; c += 16)
-                if (c / (KC / 2) != part) tmem_st16u(s_addr + c, none);
+              for (int c = 0; c < KT / 2; c += W)
+                if (c / (KC / 2) != part) tmem_stn<W>(s_addr + c, none);
             }
             uint64_t acc = f2(0.f, 0.f);
 #pragma unroll
-            for (int g = 0; g < NG; g += 2) {
-              uint32_t pk[16];
+            for (int g = 0; g < NG; g += GS) {
+              uint32_t pk[8 * GS];
 #pragma unroll
-              for (int q = g; q < g + 2; ++q) {
+              for (int q = g; q < g + GS; ++q) {
                 // (a group that is hidden from the row has scores of -inf, whatever its scales)
                 float lv = scq[32 + q], iv = scq[64 + q];
                 if (__builtin_expect(diag, 0) && 16 * q > lim) {
@@ -739,8 +765,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 }
                 acc = f2_fma(sum, f2(iv, iv), acc);
               }
-              tmem_st16u(s_addr + part * (KC / 2) + 8 * g, pk);
-              if (CP == 1 && g + 2 == NG / 2) {
+              tmem_stn<8 * GS>(s_addr + part * (KC / 2) + 8 * g, pk);
+              if (HALVES && g + 2 == NG / 2) {
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -752,16 +778,14 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               l += rs.x + rs.y;
             }
             tmem_wait_st();
-          } else if (CP == 1 && lane == 0) {
+          } else if (HALVES && lane == 0) {
             mbar_arrive(PF(x, 0));
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if (CP > 1) mbar_arrive(PF(x, 0));
-            mbar_arrive(PF(x, 1));
-          }
+          if (lane == 0) mbar_arrive(PF(x, HALVES ? 1 : place(n_tile)));
           ++n_tile;
+          if (!ok) break;
         }
         if (jj % NB == NB - 1 || jj == nt - 1) {
           __syncwarp();
@@ -1159,10 +1183,10 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       const uint64_t dq = smem_desc(sbase + S::OFF_Q + (ALT ? 0 : x) * S::Q_BYTES, 16, 8 * SPAN, SWZ);
       const uint64_t dk0 = smem_desc(sbase + S::OFF_K, 16, 8 * SPAN, SWZ);
       const uint64_t dv0 = smem_desc(sbase + S::OFF_V, KT * SPAN, 8 * SPAN, SWZ);
-      const uint32_t s_tmem = tmem + S::TM_S + x * KT, o_tmem = tmem + S::TM_O + x * D;
+      const uint32_t s_tmem = tmem + S::TM_S + S::SB * x * KT, o_tmem = tmem + S::TM_O + x * D;
       const bool leader = elect_one();
       int kt = 0;                        // key tiles of the fragments before
-      int n_q = 0, n_p = 0, n_d = 0;     // query tiles, tiles of P, waits for the end of P V
+      int n_q = 0, n_s = 0, n_p = 0;     // query tiles, tiles of S and of P
       auto wait = [&](uint32_t b, int parity, int site) {
         return __all_sync(0xffffffffu, extend_wait(b, parity, failed, site)) != 0;
       };
@@ -1177,12 +1201,13 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off_q = ((kk * 32) / SPAN) * 128 * SPAN + (kk * 32) % SPAN;
             const uint32_t off_k = ((kk * 32) / SPAN) * KT * SPAN + (kk * 32) % SPAN;
-            umma_f16_ss(s_tmem, dq + (off_q >> 4), dk + (off_k >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
+            umma_f16_ss(s_tmem + place(n_s) * KT, dq + (off_q >> 4), dk + (off_k >> 4), IDESC_QK, kk > 0 ? 1u : 0u);
           }
-          umma_commit(SF(x));
+          umma_commit(SF(x, place(n_s)));
           umma_commit(KE(st));
         }
         __syncwarp();
+        ++n_s;
       };
       while (ok) {
         const ExtendFrag f = take();
@@ -1191,33 +1216,36 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         const int step = ALT ? 2 : 1, first = ALT ? x : 0;
         if (ALT || n > 0) ok = wait(QF(ALT ? 0 : x), n_q++ & 1, 530);
         if (ok && n > 0) scores(first);
+        if (S::SB == 2 && ok && n > 1) scores(first + step);
         for (int i = 0; ok && i < n; ++i) {
           const int jj = first + i * step, st = (kt + jj) % NV;
           if (!(ok = wait(VF(st), ((kt + jj) / NV) & 1, 532))) break;
           const uint64_t dv = dv0 + static_cast<uint64_t>((st * S::T_BYTES) >> 4);
+          constexpr int PH = HALVES ? 2 : 1;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (!(ok = wait(PF(x, half), n_p & 1, 531))) break;
+          for (int half = 0; half < PH; ++half) {
+            if (!(ok = wait(PF(x, HALVES ? half : place(n_p)), turn(n_p), 531))) break;
             tc_fence_after();
             if (leader) {
 #pragma unroll
-              for (int kk = half * (KT / 32); kk < (half + 1) * (KT / 32); ++kk)
-                umma_f16_ts(o_tmem, s_tmem + kk * 8, dv + static_cast<uint64_t>((kk * 16 * SPAN) >> 4), IDESC_PV, (i > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = half * (KT / 16 / PH); kk < (half + 1) * (KT / 16 / PH); ++kk)
+                umma_f16_ts(o_tmem, s_tmem + place(n_p) * KT + kk * 8, dv + static_cast<uint64_t>((kk * 16 * SPAN) >> 4), IDESC_PV, (i > 0 || kk > 0) ? 1u : 0u);
             }
             __syncwarp();
           }
           if (!ok) break;
-          ++n_p;
           if (leader) {
             umma_commit(VE(st));
+            if (!ORDERED) umma_commit(OD(x));
             if (i == n - 1) umma_commit(OF(x));
-            else if (!ORDERED) umma_commit(OD(x));
           }
           __syncwarp();
-          if (i + 1 < n) {
-            if (!ORDERED && !(ok = wait(OD(x), n_d++ & 1, 534))) break;
-            scores(jj + step);
+          // The next S (but one, with two) overwrites this P.
+          if (i + S::SB < n) {
+            if (!ORDERED && !(ok = wait(OD(x), n_p & 1, 534))) break;
+            scores(jj + S::SB * step);
           }
+          ++n_p;
         }
         if (NT == 2) {
           // Tiles that only the other stream has: released as they come.
