@@ -40,6 +40,16 @@
 //    warps take half (a quarter) of each tile's keys, P being zero for the others. Each copy is a part of its
 //    rows of its own. (At head_dim 256 joining the copies cost as much as they gave.)
 //
+// Bounds and measures (device time): where a stream has its own rows, the exponentials and what a warp does
+// around them: of the ~2400 clocks that a stream takes for 128 rows and 64 keys 512 are the special function
+// unit's, ~600 other instructions of the same warp and the rest waits (32 heads on 8 of 128: the last 2048 of
+// 32768 tokens 1.19 ms, 900 TFLOP/s, 54 % of a bf16 product's rate; 256 behind 32512 178 us; 8 requests of up to 777 tokens,
+// 32 heads of 64, up to 2048 keys 164 us). Where streams share rows, shared memory: per 128 keys at head_dim 128 it
+// moves 32 KB raw in and out, 64 KB widened in and out again and the query rows' 32 KB, at least ~1800 clocks
+// against 1400 that the cached bytes take from HBM; then the beginnings and ends of fragments, ~10000 clocks
+// each (64 requests of up to 4096, 4 new tokens, 32 heads on 8 of 128: 109 us, 2.5 TB/s; 16 of up to 20001, 16
+// tokens, 64 on 8: 115 us). A small call is its launches and a chain of dependent loads (8.4 us).
+//
 // Warps (512 threads): 0-3 and 4-7 softmax; 8-11 widen K and V (4-11 at head_dim 256); 12 bulk copies of K;
 // 13 walks the fragments, fetches the scales and copies V; 14 and 15 the products of a stream each (14: and
 // TMEM). Every wait is bounded.
@@ -128,7 +138,9 @@ struct ExtendShape {
   static constexpr int SW = 4 * NS;      // softmax warps
   static constexpr int WC = NS == 2 ? 2 : 4;  // warps that widen K, and as many V
   static constexpr int REG_SOFTMAX = 200, REG_WIDEN = NS == 2 ? 64 : 112, REG_ISSUE = NS == 2 ? 48 : 88;
-  // Tiles that an item's beginning is charged with.
+  // Tiles that an item's beginning is charged with. (Of 128 keys, with 4 / 5 / 7: 64 requests of up to 4096 111 /
+  // 109 / 105 us, 128 of 1000 110 / 116 / 117, 16 of up to 20001 116 / 115 / 117, 16 of 2048 at head_dim 64 84 /
+  // 79 / 80; of 64 keys, with 4 / 5 / 6: 163 / 163 / 164, 256 tokens behind 32512 180 / 179 / 178.)
   static constexpr int PEN = KT == 64 ? 6 : 5;
   static constexpr int KC = KT / CP;             // keys of a tile that a softmax warp takes
   static constexpr int RW = 4 / CP;              // softmax warps of a copy

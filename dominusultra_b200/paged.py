@@ -251,7 +251,8 @@ def dominus_ultra_paged_tables(
     over a block's end take blocks from the ring of free ones, in order of ``b`` from its head, as
     long as the needs up to a request are covered; a request that is not served keeps its length.
     Requests that shrink give blocks back behind the ring's tail, free from the next call on; a block is
-    held by one request only (a block in two rows would be given back twice).
+    held by one request only (a block in two rows would be given back twice). Requests that share blocks
+    shrink and end through ``dominus_ultra_paged_fork``; they grow here.
 
     ``block_table`` (new entries) and ``free_blocks`` (given-back ids) are updated in place; the
     lengths and ``free_state`` are not: pass the returned ones to the next call, or copy them

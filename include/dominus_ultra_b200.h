@@ -333,8 +333,11 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
  * the table's row and rope_positions) give zeros and code 6; a block id out of range gives NaN in the
  * rows that see its keys, and code 7. workspace: du_extend_paged_workspace_size bytes, 16-byte
  * aligned, any contents; calls that may overlap on the GPU, replayed graphs among them, need one each.
- * A table row covers at most 2^27 tokens. The caches are as du_paged_write leaves them:
- * no value that is not a number under a finite scale.
+ * A table row covers at most 2^27 tokens; Hq is at most 65536, T 2^20, T Hq / Hkv 2^24 and B 2^20. The caches are
+ * as du_paged_write leaves them: no value that is not a number under a finite scale. Scales as in
+ * du_decode_paged. Precision: query rows and softmax weights are carried as fp16 (to 2^-11 of
+ * themselves; weights below 2^-22 of a row's largest, times its value scale, to 2^-33 of that), sums and
+ * outputs in fp32; the order of the sums, and so every bit, depends on the sizes and lengths only.
  */
 size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size,
                                       int max_blocks);
