@@ -31,9 +31,8 @@
 //  - NT = 2 (more than 128 rows in an item): a stream is a tile of 128 rows. It has two tiles of S of 64 keys, so
 //    that a warpgroup goes from tile to tile without waiting for products (also at head_dim 256, with one row tile).
 //  - NT = 1: the streams share the one row tile and take every other key tile of 128 each; a row then has two
-//    parts, each with a maximum, sum and O of its own, joined at the fragment's end. What bounds these is shared
-//    memory: of the bytes that widening and products move per key there, the query rows' are per tile, so tiles are
-//    long (with 64 keys 117 -> 122 us for 16 requests of 128 rows behind 10000 keys), and the other stream's
+//    parts, each with a maximum, sum and O of its own, joined at the fragment's end. Of the bytes that widening and
+//    products move through shared memory the query rows' are per tile, and so are the hand-offs, so tiles are long (with 64 keys 117 -> 122 us for 16 requests of 128 rows behind 10000 keys), and the other stream's
 //    softmax fills the time in which one waits.
 //  - Copies: a softmax warp has 32 of the row tile's rows, so with 64 rows or fewer most would idle while one has all
 //    the keys of a tile to do: there the tile holds two (or, with 32 rows, four) copies of the rows, and a copy's
@@ -44,7 +43,7 @@
 // around them: of the ~2400 clocks that a stream takes for 128 rows and 64 keys 512 are the special function
 // unit's, ~600 other instructions of the same warp and the rest waits (32 heads on 8 of 128: the last 2048 of
 // 32768 tokens 1.19 ms, 900 TFLOP/s, 54 % of a bf16 product's rate; 256 behind 32512 178 us; 8 requests of up to 777 tokens,
-// 32 heads of 64, up to 2048 keys 164 us). Where streams share rows, shared memory: per 128 keys at head_dim 128 it
+// 32 heads of 64, up to 2048 keys 164 us). Where streams share rows, latency too (no unit is half busy), then shared memory: per 128 keys at head_dim 128 it
 // moves 32 KB raw in and out, 64 KB widened in and out again and the query rows' 32 KB, at least ~1800 clocks
 // against 1400 that the cached bytes take from HBM; then the beginnings and ends of fragments, ~10000 clocks
 // each (64 requests of up to 4096, 4 new tokens, 32 heads on 8 of 128: 109 us, 2.5 TB/s; 16 of up to 20001, 16
