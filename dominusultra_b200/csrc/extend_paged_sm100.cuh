@@ -975,8 +975,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       } else {
         if (f.nf > 1 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = lse;
         if (n > 0 && warp_rows) {
-          // Whole items' rows go out through shared memory, where the query rows were, so that lanes share lines.
-          const uint32_t mine = q_tile + row * (2 * D);
+          // Whole items' rows go out through shared memory, so that lanes share lines: each where its own query row
+          // was, piece for piece. A warp so writes no bytes but those of its own query rows, which it is the next to
+          // write, and no warp waits for the others; row after row, warps would share bytes from head_dim 128 on.
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             float o[16];
@@ -993,7 +994,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 }
               } else {
                 const uint2 u = pack4(o + k), v = pack4(o + k + 4);
-                st_shared_v4(mine + 16 * (((c + k) / 8 + row) % (D / 8)), make_uint4(u.x, u.y, v.x, v.y));
+                st_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, row, (c + k) / 8), make_uint4(u.x, u.y, v.x, v.y));
               }
             }
           }
@@ -1006,7 +1007,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               const int from = i * RPO + lane / LPO, at = 32 * w4 + from;
               const long long to = static_cast<long long>(__shfl_sync(0xffffffffu, q_row_hi, from)) << 32 |
                                    static_cast<uint32_t>(__shfl_sync(0xffffffffu, q_row_lo, from));
-              const uint4 v = ld_shared_v4(q_tile + at * (2 * D) + 16 * ((lane % LPO + at) % LPO));
+              const uint4 v = ld_shared_v4(q_tile + swz_chunk_offset<SPAN>(128, at, lane % LPO));
               if (r_item - lane + from < f.rows) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + to * (2 * D) + 16 * (lane % LPO)) = v;
             }
             __syncwarp();
