@@ -682,6 +682,8 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
                 mx = fmaxf(mx, fmaf(ga[g], kq[g], scq[32 + g]));
               }
             }
+            // (a row that is not there has whatever shared memory held, and no say in what its warp does)
+            if (!row_ok) mx = -INFINITY;
             const float m_old = m, mlo_old = mlo;
             bool moved = mx > m + mlo + EXTEND_MOVE;
             float base = 0.f;  // what is taken off log2 vs
@@ -702,6 +704,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
               float hi = -INFINITY, lo = -INFINITY;
 #pragma unroll
               for (int g = 0; g < NG; ++g) hi = fmaxf(hi, ga[g] * kq[g]);
+              if (!row_ok) hi = -INFINITY;
               const float h0 = hi == -INFINITY ? 0.f : hi;
 #pragma unroll
               for (int g = 0; g < NG; ++g) lo = fmaxf(lo, less(ga[g], kq[g], h0) + scq[32 + g]);

@@ -337,7 +337,8 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
  * as du_paged_write leaves them: no value that is not a number under a finite scale. Scales as in
  * du_decode_paged. Precision: query rows and softmax weights are carried as fp16 (to 2^-11 of
  * themselves; weights below 2^-22 of a row's largest, times its value scale, to 2^-33 of that), sums and
- * outputs in fp32; the order of the sums, and so every bit, depends on the sizes and lengths only.
+ * outputs in fp32. The order of the sums depends on the sizes and lengths only, so the same inputs give the same
+ * bits; a row with scores beyond 2^10 (of the base-2 exponential) may change the last bits of rows beside it.
  */
 size_t du_extend_paged_workspace_size(int B, int Hq, int Hkv, int T, int D, int block_size,
                                       int max_blocks);

@@ -44,3 +44,28 @@ def test_items_one_after_the_other(name, busy):
         out = _call(c)
         assert ((out.double() - ref).abs() <= tol).all()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("name", UNCUT)
+def test_the_same_bits_every_time(name):
+    Hq, Hkv, D, T, new, past, dtype = UNCUT[name]
+    c = _case(Hq, Hkv, D, T, past, new, 16, dtype, seed=len(new) + T + D)
+    want = _call(c)
+    for _ in range(20):
+        assert torch.equal(_call(c), want)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("T", [1, 5, 16, 33, 70])
+def test_rows_that_are_not_there_have_no_say(D, T):
+    """The same bits, whatever a call before left in the shared memory of rows that a request does not fill."""
+    c = _case(2, 2, D, T, [700] * 40, [T] * 40, 16, torch.bfloat16, seed=D + T)
+    c["q"] = c["q"] * 2.0**-6
+    c["ks"] = c["ks"] * 2.0**6
+    before = _case(2, 2, D, 256, [64] * 80, [256] * 80, 16, torch.bfloat16, seed=1)
+    want = None
+    for factor in (0.0, 1.0, 2.0**8):
+        _call(dict(before, q=before["q"] * factor))
+        out = _call(c)
+        want = out if want is None else want
+        assert torch.equal(out, want)
