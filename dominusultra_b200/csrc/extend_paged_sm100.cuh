@@ -813,8 +813,9 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
       if (S::PARTS > 1 ? softmax_any<ST>(!ok) : !ok) break;
       tc_fence_after();
       // The log2 of the row's (or its part's) sum, in two parts; and what brings O to the fragment's output,
-      // O 2^(m + mlo - 8) over the sum, in two factors since the exponent may be large.
-      float2 lse = l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m, lg2(l) + (far ? eo : mlo - EXTEND_TOP - vr));
+      // O 2^(m + mlo - 8) over the sum, in two factors since the exponent may be large. A sum that is not a number
+      // (a block's scale, or a block without an id) must not look like no keys: the maximum passes over such scores.
+      float2 lse = l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(l == l ? m : l, lg2(l) + (far ? eo : mlo - EXTEND_TOP - vr));
       float w1 = 0.f, w2 = 0.f;
       if (l != 0.f) {
         const float ex = far ? mlo - EXTEND_TOP - eo : vr, half = rintf(0.5f * ex);
