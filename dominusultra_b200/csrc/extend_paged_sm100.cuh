@@ -822,6 +822,10 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         w2 = ex2(half);
         w1 = ex2(ex - half) / l;
       }
+      // A row of a whole item sees a key at least. Where all that it sees have scores of -inf (an infinite query), its
+      // softmax is not a number, as it is in an item that is cut, where the joining kernel divides by no weight.
+      const bool whole = f.nf == 1;
+      constexpr float not_a_number = __builtin_nanf("");
       float4* const part_o = reinterpret_cast<float4*>(p.part);
       float2* const part_l = reinterpret_cast<float2*>(p.part + 2LL * gridDim.x * RP * D);
       auto part_at = [&](int slot, int col, int r) { return (static_cast<long long>(slot) * (D / 4) + col / 4) * RP + r; };
@@ -869,6 +873,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         softmax_sync<ST>();
         if (lse.x != -INFINITY) w1 *= ex2((lse.x - top.x) + (lse.y - top.y)) / sum;
         if (top.x != -INFINITY) top.y += lg2(sum);
+        else if (whole) w1 = not_a_number;
         if (f.nf > 1 && mine == 0 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = top;
         // (two quarters, or all, where half or a quarter of the rows are there)
         const int at_once = f.rows > ROWS / 2 ? 1 : (f.rows > ROWS / 4 ? 2 : 4), rows_p = ROWS / at_once;
@@ -927,6 +932,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
             lse.y += lg2(total);
           }
         }
+        if (whole && lse.x == -INFINITY) w1 = not_a_number;
         if (f.nf > 1 && x == 0 && row_ok) part_l[static_cast<long long>(f.slot) * RP + row] = lse;
         constexpr int CB = D / 4, PC = CB / 4;
         float4* buf = reinterpret_cast<float4*>(sgen + S::OFF_Q);
@@ -978,6 +984,7 @@ __global__ void __launch_bounds__(EXTEND_THREADS, 1) extend_paged_kernel(const E
         }
       } else {
         if (f.nf > 1 && row_ok) part_l[static_cast<long long>(f.slot) * RP + r_item] = lse;
+        if (whole && l == 0.f) w1 = not_a_number;
         if (n > 0 && warp_rows) {
           // Whole items' rows go out through shared memory, so that lanes share lines: each where its own query row
           // was, piece for piece. A warp so writes no bytes but those of its own query rows, which it is the next to

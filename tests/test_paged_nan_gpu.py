@@ -62,3 +62,24 @@ def test_a_fragment_without_a_number(D, T, where, which):
     assert torch.equal(out[0, heads][:, ~seen], clean[0, heads][:, ~seen])
     if which != "id":
         assert torch.equal(out[0, 2:], clean[0, 2:])
+
+
+@pytest.mark.parametrize("cut", [False, True], ids=["whole", "cut"])
+@pytest.mark.parametrize("T", ROWS)
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+def test_scores_that_are_all_minus_infinity(D, T, cut):
+    """The softmax of a row that has no other scores is not a number, however its keys are cut."""
+    n = 20000 if cut else T + 3
+    c = _case(4, 2, D, T, [n - T], [T], 16, torch.float16, seed=1)
+    c["cos"].fill_(0.75)
+    c["sin"].fill_(0.5)
+    for i in (0, D // 2):
+        c["k"].view(torch.uint8)[..., i] = 0xB8  # -1 in the pair of coordinates that the infinity turns into
+    clean = _call(c)
+    c["q"][0, 1, 0, 0] = float("inf")
+    if T > 1:
+        c["q"][0, 3, T - 1, 0] = float("inf")
+    out = _call(c)
+    bad = torch.isinf(c["q"][0]).any(-1)
+    assert torch.isfinite(clean).all()
+    assert torch.isnan(out[0][bad]).all() and torch.equal(out[0][~bad], clean[0][~bad])
