@@ -155,12 +155,14 @@ __device__ __forceinline__ int paged_fork_slot(int id, int slots) {
 constexpr int PAGED_FORK_BLOCKS = (1 << 19) - 1;  // ids of 19 bits beside the requests' 13
 
 // What request b takes over: the first `n` tokens of row `src`. A request with a length, source or
-// wanted length out of range is kept: its row is copied as it is, and it holds its blocks whole (none,
-// if its own length is out of range).
+// wanted length out of range is kept: its row is copied as it is, and it holds its blocks whole. Where its own
+// length is out of range nobody knows which of the row's entries are its blocks, so all that are block ids count
+// as held after the call: others may share them, and none is given back. (They do not count as held before: a block
+// that nobody else holds then stays out of the ring, as the row that names it stays.)
 struct PagedForkAsk {
   int src, n;
   int pages, old_pages;  // blocks that it holds after and before
-  bool kept;
+  bool kept, lost;       // lost: its own length is out of range
 };
 __device__ __forceinline__ PagedForkAsk paged_fork_ask(const PagedForkParams& p, int b) {
   PagedForkAsk a;
@@ -169,11 +171,12 @@ __device__ __forceinline__ PagedForkAsk paged_fork_ask(const PagedForkParams& p,
   const bool own = len >= 0 && len <= cap;
   const bool from = s >= 0 && s < p.B;
   const int ls = p.lens[from ? s : b];
+  a.lost = !own;
   a.kept = !own || !from || ls < 0 || ls > cap || w < 0 || w > ls;
   a.src = a.kept ? b : s;
   a.n = a.kept ? len : w;
   a.old_pages = own ? (len + p.block - 1) >> p.shift : 0;
-  a.pages = a.kept ? a.old_pages : (w + p.block - 1) >> p.shift;
+  a.pages = a.lost ? p.width : (a.kept ? a.old_pages : (w + p.block - 1) >> p.shift);
   return a;
 }
 
@@ -237,14 +240,15 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
     // (a piece's entries are on their way while those of the one before are marked)
     int old_ids[PAGED_SET_PAGES / 32], new_ids[PAGED_SET_PAGES / 32];
     int b = 0, c0 = 0, pages = 0, partly = -1, tokens = 0, bad = 0;
-    bool any_bad = false;
+    bool any_bad = false, lost = false;
 #pragma unroll 1
     for (int i = 0; i <= nq; ++i) {
       int next_old[PAGED_SET_PAGES / 32], next_new[PAGED_SET_PAGES / 32];
       const int nb = __shfl_sync(0xffffffffu, my_b, i), nc0 = __shfl_sync(0xffffffffu, my_c0, i);
       const int src = __shfl_sync(0xffffffffu, a.src, i), n = __shfl_sync(0xffffffffu, a.n, i);
       const int npages = __shfl_sync(0xffffffffu, a.pages, i), old_pages = __shfl_sync(0xffffffffu, a.old_pages, i);
-      const bool kept = __shfl_sync(0xffffffffu, static_cast<int>(a.kept), i) != 0;
+      const int how = __shfl_sync(0xffffffffu, static_cast<int>(a.kept) + static_cast<int>(a.lost), i);
+      const bool kept = how != 0;
       if (i < nq) {
         const int* row_old = p.table + static_cast<long long>(nb) * p.width + nc0 + lane;
         const int* row_new = p.table + static_cast<long long>(src) * p.width + nc0 + lane;
@@ -267,7 +271,7 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
             if (static_cast<unsigned>(y) < static_cast<unsigned>(p.N)) {
               set_bit(after, y);
               if (page != partly) set_bit(whole, y);
-            } else {
+            } else if (!lost) {
               any_bad = true;
               bad = y;
             }
@@ -293,6 +297,7 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
       b = nb;
       c0 = nc0;
       pages = npages;
+      lost = how == 2;
       partly = !kept && (n & (p.block - 1)) != 0 ? npages - 1 : -1;
       tokens = kept ? -1 : n;
     }

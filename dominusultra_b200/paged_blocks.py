@@ -113,7 +113,8 @@ def dominus_ultra_paged_fork(
     Args:
         block_table: [batch, max_blocks] int32
         cache_seqlens: [batch] integer tokens cached (int32 or int64; on the CPU they are checked
-            here, on the GPU a request out of range keeps its row and ``_lib.read_status()`` reports 6)
+            here, on the GPU a request out of range keeps its row and every block in it, and
+            ``_lib.read_status()`` reports 6)
         sources: [batch] integer requests to continue from
         new_seqlens: [batch] integer tokens to take over, at most the source's
         free_blocks: [num_blocks] int32, a ring of free block ids

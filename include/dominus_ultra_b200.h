@@ -360,7 +360,8 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
  * whole blocks: seqlens_out[b] says so. Blocks that were held before and are not held any more go
  * behind the ring's tail in order of their ids, free from the next call on. free_blocks is updated in
  * place, nothing else is: outputs must not be inputs. A request whose lengths or source are out of
- * range keeps its row and its blocks (code 6); if more is given back than the ring has room for, or its
+ * range keeps its row and its blocks (code 6; where its own length is, every block id in its row counts as held, so
+ * that none is given back or written by others); if more is given back than the ring has room for, or its
  * state is out of range, nothing changes (code 7). num_blocks and B are bounded by the kernel's 200 KB of
  * sets: 3 bits a block and 112 a request (at most 8192 requests, and 524287 blocks or, with 8192 requests,
  * 240000).
