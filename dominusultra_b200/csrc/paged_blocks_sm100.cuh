@@ -59,6 +59,17 @@ __device__ __forceinline__ void cluster_store2(const int2* here, uint32_t rank, 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(here)), "r"(rank));
   asm volatile("st.shared::cluster.v2.s32 [%0], {%1, %2};" :: "r"(a), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void cluster_store1(const int* here, uint32_t rank, int x) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(here)), "r"(rank));
+  asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(a), "r"(x) : "memory");
+}
+// Bits taken out of a word of another CTA's.
+__device__ __forceinline__ void cluster_and(const uint32_t* here, uint32_t rank, uint32_t mask) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(here)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.and.b32 [%0], %1;" :: "r"(a), "r"(mask) : "memory");
+}
 // A set of p.N ids as bits: words, and the share of them that a CTA joins (both whole 16-byte pieces).
 __host__ __device__ __forceinline__ int set_words(int n) { return ((n + 127) >> 7) << 2; }
 __host__ __device__ __forceinline__ int set_slice(int words) { return ((words + 4 * PAGED_SET_CTAS - 1) / (4 * PAGED_SET_CTAS)) * 4; }
@@ -439,6 +450,10 @@ struct PagedCompactParams {
 // ascending order from its start. Blocks that are in neither set belong to others and stay. A ring whose
 // entries are not `count` different block ids that no request holds is not the tables': nothing moves.
 //
+// A request whose length is out of range keeps its row as it is, so none of the blocks in it may move, whoever else
+// holds them: where there is such a request (every CTA is told), its entries are taken out of U again once U is
+// joined, at the price of two more barriers.
+//
 // Ranks are counts of bits: of the slices before, of the words before in the slice, of the bits before in
 // the word. The destinations are listed here, by rank; the second kernel looks a table's entry up by its
 // rank, and lists sources and free ids.
@@ -453,6 +468,7 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
   __shared__ unsigned long long part[PAGED_SET_WARPS];
   __shared__ int2 told[2 * PAGED_SET_CTAS];  // {ids in use, free ids}, {ids that are both, -} of CTA r's slice: each tells all
   __shared__ int end_here[3];   // the end, ids in use and free ids before it in its slice
+  __shared__ int lost;          // some request's length is out of range
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   const int words = set_words(p.N), slice = set_slice(words);
@@ -461,6 +477,9 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
   int* rank_of = reinterpret_cast<int*>(spare + words);  // [slice] free ids below the end before each word of this slice
 #pragma unroll 1
   for (int i = tid; i < 2 * words; i += PAGED_SET_THREADS) sm_set[i] = 0u;
+  if (tid == 0) lost = 0;
+  __syncwarp();
+  cluster_arrive();
   griddep_launch_dependents();
   griddep_wait();
   const int head = p.state[0], count = p.state[1];
@@ -478,12 +497,14 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
   const int share = (pieces + all_warps - 1) / all_warps;
   const int q_first = min((static_cast<int>(rank) * PAGED_SET_WARPS + warp) * share, pieces);
   const int q_end = min(q_first + share, pieces);
+  bool any_lost = false;
 #pragma unroll 1
   for (int q0 = q_first; q0 < q_end; q0 += 32) {
     const int nq = min(32, q_end - q0);
     const int my_b = (q0 + min(lane, nq - 1)) / per_row, my_c0 = (q0 + min(lane, nq - 1) - my_b * per_row) * PAGED_SET_PAGES;
     const int len = p.lens[my_b];
     const bool bad = len < 0 || len > cap;
+    any_lost = any_lost || bad;
     if (bad && lane < nq) paged_set_error(6u, static_cast<unsigned>(my_b), static_cast<unsigned>(len));
     const int held = bad || lane >= nq ? 0 : (len + p.block - 1) >> p.shift;
     int ids[PAGED_SET_PAGES / 32], b = 0, left = 0, bad_id = 0;
@@ -531,11 +552,33 @@ __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_S
     for (int k = 0; k < RING; ++k)
       if (static_cast<unsigned>(ring[k]) < static_cast<unsigned>(p.N)) set_bit(spare, ring[k]);
   }
+  any_lost = __any_sync(0xffffffffu, any_lost);
+  cluster_wait();  // (the cluster's CTAs run)
+  if (any_lost && lane < PAGED_SET_CTAS) cluster_store1(&lost, static_cast<uint32_t>(lane), 1);
   cluster_sync();
 
   // This CTA's slice of the ids: the eight CTAs' bits joined and counted.
   const int w0 = min(static_cast<int>(rank) * slice, words), w1 = min(w0 + slice, words);
   join_slices(sm_set, words, 2, w0, w1);
+  if (lost) {
+    cluster_sync();
+#pragma unroll 1
+    for (int q = q_first; q < q_end; ++q) {
+      const int b = q / per_row, c0 = (q - b * per_row) * PAGED_SET_PAGES, len = p.lens[b];
+      if (len >= 0 && len <= cap) continue;
+#pragma unroll 1
+      for (int page = c0 + lane; page < min(c0 + PAGED_SET_PAGES, p.width); page += 32) {
+        const int id = p.table[static_cast<long long>(b) * p.width + page];
+        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.N)) continue;
+        const int w = id >> 5;
+        const uint32_t owner = static_cast<uint32_t>(w / slice), bit = 1u << (id & 31);
+        // (one that is in the ring too stays: the ring is not the tables' then)
+        if (!(cluster_load(spare + w, owner) & bit)) cluster_and(used + w, owner, ~bit);
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   unsigned long long n3 = 0, below;
 #pragma unroll 1
   for (int w = w0 + tid; w < w1; w += PAGED_SET_THREADS) n3 += count3(__popc(used[w]), __popc(spare[w]), __popc(used[w] & spare[w]));
@@ -651,7 +694,9 @@ __global__ void __launch_bounds__(PAGED_APPLY_THREADS) paged_compact_rows_kernel
         x = -1;
       } else if (x >= end && x < p.N) {
         const int4 m = __ldcg(p.map + 1 + (x >> 5));
-        x = __ldcg(p.copies + 2LL * (m.y + __popc(static_cast<uint32_t>(m.x) & ((1u << (x & 31)) - 1u))) + 1);
+        const uint32_t bit = 1u << (x & 31);
+        if (static_cast<uint32_t>(m.x) & bit)  // (else it stays)
+          x = __ldcg(p.copies + 2LL * (m.y + __popc(static_cast<uint32_t>(m.x) & (bit - 1u))) + 1);
       }
     }
     p.table_out[e] = x;

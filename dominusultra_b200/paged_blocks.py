@@ -240,8 +240,8 @@ def dominus_ultra_paged_compact(
     Args:
         block_table: [batch, max_blocks] int32
         cache_seqlens: [batch] integer tokens cached (int32 or int64; on the CPU they are checked
-            here, on the GPU a request out of range keeps its row and its blocks, and
-            ``_lib.read_status()`` reports 6)
+            here, on the GPU a request out of range keeps its row, every block in it stays where it is,
+            and ``_lib.read_status()`` reports 6)
         free_blocks: [num_blocks] int32, a ring of free block ids
         free_state: [2] int32, {head, count} of the ring; if that does not hold ``count`` different
             blocks that nobody uses, nothing moves, and the status is 7

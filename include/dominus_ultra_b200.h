@@ -386,8 +386,8 @@ int du_paged_copy(void* k_cache, void* v_cache, float* k_scale, float* v_scale, 
  * ones among them, in ascending order, and their pairs are left in copies [num_blocks / 2, 2] for
  * du_paged_copy, the rest {-1, -1}. table_out [B, max_blocks] has the new ids up to each request's pages,
  * then -1; free_blocks_out [num_blocks] the free ids in ascending order, then -1, with free_state_out
- * {0, count}. Outputs must not be inputs. A request whose length is out of range keeps its row, and its
- * blocks stay (code 6). A ring that does not hold `count` different block ids, none of them in use,
+ * {0, count}. Outputs must not be inputs. A request whose length is out of range keeps its row, and every
+ * block in it that is not free stays, whoever else holds it (code 6). A ring that does not hold `count` different block ids, none of them in use,
  * leaves everything as it is (code 7). At most 770000 blocks. workspace:
  * du_paged_compact_workspace_size bytes, 16-byte aligned, any contents; calls that may overlap on the
  * GPU, replayed graphs among them, need one each.
