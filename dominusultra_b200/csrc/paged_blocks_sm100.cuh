@@ -211,7 +211,7 @@ __device__ __forceinline__ PagedForkAsk paged_fork_ask(const PagedForkParams& p,
 // 256 entries 9.9 us, 512 of 256 18.3 us.
 __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_SET_THREADS, 1)
     paged_fork_kernel(const PagedForkParams p) {
-  extern __shared__ uint32_t sm_set[];
+  extern __shared__ __align__(16) uint32_t sm_set[];  // (taken in pieces of 16 bytes)
   __shared__ int part[PAGED_SET_WARPS];
   __shared__ int2 freed_of[PAGED_SET_CTAS];  // {ids given back in CTA r's slice, -}: each tells all
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -464,7 +464,7 @@ struct PagedCompactParams {
 // took the cluster's eight SMs 20 us.
 __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_SET_THREADS, 1)
     paged_compact_kernel(const PagedCompactParams p) {
-  extern __shared__ uint32_t sm_set[];
+  extern __shared__ __align__(16) uint32_t sm_set[];  // (taken in pieces of 16 bytes)
   __shared__ unsigned long long part[PAGED_SET_WARPS];
   __shared__ int2 told[2 * PAGED_SET_CTAS];  // {ids in use, free ids}, {ids that are both, -} of CTA r's slice: each tells all
   __shared__ int end_here[3];   // the end, ids in use and free ids before it in its slice
