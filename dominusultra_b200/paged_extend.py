@@ -32,13 +32,18 @@ from .paged import (
 __all__ = ["dominus_ultra_extend_paged"]
 
 _I32 = torch.int32
+# Sizes by what they depend on (head_dim, and whether the new tokens' rows of a KV head fill a row tile), so that a
+# server whose batches, chunks and tables vary keeps no more than a few.
 _WS_SIZES = {}
 
 
-def _workspace_size(*key) -> int:
+def _workspace_size(B, Hq, Hkv, T, D, block_size, max_blocks, index) -> int:
+    key = (D, T * (Hq // Hkv) > 128, index)
     n = _WS_SIZES.get(key)
     if n is None:
-        n = _WS_SIZES[key] = int(_lib.load().du_extend_paged_workspace_size(*key[:-1]))
+        n = int(_lib.load().du_extend_paged_workspace_size(B, Hq, Hkv, T, D, block_size, max_blocks))
+        if n:  # (0: sizes that the call will refuse)
+            _WS_SIZES[key] = n
     return n
 
 
