@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(PAGED_COPY_THREADS) paged_copy_kernel(const Pa
     const bool values = rest >= p.parts;
     const int part = values ? rest - p.parts : rest;
     const int2 c = make_int2(p.copies[2 * pair], p.copies[2 * pair + 1]);
-    if (c.x < 0 && c.y < 0) continue;
+    if (c.x == -1 && c.y == -1) continue;
     if (static_cast<unsigned>(c.x) >= static_cast<unsigned>(p.N) || static_cast<unsigned>(c.y) >= static_cast<unsigned>(p.N)) {
       if (lane == 0 && rest == 0)
         record_error(7u, static_cast<unsigned>(pair), static_cast<unsigned>(static_cast<unsigned>(c.x) >= static_cast<unsigned>(p.N) ? c.x : c.y));
