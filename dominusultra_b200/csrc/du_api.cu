@@ -1598,6 +1598,8 @@ int launch_paged_sets(void (*kern)(Params), const Params& prm, long long set_wor
 //    of up to 777 tokens at head_dim 64 190 instead of 165. Up to 128 rows the second would be empty.
 //  - Copies where the rows leave softmax warps without any. 64 requests of 16 rows, one / two / four copies: 126 /
 //    112 / 109 us; at head_dim 64 103 / 83 / 80. Not at head_dim 256: 4 requests of 64 rows 45.5 us, with two copies 47.2.
+// The lengths are on the GPU, so this is decided by the most new tokens that a request can have, for the whole call:
+// single tokens beside a long chunk are items of two row tiles too, one of them empty.
 struct ExtendPlan {
   int nt, copies, grid;
 };

@@ -32,8 +32,9 @@
 //    that a warpgroup goes from tile to tile without waiting for products (also at head_dim 256, with one row tile).
 //  - NT = 1: the streams share the one row tile and take every other key tile of 128 each; a row then has two
 //    parts, each with a maximum, sum and O of its own, joined at the fragment's end. Of the bytes that widening and
-//    products move through shared memory the query rows' are per tile, and so are the hand-offs, so tiles are long (with 64 keys 117 -> 122 us for 16 requests of 128 rows behind 10000 keys), and the other stream's
-//    softmax fills the time in which one waits.
+//    products move through shared memory the query rows' are per tile, and so are the hand-offs, so tiles are long
+//    (with 64 keys 117 -> 122 us for 16 requests of 128 rows behind 10000 keys), and the other stream's softmax
+//    fills the time in which one waits.
 //  - Copies: a softmax warp has 32 of the row tile's rows, so with 64 rows or fewer most would idle while one has all
 //    the keys of a tile to do: there the tile holds two (or, with 32 rows, four) copies of the rows, and a copy's
 //    warps take half (a quarter) of each tile's keys, P being zero for the others. Each copy is a part of its
@@ -42,12 +43,15 @@
 // Bounds and measures (device time): where a stream has its own rows, the exponentials and what a warp does
 // around them: of the ~2400 clocks that a stream takes for 128 rows and 64 keys 512 are the special function
 // unit's, ~600 other instructions of the same warp and the rest waits (32 heads on 8 of 128: the last 2048 of
-// 32768 tokens 1.19 ms, 900 TFLOP/s, 54 % of a bf16 product's rate; 256 behind 32512 178 us; 8 requests of up to 777 tokens,
-// 32 heads of 64, up to 2048 keys 164 us). Where streams share rows, latency too (no unit is half busy), then shared memory: per 128 keys at head_dim 128 it
-// moves 32 KB raw in and out, 64 KB widened in and out again and the query rows' 32 KB, at least ~1800 clocks
-// against 1400 that the cached bytes take from HBM; then the beginnings and ends of fragments, ~10000 clocks
-// each (64 requests of up to 4096, 4 new tokens, 32 heads on 8 of 128: 109 us, 2.5 TB/s; 16 of up to 20001, 16
-// tokens, 64 on 8: 115 us). A small call is its launches and a chain of dependent loads (8.4 us).
+// 32768 tokens 1.20 ms, 890 TFLOP/s, 54 % of a bf16 product's rate; 256 behind 32512 177 us; 8 requests of up to
+// 777 tokens, 32 heads of 64, up to 2048 keys 165 us). Where streams share rows, latency too (no unit is half
+// busy), then shared memory: per 128 keys at head_dim 128 it moves 32 KB raw in and out, 64 KB widened in and out
+// again and the query rows' 32 KB, at least ~1800 clocks against 1400 that the cached bytes take from HBM; then the
+// beginnings and ends of fragments, ~10000 clocks each (64 requests of up to 4096, 4 new tokens, 32 heads on 8 of
+// 128: 109 us, 2.5 TB/s; 16 of up to 20001, 16 tokens, 64 on 8: 115 us). These are the bounds of this schedule: the
+// single-token kernel, which feeds cached bytes to the tensor cores as they are, streams such caches in half the
+// time. A small call is its launches and a chain of dependent loads (8.5 us where one key tile covers the table's
+// row, so that nothing is to be joined).
 //
 // Warps (512 threads): 0-3 and 4-7 softmax; 8-11 widen K and V (4-11 at head_dim 256); 12 bulk copies of K;
 // 13 walks the fragments, fetches the scales and copies V; 14 and 15 the products of a stream each (14: and

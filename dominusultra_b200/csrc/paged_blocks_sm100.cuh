@@ -201,14 +201,14 @@ __device__ __forceinline__ PagedForkAsk paged_fork_ask(const PagedForkParams& p,
 //
 // With the sets O (held before), N (held after), W (held whole after): given back = O \ N, and b keeps
 // its last block x iff x is not in W and no lower request ends partly in x. Marks are bits in shared
-// memory; a warp takes 128 entries at a time, and its lanes fetch the lengths of 32 such pieces at once. The new rows are written while they are marked, all but the blocks that turn out to be
-// the requests' own (written at the end, the rows cost a second pass: 8 us for 131072 entries, or the
-// 4 us of a second launch). Whoever sees a partly filled last block tells all CTAs, and each finds the
+// memory; a warp takes 128 entries at a time, and its lanes fetch the lengths of 32 such pieces at once. The
+// new rows are written while they are marked, all but the blocks that turn out to be the requests' own (written
+// at the end, the rows cost a second pass: 8 us for 131072 entries, or the 4 us of a second launch). Whoever sees a partly filled last block tells all CTAs, and each finds the
 // lowest request of every such block in a hash table of its own (entries {id, request} of 19 and 13 bits,
 // the lowest stays).
 //
 // Bound by latency: chains of loads (source, length, entry; ring), two cluster barriers. 64 requests of
-// 256 entries 9.9 us, 512 of 256 18.3 us.
+// 256 entries 9.8 us, 512 of 256 18.3 us.
 __global__ void __cluster_dims__(PAGED_SET_CTAS, 1, 1) __launch_bounds__(PAGED_SET_THREADS, 1)
     paged_fork_kernel(const PagedForkParams p) {
   extern __shared__ __align__(16) uint32_t sm_set[];  // (taken in pieces of 16 bytes)
@@ -458,7 +458,7 @@ struct PagedCompactParams {
 // the word. The destinations are listed here, by rank; the second kernel looks a table's entry up by its
 // rank, and lists sources and free ids.
 //
-// Bound by latency, as the fork; two cluster barriers. 16 requests of 64 entries 9.9 us, 256 of 512
+// Bound by latency, as the fork; two cluster barriers. 16 requests of 64 entries 10.0 us, 256 of 512
 // entries 17.7 us. The table's rows and the lists are written by a
 // second launch over all SMs, whose CTAs are resident before the cluster ends: looking up 131072 entries
 // took the cluster's eight SMs 20 us.

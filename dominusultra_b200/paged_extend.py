@@ -68,6 +68,10 @@ def dominus_ultra_extend_paged(
     up to its own. Rows behind a request's last new token are zeros. Rows of a block behind the length are
     never used, whatever they hold.
 
+    Query rows and softmax weights are carried as fp16, as in ``dominus_ultra_prefill``. On unit-normal queries fp16
+    outputs are off by about 0.0005 of their norm, 2.5 times what their own rounding takes (and
+    ``dominus_ultra_decode_paged`` with it); bf16 outputs by no more than their own rounding.
+
     Lengths and table are read on the GPU: lengths out of range give zeros, a block id out of range
     NaN in the rows that see its keys, and ``_lib.read_status()`` reports code 6 or 7. Given on the CPU,
     they are checked here.
