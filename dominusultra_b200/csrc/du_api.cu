@@ -179,6 +179,12 @@ cudaError_t ensure_smem_attr(Kern kern, int bytes) {
   return e;
 }
 
+// Held over the launches of a call that hands something from one kernel to the next through its workspace, and of the
+// calls that share that workspace: host threads that call on one stream share one, and kernels of another thread's
+// call between two of this one's would overwrite what the second is to read (its indices among them).
+std::mutex g_launch_mu;
+using LaunchOrder = std::lock_guard<std::mutex>;
+
 // Launch on `st`; with `pdl` as a programmatic dependent of the stream's previous kernel (the
 // kernel must call griddep_wait before touching that kernel's outputs).
 template <typename... KArgs, typename... Args>
@@ -1525,6 +1531,7 @@ int du_decode_paged(const void* q, const void* k_cache, const void* v_cache, con
   static_assert(du::DECODE_PAGED_MAX_CTAS <= DU_PAGED_TICKETS, "a ticket for each block of threads");
   if (!workspace || workspace_bytes < paged_ws_bytes(grid, Hq, Hkv, D) || !aligned16(workspace))
     return fail(DU_ERR_WORKSPACE, "workspace missing, misaligned or smaller than du_decode_paged_workspace_size");
+  const LaunchOrder order(g_launch_mu);
   du::DecodePagedParams prm{};
   prm.q = q;
   prm.ks = k_scale;
@@ -1742,6 +1749,7 @@ int du_paged_compact(const int* block_table, const int* cache_seqlens, const int
   prm.block = block_size;
   prm.shift = log2_of(block_size);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const LaunchOrder order(g_launch_mu);
   rc = launch_paged_sets(du::paged_compact_kernel, prm, words, st, "paged compact launch");
   if (rc != DU_OK) return rc;
   // a thread per entry of the table and per block
@@ -1862,6 +1870,7 @@ int du_extend_paged(const void* q, const void* k_cache, const void* v_cache, con
   prm.block_log2 = block_size == 16 ? 4 : (block_size == 32 ? 5 : (block_size == 64 ? 6 : 7));
   prm.scale_log2 = scale * 1.4426950408889634f;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const LaunchOrder order(g_launch_mu);
   switch (D) {
     case 16: return launch_extend<16>(prm, plan, st);
     case 32: return launch_extend<32>(prm, plan, st);
