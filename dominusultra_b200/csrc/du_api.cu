@@ -642,6 +642,7 @@ int decode_impl(const void* q, const void* kc, const void* vc, const void* cos, 
     return fail(DU_ERR_INVALID, "rope tables do not cover the query / key positions");
   if (!(scale > 0.f)) return fail(DU_ERR_INVALID, "scale must be positive");
   const DecodePlan pl = plan_decode(B, Hq, Hkv, L, D);
+  const LaunchOrder order(g_launch_mu);
   du::DecodeParams prm{};
   prm.q = q;
   prm.k = kc;
@@ -838,6 +839,7 @@ int decode_kvcache_impl(const void* q, const void* k_new, const void* v_new, voi
     return fail(DU_ERR_WORKSPACE, "decode_kvcache workspace of " + std::to_string(ly.total) +
                                       " bytes (256-byte aligned) is required");
   uint8_t* w8 = static_cast<uint8_t*>(ws);
+  const LaunchOrder order(g_launch_mu);
   du::DecodePrepParams pp{};
   pp.seqlens = seqlens;
   pp.k_new = k_new;
@@ -942,6 +944,7 @@ int du_prefill(const void* q, const void* k, const void* v, const void* cos, con
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
     return fail(DU_ERR_WORKSPACE, "prefill workspace of " + std::to_string(need) +
                                       " bytes (16-byte aligned) is required");
+  const LaunchOrder order(g_launch_mu);
   du::PrefillParams prm{};
   prm.cos = cos;
   prm.sin = sin;

@@ -17,8 +17,10 @@ def _body(name):
     return re.search(r"\nint " + name + r"\([^;{]*\) \{\n(.*?)\n\}\n", text, re.S).group(1)
 
 
-@pytest.mark.parametrize("name", ["du_extend_paged", "du_paged_compact", "du_decode_paged"])
-def test_launches_of_the_paged_scratch_are_held_together(name):
+@pytest.mark.parametrize(
+    "name", ["du_extend_paged", "du_paged_compact", "du_decode_paged", "du_prefill", "decode_impl", "decode_kvcache_impl"]
+)
+def test_launches_over_a_workspace_are_held_together(name):
     body = _body(name)
     assert body.count(HELD) == 1
     assert not re.search(r"\blaunch_\w+(<[^;]*?>)?\(", body[: body.index(HELD)])
