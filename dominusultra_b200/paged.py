@@ -210,16 +210,17 @@ def _workspace(nbytes: int, index: int, stream: int):
         return ws.data_ptr(), ws
     pair = _SCRATCH.get((index, stream))
     if pair is None or pair[2] < nbytes:
-        pair = _grow_scratch(nbytes, index, stream)
+        pair = _grow_scratch(nbytes, index, stream, slab_too=False)
     return pair[1], pair
 
 
-def _grow_scratch(nbytes: int, index: int, stream: int):
-    """A (device, stream)'s scratch of at least nbytes, and a ticket slab with room for captures."""
+def _grow_scratch(nbytes: int, index: int, stream: int, slab_too: bool = True):
+    """A (device, stream)'s scratch of at least nbytes, and (for calls that take tickets) a ticket slab with room
+    for captures, which is waited for."""
     device = torch.device("cuda", index)
     with _SLAB_LOCK:
         slab = _SLABS.get(index)
-        if slab is None or slab[1] > _SLAB_WORDS // 2:
+        if slab_too and (slab is None or slab[1] > _SLAB_WORDS // 2):
             if slab is not None:
                 _RETIRED.append(slab[0])  # graphs count in it
             # (a copy from the host has ended when it returns: the zeros are there for any stream)
