@@ -17,6 +17,7 @@ from .paged import (
     _CODES,
     _GET_DEVICE,
     _HEAD_DIMS,
+    _check_host_lengths,
     _check_host_table,
     _device_int32,
     _fit_cache,
@@ -74,7 +75,7 @@ def dominus_ultra_extend_paged(
 
     Lengths and table are read on the GPU: lengths out of range give zeros, a block id out of range
     NaN in the rows that see its keys, and ``_lib.read_status()`` reports code 6 or 7. Given on the CPU,
-    they are checked here.
+    they are checked here (a table only if ``cache_seqlens`` is there too).
 
     Args:
         q_new: [batch, num_heads, T, head_dim], not rotated
@@ -169,6 +170,8 @@ def _check_extend(q_new, k_cache, v_cache, k_scale, v_scale, block_table, past_s
                     raise ValueError(f"past_seqlens[{b}] = {p} is outside [{max(0, n - T)}, {n}]")
         if block_table.device.type == "cpu":
             _check_host_table(block_table, cache_seqlens, block_size, num_blocks)
+    elif past_seqlens.device.type == "cpu":
+        _check_host_lengths("past_seqlens", past_seqlens, most)
     with _OnDevice(device):
         if block_table.device.type == "cpu" and block_table.dtype == torch.int32:
             block_table = block_table.to(device)
