@@ -9,7 +9,7 @@
 // result.
 //
 // A call takes 10 to 18 us, all of it latency: loads that wait for loads, barriers, and the instructions' own
-// way from L2, since a call runs through the code once (a fork of 64 requests, which takes 9.9 us now, took
+// way from L2, since a call runs through the code once (a fork of 64 requests, which takes 9.8 us now, took
 // 12.6 with its loops unrolled, 42 KB of code instead of 21). Counts that all CTAs need are pushed into their
 // shared memory before a barrier: pulled after it, eight CTAs' warps queued at one word for up to 2 us.
 #pragma once
@@ -203,9 +203,9 @@ __device__ __forceinline__ PagedForkAsk paged_fork_ask(const PagedForkParams& p,
 // its last block x iff x is not in W and no lower request ends partly in x. Marks are bits in shared
 // memory; a warp takes 128 entries at a time, and its lanes fetch the lengths of 32 such pieces at once. The
 // new rows are written while they are marked, all but the blocks that turn out to be the requests' own (written
-// at the end, the rows cost a second pass: 8 us for 131072 entries, or the 4 us of a second launch). Whoever sees a partly filled last block tells all CTAs, and each finds the
-// lowest request of every such block in a hash table of its own (entries {id, request} of 19 and 13 bits,
-// the lowest stays).
+// at the end, the rows cost a second pass: 8 us for 131072 entries, or the 4 us of a second launch). Whoever
+// sees a partly filled last block tells all CTAs, and each finds the lowest request of every such block in a hash
+// table of its own (entries {id, request} of 19 and 13 bits, the lowest stays).
 //
 // Bound by latency: chains of loads (source, length, entry; ring), two cluster barriers. 64 requests of
 // 256 entries 9.8 us, 512 of 256 18.3 us.
